@@ -1,0 +1,144 @@
+// Attention under score rules (capped, biased by distance, masked by documents, prefixes or lengths; shared heads of keys), forward and backward.
+#include <math.h>
+
+#include "attn_rules.h"
+
+namespace {
+using namespace axhip;
+
+// One wave a row of queries, or a row of keys
+__global__ void __launch_bounds__(256) k_attn_rows(AttnArgs a, int64_t first) {
+    const int64_t n = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= (int64_t)a.B * a.H * a.Sq) return;
+    const int i = (int)(n % a.Sq), head = (int)(n / a.Sq % a.H), b = (int)(n / a.Sq / a.H);
+    attn_fwd_row(a, b, head, i, threadIdx.x & 63);
+}
+__global__ void __launch_bounds__(256) k_attn_dq_rows(AttnArgs a, int64_t first) {
+    const int64_t n = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= (int64_t)a.B * a.H * a.Sq) return;
+    const int i = (int)(n % a.Sq), head = (int)(n / a.Sq % a.H), b = (int)(n / a.Sq / a.H);
+    attn_dq_row(a, b, head, i, threadIdx.x & 63);
+}
+__global__ void __launch_bounds__(256) k_attn_dkv_rows(AttnArgs a, int64_t first) {
+    const int64_t n = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= (int64_t)a.B * a.Hkv * a.Sk) return;
+    const int j = (int)(n % a.Sk), hk = (int)(n / a.Sk % a.Hkv), b = (int)(n / a.Sk / a.Hkv);
+    attn_dkv_row(a, b, hk, j, threadIdx.x & 63);
+}
+
+// Workgroups of four waves for n waves, in launches that a grid holds
+template <typename Kernel>
+int launch_rows(Kernel kernel, const AttnArgs &a, int64_t n, const char *what) {
+    constexpr int64_t MOST = int64_t(1) << 23;   // workgroups: a grid holds fewer than 2^32 threads
+    for (int64_t first = 0; first < n; first += MOST * 4) {
+        const int64_t left = (n - first + 3) / 4;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(left < MOST ? left : MOST)), dim3(256), 0, kStream, a, first);
+        if (int rc = check_launch(what)) return rc;
+    }
+    return AXHIP_OK;
+}
+
+struct Tensor {
+    const void *at;
+    int64_t ld, heads;
+};
+
+// Checks that both entry points make, and the arguments that both pass on
+int attn_arguments(const char *who, AttnArgs &a, const Tensor *tensors, int n, int64_t kv_rows, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk,
+                   int64_t dk, float scale, const axhip_attn_rules *rules) {
+    for (int t = 0; t < n; t++)
+        if (!tensors[t].at) return fail(AXHIP_ERR_NULL_ARG, "%s: NULL tensor", who);
+    constexpr int64_t LONG = 1 << 24;
+    if (B < 0 || H <= 0 || Hkv <= 0 || Sq < 0 || Sk < 0 || Sq > LONG || Sk > LONG) return fail(AXHIP_ERR_SHAPE, "%s: bad extent", who);
+    if (H % Hkv != 0) return fail(AXHIP_ERR_SHAPE, "%s: query heads must be a multiple of the heads of keys", who);
+    if (dk < 4 || dk > 128 || dk % 4 != 0) return fail(AXHIP_ERR_NOT_IMPLEMENTED, "%s: head size %lld (multiples of 4 up to 128 only)", who, (long long)dk);
+    if (kv_rows < Sk) return fail(AXHIP_ERR_SHAPE, "%s: kv_rows must hold Sk rows", who);
+    for (int t = 0; t < n; t++) {
+        if (tensors[t].ld < tensors[t].heads * dk || tensors[t].ld % 4 != 0 || tensors[t].ld > (1 << 22))
+            return fail(AXHIP_ERR_SHAPE, "%s: row pitch must hold the heads, be a multiple of 4 and at most 2^22 floats", who);
+        if (((uintptr_t)tensors[t].at & 15) != 0) return fail(AXHIP_ERR_SHAPE, "%s: tensors must be 16-byte aligned", who);
+    }
+    if (B > 0x7fffff || B * H > 0x7fffffff || kv_rows > ((int64_t)1 << 40)) return fail(AXHIP_ERR_SHAPE, "%s: too many sequences", who);
+    axhip_attn_rules r = {};
+    if (rules) r = *rules;
+    if (!(r.cap >= 0.0f) || isinf(r.cap)) return fail(AXHIP_ERR_SHAPE, "%s: the cap must be zero or positive", who);
+    if (r.prefix && !r.causal) return fail(AXHIP_ERR_SHAPE, "%s: a prefix without a causal mask", who);
+    if ((r.doc_q == nullptr) != (r.doc_k == nullptr)) return fail(AXHIP_ERR_NULL_ARG, "%s: documents of queries and of keys, or neither", who);
+    a.kv_rows = kv_rows;
+    a.B = (int)B;
+    a.H = (int)H;
+    a.Hkv = (int)Hkv;
+    a.G = (int)(H / Hkv);
+    a.Sq = (int)Sq;
+    a.Sk = (int)Sk;
+    a.dk = (int)dk;
+    a.scale = scale;
+    a.q_up = r.cap > 0.0f ? scale / r.cap : scale * LOG2E;
+    a.cap2 = r.cap * LOG2E;
+    a.bias2 = LOG2E;
+    a.slopes = r.slopes;
+    a.prefix = r.prefix;
+    a.start = r.start;
+    a.lens = r.lens;
+    a.doc_q = r.doc_q;
+    a.doc_k = r.doc_k;
+    a.causal = r.causal != 0;
+    return AXHIP_OK;
+}
+
+}  // namespace
+
+extern "C" int axhip_attn_fwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, const float *V, int64_t ldv, int64_t kv_rows, float *O, int64_t ldo,
+                              float *L, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t dk, float scale, const axhip_attn_rules *rules) {
+    if (int rc = ensure_ready()) return rc;
+    AttnArgs a = {};
+    const Tensor tensors[] = {{Q, ldq, H}, {K, ldk, Hkv}, {V, ldv, Hkv}, {O, ldo, H}};
+    if (int rc = attn_arguments("attn_fwd", a, tensors, 4, kv_rows, B, H, Hkv, Sq, Sk, dk, scale, rules)) return rc;
+    if (B == 0 || Sq == 0) return AXHIP_OK;
+    a.Q = Q;
+    a.K = K;
+    a.V = V;
+    a.O = O;
+    a.L = L;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.ldo = ldo;
+    note_kernel("attn_rows");
+    return launch_rows(k_attn_rows, a, B * H * Sq, "attn_fwd");
+}
+
+extern "C" int axhip_attn_bwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, const float *V, int64_t ldv, int64_t kv_rows, const float *O,
+                              int64_t ldo, const float *L, const float *dO, int64_t lddo, float *dQ, int64_t lddq, float *dK, int64_t lddk, float *dV,
+                              int64_t lddv, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t dk, float scale,
+                              const axhip_attn_rules *rules) {
+    if (int rc = ensure_ready()) return rc;
+    if (!L) return fail(AXHIP_ERR_NULL_ARG, "attn_bwd: NULL log-sum-exp");
+    AttnArgs a = {};
+    const Tensor tensors[] = {{Q, ldq, H}, {K, ldk, Hkv}, {V, ldv, Hkv}, {O, ldo, H}, {dO, lddo, H}, {dQ, lddq, H}, {dK, lddk, Hkv}, {dV, lddv, Hkv}};
+    if (int rc = attn_arguments("attn_bwd", a, tensors, 8, kv_rows, B, H, Hkv, Sq, Sk, dk, scale, rules)) return rc;
+    if (B == 0) return AXHIP_OK;
+    a.Q = Q;
+    a.K = K;
+    a.V = V;
+    a.Oin = O;
+    a.Lin = L;
+    a.dO = dO;
+    a.dQ = dQ;
+    a.dK = dK;
+    a.dV = dV;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.ldo = ldo;
+    a.lddo = lddo;
+    a.lddq = lddq;
+    a.lddk = lddk;
+    a.lddv = lddv;
+    a.delta = static_cast<float *>(workspace((size_t)B * H * Sq * sizeof(float)));
+    if (!a.delta) return AXHIP_ERR_ALLOC;
+    note_kernel("attn_grad_rows");
+    if (Sq > 0)
+        if (int rc = launch_rows(k_attn_dq_rows, a, B * H * Sq, "attn_bwd queries")) return rc;
+    return launch_rows(k_attn_dkv_rows, a, B * Hkv * Sk, "attn_bwd keys");
+}

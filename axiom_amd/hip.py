@@ -9,8 +9,15 @@ LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libaxhip.so")
 
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_BY_PARTS = 0, 1, 2, 3
+ROPE_INTERLEAVED, ROPE_HALVES = 0, 1
 i64 = C.c_int64
 vp = C.c_void_p
+
+class AttnRules(C.Structure):
+    """axhip_attn_rules: AttnRules(cap=50.0, causal=1, lens=ptr), device pointers as integers."""
+    _fields_ = [("cap", C.c_float), ("causal", C.c_int32), ("slopes", vp), ("prefix", vp), ("start", vp), ("lens", vp), ("doc_q", vp), ("doc_k", vp)]
+
 
 # every symbol include/axhip.h declares: (restype, argtypes)
 SIGNATURES = {
@@ -61,6 +68,13 @@ SIGNATURES = {
     "axhip_layernorm_fwd": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, i64, C.c_float]),
     "axhip_adam_update": (C.c_int, [vp, vp, vp, vp, i64] + [C.c_float] * 7 + [C.c_int]),
     "axhip_sgd_update": (C.c_int, [vp, vp, vp, i64, C.c_float, C.c_float, C.c_float, C.c_int]),
+    "axhip_rope_frequencies": (C.c_int, [vp, i64, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, i64]),
+    "axhip_rope_rows": (C.c_int, [vp, i64, vp, i64, vp, vp, i64, i64, i64, i64, C.c_float, C.c_int, C.c_int]),
+    "axhip_qk_norm_rope_fwd": (C.c_int, [vp, i64, vp, i64, vp, vp, vp, C.c_float, vp, vp, i64, i64, i64, i64, i64, C.c_float, C.c_int]),
+    "axhip_qk_norm_rope_bwd": (C.c_int, [vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, C.c_float, C.c_int]),
+    "axhip_attn_fwd": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, i64, i64, i64, i64, C.c_float, C.POINTER(AttnRules)]),
+    "axhip_attn_bwd": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i64, i64, i64, i64,
+                                 C.c_float, C.POINTER(AttnRules)]),
     "axhip_head_split_qkv": (C.c_int, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64]),
     "axhip_head_interleave": (C.c_int, [vp, vp, i64, i64, i64, i64]),
     "axhip_head_deinterleave": (C.c_int, [vp, vp, i64, i64, i64, i64]),

@@ -338,6 +338,80 @@ int axhip_sdpa_fwd(const float *Q, const float *K, const float *V, float *O, flo
 int axhip_sdpa_fwd_rows(const float *Q, const float *K, const float *V, int64_t ld, float *O, int64_t ldo,
                         float *L, int64_t B, int64_t H, int64_t S, int64_t dk, float scale, int causal);
 
+/* ---- between the projections of a decoder's attention layer ------------------------------------
+ * Rows are tokens; a row holds heads of dk floats side by side, as a fused projection writes them, and row pitches are
+ * in floats.  The reference's GPU backend has only the gradient of plain attention among these (the sdpa_bwd member of its extension
+ * table, include/axiom/internal/cuda_extension.h).  No result depends on the order in which workgroups run. */
+
+/* Frequencies of a rotation, freq[i], i < rot / 2, written to device memory (blocking): f = theta^(-2 i / rot), then by `scaling`
+ *   AXHIP_ROPE_PLAIN     f
+ *   AXHIP_ROPE_LINEAR    f / factor
+ *   AXHIP_ROPE_NTK       as f with theta * factor^(rot / (rot - 2)) for theta: the slowest turns `factor` times slower, the fastest as before
+ *                        (rot = 2: f)
+ *   AXHIP_ROPE_BY_PARTS  by the turns that f makes in `trained` positions, n = trained f / 2 pi: f from n = fast on, f / factor up to
+ *                        n = slow, between them the mean of the two weighted by (n - slow) / (fast - slow)
+ * factor >= 1; 0 <= slow < fast and trained >= 1 for AXHIP_ROPE_BY_PARTS (unused otherwise). */
+enum { AXHIP_ROPE_PLAIN = 0, AXHIP_ROPE_LINEAR = 1, AXHIP_ROPE_NTK = 2, AXHIP_ROPE_BY_PARTS = 3 };
+int axhip_rope_frequencies(float *freq, int64_t rot, double theta, int scaling, double factor, double slow, double fast, int64_t trained);
+
+/* Which values of a head form the pairs (x, y) that are turned to (x cos a - y sin a, y cos a + x sin a): 2 i and 2 i + 1, or
+ * i and i + rot / 2. */
+enum { AXHIP_ROPE_INTERLEAVED = 0, AXHIP_ROPE_HALVES = 1 };
+
+/* Rotary positions: the first rot columns of each of H heads of x [rows, H * dk] turned by a = pos[row] * freq[i] and taken times
+ * `amplitude`, the others as they are, to y (the whole heads; y may be x with the same pitch, and must not overlap it otherwise).  The angle is the exact product of the int32 position and the float
+ * frequency, reduced in 64 bits.  backward != 0: the transpose, y = amplitude * (turned by -a) of x: the gradient.
+ * rot even, 0 <= rot <= dk <= 4096 (rot = 0 copies; pos and freq may then be NULL). */
+int axhip_rope_rows(const float *x, int64_t ldx, float *y, int64_t ldy, const int32_t *pos, const float *freq, int64_t rows, int64_t H,
+                    int64_t dk, int64_t rot, float amplitude, int layout, int backward);
+
+/* Norm of each query and key head and its rotation in one pass.  A row of x holds H query heads and behind them Hk key heads (what
+ * follows them, the values, is not looked at):
+ *   r = 1 / sqrt(mean(x^2) + eps),  y = rotation(gamma * x * r)        gamma_q [dk] for the query heads, gamma_k [dk] for the key heads
+ * (NULL: ones).  inv_rms [rows, H + Hk] receives r, or is NULL.  y may be x with the same pitch when no gradient is wanted.  Rotation and limits as in axhip_rope_rows;
+ * H or Hk may be zero. */
+int axhip_qk_norm_rope_fwd(const float *x, int64_t ldx, float *y, int64_t ldy, float *inv_rms, const float *gamma_q, const float *gamma_k,
+                           float eps, const int32_t *pos, const float *freq, int64_t rows, int64_t H, int64_t Hk, int64_t dk, int64_t rot,
+                           float amplitude, int layout);
+/* Its gradient: from dy, the x of the forward pass and its inv_rms, dx and the sums over rows and heads dgamma_q, dgamma_k (each may be
+ * NULL; all outputs are overwritten, with zero rows or heads the sums are zeros).  dx may be dy with the same pitch. */
+int axhip_qk_norm_rope_bwd(const float *dy, int64_t lddy, const float *x, int64_t ldx, const float *inv_rms, float *dx, int64_t lddx,
+                           const float *gamma_q, const float *gamma_k, float *dgamma_q, float *dgamma_k, const int32_t *pos, const float *freq,
+                           int64_t rows, int64_t H, int64_t Hk, int64_t dk, int64_t rot, float amplitude, int layout);
+
+/* Rules for the scores of axhip_attn_fwd / axhip_attn_bwd.  Zeroes and NULLs, or no rules at all, are plain attention.  With
+ * query i of sequence b at position p = start[b] + i (start NULL: Sk - Sq + i, the queries are the last ones) and key j at j:
+ *   x = scale * (q . k);   cap > 0: x = cap * tanh(x / cap);   slopes: x = x - slopes[h] * |p - j|
+ * and the query sees the key if all of these hold
+ *   j < lens[b]                                        (lens NULL: Sk; taken as 0 below 0 and as Sk above Sk)
+ *   causal: p < lens[b], and j <= p or j < prefix[b]   (prefix NULL: 0; only with causal)
+ *   documents: doc_q[b, i] == doc_k[b, j] >= 0         (both or neither; ids may come in any order, negative ones see and show nothing)
+ * A key that a query does not see has no part in its results, whatever it holds (infinities and NaNs too); a query that sees no key gets
+ * O = 0, L = -infinity and gives no gradient.  Arrays in device memory; start within 2^24 of zero. */
+typedef struct {
+    float cap;
+    int32_t causal;
+    const float *slopes;        /* [H] */
+    const int32_t *prefix;      /* [B] */
+    const int32_t *start;       /* [B] */
+    const int32_t *lens;        /* [B] */
+    const int32_t *doc_q;       /* [B, Sq] */
+    const int32_t *doc_k;       /* [B, Sk] */
+} axhip_attn_rules;
+
+/* Attention under these rules, O = softmax(x) V, for H query heads that share Hkv heads of keys and values (H a multiple of Hkv: query head
+ * h reads head h / (H / Hkv)).  Query i of sequence b is row b * Sq + i of Q and O, its key j row b * kv_rows + j of K and V (kv_rows >= Sk:
+ * rows that a cache holds for each sequence).  L [B, H, Sq] is the log-sum-exp of each row of scores, or NULL.  For prompts, training and, with Sq = 1 or a
+ * few, single tokens over a cache.  dk a multiple of 4 up to 128 (AXHIP_ERR_NOT_IMPLEMENTED otherwise), pitches multiples of 4 floats up to
+ * 2^22, Q, K, V, O 16-byte aligned, Sq and Sk up to 2^24.  `rules` is read before the call returns; what it points to when the kernels run. */
+int axhip_attn_fwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, const float *V, int64_t ldv, int64_t kv_rows, float *O, int64_t ldo,
+                   float *L, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t dk, float scale, const axhip_attn_rules *rules);
+/* Its gradient from dO, with the O and L that the forward pass gave for the same arguments: dQ (rows and columns as Q), dK and dV (as K and
+ * V; rows Sk .. kv_rows - 1 of a sequence are left as they are), all overwritten, the gradients of shared heads summed. */
+int axhip_attn_bwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, const float *V, int64_t ldv, int64_t kv_rows, const float *O, int64_t ldo,
+                   const float *L, const float *dO, int64_t lddo, float *dQ, int64_t lddq, float *dK, int64_t lddk, float *dV, int64_t lddv,
+                   int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t dk, float scale, const axhip_attn_rules *rules);
+
 /* ---- layout transforms around attention (the layout members of the reference's GPU extension
  * table, include/axiom/internal/cuda_extension.h:45-84) ------------------------------------- */
 /* qkv [B*S, 3D] (row = [q | k | v], D = H*dk) -> q, k, v each [B*H, S, dk]; bqkv [3D] is added
