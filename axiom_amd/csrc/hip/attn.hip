@@ -1,18 +1,12 @@
 // Attention under score rules (capped, biased by distance, masked by documents, prefixes or lengths; shared heads of keys), forward and backward.
 #include <math.h>
 
-#include "attn_rules.h"
+#include "attn_launch.h"
 
 namespace {
 using namespace axhip;
 
 // One wave a row of queries, or a row of keys
-__global__ void __launch_bounds__(256) k_attn_rows(AttnArgs a, int64_t first) {
-    const int64_t n = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= (int64_t)a.B * a.H * a.Sq) return;
-    const int i = (int)(n % a.Sq), head = (int)(n / a.Sq % a.H), b = (int)(n / a.Sq / a.H);
-    attn_fwd_row(a, b, head, i, threadIdx.x & 63);
-}
 __global__ void __launch_bounds__(256) k_attn_dq_rows(AttnArgs a, int64_t first) {
     const int64_t n = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (n >= (int64_t)a.B * a.H * a.Sq) return;
@@ -104,8 +98,7 @@ extern "C" int axhip_attn_fwd(const float *Q, int64_t ldq, const float *K, int64
     a.ldk = ldk;
     a.ldv = ldv;
     a.ldo = ldo;
-    note_kernel("attn_rows");
-    return launch_rows(k_attn_rows, a, B * H * Sq, "attn_fwd");
+    return attn_fwd_tiles(a);
 }
 
 extern "C" int axhip_attn_bwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, const float *V, int64_t ldv, int64_t kv_rows, const float *O,

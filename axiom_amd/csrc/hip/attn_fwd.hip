@@ -1,0 +1,421 @@
+// Attention forward under score rules: tiles of queries on the f16 matrix core.
+//
+// A workgroup of four or eight waves owns 128 or 256 rows of queries, a wave 32 of them; the rows are those of one query head, or, where a head has
+// few, of all heads that share keys, one after the other.  Keys and values stream through LDS in blocks of 64, cut into f16 terms on the way (f16x2.h; a
+// query's row once, a probability when it is used).  As in plain attention (sdpa.hip) a lane owns query (l & 31) in the score tile and in the output:
+//   S^T tile   A = keys' rows, B = the wave's queries; register v of a lane is key 8 (v >> 2) + 4 (l >> 5) + (v & 3)
+//   softmax    online, in log2 units; the reference point moves only when a maximum exceeds it by 2^8
+//   O^T tile   A = V^T, read from the rows by transposing LDS reads, B = the probabilities where the score tile left them
+// What a query sees is the keys before `end` that have its document (AttnRow).  Blocks that no row of the workgroup sees are not fetched, 32-key tiles that no row of a
+// wave sees not computed, and only tiles that some row sees in part pay for the mask; with documents the ranges of ids of each 32 keys, formed by a first
+// launch, decide that.  A row whose sums are not finite (infinities or NaNs that it sees, or that a masked key of a tile holds) is formed again with fp32
+// instructions by its wave.
+#include "attn_launch.h"
+#include "attn_tiles.h"
+
+namespace {
+using namespace axhip;
+
+template <int DK, int WAVES>
+struct FwdGeom {
+    static constexpr int BQ = 32 * WAVES, BKV = 64;
+    using B = Block<DK, BKV>;
+    static constexpr bool DOUBLE = WAVES == 8;   // two blocks in LDS, or two workgroups a CU
+    static constexpr int FACTORS_AT = 2 * B::BYTES;              // of each eight keys: 2^-e of K (float), e of V (int)
+    static constexpr int DOCS_AT = FACTORS_AT + BKV / 8 * 8;     // documents of the keys, then the ranges of their two tiles
+    static constexpr int STAGE = DOCS_AT + BKV * 4 + 2 * 8;
+    static constexpr int META_AT = (DOUBLE ? 2 : 1) * STAGE;     // a row of four ints a wave
+    static constexpr int SMEM = META_AT + 16 * WAVES;
+    static_assert(STAGE % 16 == 0 && SMEM * (DOUBLE ? 1 : 2) <= 160 * 1024, "eight waves a CU");
+};
+
+constexpr int P_UP = 6;                          // probabilities are at most 2^8 times the reference point's
+
+template <int DK, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid grid) {
+    using G = FwdGeom<DK, WAVES>;
+    using B = typename G::B;
+    constexpr int KS = DK / 16, DT = DK / 32, BKV = G::BKV;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
+
+    // Eight units (heads, or groups of heads) go to the eight XCDs in turn; a unit's tiles to one, causal ones from the last, the longest, on.
+    const int64_t lin = grid.first + blockIdx.x, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
+    const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8, unit = group * 8 + r8 % width;
+    const int tile = a.causal ? grid.tiles - 1 - (int)(r8 / width) : (int)(r8 / width);
+    const int per_b = a.H / grid.pack, b = (int)(unit / per_b), h0 = (int)(unit - (int64_t)b * per_b) * grid.pack, hk = h0 / a.G;
+    const int rows = grid.pack * a.Sq, r = tile * G::BQ + wave * 32 + frow;
+    const bool valid = r < rows;
+    const int over = grid.pack == 1 ? 0 : (valid ? r : rows - 1) / a.Sq, head = h0 + over, i = (valid ? r : rows - 1) - over * a.Sq;
+    AttnRow row = attn_row(a, b, head, i);
+    if (!valid) row.end = 0;
+    const bool live = row.end > 0;
+
+    // what the wave sees, and what the workgroup does: the last end, the first end of rows that see anything, the range of documents
+    int last = row.end, sure = live ? row.end : 0x7fffffff, d_low = live ? row.doc : 0x7fffffff, d_high = live ? row.doc : -1;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        last = max(last, __shfl_xor(last, off, 64));
+        sure = min(sure, __shfl_xor(sure, off, 64));
+        d_low = min(d_low, __shfl_xor(d_low, off, 64));
+        d_high = max(d_high, __shfl_xor(d_high, off, 64));
+    }
+    last = __builtin_amdgcn_readfirstlane(last);
+    sure = __builtin_amdgcn_readfirstlane(sure);
+    d_low = __builtin_amdgcn_readfirstlane(d_low);
+    d_high = __builtin_amdgcn_readfirstlane(d_high);
+    int *meta = reinterpret_cast<int *>(lds + G::META_AT);
+    if (lane == 0) *reinterpret_cast<v4i *>(meta + 4 * wave) = v4i{last, 0, d_low, d_high};
+    __syncthreads();
+    int wg_last = 0, wg_low = 0x7fffffff, wg_high = -1;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        const v4i m = *reinterpret_cast<const v4i *>(meta + 4 * w);
+        wg_last = max(wg_last, m[0]);
+        wg_low = min(wg_low, m[2]);
+        wg_high = max(wg_high, m[3]);
+    }
+    wg_last = __builtin_amdgcn_readfirstlane(wg_last);
+    wg_low = __builtin_amdgcn_readfirstlane(wg_low);
+    wg_high = __builtin_amdgcn_readfirstlane(wg_high);
+    const int nblocks = (wg_last + BKV - 1) / BKV;
+    const bool docs = a.doc_q != nullptr;
+
+    // the next block from `blk` on that some row may see: 64 at a time, a lane each
+    const DocRange *ranges = grid.ranges + (int64_t)b * grid.range_tiles;
+    uint64_t window = 0;
+    int window_at = -64;
+    auto next = [&](int blk) -> int {
+        if (!docs) return blk;
+        while (blk < nblocks) {
+            if (blk - window_at >= 64) {
+                window_at = blk & ~63;
+                const int mine = window_at + lane;
+                bool meets = false;
+                if (mine < nblocks) {
+                    meets = ranges[2 * mine].meets(wg_low, wg_high);
+                    if (2 * mine + 1 < grid.range_tiles) meets |= ranges[2 * mine + 1].meets(wg_low, wg_high);
+                }
+                window = __builtin_amdgcn_ballot_w64(meets);
+            }
+            const uint64_t ahead = window >> (blk - window_at);
+            if (ahead) return blk + __builtin_ctzll(ahead);
+            blk = window_at + 64;
+        }
+        return nblocks;
+    };
+
+    const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;
+    Stage<DK, BKV, WAVES> ks, vs;
+    int doc_here = -1;
+    DocRange range_here = {0, 0};
+    auto load = [&](int blk) {
+        const int64_t k0 = (int64_t)blk * BKV;
+        const int end = wg_last - 1 - (int)k0;       // rows past it are read as it
+        ks.load(Kb + k0 * a.ldk, a.ldk, end, wave, lane, a.dk);
+        vs.load(Vb + k0 * a.ldv, a.ldv, end, wave, lane, a.dk);
+        if (docs && threadIdx.x < BKV) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
+        if (docs && threadIdx.x < 2) range_here = 2 * blk + (int)threadIdx.x < grid.range_tiles ? ranges[2 * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
+    };
+    auto stage = [&](unsigned char *at) {
+        const int ke = ks.put(at, wave, lane, 1.0f), ve = vs.put(at + B::BYTES, wave, lane, 1.0f);
+        constexpr int SLOTS = Stage<DK, BKV, WAVES>::RPW / 8;
+        if (lane < SLOTS) {
+            reinterpret_cast<float *>(at + G::FACTORS_AT)[wave * SLOTS + lane] = two_to(-ke);
+            reinterpret_cast<int *>(at + G::FACTORS_AT + BKV / 2)[wave * SLOTS + lane] = ve;
+        }
+        if (docs && threadIdx.x < BKV) reinterpret_cast<int *>(at + G::DOCS_AT)[threadIdx.x] = doc_here;
+        if (docs && threadIdx.x < 2) reinterpret_cast<DocRange *>(at + G::DOCS_AT + BKV * 4)[threadIdx.x] = range_here;
+    };
+
+    int blk = next(0), ahead = nblocks;
+    if (blk < nblocks) load(blk);
+    v4i qf[KS][2];                                   // step s: columns 16 s + 8 * half .. + 7 of this lane's query
+    float q_down;
+    {
+        const float *q = a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk;
+        float x[KS][8], most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int col = 16 * s + 8 * fhalf + 4 * h;
+                v4f v = {0.f, 0.f, 0.f, 0.f};
+                if (live && (a.dk == DK || col < a.dk)) v = *reinterpret_cast<const v4f *>(q + col);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[s][4 * h + e] = v[e] * a.q_up;
+                    most = fmaxf(most, __builtin_fabsf(x[s][4 * h + e]));
+                }
+            }
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const int up = up_of(most);
+        q_down = two_to(-up);
+#pragma unroll
+        for (int s = 0; s < KS; s++) cut_halves(x[s], two_to(up), qf[s]);
+    }
+    if (blk < nblocks) {
+        stage(lds);
+        ahead = next(blk + 1);
+        if (G::DOUBLE && ahead < nblocks) load(ahead);
+    }
+    __syncthreads();
+
+    v16f acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
+    float m_run = ATTN_LOWEST, l_run = 0.0f;         // l_run: this lane half's share of the row sum
+    int v_up = MOST_UP;                              // acc is 2^(P_UP + v_up) times the sum; v_up the least of the values' exponents so far
+
+    auto attend = [&](int blk, const unsigned char *at) {
+#pragma unroll 1
+        for (int kt = 0; kt < BKV / 32; kt++) {
+            const int kt0 = blk * BKV + 32 * kt;
+            if (kt0 >= last) break;
+            bool partly = kt0 + 32 > sure;
+            if (docs) {
+                const v2i32 range = *reinterpret_cast<const v2i32 *>(at + G::DOCS_AT + BKV * 4 + 8 * kt);
+                const DocRange here = {__builtin_amdgcn_readfirstlane(range[0]), __builtin_amdgcn_readfirstlane(range[1])};
+                if (!here.meets(d_low, d_high)) continue;
+                partly |= here.low != here.high || here.low != d_low || d_low != d_high;
+            }
+            // ---- scores ----
+            v16f s;
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[v] = 0.0f;
+            __builtin_amdgcn_s_setprio(1);           // matrix phases go ahead of the co-resident wave's vector work
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const v4i kf[2] = {B::rows(at, 32 * kt, k, lane, 0), B::rows(at, 32 * kt, k, lane, 1)};
+                s = mfma_cut(kf, qf[k], s);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            const v4f down = *reinterpret_cast<const v4f *>(at + G::FACTORS_AT + 16 * kt);
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float f = down[g] * q_down;
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[4 * g + e] *= f;
+            }
+            if (a.cap2 > 0.0f) {
+                float big = 0.0f;
+#pragma unroll
+                for (int v = 0; v < 16; v++) big = fmaxf(big, __builtin_fabsf(s[v]));
+                if (__builtin_amdgcn_ballot_w64(!(big < TANH_NEAR)))
+#pragma unroll
+                    for (int v = 0; v < 16; v++) s[v] = a.cap2 * tanh_of(s[v]).value;
+                else
+#pragma unroll
+                    for (int v = 0; v < 16; v++) s[v] = a.cap2 * tanh_near(s[v]);
+            }
+            if (a.slopes) {
+                const float from = (float)(row.p - kt0 - 4 * fhalf);
+#pragma unroll
+                for (int v = 0; v < 16; v++) s[v] = __builtin_fmaf(-row.slope2, __builtin_fabsf(from - (float)(8 * (v >> 2) + (v & 3))), s[v]);
+            }
+            if (partly) {
+                const int end = row.end - kt0 - 4 * fhalf;
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    if (8 * (v >> 2) + (v & 3) >= end) s[v] = -INFINITY;
+                if (docs) {
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const v4i d = *reinterpret_cast<const v4i *>(at + G::DOCS_AT + 4 * (32 * kt + 8 * g + 4 * fhalf));
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (d[e] != row.doc) s[4 * g + e] = -INFINITY;
+                    }
+                }
+            }
+            // ---- online softmax ----
+            float m_blk = s[0];
+#pragma unroll
+            for (int v = 1; v < 16; v++) m_blk = fmaxf(m_blk, s[v]);
+            m_blk = fmaxf(m_blk, __shfl_xor(m_blk, 32, 64));
+            if (__builtin_amdgcn_ballot_w64(m_blk > m_run + 8.0f)) {
+                const float m_new = fmaxf(m_run, m_blk), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+                l_run *= alpha;
+                m_run = m_new;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) acc[d][v] *= alpha;
+            }
+            float l_blk = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                s[v] = __builtin_amdgcn_exp2f(s[v] - m_run);
+                l_blk += s[v];
+            }
+            l_run += l_blk;
+            // ---- O^T += V^T P^T ----
+            int ve[4];
+            const v4i ve4 = *reinterpret_cast<const v4i *>(at + G::FACTORS_AT + BKV / 2 + 16 * kt);
+#pragma unroll
+            for (int g = 0; g < 4; g++) ve[g] = __builtin_amdgcn_readfirstlane(ve4[g]);
+            const int least = min(min(ve[0], ve[1]), min(ve[2], ve[3]));
+            if (least < v_up) {
+                const float by = two_to(least - v_up);
+                v_up = least;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) acc[d][v] *= by;
+            }
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                v4i pf[2];
+                v2i32 pa[2], pb[2];
+                const float x[4] = {s[8 * st], s[8 * st + 1], s[8 * st + 2], s[8 * st + 3]}, y[4] = {s[8 * st + 4], s[8 * st + 5], s[8 * st + 6], s[8 * st + 7]};
+                cut_halves(x, two_to(P_UP + v_up - ve[2 * st]), pa);
+                cut_halves(y, two_to(P_UP + v_up - ve[2 * st + 1]), pb);
+#pragma unroll
+                for (int t = 0; t < 2; t++) pf[t] = v4i{pa[t][0], pa[t][1], pb[t][0], pb[t][1]};
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const v4i vf[2] = {B::columns(at + B::BYTES, 32 * kt + 16 * st, d, lane, 0), B::columns(at + B::BYTES, 32 * kt + 16 * st, d, lane, 1)};
+                    acc[d] = mfma_cut(vf, pf, acc[d]);
+                }
+            }
+        }
+    };
+    if constexpr (G::DOUBLE) {
+        // Two blocks in LDS and the next in registers.  The two waves of a SIMD (w, w + 4) put it beside the current block before and after that is
+        // multiplied, so that one cuts while the other's products run.
+        unsigned cur = 0;
+        while (blk < nblocks) {
+            const bool more = ahead < nblocks;
+            int after = nblocks;
+            auto bring = [&]() {
+                stage(lds + (cur ^ G::STAGE));
+                after = next(ahead + 1);
+                if (after < nblocks) load(after);
+            };
+            if (more && wave >= 4) bring();
+            attend(blk, lds + cur);
+            if (more && wave < 4) bring();
+            __syncthreads();
+            blk = ahead;
+            ahead = after;
+            cur ^= G::STAGE;
+        }
+    } else {
+        while (blk < nblocks) {
+            const bool more = ahead < nblocks;
+            if (more) load(ahead);
+            attend(blk, lds);
+            __syncthreads();                         // the block has been read
+            if (more) {
+                stage(lds);
+                __syncthreads();
+            }
+            blk = ahead;
+            ahead = more ? next(ahead + 1) : nblocks;
+        }
+    }
+
+    // ---- normalise and write: a lane owns its query's columns 32 d + 8 g + 4 * half .. + 3 ----
+    float seen = l_run * 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) seen = __builtin_fmaf(acc[d][v], 0.0f, seen);
+    const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+    const bool unfit = live && (!(seen == 0.0f) || l_tot == 0.0f);
+    uint64_t again = __builtin_amdgcn_ballot_w64(unfit);
+    again |= again >> 32;
+    const bool fit = !((again >> frow) & 1);
+    const float inv = live ? 1.0f / l_tot * two_to(-P_UP - v_up) : 0.0f;
+    if (valid && fit) {
+        float *o = a.O + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int col = 32 * d + 8 * g + 4 * fhalf;
+                v4f out;
+#pragma unroll
+                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * inv : 0.0f;
+                if (a.dk == DK || col < a.dk) *reinterpret_cast<v4f *>(o + col) = out;
+            }
+        if (a.L && fhalf == 0) a.L[((int64_t)b * a.H + head) * a.Sq + i] = live ? (m_run + __builtin_amdgcn_logf(l_tot)) * LN2 : -INFINITY;
+    }
+    for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) {
+        const int n = __builtin_ctz(rest);
+        attn_fwd_row(a, b, __builtin_amdgcn_readlane(head, n), __builtin_amdgcn_readlane(i, n), lane);
+    }
+}
+
+// The ranges of documents of each 32 ids, a wave each
+__global__ void __launch_bounds__(256) k_doc_ranges(const int32_t *ids, int64_t sequences, int S, int tiles, DocRange *out) {
+    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (n >= sequences * tiles) return;
+    const int64_t b = n / tiles;
+    const int at = (int)(n - b * tiles) * 32 + (threadIdx.x & 31);
+    const int id = at < S ? ids[b * S + at] : -1;
+    int low = id < 0 ? 0x7fffffff : id, high = id;
+    bool none = id < 0 && at < S;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        low = min(low, __shfl_xor(low, off, 32));
+        high = max(high, __shfl_xor(high, off, 32));
+        none |= __shfl_xor((int)none, off, 32) != 0;
+    }
+    if ((threadIdx.x & 31) == 0) out[n] = high < 0 ? DocRange{0x7fffffff, -1} : DocRange{none ? ~low : low, high};
+}
+
+template <int DK, int WAVES>
+int launch_fwd(const AttnArgs &a, FwdGrid grid) {
+    using G = FwdGeom<DK, WAVES>;
+    static bool attr_set = false;
+    if (!attr_set) {
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_fwd<DK, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
+        attr_set = true;
+    }
+    grid.tiles = (int)(((int64_t)grid.pack * a.Sq + G::BQ - 1) / G::BQ);
+    const int64_t all = grid.units * grid.tiles;
+    note_kernel(WAVES == 8 ? "attn_tiles_w8" : "attn_tiles");
+    for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
+        const int64_t left = all - grid.first;
+        hipLaunchKernelGGL((k_attn_fwd<DK, WAVES>), dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
+        if (int rc = check_launch("attn_fwd")) return rc;
+    }
+    return AXHIP_OK;
+}
+
+}  // namespace
+
+namespace axhip {
+
+int doc_ranges(const int32_t *ids, int64_t B, int64_t S, void *out) {
+    const int64_t tiles = (S + 31) / 32, n = B * tiles;
+    if (n == 0) return AXHIP_OK;
+    if ((n + 7) / 8 > GRID_MOST) return fail(AXHIP_ERR_SHAPE, "attention: too many documents");
+    hipLaunchKernelGGL(k_doc_ranges, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, kStream, ids, B, (int)S, (int)tiles, static_cast<DocRange *>(out));
+    return check_launch("document ranges");
+}
+
+int attn_fwd_tiles(const AttnArgs &a) {
+    FwdGrid grid = {};
+    // rows of all heads that share keys in one tile, where a head's own would leave most of it empty
+    grid.pack = a.G > 1 && a.Sq <= 64 ? a.G : 1;
+    grid.units = (int64_t)a.B * (a.H / grid.pack);
+    if (a.doc_k) {
+        grid.range_tiles = (int)(((int64_t)a.Sk + 31) / 32);
+        void *ranges = workspace((size_t)a.B * grid.range_tiles * sizeof(DocRange));
+        if (!ranges) return AXHIP_ERR_ALLOC;
+        if (int rc = doc_ranges(a.doc_k, a.B, a.Sk, ranges)) return rc;
+        grid.ranges = static_cast<DocRange *>(ranges);
+    }
+    const int64_t rows = (int64_t)grid.pack * a.Sq, wide = (rows + 255) / 256 * grid.units;
+    const bool eight = wide >= cu_count();
+    if (a.dk <= 32) return launch_fwd<32, 4>(a, grid);
+    if (a.dk <= 64) return eight ? launch_fwd<64, 8>(a, grid) : launch_fwd<64, 4>(a, grid);
+    if (a.dk <= 96) return eight ? launch_fwd<96, 8>(a, grid) : launch_fwd<96, 4>(a, grid);
+    return eight ? launch_fwd<128, 8>(a, grid) : launch_fwd<128, 4>(a, grid);
+}
+
+}  // namespace axhip
