@@ -6,32 +6,6 @@
 namespace {
 using namespace axhip;
 
-// One wave a row of queries, or a row of keys
-__global__ void __launch_bounds__(256) k_attn_dq_rows(AttnArgs a, int64_t first) {
-    const int64_t n = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= (int64_t)a.B * a.H * a.Sq) return;
-    const int i = (int)(n % a.Sq), head = (int)(n / a.Sq % a.H), b = (int)(n / a.Sq / a.H);
-    attn_dq_row(a, b, head, i, threadIdx.x & 63);
-}
-__global__ void __launch_bounds__(256) k_attn_dkv_rows(AttnArgs a, int64_t first) {
-    const int64_t n = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= (int64_t)a.B * a.Hkv * a.Sk) return;
-    const int j = (int)(n % a.Sk), hk = (int)(n / a.Sk % a.Hkv), b = (int)(n / a.Sk / a.Hkv);
-    attn_dkv_row(a, b, hk, j, threadIdx.x & 63);
-}
-
-// Workgroups of four waves for n waves, in launches that a grid holds
-template <typename Kernel>
-int launch_rows(Kernel kernel, const AttnArgs &a, int64_t n, const char *what) {
-    constexpr int64_t MOST = int64_t(1) << 23;   // workgroups: a grid holds fewer than 2^32 threads
-    for (int64_t first = 0; first < n; first += MOST * 4) {
-        const int64_t left = (n - first + 3) / 4;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(left < MOST ? left : MOST)), dim3(256), 0, kStream, a, first);
-        if (int rc = check_launch(what)) return rc;
-    }
-    return AXHIP_OK;
-}
-
 struct Tensor {
     const void *at;
     int64_t ld, heads;
@@ -128,10 +102,5 @@ extern "C" int axhip_attn_bwd(const float *Q, int64_t ldq, const float *K, int64
     a.lddq = lddq;
     a.lddk = lddk;
     a.lddv = lddv;
-    a.delta = static_cast<float *>(workspace((size_t)B * H * Sq * sizeof(float)));
-    if (!a.delta) return AXHIP_ERR_ALLOC;
-    note_kernel("attn_grad_rows");
-    if (Sq > 0)
-        if (int rc = launch_rows(k_attn_dq_rows, a, B * H * Sq, "attn_bwd queries")) return rc;
-    return launch_rows(k_attn_dkv_rows, a, B * Hkv * Sk, "attn_bwd keys");
+    return Sk == 0 && Sq == 0 ? AXHIP_OK : attn_bwd_tiles(a);
 }

@@ -1,0 +1,718 @@
+// Attention backward under score rules: tiles on the f16 matrix core, no atomics.
+//   P = 2^(x - lse), dP = dO V^T, ds = P (dP - delta) slope, delta = sum dO O
+//   dQ = scale ds K (k_attn_dq, a tile of queries over the keys that it sees), dK = scale ds^T Q and dV = P^T dO (k_attn_dkv, a tile of keys over the rows that see
+//   it, of all query heads that share it).  Scores and dP are formed by both: seven products a pair where five would do, for sums in a fixed order.
+// Operands are cut into f16 terms as in the forward pass (f16x2.h).  ds and P have no scale of their own: a running exponent for each row (or key) keeps the largest so
+// far at 2^10 to 2^15, and the sum is rescaled when it moves, as an online softmax does.  In k_attn_dkv the key is on the lane side: a lane owns key (l & 31), its
+// registers are 16 rows, and what these need (lse, delta, end, document) lies in LDS beside the block.  Rows (keys) whose sums are not finite are formed again
+// with fp32 instructions.
+#include "attn_launch.h"
+#include "attn_tiles.h"
+
+namespace {
+using namespace axhip;
+
+template <int DT>
+__device__ __forceinline__ void times(v16f (&acc)[DT], float by) {
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) acc[d][v] *= by;
+}
+
+template <int KS>
+__device__ __forceinline__ void load_row(float (&x)[KS][8], const float *row, bool live, int fhalf, int dk) {
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int col = 16 * s + 8 * fhalf + 4 * h;
+            v4f v = {0.f, 0.f, 0.f, 0.f};
+            if (live && (dk == 16 * KS || col < dk)) v = *reinterpret_cast<const v4f *>(row + col);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[s][4 * h + e] = v[e];
+        }
+}
+
+// Scores of a tile (products already scaled) after cap and distance; `slope` the cap's derivative.  from[v]: position less key of register v.
+template <typename Distance>
+__device__ __forceinline__ void score_tile(const AttnArgs &a, v16f &s, v16f &slope, Distance distance) {
+    if (a.cap2 > 0.0f) {
+        float big = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 16; v++) big = fmaxf(big, __builtin_fabsf(s[v]));
+        if (__builtin_amdgcn_ballot_w64(!(big < TANH_NEAR)))
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const Tanh t = tanh_of(s[v]);
+                s[v] = a.cap2 * t.value;
+                slope[v] = t.slope;
+            }
+        else
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const float t = tanh_near(s[v]);
+                s[v] = a.cap2 * t;
+                slope[v] = __builtin_fmaf(-t, t, 1.0f);
+            }
+    }
+    if (a.slopes)
+#pragma unroll
+        for (int v = 0; v < 16; v++) s[v] -= distance(v);
+}
+
+// The next 64-row block from `blk` on, below n, of which some tile's documents meet [low, high]: 64 blocks at a time, a lane each
+struct Blocks {
+    const DocRange *ranges;                      // NULL: every block
+    int n, tiles, low, high, at;
+    uint64_t window;
+    __device__ Blocks(const DocRange *r, int blocks, int range_tiles, int from, int to) : ranges(r), n(blocks), tiles(range_tiles), low(from), high(to), at(-64), window(0) {}
+    __device__ __forceinline__ int next(int blk, int lane) {
+        if (!ranges) return blk < n ? blk : n;
+        while (blk < n) {
+            if (blk < at || blk - at >= 64) {
+                at = blk & ~63;
+                const int mine = at + lane;
+                bool meets = false;
+                if (mine < n) {
+                    meets = ranges[2 * mine].meets(low, high);
+                    if (2 * mine + 1 < tiles) meets |= ranges[2 * mine + 1].meets(low, high);
+                }
+                window = __builtin_amdgcn_ballot_w64(meets);
+            }
+            const uint64_t ahead = window >> (blk - at);
+            if (ahead) {
+                const int found = blk + __builtin_ctzll(ahead);
+                return found < n ? found : n;
+            }
+            blk = at + 64;
+        }
+        return n;
+    }
+};
+
+constexpr int WAVES = 4, ROWS = 64;              // rows of a block
+
+template <int DK>
+struct DqGeom {
+    using B = Block<DK, ROWS>;
+    static constexpr int FACTORS_AT = 2 * B::BYTES;              // of each key row, then of each value row
+    static constexpr int DOCS_AT = FACTORS_AT + ROWS * 8;
+    static constexpr int META_AT = DOCS_AT + ROWS * 4 + 2 * 8;
+    static constexpr int SMEM = META_AT + 16 * WAVES;
+    static constexpr int PER_SIMD = DK <= 64 ? 2 : 1;
+};
+
+template <int DK>
+__global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(AttnArgs a, BwdGrid grid) {
+    using G = DqGeom<DK>;
+    using B = typename G::B;
+    constexpr int KS = DK / 16, DT = DK / 32;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
+    const int64_t lin = grid.first + blockIdx.x, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
+    const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8, unit = group * 8 + r8 % width;
+    const int tile = a.causal ? grid.tiles - 1 - (int)(r8 / width) : (int)(r8 / width);
+    const int b = (int)(unit / a.H), head = (int)(unit - (int64_t)b * a.H), hk = head / a.G;
+    const int r = tile * 32 * WAVES + wave * 32 + frow, i = r < a.Sq ? r : a.Sq - 1;
+    const bool valid = r < a.Sq;
+    AttnRow row = attn_row(a, b, head, i);
+    if (!valid) row.end = 0;
+    const bool live = row.end > 0, docs = a.doc_q != nullptr;
+    int last = row.end, sure = live ? row.end : 0x7fffffff, d_low = live ? row.doc : 0x7fffffff, d_high = live ? row.doc : -1;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        last = max(last, __shfl_xor(last, off, 64));
+        sure = min(sure, __shfl_xor(sure, off, 64));
+        d_low = min(d_low, __shfl_xor(d_low, off, 64));
+        d_high = max(d_high, __shfl_xor(d_high, off, 64));
+    }
+    last = __builtin_amdgcn_readfirstlane(last);
+    sure = __builtin_amdgcn_readfirstlane(sure);
+    d_low = __builtin_amdgcn_readfirstlane(d_low);
+    d_high = __builtin_amdgcn_readfirstlane(d_high);
+    int *meta = reinterpret_cast<int *>(lds + G::META_AT);
+    if (lane == 0) *reinterpret_cast<v4i *>(meta + 4 * wave) = v4i{last, 0, d_low, d_high};
+    __syncthreads();
+    int wg_last = 0, wg_low = 0x7fffffff, wg_high = -1;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        const v4i m = *reinterpret_cast<const v4i *>(meta + 4 * w);
+        wg_last = max(wg_last, m[0]);
+        wg_low = min(wg_low, m[2]);
+        wg_high = max(wg_high, m[3]);
+    }
+    wg_last = __builtin_amdgcn_readfirstlane(wg_last);
+    wg_low = __builtin_amdgcn_readfirstlane(wg_low);
+    wg_high = __builtin_amdgcn_readfirstlane(wg_high);
+    const DocRange *ranges = docs ? grid.key_ranges + (int64_t)b * grid.key_tiles : nullptr;
+    Blocks blocks(ranges, (wg_last + ROWS - 1) / ROWS, grid.key_tiles, wg_low, wg_high);
+
+    const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;
+    Stage<DK, ROWS, WAVES> ks, vs;
+    int doc_here = -1;
+    DocRange range_here = {0, 0};
+    auto load = [&](int blk) {
+        const int64_t k0 = (int64_t)blk * ROWS;
+        const int end = wg_last - 1 - (int)k0;
+        ks.load(Kb + k0 * a.ldk, a.ldk, end, wave, lane, a.dk);
+        vs.load(Vb + k0 * a.ldv, a.ldv, end, wave, lane, a.dk);
+        if (docs && threadIdx.x < ROWS) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
+        if (docs && threadIdx.x < 2) range_here = 2 * blk + (int)threadIdx.x < grid.key_tiles ? ranges[2 * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
+    };
+    auto stage = [&]() {
+        float *factors = reinterpret_cast<float *>(lds + G::FACTORS_AT);
+        ks.put(lds, factors, wave, lane, 1.0f);
+        vs.put(lds + B::BYTES, factors + ROWS, wave, lane, 1.0f);
+        if (docs && threadIdx.x < ROWS) reinterpret_cast<int *>(lds + G::DOCS_AT)[threadIdx.x] = doc_here;
+        if (docs && threadIdx.x < 2) reinterpret_cast<DocRange *>(lds + G::DOCS_AT + ROWS * 4)[threadIdx.x] = range_here;
+    };
+
+    int blk = blocks.next(0, lane);
+    if (blk < blocks.n) load(blk);
+    // ---- the row: query, gradient, delta ----
+    const int64_t at = ((int64_t)b * a.H + head) * a.Sq + i;
+    v4i qf[KS][2], of[KS][2];
+    float q_down, o_down, delta = 0.0f;
+    {
+        float x[KS][8], y[KS][8];
+        load_row(x, a.Oin + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk, live, fhalf, a.dk);
+        load_row(y, a.dO + ((int64_t)b * a.Sq + i) * a.lddo + (int64_t)head * a.dk, live, fhalf, a.dk);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) delta = __builtin_fmaf(x[s][e], y[s][e], delta);
+        delta += __shfl_xor(delta, 32, 64);
+        o_down = cut_row(y, of);
+        load_row(x, a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk, live, fhalf, a.dk);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[s][e] *= a.q_up;
+        q_down = cut_row(x, qf);
+    }
+    if (valid && fhalf == 0) a.delta[at] = delta;
+    float lse2 = live ? a.Lin[at] * LOG2E : INFINITY;
+    if (lse2 == -INFINITY) lse2 = INFINITY;          // a row that saw nothing: no probability
+    if (blk < blocks.n) stage();
+    __syncthreads();
+
+    v16f acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
+    int d_up = MOST_UP;                              // acc is 2^(BIAS + d_up) times the sum: the running exponent of ds times its key row's factor
+
+    auto attend = [&](int blk) {
+#pragma unroll 1
+        for (int kt = 0; kt < 2; kt++) {
+            const int kt0 = blk * ROWS + 32 * kt;
+            if (kt0 >= last) break;
+            bool partly = kt0 + 32 > sure;
+            if (docs) {
+                const v2i32 range = *reinterpret_cast<const v2i32 *>(lds + G::DOCS_AT + ROWS * 4 + 8 * kt);
+                const DocRange here = {__builtin_amdgcn_readfirstlane(range[0]), __builtin_amdgcn_readfirstlane(range[1])};
+                if (!here.meets(d_low, d_high)) continue;
+                partly |= here.low != here.high || here.low != d_low || d_low != d_high;
+            }
+            v16f s, dp, slope;
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[v] = dp[v] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const v4i kf[2] = {B::rows(lds, 32 * kt, k, lane, 0), B::rows(lds, 32 * kt, k, lane, 1)};
+                s = mfma_cut(kf, qf[k], s);
+            }
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const v4i vf[2] = {B::rows(lds + B::BYTES, 32 * kt, k, lane, 0), B::rows(lds + B::BYTES, 32 * kt, k, lane, 1)};
+                dp = mfma_cut(vf, of[k], dp);
+            }
+            auto factors = [&](int what, int g) {    // of keys 8 g + 4 * half + 0..3 of the tile
+                return *reinterpret_cast<const v4f *>(lds + G::FACTORS_AT + what * ROWS * 4 + 4 * (32 * kt + 8 * g + 4 * fhalf));
+            };
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const v4f f = factors(0, g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e] * q_down;
+            }
+            const float from = (float)(row.p - kt0 - 4 * fhalf);
+            score_tile(a, s, slope, [&](int v) { return row.slope2 * __builtin_fabsf(from - (float)(8 * (v >> 2) + (v & 3))); });
+            if (partly) {
+                const int end = row.end - kt0 - 4 * fhalf;
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    if (8 * (v >> 2) + (v & 3) >= end) s[v] = -INFINITY;
+                if (docs) {
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const v4i d = *reinterpret_cast<const v4i *>(lds + G::DOCS_AT + 4 * (32 * kt + 8 * g + 4 * fhalf));
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (d[e] != row.doc) s[4 * g + e] = -INFINITY;
+                    }
+                }
+            }
+            float most = 0.0f;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const v4f kf = factors(0, g), vf = factors(1, g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int v = 4 * g + e;
+                    const float p = __builtin_amdgcn_exp2f(s[v] - lse2);
+                    s[v] = p * __builtin_fmaf(dp[v] * vf[e], o_down, -delta);
+                    if (a.cap2 > 0.0f) s[v] *= slope[v];
+                    s[v] *= kf[e];
+                    most = fmaxf(most, __builtin_fabsf(s[v]));
+                }
+            }
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            if (__builtin_amdgcn_ballot_w64(outgrown(most, d_up))) {
+                const int grown = regrown(most, d_up);
+                times(acc, two_to(grown - d_up));
+                d_up = grown;
+            }
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                v4i df[2];
+                cut_result(s, st, two_to(d_up), df);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const v4i kf[2] = {B::columns(lds, 32 * kt + 16 * st, d, lane, 0), B::columns(lds, 32 * kt + 16 * st, d, lane, 1)};
+                    acc[d] = mfma_cut(kf, df, acc[d]);
+                }
+            }
+        }
+    };
+    while (blk < blocks.n) {
+        const int ahead = blocks.next(blk + 1, lane);
+        if (ahead < blocks.n) load(ahead);
+        attend(blk);
+        __syncthreads();                             // the block has been read
+        if (ahead < blocks.n) {
+            stage();
+            __syncthreads();
+        }
+        blk = ahead;
+    }
+
+    float seen = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) seen = __builtin_fmaf(acc[d][v], 0.0f, seen);
+    uint64_t again = __builtin_amdgcn_ballot_w64(live && !(seen == 0.0f));
+    again |= again >> 32;
+    if (valid && !((again >> frow) & 1)) {
+        const float down = two_to(-d_up - BIAS);
+        float *dq = a.dQ + ((int64_t)b * a.Sq + i) * a.lddq + (int64_t)head * a.dk;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int col = 32 * d + 8 * g + 4 * fhalf;
+                v4f out;
+#pragma unroll
+                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * down * a.scale : 0.0f;
+                if (a.dk == DK || col < a.dk) *reinterpret_cast<v4f *>(dq + col) = out;
+            }
+    }
+    for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) {
+        const int n = __builtin_ctz(rest);
+        attn_dq_row(a, b, head, __builtin_amdgcn_readlane(i, n), lane);
+    }
+}
+
+template <int DK>
+struct DkvGeom {
+    using B = Block<DK, ROWS>;
+    static constexpr int ROW_AT = 2 * B::BYTES;                  // of each row: factors of Q and dO, lse, delta, slope (floats), end, position, document (ints)
+    static constexpr int TILE_AT = ROW_AT + ROWS * 32;           // of each 32 rows: last end, first end, range of documents
+    static constexpr int SMEM = TILE_AT + 2 * 16;
+    static constexpr int PER_SIMD = DK <= 64 ? 2 : 1;
+    // the sums of the waves that share keys: [2 DT][64 lanes][16]
+    static constexpr int JOIN = 2 * (DK / 32) * 64 * 64;
+};
+
+// KW waves side by side along the keys, 32 each; the others take the other tile of each block's rows, and their sums are added in the end
+template <int DK, int KW>
+__global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dkv(AttnArgs a, BwdGrid grid) {
+    using G = DkvGeom<DK>;
+    using B = typename G::B;
+    constexpr int KS = DK / 16, DT = DK / 32;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
+    const int64_t lin = grid.first + blockIdx.x, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
+    const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8, unit = group * 8 + r8 % width;
+    const int tile = (int)(r8 / width);              // causal: the first keys, which most rows see, go out first
+    const int b = (int)(unit / a.Hkv), hk = (int)(unit - (int64_t)b * a.Hkv);
+    const int k0 = tile * 32 * KW, kw0 = k0 + wave % KW * 32, key = kw0 + frow;
+    const int len = attn_len(a, b), start = attn_start(a, b);
+    const bool valid = key < a.Sk, live = key < len, docs = a.doc_q != nullptr;
+    int doc = 0, d_low = 0, d_high = 0, wg_low = 0, wg_high = 0;
+    if (docs) {
+        doc = live ? a.doc_k[(int64_t)b * a.Sk + key] : -1;
+        // the ranges of the wave's keys and of the workgroup's, from those of 32
+        const DocRange *ranges = grid.key_ranges + (int64_t)b * grid.key_tiles;
+        d_low = wg_low = 0x7fffffff;
+        d_high = wg_high = -1;
+#pragma unroll
+        for (int w = 0; w < KW; w++)
+            if (k0 / 32 + w < grid.key_tiles) {
+                const DocRange range = ranges[k0 / 32 + w];
+                const int low = range.low < 0 ? ~range.low : range.low;
+                wg_low = min(wg_low, low);
+                wg_high = max(wg_high, range.high);
+                if (w == wave % KW) {
+                    d_low = low;
+                    d_high = range.high;
+                }
+            }
+        d_low = __builtin_amdgcn_readfirstlane(d_low);
+        d_high = __builtin_amdgcn_readfirstlane(d_high);
+        wg_low = __builtin_amdgcn_readfirstlane(wg_low);
+        wg_high = __builtin_amdgcn_readfirstlane(wg_high);
+    }
+    // rows of a head that may see the workgroup's keys
+    int first = 0, rows_end = a.Sq;
+    if (a.causal) {
+        if (!(a.prefix && a.prefix[b] > k0)) first = k0 - start > 0 ? k0 - start : 0;
+        if (len - start < rows_end) rows_end = len - start;
+    }
+    if (k0 >= len || first >= rows_end) rows_end = 0;
+    first = __builtin_amdgcn_readfirstlane(first);
+    rows_end = __builtin_amdgcn_readfirstlane(rows_end);
+    const DocRange *row_ranges = docs ? grid.row_ranges + (int64_t)b * grid.row_tiles : nullptr;
+    Blocks blocks(row_ranges, rows_end > 0 ? (rows_end + ROWS - 1) / ROWS : 0, grid.row_tiles, wg_low, wg_high);
+
+    // head `g` of the group, block `blk` of it: the place of the work, and the next one
+    struct Place {
+        int g, blk;
+    };
+    auto settle = [&](Place p) -> Place {            // the first place from p on with work
+        while (p.g < a.G) {
+            p.blk = blocks.next(p.blk, lane);
+            if (p.blk < blocks.n) return p;
+            p.g = blocks.n > 0 ? p.g + 1 : a.G;
+            p.blk = first / ROWS;
+        }
+        return p;
+    };
+    Stage<DK, ROWS, WAVES> qs, os;
+    float r_lse = INFINITY, r_delta = 0.0f, r_slope = 0.0f;
+    AttnRow r_row = {0, 0, -1, 0.0f};
+    auto load = [&](Place p) {
+        const int head = hk * a.G + p.g, i0 = p.blk * ROWS, end = rows_end - 1 - i0;
+        qs.load(a.Q + ((int64_t)b * a.Sq + i0) * a.ldq + (int64_t)head * a.dk, a.ldq, end, wave, lane, a.dk);
+        os.load(a.dO + ((int64_t)b * a.Sq + i0) * a.lddo + (int64_t)head * a.dk, a.lddo, end, wave, lane, a.dk);
+        if (threadIdx.x < ROWS) {
+            const int i = i0 + threadIdx.x;
+            r_row.end = 0;
+            r_lse = INFINITY;
+            r_delta = 0.0f;
+            if (i < rows_end) {
+                r_row = attn_row(a, b, head, i);
+                const int64_t at = ((int64_t)b * a.H + head) * a.Sq + i;
+                r_lse = a.Lin[at] * LOG2E;
+                if (r_lse == -INFINITY) r_lse = INFINITY;
+                r_delta = a.delta[at];
+            }
+            r_slope = r_row.slope2;
+        }
+    };
+    auto stage = [&]() {
+        float *of_rows = reinterpret_cast<float *>(lds + G::ROW_AT);
+        qs.put(lds, of_rows, wave, lane, a.q_up);
+        os.put(lds + B::BYTES, of_rows + ROWS, wave, lane, 1.0f);
+        if (threadIdx.x < ROWS) {
+            float *at = of_rows + threadIdx.x;
+            int *ints = reinterpret_cast<int *>(at);
+            at[2 * ROWS] = r_lse;
+            at[3 * ROWS] = r_delta;
+            at[4 * ROWS] = r_slope;
+            ints[5 * ROWS] = r_row.end;
+            ints[6 * ROWS] = r_row.p;
+            ints[7 * ROWS] = r_row.doc;
+            int last = r_row.end, sure = r_row.end, low = r_row.end > 0 ? r_row.doc : 0x7fffffff, high = r_row.end > 0 ? r_row.doc : -1;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) {
+                last = max(last, __shfl_xor(last, off, 64));
+                sure = min(sure, __shfl_xor(sure, off, 64));
+                low = min(low, __shfl_xor(low, off, 64));
+                high = max(high, __shfl_xor(high, off, 64));
+            }
+            if (frow == 0) *reinterpret_cast<v4i *>(lds + G::TILE_AT + 16 * fhalf) = v4i{last, sure, low, high};
+        }
+    };
+
+    Place at = settle({0, first / ROWS});
+    if (at.g < a.G) load(at);
+    v4i kf[KS][2], vf[KS][2];                        // this lane's key and value rows
+    float k_down, v_down;
+    {
+        float x[KS][8];
+        load_row(x, a.K + ((int64_t)b * a.kv_rows + key) * a.ldk + (int64_t)hk * a.dk, live, fhalf, a.dk);
+        k_down = cut_row(x, kf);
+        load_row(x, a.V + ((int64_t)b * a.kv_rows + key) * a.ldv + (int64_t)hk * a.dk, live, fhalf, a.dk);
+        v_down = cut_row(x, vf);
+    }
+    if (at.g < a.G) stage();
+    __syncthreads();
+
+    v16f acc_k[DT], acc_v[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) acc_k[d][v] = acc_v[d][v] = 0.0f;
+    // acc_k is 2^(BIAS + d_up) times the sum of ds q, acc_v 2^(BIAS + p_up) times that of P dO: running exponents of ds and P times their rows' factors
+    int d_up = MOST_UP, p_up = MOST_UP;
+
+    auto attend = [&](int qt) {
+        const v4i whole = *reinterpret_cast<const v4i *>(lds + G::TILE_AT + 16 * qt);
+        const int t_last = __builtin_amdgcn_readfirstlane(whole[0]), t_sure = __builtin_amdgcn_readfirstlane(whole[1]);
+        if (t_last <= kw0) return;
+        bool partly = t_sure < kw0 + 32;
+        if (docs) {
+            const int t_low = __builtin_amdgcn_readfirstlane(whole[2]), t_high = __builtin_amdgcn_readfirstlane(whole[3]);
+            if (t_high < d_low || t_low > d_high) return;
+            partly = true;
+        }
+        v16f s, dp, slope;
+#pragma unroll
+        for (int v = 0; v < 16; v++) s[v] = dp[v] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const v4i qf[2] = {B::rows(lds, 32 * qt, k, lane, 0), B::rows(lds, 32 * qt, k, lane, 1)};
+            s = mfma_cut(qf, kf[k], s);
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const v4i of[2] = {B::rows(lds + B::BYTES, 32 * qt, k, lane, 0), B::rows(lds + B::BYTES, 32 * qt, k, lane, 1)};
+            dp = mfma_cut(of, vf[k], dp);
+        }
+        const unsigned char *mine = lds + G::ROW_AT + 4 * (32 * qt + 4 * fhalf);     // rows 8 g + 0..3 from here: 16 bytes at 32 g
+        auto of_rows = [&](int what, int g) { return *reinterpret_cast<const v4i *>(mine + what * ROWS * 4 + 32 * g); };
+        auto floats = [&](int what, int g) { return __builtin_bit_cast(v4f, of_rows(what, g)); };
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const v4f f = floats(0, g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e] * k_down;
+        }
+        if (a.cap2 > 0.0f || a.slopes) {
+            v16f far;
+            if (a.slopes)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const v4f sl = floats(4, g);
+                    const v4i p = of_rows(6, g);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) far[4 * g + e] = sl[e] * __builtin_fabsf((float)(p[e] - key));
+                }
+            score_tile(a, s, slope, [&](int v) { return far[v]; });
+        }
+        if (partly)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const v4i end = of_rows(5, g);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (key >= end[e]) s[4 * g + e] = -INFINITY;
+                if (docs) {
+                    const v4i d = of_rows(7, g);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (d[e] != doc) s[4 * g + e] = -INFINITY;
+                }
+            }
+        float most_d = 0.0f, most_p = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const v4f qf = floats(0, g), of = floats(1, g), lse = floats(2, g), delta = floats(3, g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int v = 4 * g + e;
+                const float p = __builtin_amdgcn_exp2f(s[v] - lse[e]);
+                dp[v] = p * __builtin_fmaf(dp[v] * of[e], v_down, -delta[e]);
+                if (a.cap2 > 0.0f) dp[v] *= slope[v];
+                dp[v] *= qf[e];
+                s[v] = p * of[e];
+                most_p = fmaxf(most_p, s[v]);
+                most_d = fmaxf(most_d, __builtin_fabsf(dp[v]));
+            }
+        }
+        most_p = fmaxf(most_p, __shfl_xor(most_p, 32, 64));
+        most_d = fmaxf(most_d, __shfl_xor(most_d, 32, 64));
+        if (__builtin_amdgcn_ballot_w64(outgrown(most_d, d_up))) {
+            const int grown = regrown(most_d, d_up);
+            times(acc_k, two_to(grown - d_up));
+            d_up = grown;
+        }
+        if (__builtin_amdgcn_ballot_w64(outgrown(most_p, p_up))) {
+            const int grown = regrown(most_p, p_up);
+            times(acc_v, two_to(grown - p_up));
+            p_up = grown;
+        }
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+            v4i pf[2], df[2];
+            cut_result(s, st, two_to(p_up), pf);
+            cut_result(dp, st, two_to(d_up), df);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const v4i of[2] = {B::columns(lds + B::BYTES, 32 * qt + 16 * st, d, lane, 0), B::columns(lds + B::BYTES, 32 * qt + 16 * st, d, lane, 1)};
+                acc_v[d] = mfma_cut(of, pf, acc_v[d]);
+                const v4i qf[2] = {B::columns(lds, 32 * qt + 16 * st, d, lane, 0), B::columns(lds, 32 * qt + 16 * st, d, lane, 1)};
+                acc_k[d] = mfma_cut(qf, df, acc_k[d]);
+            }
+        }
+    };
+    while (at.g < a.G) {
+        const Place ahead = settle({at.g, at.blk + 1});
+        if (ahead.g < a.G) load(ahead);
+        if (KW == WAVES) {
+#pragma unroll 1
+            for (int qt = 0; qt < 2; qt++) attend(qt);
+        } else {
+            attend(wave / KW);
+        }
+        __syncthreads();                             // the block has been read
+        if (ahead.g < a.G) {
+            stage();
+            __syncthreads();
+        }
+        at = ahead;
+    }
+
+    const float k_out = a.cap2 > 0.0f ? a.cap2 * LN2 : LN2;      // scale over what the rows of Q were taken times
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+            acc_k[d][v] = acc_k[d][v] * two_to(-d_up - BIAS) * k_out;
+            acc_v[d][v] = acc_v[d][v] * two_to(-p_up - BIAS);
+        }
+    if constexpr (KW < WAVES) {
+        static_assert(WAVES == 2 * KW, "two waves share keys");
+        v4f *part = reinterpret_cast<v4f *>(lds + wave % KW * G::JOIN) + lane;
+        if (wave >= KW)
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    part[64 * (8 * d + g)] = v4f{acc_k[d][4 * g], acc_k[d][4 * g + 1], acc_k[d][4 * g + 2], acc_k[d][4 * g + 3]};
+                    part[64 * (8 * d + 4 + g)] = v4f{acc_v[d][4 * g], acc_v[d][4 * g + 1], acc_v[d][4 * g + 2], acc_v[d][4 * g + 3]};
+                }
+        __syncthreads();
+        if (wave >= KW) return;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const v4f pk = part[64 * (8 * d + g)], pv = part[64 * (8 * d + 4 + g)];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    acc_k[d][4 * g + e] += pk[e];
+                    acc_v[d][4 * g + e] += pv[e];
+                }
+            }
+    }
+    float seen = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) seen = __builtin_fmaf(acc_v[d][v], 0.0f, __builtin_fmaf(acc_k[d][v], 0.0f, seen));
+    uint64_t again = __builtin_amdgcn_ballot_w64(live && !(seen == 0.0f));
+    again |= again >> 32;
+    if (valid && !((again >> frow) & 1)) {
+        const int64_t row = (int64_t)b * a.kv_rows + key;
+        float *dk = a.dK + row * a.lddk + (int64_t)hk * a.dk, *dv = a.dV + row * a.lddv + (int64_t)hk * a.dk;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int col = 32 * d + 8 * g + 4 * fhalf;
+                v4f ok, ov;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    ok[e] = live ? acc_k[d][4 * g + e] : 0.0f;
+                    ov[e] = live ? acc_v[d][4 * g + e] : 0.0f;
+                }
+                if (a.dk == DK || col < a.dk) {
+                    *reinterpret_cast<v4f *>(dk + col) = ok;
+                    *reinterpret_cast<v4f *>(dv + col) = ov;
+                }
+            }
+    }
+    for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) attn_dkv_row(a, b, hk, kw0 + __builtin_ctz(rest), lane);
+}
+
+template <typename Kernel>
+int launch_tiles(Kernel kernel, int smem, const AttnArgs &a, BwdGrid grid, const char *what) {
+    const int64_t all = grid.units * grid.tiles;
+    for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
+        const int64_t left = all - grid.first;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), smem, kStream, a, grid);
+        if (int rc = check_launch(what)) return rc;
+    }
+    return AXHIP_OK;
+}
+
+template <int DK>
+int launch_bwd(const AttnArgs &a, BwdGrid grid) {
+    constexpr int SHARED_KEYS = 2 * DkvGeom<DK>::JOIN > DkvGeom<DK>::SMEM ? 2 * DkvGeom<DK>::JOIN : DkvGeom<DK>::SMEM;
+    static bool attr_set = false;
+    if (!attr_set) {
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_dq<DK>), hipFuncAttributeMaxDynamicSharedMemorySize, DqGeom<DK>::SMEM), "hipFuncSetAttribute");
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_dkv<DK, 4>), hipFuncAttributeMaxDynamicSharedMemorySize, DkvGeom<DK>::SMEM), "hipFuncSetAttribute");
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_dkv<DK, 2>), hipFuncAttributeMaxDynamicSharedMemorySize, SHARED_KEYS), "hipFuncSetAttribute");
+        attr_set = true;
+    }
+    if (a.Sq > 0) {
+        grid.units = (int64_t)a.B * a.H;
+        grid.tiles = (a.Sq + 32 * WAVES - 1) / (32 * WAVES);
+        if (int rc = launch_tiles(k_attn_dq<DK>, DqGeom<DK>::SMEM, a, grid, "attn_bwd queries")) return rc;
+    }
+    grid.units = (int64_t)a.B * a.Hkv;
+    const int64_t wide = (a.Sk + 127) / 128 * grid.units;
+    if (wide > 2 * cu_count()) {
+        grid.tiles = (a.Sk + 127) / 128;
+        return launch_tiles(k_attn_dkv<DK, 4>, DkvGeom<DK>::SMEM, a, grid, "attn_bwd keys");
+    }
+    grid.tiles = (a.Sk + 63) / 64;
+    return launch_tiles(k_attn_dkv<DK, 2>, SHARED_KEYS, a, grid, "attn_bwd keys");
+}
+
+}  // namespace
+
+namespace axhip {
+
+int attn_bwd_tiles(AttnArgs &a) {
+    BwdGrid grid = {};
+    const size_t deltas = ((size_t)a.B * a.H * a.Sq * sizeof(float) + 15) & ~size_t(15);
+    size_t bytes = deltas;
+    if (a.doc_k) {
+        grid.key_tiles = (int)(((int64_t)a.Sk + 31) / 32);
+        grid.row_tiles = (int)(((int64_t)a.Sq + 31) / 32);
+        bytes += (size_t)a.B * (grid.key_tiles + grid.row_tiles) * 8;
+    }
+    char *ws = static_cast<char *>(workspace(bytes));
+    if (!ws) return AXHIP_ERR_ALLOC;
+    a.delta = reinterpret_cast<float *>(ws);
+    if (a.doc_k) {
+        grid.key_ranges = reinterpret_cast<DocRange *>(ws + deltas);
+        grid.row_ranges = reinterpret_cast<DocRange *>(ws + deltas + (size_t)a.B * grid.key_tiles * 8);
+        if (int rc = doc_ranges(a.doc_k, a.B, a.Sk, ws + deltas)) return rc;
+        if (int rc = doc_ranges(a.doc_q, a.B, a.Sq, ws + deltas + (size_t)a.B * grid.key_tiles * 8)) return rc;
+    }
+    note_kernel("attn_grad_tiles");
+    if (a.dk <= 32) return launch_bwd<32>(a, grid);
+    if (a.dk <= 64) return launch_bwd<64>(a, grid);
+    if (a.dk <= 96) return launch_bwd<96>(a, grid);
+    return launch_bwd<128>(a, grid);
+}
+
+}  // namespace axhip

@@ -21,15 +21,13 @@ struct FwdGeom {
     static constexpr int BQ = 32 * WAVES, BKV = 64;
     using B = Block<DK, BKV>;
     static constexpr bool DOUBLE = WAVES == 8;   // two blocks in LDS, or two workgroups a CU
-    static constexpr int FACTORS_AT = 2 * B::BYTES;              // of each eight keys: 2^-e of K (float), e of V (int)
-    static constexpr int DOCS_AT = FACTORS_AT + BKV / 8 * 8;     // documents of the keys, then the ranges of their two tiles
+    static constexpr int FACTORS_AT = 2 * B::BYTES;              // of each key row, then of each value row
+    static constexpr int DOCS_AT = FACTORS_AT + BKV * 8;         // documents of the keys, then the ranges of their two tiles
     static constexpr int STAGE = DOCS_AT + BKV * 4 + 2 * 8;
     static constexpr int META_AT = (DOUBLE ? 2 : 1) * STAGE;     // a row of four ints a wave
     static constexpr int SMEM = META_AT + 16 * WAVES;
     static_assert(STAGE % 16 == 0 && SMEM * (DOUBLE ? 1 : 2) <= 160 * 1024, "eight waves a CU");
 };
-
-constexpr int P_UP = 6;                          // probabilities are at most 2^8 times the reference point's
 
 template <int DK, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid grid) {
@@ -118,12 +116,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
         if (docs && threadIdx.x < 2) range_here = 2 * blk + (int)threadIdx.x < grid.range_tiles ? ranges[2 * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
     };
     auto stage = [&](unsigned char *at) {
-        const int ke = ks.put(at, wave, lane, 1.0f), ve = vs.put(at + B::BYTES, wave, lane, 1.0f);
-        constexpr int SLOTS = Stage<DK, BKV, WAVES>::RPW / 8;
-        if (lane < SLOTS) {
-            reinterpret_cast<float *>(at + G::FACTORS_AT)[wave * SLOTS + lane] = two_to(-ke);
-            reinterpret_cast<int *>(at + G::FACTORS_AT + BKV / 2)[wave * SLOTS + lane] = ve;
-        }
+        float *factors = reinterpret_cast<float *>(at + G::FACTORS_AT);
+        ks.put(at, factors, wave, lane, 1.0f);
+        vs.put(at + B::BYTES, factors + BKV, wave, lane, 1.0f);
         if (docs && threadIdx.x < BKV) reinterpret_cast<int *>(at + G::DOCS_AT)[threadIdx.x] = doc_here;
         if (docs && threadIdx.x < 2) reinterpret_cast<DocRange *>(at + G::DOCS_AT + BKV * 4)[threadIdx.x] = range_here;
     };
@@ -134,7 +129,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     float q_down;
     {
         const float *q = a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk;
-        float x[KS][8], most = 0.0f;
+        float x[KS][8];
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -143,16 +138,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 v4f v = {0.f, 0.f, 0.f, 0.f};
                 if (live && (a.dk == DK || col < a.dk)) v = *reinterpret_cast<const v4f *>(q + col);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[s][4 * h + e] = v[e] * a.q_up;
-                    most = fmaxf(most, __builtin_fabsf(x[s][4 * h + e]));
-                }
+                for (int e = 0; e < 4; e++) x[s][4 * h + e] = v[e] * a.q_up;
             }
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        const int up = up_of(most);
-        q_down = two_to(-up);
-#pragma unroll
-        for (int s = 0; s < KS; s++) cut_halves(x[s], two_to(up), qf[s]);
+        q_down = cut_row(x, qf);
     }
     if (blk < nblocks) {
         stage(lds);
@@ -167,7 +155,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
 #pragma unroll
         for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
     float m_run = ATTN_LOWEST, l_run = 0.0f;         // l_run: this lane half's share of the row sum
-    int v_up = MOST_UP;                              // acc is 2^(P_UP + v_up) times the sum; v_up the least of the values' exponents so far
+    int p_up = MOST_UP;                              // acc is 2^(BIAS + p_up) times the sum: the running exponent of p times its value row's factor
 
     auto attend = [&](int blk, const unsigned char *at) {
 #pragma unroll 1
@@ -192,13 +180,21 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 s = mfma_cut(kf, qf[k], s);
             }
             __builtin_amdgcn_s_setprio(0);
-            const v4f down = *reinterpret_cast<const v4f *>(at + G::FACTORS_AT + 16 * kt);
+            auto factors = [&](int what, int g) {    // of keys 8 g + 4 * half + 0..3 of the tile
+                return *reinterpret_cast<const v4f *>(at + G::FACTORS_AT + what * BKV * 4 + 4 * (32 * kt + 8 * g + 4 * fhalf));
+            };
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const float f = down[g] * q_down;
+                const v4f f = factors(0, g);
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[4 * g + e] *= f;
+                for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e];
             }
+            // what is left to the score: q_down, here where more is done to it, in the exponential's multiply-add otherwise
+            const bool plain = a.cap2 == 0.0f && !a.slopes;
+            const float down = plain ? q_down : 1.0f;
+            if (!plain)
+#pragma unroll
+                for (int v = 0; v < 16; v++) s[v] *= q_down;
             if (a.cap2 > 0.0f) {
                 float big = 0.0f;
 #pragma unroll
@@ -234,7 +230,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
             float m_blk = s[0];
 #pragma unroll
             for (int v = 1; v < 16; v++) m_blk = fmaxf(m_blk, s[v]);
-            m_blk = fmaxf(m_blk, __shfl_xor(m_blk, 32, 64));
+            m_blk = fmaxf(m_blk, __shfl_xor(m_blk, 32, 64)) * down;
             if (__builtin_amdgcn_ballot_w64(m_blk > m_run + 8.0f)) {
                 const float m_new = fmaxf(m_run, m_blk), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
                 l_run *= alpha;
@@ -247,19 +243,26 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
             float l_blk = 0.0f;
 #pragma unroll
             for (int v = 0; v < 16; v++) {
-                s[v] = __builtin_amdgcn_exp2f(s[v] - m_run);
+                s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], down, -m_run));
                 l_blk += s[v];
             }
             l_run += l_blk;
             // ---- O^T += V^T P^T ----
-            int ve[4];
-            const v4i ve4 = *reinterpret_cast<const v4i *>(at + G::FACTORS_AT + BKV / 2 + 16 * kt);
+            float most = 0.0f;
 #pragma unroll
-            for (int g = 0; g < 4; g++) ve[g] = __builtin_amdgcn_readfirstlane(ve4[g]);
-            const int least = min(min(ve[0], ve[1]), min(ve[2], ve[3]));
-            if (least < v_up) {
-                const float by = two_to(least - v_up);
-                v_up = least;
+            for (int g = 0; g < 4; g++) {
+                const v4f f = factors(1, g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[4 * g + e] *= f[e];
+                    most = fmaxf(most, s[4 * g + e]);
+                }
+            }
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            if (__builtin_amdgcn_ballot_w64(outgrown(most, p_up))) {
+                const int grown = regrown(most, p_up);
+                const float by = two_to(grown - p_up);
+                p_up = grown;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -268,12 +271,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
 #pragma unroll
             for (int st = 0; st < 2; st++) {
                 v4i pf[2];
-                v2i32 pa[2], pb[2];
-                const float x[4] = {s[8 * st], s[8 * st + 1], s[8 * st + 2], s[8 * st + 3]}, y[4] = {s[8 * st + 4], s[8 * st + 5], s[8 * st + 6], s[8 * st + 7]};
-                cut_halves(x, two_to(P_UP + v_up - ve[2 * st]), pa);
-                cut_halves(y, two_to(P_UP + v_up - ve[2 * st + 1]), pb);
-#pragma unroll
-                for (int t = 0; t < 2; t++) pf[t] = v4i{pa[t][0], pa[t][1], pb[t][0], pb[t][1]};
+                cut_result(s, st, two_to(p_up), pf);
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     const v4i vf[2] = {B::columns(at + B::BYTES, 32 * kt + 16 * st, d, lane, 0), B::columns(at + B::BYTES, 32 * kt + 16 * st, d, lane, 1)};
@@ -328,7 +326,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     uint64_t again = __builtin_amdgcn_ballot_w64(unfit);
     again |= again >> 32;
     const bool fit = !((again >> frow) & 1);
-    const float inv = live ? 1.0f / l_tot * two_to(-P_UP - v_up) : 0.0f;
+    const float inv = 1.0f / l_tot, p_down = two_to(-p_up - BIAS);
     if (valid && fit) {
         float *o = a.O + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk;
 #pragma unroll
@@ -338,7 +336,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 const int col = 32 * d + 8 * g + 4 * fhalf;
                 v4f out;
 #pragma unroll
-                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * inv : 0.0f;
+                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * p_down * inv : 0.0f;
                 if (a.dk == DK || col < a.dk) *reinterpret_cast<v4f *>(o + col) = out;
             }
         if (a.L && fhalf == 0) a.L[((int64_t)b * a.H + head) * a.Sq + i] = live ? (m_run + __builtin_amdgcn_logf(l_tot)) * LN2 : -INFINITY;

@@ -14,8 +14,16 @@ struct FwdGrid {
     int range_tiles;
 };
 
+struct BwdGrid {
+    int64_t first, units;                        // units: query heads, or heads of keys
+    int tiles;
+    const DocRange *key_ranges, *row_ranges;     // [B, key_tiles], [B, row_tiles], with documents
+    int key_tiles, row_tiles;
+};
+
 // The ranges of ids [B, S] in each 32 (8 bytes each)
 int doc_ranges(const int32_t *ids, int64_t B, int64_t S, void *out);
 int attn_fwd_tiles(const AttnArgs &a);
+int attn_bwd_tiles(AttnArgs &a);
 
 }  // namespace axhip

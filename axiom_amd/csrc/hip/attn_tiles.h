@@ -29,52 +29,52 @@ struct Block {
     }
 };
 
-// How the waves of a workgroup bring a block from memory: wave w rows RPW w .. RPW w + RPW - 1, a lane PIECES pieces of E columns of a row.
+// How the waves of a workgroup bring a block from memory: wave w rows RPW w .. RPW w + RPW - 1, eight columns a lane and piece, LANES lanes a row.
 template <int DK, int ROWS, int WAVES>
 struct Stage {
-    static constexpr int RPW = ROWS / WAVES;
-    static constexpr int E = RPW * DK % 512 == 0 ? 8 : 4;
-    static constexpr int PIECES = RPW * DK / (64 * E);
-    static_assert(RPW % 8 == 0 && PIECES * 64 * E == RPW * DK, "a block divides over the lanes");
+    static constexpr int RPW = ROWS / WAVES, LANES = DK <= 32 ? 4 : DK <= 64 ? 8 : 16, PIECES = RPW * LANES / 64;
+    static_assert(PIECES * 64 == RPW * LANES, "a block divides over the lanes");
     using B = Block<DK, ROWS>;
-    float x[PIECES][E];
+    float x[PIECES][8];
+    __device__ static int row_of(int piece, int wave, int lane) { return wave * RPW + piece * (64 / LANES) + lane / LANES; }
     // row r of the block is at base + min(r, last) * pitch; columns from dk on are zero
     __device__ __forceinline__ void load(const float *base, int64_t pitch, int last, int wave, int lane, int dk) {
+        const int col = lane % LANES * 8;
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            const int q = lane + 64 * i, row = wave * RPW + q / (DK / E), col = q % (DK / E) * E;
+            const int row = row_of(i, wave, lane);
             const float *p = base + (int64_t)(row < last ? row : last) * pitch + col;
 #pragma unroll
-            for (int h = 0; h < E / 4; h++) {
+            for (int h = 0; h < 2; h++) {
                 v4f a = {0.f, 0.f, 0.f, 0.f};
-                if (dk == DK || col + 4 * h < dk) a = *reinterpret_cast<const v4f *>(p + 4 * h);
+                if ((dk == DK && DK == 8 * LANES) || col + 4 * h < dk) a = *reinterpret_cast<const v4f *>(p + 4 * h);
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[i][4 * h + e] = a[e];
             }
         }
     }
-    // to LDS, cut; returns the exponent that this wave's rows were taken up by
-    __device__ __forceinline__ int put(unsigned char *block, int wave, int lane, float factor) {
-        float most = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PIECES; i++)
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                if (factor != 1.0f) x[i][e] *= factor;
-                most = fmaxf(most, __builtin_fabsf(x[i][e]));
-            }
-        const int up = up_of(most_of_wave(most));
-        const float by = two_to(up);
+    // to LDS, times `by`, cut; the rows' factors beside them
+    __device__ __forceinline__ void put(unsigned char *block, float *factors, int wave, int lane, float by) {
+        const int chunk = lane % LANES;
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            const int q = lane + 64 * i, row = wave * RPW + q / (DK / E), col = q % (DK / E) * E;
-            Half<E> t[2];
-            cut_halves(x[i], by, t);
-            unsigned char *to = block + B::at(row, col / 8) + col % 8 * 2;
-            *reinterpret_cast<Half<E> *>(to) = t[0];
-            *reinterpret_cast<Half<E> *>(to + B::PLANE) = t[1];
+            const int row = row_of(i, wave, lane);
+            float most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) most = fmaxf(most, __builtin_fabsf(x[i][e]));
+            const int up = up_of(most_of_lanes<LANES>(most * __builtin_fabsf(by)));
+            v4i t[2];
+            if (by != 1.0f)
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] *= by;
+            cut_halves(x[i], two_to(up), t);
+            if (8 * LANES == DK || 8 * chunk < DK) {
+                unsigned char *to = block + B::at(row, chunk);
+                *reinterpret_cast<v4i *>(to) = t[0];
+                *reinterpret_cast<v4i *>(to + B::PLANE) = t[1];
+            }
+            if (chunk == 0) factors[row] = factor_of(up);
         }
-        return up;
     }
 };
 

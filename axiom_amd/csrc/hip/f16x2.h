@@ -1,9 +1,11 @@
 // fp32 products on the f16 matrix core: every operand as the sum of two f16 terms under a power of two of its own.
 //
-// A group of values (a row, or eight rows, of a head) is taken times 2^e so that its largest lies in [2^14, 2^15), and each is cut into hi = f16(x) and
-// lo = f16(x - hi): 11 bits each, so hi + lo is x to 2^-23 of itself.  A product of two values is formed of three products of terms, hi hi + hi lo + lo hi,
-// added in fp32; lo lo, left out, is at most 2^-22 of it.  Half of what six products of bf16 terms cost (bf16x3.h), for one bit of each operand: the matrix core
-// multiplies f16 subnormals exactly (measured), so what a value below 2^-17 of its group's largest loses is an absolute 2^-40 of that.
+// A row of a head is taken times 2^e so that its largest value lies in [2^14, 2^15), and each value is cut into hi = f16(x) and lo = f16(x - hi): 11 bits each,
+// so hi + lo is x to 2^-23 of itself.  A product of two values is formed of three products of terms, hi hi + hi lo + lo hi, added in fp32; lo lo, left out,
+// is at most 2^-22 of it.  Half of what six products of bf16 terms cost (bf16x3.h), for one bit of each operand.  The matrix core multiplies f16
+// subnormals exactly (measured), so what a value below 2^-17 of its row's largest loses is an absolute 2^-40 of that.
+// Every row has a power of its own, and not a block: a row of 1e30 that a mask hides would otherwise take the bits of its neighbours.  Where rows are summed over
+// (P V), their powers go to the other operand, whose largest so far a running exponent holds.
 // Cutting a pair: two products, two conversions of pairs, two mixed multiply-adds.
 // (Sums of products of split operands: Dekker, "A floating-point technique for extending the available precision", 1971.)
 #pragma once
@@ -41,28 +43,55 @@ __device__ __forceinline__ v16f mfma_cut(const v4i (&a)[2], const v4i (&b)[2], v
     return mfma_halves(a[0], b[0], c);
 }
 
-// The exponent e of a group whose largest magnitude is `most`.  At most 120, which a group of zeros gets too, so that 2^e and 2^-e are floats.
-constexpr int MOST_UP = 120;
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigned)((e < -126 ? -126 : e) + 127) << 23); }
+
+// The exponent e of a row whose largest magnitude is `most`: at most MOST_UP, which a row of zeros gets.  The factor kept with a row is 2^(BIAS - e): times it, what
+// small rows are multiplied by does not run out of exponents.  (Rows past 2^100 get an infinite factor, and what it meets is formed again.)
+constexpr int MOST_UP = 100, BIAS = 24;
 __device__ __forceinline__ int up_of(float most) {
     const int e = 15 - __builtin_amdgcn_frexp_expf(most);
     return most == 0.0f || e > MOST_UP ? MOST_UP : e;
 }
-__device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigned)((e < -126 ? -126 : e) + 127) << 23); }
+__device__ __forceinline__ float factor_of(int e) { return BIAS - e > 127 ? INFINITY : two_to(BIAS - e); }
 
-// The largest of the 64 lanes' values, in every lane
-__device__ __forceinline__ float most_of_wave(float v) {
-#define AX_ROTATED(ctrl) v = fmaxf(v, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), ctrl, 0xf, 0xf, true)))
-    AX_ROTATED(0x128);                           // rotations by 8, 4, 2 and 1 within each row of 16 lanes
-    AX_ROTATED(0x124);
-    AX_ROTATED(0x122);
-    AX_ROTATED(0x121);
-#undef AX_ROTATED
-    const unsigned u = __float_as_uint(v);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    const unsigned w = __float_as_uint(v);
-    const auto h = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+// The largest of each LANES neighbouring lanes' values (4, 8 or 16), in all of them
+template <int LANES>
+__device__ __forceinline__ float most_of_lanes(float v) {
+#define AX_MOVED(ctrl) v = fmaxf(v, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), ctrl, 0xf, 0xf, true)))
+    AX_MOVED(0xb1);                              // lane ^ 1, lane ^ 2, then 8 and 16 lanes mirrored
+    AX_MOVED(0x4e);
+    if (LANES >= 8) AX_MOVED(0x141);
+    if (LANES >= 16) AX_MOVED(0x140);
+#undef AX_MOVED
+    return v;
+}
+
+// A running exponent `up` for sums over what has no scale of its own: `most`, the largest factor yet, may not exceed 2^15 times it; it starts at MOST_UP and
+// falls so that the largest lies at 2^10, which leaves room for others.
+__device__ __forceinline__ bool outgrown(float most, int up) { return most > two_to(15 - up); }
+__device__ __forceinline__ int regrown(float most, int up) {
+    const int e = 10 - __builtin_amdgcn_frexp_expf(most);
+    return outgrown(most, up) ? (e < MOST_UP ? e : MOST_UP) : up;
+}
+
+// Registers 8 s .. 8 s + 7 of a result tile as an operand, times `up`
+__device__ __forceinline__ void cut_result(const v16f &x, int s, float up, v4i (&t)[2]) {
+    const float part[8] = {x[8 * s], x[8 * s + 1], x[8 * s + 2], x[8 * s + 3], x[8 * s + 4], x[8 * s + 5], x[8 * s + 6], x[8 * s + 7]};
+    cut_halves(part, up, t);
+}
+
+// A lane's row (its other half in lane ^ 32) as operand terms, columns 16 s + 8 * half .. + 7 for step s; gives back the 2^-e that its products are taken times, less BIAS
+template <int KS>
+__device__ __forceinline__ float cut_row(float (&x)[KS][8], v4i (&t)[KS][2]) {
+    float most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) most = fmaxf(most, __builtin_fabsf(x[s][e]));
+    const int up = up_of(fmaxf(most, __shfl_xor(most, 32, 64)));
+#pragma unroll
+    for (int s = 0; s < KS; s++) cut_halves(x[s], two_to(up), t[s]);
+    return two_to(-up - BIAS);
 }
 
 // Four rows of one column each from LDS: lane l of a group of 16 lanes gives the address of four columns of one row (rows go with l / 4, columns with

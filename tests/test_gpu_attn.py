@@ -304,3 +304,21 @@ def test_layer_between_its_projections(hip):
     hip.check(L.axhip_attn_fwd(dl.ptr, H * dk, y.ptr + at, ldn, x.ptr + vat, ld, S, o1.ptr, H * dk, None, B, H, Hkv, 1, S, dk, 0.125, C.byref(step)))
     prompt = o.numpy().reshape(B, S, H * dk)
     assert near(o1.numpy(), np.stack([prompt[b, lens[b] - 1] for b in range(B)]))
+
+
+@pytest.mark.parametrize("dk", [32, 64, 96, 128])
+def test_large_rows_beside_ordinary_ones(hip, dk):
+    """Keys, values, queries and gradients whose rows differ by 10^15 and more, next to each other: what does not see the large ones, and what sees them with a probability
+    of nothing, is held to its own size."""
+    say("attn large rows", dk)
+    B, S, H = 1, 130, 2
+    rng, q, k, v, d_o = draw(14, B, S, S, H, 1, dk)
+    v[0, 70] *= np.float32(1e20)                          # rows 0 .. 69 do not see it
+    k[0, 75, 0, 0], q[0, :, :, 0] = 1e18, -1e-3           # seen with a score of -1e15 scale
+    q[0, 20:22] *= np.float32(1e-15)
+    d_o[0, 90] *= np.float32(1e-12)
+    d_o[0, 33] *= np.float32(1e12)
+    rules = Rules(causal=1)
+    want = attention(q, k, v, dk ** -0.5, rules, d_o)
+    # what the large value and gradient add to others is in their bounds, as in any fp32 sum
+    check(hip, q, k, v, dk ** -0.5, rules, d_o, want=want)
