@@ -72,7 +72,8 @@ extern "C" int axhip_attn_fwd(const float *Q, int64_t ldq, const float *K, int64
     a.ldk = ldk;
     a.ldv = ldv;
     a.ldo = ldo;
-    return attn_fwd_tiles(a);
+    int rc = AXHIP_OK;
+    return attn_fwd_few(a, rc) ? rc : attn_fwd_tiles(a);
 }
 
 extern "C" int axhip_attn_bwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, const float *V, int64_t ldv, int64_t kv_rows, const float *O,

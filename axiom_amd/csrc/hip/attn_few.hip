@@ -1,0 +1,351 @@
+// Attention forward under score rules for few rows: tokens over a cache, short prompts.
+//
+// Bound by how fast K and V come in.  32 rows (the new tokens of all query heads that share keys, one head after the other) meet one head of keys, and the keys are
+// shared out twice: over workgroups, `splits` ranges of a sequence's 32-key tiles, and over the four waves of each, which take its tiles in turn.  A wave brings its own
+// tile, whole rows of K and V by 16-byte loads with the next tile in registers meanwhile, cuts it into an LDS block of its own (no barrier until the end) and goes through it as
+// the tile kernel does (attn_fwd.hip).  Maxima, sums and outputs of the waves meet in LDS, those of the ranges in memory, where the last workgroup of the rows to arrive adds
+// them, in order: one launch, and the same bits whoever is last.
+#include "attn_launch.h"
+#include "attn_tiles.h"
+
+namespace {
+using namespace axhip;
+
+constexpr int WAVES = 4;
+
+template <int DK>
+struct FewGeom {
+    using B = Block<DK, 32>;
+    static constexpr int DT = DK / 32, PIECES = 4 * DT;          // a lane's output in pieces of four
+    static constexpr int FACTORS_AT = 2 * B::BYTES, DOCS_AT = FACTORS_AT + 256, BLOCK = DOCS_AT + 128;
+    static constexpr int JOIN_AT = 0, ML_AT = WAVES * PIECES * 1024;   // of the waves: pieces [64] v4f, then maxima and sums [2][32]
+    static constexpr int BLOCKS = WAVES * BLOCK, JOINED = ML_AT + WAVES * 256;
+    static constexpr int FLAGS_AT = BLOCKS > JOINED ? BLOCKS : JOINED;   // a word a wave: the rows whose sums are not finite; then who is last
+    static constexpr int SMEM = FLAGS_AT + 4 * WAVES + 16;
+    static_assert(BLOCK % 16 == 0 && SMEM <= 160 * 1024, "LDS");
+    static constexpr int PART = PIECES * 64 * 4 + 64;            // floats that a range leaves in memory
+};
+
+template <int DK>
+__global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(AttnArgs a, FewGrid grid) {
+    using G = FewGeom<DK>;
+    using B = typename G::B;
+    constexpr int KS = DK / 16, DT = DK / 32, PIECES = G::PIECES;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
+    // ranges of one set of rows follow each other, so that they go to different XCDs
+    const int64_t unit = blockIdx.x / grid.splits;
+    const int split = (int)(blockIdx.x - unit * grid.splits);
+    const int64_t bh = unit / grid.row_tiles;
+    const int rt = (int)(unit - bh * grid.row_tiles), b = (int)(bh / a.Hkv), hk = (int)(bh - (int64_t)b * a.Hkv), h0 = hk * a.G;
+    const int rows = a.G * a.Sq, r = rt * 32 + frow;
+    const bool valid = r < rows, docs = a.doc_q != nullptr;
+    const int over = (valid ? r : rows - 1) / a.Sq, head = h0 + over, i = (valid ? r : rows - 1) - over * a.Sq;
+    AttnRow row = attn_row(a, b, head, i);
+    if (!valid) row.end = 0;
+    const bool live = row.end > 0;
+    int last = row.end, sure = live ? row.end : 0x7fffffff, d_low = live ? row.doc : 0x7fffffff, d_high = live ? row.doc : -1;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        last = max(last, __shfl_xor(last, off, 64));
+        sure = min(sure, __shfl_xor(sure, off, 64));
+        d_low = min(d_low, __shfl_xor(d_low, off, 64));
+        d_high = max(d_high, __shfl_xor(d_high, off, 64));
+    }
+    last = __builtin_amdgcn_readfirstlane(last);
+    sure = __builtin_amdgcn_readfirstlane(sure);
+    d_low = __builtin_amdgcn_readfirstlane(d_low);
+    d_high = __builtin_amdgcn_readfirstlane(d_high);
+    const int all = (last + 31) / 32, t_begin = (int)((int64_t)all * split / grid.splits), t_end = (int)((int64_t)all * (split + 1) / grid.splits);
+
+    const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;
+    unsigned char *const at = lds + wave * G::BLOCK;
+    float *const row_factors = reinterpret_cast<float *>(at + G::FACTORS_AT);
+    Stage<DK, 32, 1> ks, vs;
+    int doc_here = -1;
+    auto load = [&](int t) {
+        const int64_t k0 = (int64_t)t * 32;
+        const int end = last - 1 - (int)k0;          // rows past it are read as it
+        ks.load(Kb + k0 * a.ldk, a.ldk, end, 0, lane, a.dk);
+        vs.load(Vb + k0 * a.ldv, a.ldv, end, 0, lane, a.dk);
+        if (docs) doc_here = frow <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + frow] : -1;
+    };
+    int t = t_begin + wave;
+    if (t < t_end) load(t);
+    v4i qf[KS][2];
+    float q_down;
+    {
+        const float *q = a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk;
+        float x[KS][8];
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int col = 16 * s + 8 * fhalf + 4 * h;
+                v4f v = {0.f, 0.f, 0.f, 0.f};
+                if (live && (a.dk == DK || col < a.dk)) v = *reinterpret_cast<const v4f *>(q + col);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[s][4 * h + e] = v[e] * a.q_up;
+            }
+        q_down = cut_row(x, qf);
+    }
+    v16f acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
+    float m_run = ATTN_LOWEST, l_run = 0.0f;
+    int p_up = MOST_UP;                              // acc is 2^(BIAS + p_up) times the sum: the running exponent of p times its value row's factor
+
+    for (; t < t_end; t += WAVES) {
+        const int kt0 = t * 32;
+        bool partly = kt0 + 32 > sure, meets = true;
+        if (docs) {
+            meets = __builtin_amdgcn_ballot_w64(doc_here >= d_low && doc_here <= d_high) != 0;
+            partly |= __builtin_amdgcn_ballot_w64(doc_here != d_low) != 0 || d_low != d_high;
+        }
+        order_in_wave();                             // the last tile has been read
+        if (meets) {
+            ks.put(at, row_factors, 0, lane, 1.0f);
+            vs.put(at + B::BYTES, row_factors + 32, 0, lane, 1.0f);
+            if (docs && lane < 32) reinterpret_cast<int *>(at + G::DOCS_AT)[lane] = doc_here;
+        }
+        order_in_wave();
+        if (t + WAVES < t_end) load(t + WAVES);
+        if (!meets) continue;
+        v16f s;
+#pragma unroll
+        for (int v = 0; v < 16; v++) s[v] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const v4i kf[2] = {B::rows(at, 0, k, lane, 0), B::rows(at, 0, k, lane, 1)};
+            s = mfma_cut(kf, qf[k], s);
+        }
+        auto factors = [&](int what, int g) { return *reinterpret_cast<const v4f *>(row_factors + what * 32 + 8 * g + 4 * fhalf); };
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const v4f f = factors(0, g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e] * q_down;
+        }
+        if (a.cap2 > 0.0f) {
+            float big = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 16; v++) big = fmaxf(big, __builtin_fabsf(s[v]));
+            if (__builtin_amdgcn_ballot_w64(!(big < TANH_NEAR)))
+#pragma unroll
+                for (int v = 0; v < 16; v++) s[v] = a.cap2 * tanh_of(s[v]).value;
+            else
+#pragma unroll
+                for (int v = 0; v < 16; v++) s[v] = a.cap2 * tanh_near(s[v]);
+        }
+        if (a.slopes) {
+            const float from = (float)(row.p - kt0 - 4 * fhalf);
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[v] = __builtin_fmaf(-row.slope2, __builtin_fabsf(from - (float)(8 * (v >> 2) + (v & 3))), s[v]);
+        }
+        if (partly) {
+            const int end = row.end - kt0 - 4 * fhalf;
+#pragma unroll
+            for (int v = 0; v < 16; v++)
+                if (8 * (v >> 2) + (v & 3) >= end) s[v] = -INFINITY;
+            if (docs)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const v4i d = *reinterpret_cast<const v4i *>(at + G::DOCS_AT + 4 * (8 * g + 4 * fhalf));
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (d[e] != row.doc) s[4 * g + e] = -INFINITY;
+                }
+        }
+        float m_blk = s[0];
+#pragma unroll
+        for (int v = 1; v < 16; v++) m_blk = fmaxf(m_blk, s[v]);
+        m_blk = fmaxf(m_blk, __shfl_xor(m_blk, 32, 64));
+        if (__builtin_amdgcn_ballot_w64(m_blk > m_run + 8.0f)) {
+            const float m_new = fmaxf(m_run, m_blk), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            l_run *= alpha;
+            m_run = m_new;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) acc[d][v] *= alpha;
+        }
+        float l_blk = 0.0f, most = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const v4f f = factors(1, g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float p = __builtin_amdgcn_exp2f(s[4 * g + e] - m_run);
+                l_blk += p;
+                s[4 * g + e] = p * f[e];
+                most = fmaxf(most, s[4 * g + e]);
+            }
+        }
+        l_run += l_blk;
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        if (__builtin_amdgcn_ballot_w64(outgrown(most, p_up))) {
+            const int grown = regrown(most, p_up);
+            const float by = two_to(grown - p_up);
+            p_up = grown;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) acc[d][v] *= by;
+        }
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+            v4i pf[2];
+            cut_result(s, st, two_to(p_up), pf);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const v4i vf[2] = {B::columns(at + B::BYTES, 16 * st, d, lane, 0), B::columns(at + B::BYTES, 16 * st, d, lane, 1)};
+                acc[d] = mfma_cut(vf, pf, acc[d]);
+            }
+        }
+    }
+
+    // ---- the waves' parts together ----
+    __syncthreads();                                 // the blocks have been read
+    v4f *const part = reinterpret_cast<v4f *>(lds + G::JOIN_AT);
+    float *const ml = reinterpret_cast<float *>(lds + G::ML_AT);
+    const float p_down = two_to(-p_up - BIAS), l_wave = l_run + __shfl_xor(l_run, 32, 64);
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            part[(wave * PIECES + 4 * d + g) * 64 + lane] = v4f{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]} * p_down;
+    if (fhalf == 0) {
+        ml[wave * 64 + frow] = m_run;
+        ml[wave * 64 + 32 + frow] = l_wave;
+    }
+    __syncthreads();
+    float m_all = ATTN_LOWEST, l_all = 0.0f, weight[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) m_all = fmaxf(m_all, ml[w * 64 + frow]);
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        weight[w] = __builtin_amdgcn_exp2f(ml[w * 64 + frow] - m_all);
+        l_all = __builtin_fmaf(ml[w * 64 + 32 + frow], weight[w], l_all);
+    }
+    v4f out[DT];                                     // this wave's pieces: wave, wave + 4, ...
+#pragma unroll
+    for (int n = 0; n < DT; n++) {
+        out[n] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) out[n] += part[(w * PIECES + wave + 4 * n) * 64 + lane] * weight[w];
+    }
+    int *const flags = reinterpret_cast<int *>(lds + G::FLAGS_AT);
+    if (grid.splits > 1) {
+        // The ranges meet in memory: parts, counter and the reads below are device-scope accesses (the workgroups run on XCDs with an L2 each); the wait
+        // completes a thread's stores before the barrier, the barrier orders them before thread 0's increment.
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        float *mine = grid.parts + (unit * grid.splits + split) * G::PART;
+#pragma unroll
+        for (int n = 0; n < DT; n++) {
+            int64_t *to = reinterpret_cast<int64_t *>(mine + ((wave + 4 * n) * 64 + lane) * 4);
+            __hip_atomic_store(to, __builtin_bit_cast(int64_t, v2f{out[n][0], out[n][1]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(to + 1, __builtin_bit_cast(int64_t, v2f{out[n][2], out[n][3]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (wave == 0 && fhalf == 0)
+            __hip_atomic_store(reinterpret_cast<int64_t *>(mine + PIECES * 256 + 2 * frow), __builtin_bit_cast(int64_t, v2f{m_all, l_all}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (threadIdx.x == 0) flags[WAVES] = __hip_atomic_fetch_add(grid.arrivals + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == grid.splits - 1;
+        __syncthreads();
+        if (!flags[WAVES]) return;
+        const float *theirs = grid.parts + unit * grid.splits * G::PART;
+        auto read = [&](int64_t from) {
+            return __builtin_bit_cast(v2f, __hip_atomic_load(reinterpret_cast<const int64_t *>(theirs + from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        };
+        m_all = ATTN_LOWEST;
+        for (int s = 0; s < grid.splits; s++) m_all = fmaxf(m_all, read((int64_t)s * G::PART + PIECES * 256 + 2 * frow)[0]);
+        l_all = 0.0f;
+#pragma unroll
+        for (int n = 0; n < DT; n++) out[n] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < grid.splits; s++) {
+            const v2f both = read((int64_t)s * G::PART + PIECES * 256 + 2 * frow);
+            const float w = __builtin_amdgcn_exp2f(both[0] - m_all);
+            l_all = __builtin_fmaf(both[1], w, l_all);
+#pragma unroll
+            for (int n = 0; n < DT; n++) {
+                const int64_t from = (int64_t)s * G::PART + ((wave + 4 * n) * 64 + lane) * 4;
+                const v2f x = read(from), y = read(from + 2);
+                out[n] += v4f{x[0], x[1], y[0], y[1]} * w;
+            }
+        }
+        if (threadIdx.x == 0) __hip_atomic_store(grid.arrivals + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);       // ready for the next launch
+    }
+
+    // ---- normalise and write ----
+    float seen = l_all * 0.0f;
+#pragma unroll
+    for (int n = 0; n < DT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) seen = __builtin_fmaf(out[n][e], 0.0f, seen);
+    const uint64_t unfit = __builtin_amdgcn_ballot_w64(live && (!(seen == 0.0f) || l_all == 0.0f));
+    if (lane == 0) flags[wave] = (int)((unsigned)unfit | (unsigned)(unfit >> 32));
+    __syncthreads();
+    unsigned again = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) again |= (unsigned)flags[w];
+    again = __builtin_amdgcn_readfirstlane(again);
+    if (valid && !((again >> frow) & 1)) {
+        const float inv = 1.0f / l_all;
+        float *o = a.O + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk;
+#pragma unroll
+        for (int n = 0; n < DT; n++) {
+            const int col = 32 * n + 8 * wave + 4 * fhalf;
+            if (a.dk == DK || col < a.dk) *reinterpret_cast<v4f *>(o + col) = live ? out[n] * inv : v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        if (a.L && wave == 0 && fhalf == 0) a.L[((int64_t)b * a.H + head) * a.Sq + i] = live ? (m_all + __builtin_amdgcn_logf(l_all)) * LN2 : -INFINITY;
+    }
+    int nth = 0;
+    for (unsigned rest = again; rest; rest &= rest - 1, nth++) {
+        const int n = __builtin_ctz(rest);
+        if (nth % WAVES == wave) attn_fwd_row(a, b, __builtin_amdgcn_readlane(head, n), __builtin_amdgcn_readlane(i, n), lane);
+    }
+}
+
+template <int DK>
+int launch_few(const AttnArgs &a, FewGrid grid) {
+    using G = FewGeom<DK>;
+    static bool attr_set = false;
+    if (!attr_set) {
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_few<DK>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
+        attr_set = true;
+    }
+    const int64_t units = (int64_t)a.B * a.Hkv * grid.row_tiles;
+    if (grid.splits > 1) {
+        grid.parts = static_cast<float *>(workspace((size_t)units * grid.splits * G::PART * sizeof(float)));
+        grid.arrivals = strip_counters((size_t)units);
+        if (!grid.parts || !grid.arrivals) return AXHIP_ERR_ALLOC;
+    }
+    note_kernel(grid.splits > 1 ? "attn_few_ranges" : "attn_few");
+    hipLaunchKernelGGL(k_attn_few<DK>, dim3((unsigned)(units * grid.splits)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
+    return check_launch("attn_fwd");
+}
+
+}  // namespace
+
+namespace axhip {
+
+// Whether the few-rows form takes the call, and in how many ranges of keys.  Ranges: until there are two workgroups a CU, each wave with a tile or more.
+bool attn_fwd_few(const AttnArgs &a, int &rc) {
+    const int64_t rows = (int64_t)a.G * a.Sq, cus = cu_count();
+    FewGrid grid = {};
+    grid.row_tiles = (int)((rows + 31) / 32);
+    const int64_t units = (int64_t)a.B * a.Hkv * grid.row_tiles, tiles = ((int64_t)a.Sk + 31) / 32;
+    if (rows > 32 || units > GRID_MOST / 64) return false;
+    int64_t splits = (2 * cus + units - 1) / units;
+    if (splits > (tiles + WAVES - 1) / WAVES) splits = (tiles + WAVES - 1) / WAVES;
+    if (splits > 64) splits = 64;
+    if (splits < 1) splits = 1;
+    grid.splits = (int)splits;
+    rc = a.dk <= 32 ? launch_few<32>(a, grid) : a.dk <= 64 ? launch_few<64>(a, grid) : a.dk <= 96 ? launch_few<96>(a, grid) : launch_few<128>(a, grid);
+    return true;
+}
+
+}  // namespace axhip

@@ -14,6 +14,12 @@ struct FwdGrid {
     int range_tiles;
 };
 
+struct FewGrid {
+    int row_tiles, splits;                       // of 32 rows each; ranges of keys
+    float *parts;                                // what the ranges leave
+    int *arrivals;
+};
+
 struct BwdGrid {
     int64_t first, units;                        // units: query heads, or heads of keys
     int tiles;
@@ -24,6 +30,7 @@ struct BwdGrid {
 // The ranges of ids [B, S] in each 32 (8 bytes each)
 int doc_ranges(const int32_t *ids, int64_t B, int64_t S, void *out);
 int attn_fwd_tiles(const AttnArgs &a);
+bool attn_fwd_few(const AttnArgs &a, int &rc);
 int attn_bwd_tiles(AttnArgs &a);
 
 }  // namespace axhip
