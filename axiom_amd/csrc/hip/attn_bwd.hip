@@ -20,20 +20,6 @@ __device__ __forceinline__ void times(v16f (&acc)[DT], float by) {
         for (int v = 0; v < 16; v++) acc[d][v] *= by;
 }
 
-template <int KS>
-__device__ __forceinline__ void load_row(float (&x)[KS][8], const float *row, bool live, int fhalf, int dk) {
-#pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int col = 16 * s + 8 * fhalf + 4 * h;
-            v4f v = {0.f, 0.f, 0.f, 0.f};
-            if (live && (dk == 16 * KS || col < dk)) v = *reinterpret_cast<const v4f *>(row + col);
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[s][4 * h + e] = v[e];
-        }
-}
-
 // Scores of a tile (products already scaled) after cap and distance; `slope` the cap's derivative.  from[v]: position less key of register v.
 template <typename Distance>
 __device__ __forceinline__ void score_tile(const AttnArgs &a, v16f &s, v16f &slope, Distance distance) {
@@ -103,7 +89,7 @@ struct DqGeom {
     static constexpr int PER_SIMD = DK <= 64 ? 2 : 1;
 };
 
-template <int DK>
+template <int DK, bool PAD>
 __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(AttnArgs a, BwdGrid grid) {
     using G = DqGeom<DK>;
     using B = typename G::B;
@@ -155,8 +141,8 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
     auto load = [&](int blk) {
         const int64_t k0 = (int64_t)blk * ROWS;
         const int end = wg_last - 1 - (int)k0;
-        ks.load(Kb + k0 * a.ldk, a.ldk, end, wave, lane, a.dk);
-        vs.load(Vb + k0 * a.ldv, a.ldv, end, wave, lane, a.dk);
+        ks.template load<PAD>(Kb + k0 * a.ldk, a.ldk, end, wave, lane, a.dk);
+        vs.template load<PAD>(Vb + k0 * a.ldv, a.ldv, end, wave, lane, a.dk);
         if (docs && threadIdx.x < ROWS) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
         if (docs && threadIdx.x < 2) range_here = 2 * blk + (int)threadIdx.x < grid.key_tiles ? ranges[2 * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
     };
@@ -176,15 +162,15 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
     float q_down, o_down, delta = 0.0f;
     {
         float x[KS][8], y[KS][8];
-        load_row(x, a.Oin + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk, live, fhalf, a.dk);
-        load_row(y, a.dO + ((int64_t)b * a.Sq + i) * a.lddo + (int64_t)head * a.dk, live, fhalf, a.dk);
+        load_row<PAD>(x, a.Oin + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk, live, fhalf, a.dk);
+        load_row<PAD>(y, a.dO + ((int64_t)b * a.Sq + i) * a.lddo + (int64_t)head * a.dk, live, fhalf, a.dk);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) delta = __builtin_fmaf(x[s][e], y[s][e], delta);
         delta += __shfl_xor(delta, 32, 64);
         o_down = cut_row(y, of);
-        load_row(x, a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk, live, fhalf, a.dk);
+        load_row<PAD>(x, a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk, live, fhalf, a.dk);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -204,6 +190,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
         for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
     int d_up = MOST_UP;                              // acc is 2^(BIAS + d_up) times the sum: the running exponent of ds times its key row's factor
 
+    const unsigned row_at = B::row_place(lane), column_at = B::column_place(lane);
     auto attend = [&](int blk) {
 #pragma unroll 1
         for (int kt = 0; kt < 2; kt++) {
@@ -216,17 +203,19 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
                 if (!here.meets(d_low, d_high)) continue;
                 partly |= here.low != here.high || here.low != d_low || d_low != d_high;
             }
+            const unsigned char *tile = lds + 32 * kt * B::PITCH;
+            const unsigned row_place = afresh(row_at), column_place = afresh(column_at);
             v16f s, dp, slope;
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = dp[v] = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const v4i kf[2] = {B::rows(lds, 32 * kt, k, lane, 0), B::rows(lds, 32 * kt, k, lane, 1)};
+                const v4i kf[2] = {B::rows(tile, row_place, 0, k, 0), B::rows(tile, row_place, 0, k, 1)};
                 s = mfma_cut(kf, qf[k], s);
             }
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const v4i vf[2] = {B::rows(lds + B::BYTES, 32 * kt, k, lane, 0), B::rows(lds + B::BYTES, 32 * kt, k, lane, 1)};
+                const v4i vf[2] = {B::rows(tile + B::BYTES, row_place, 0, k, 0), B::rows(tile + B::BYTES, row_place, 0, k, 1)};
                 dp = mfma_cut(vf, of[k], dp);
             }
             auto factors = [&](int what, int g) {    // of keys 8 g + 4 * half + 0..3 of the tile
@@ -281,7 +270,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
                 cut_result(s, st, two_to(d_up), df);
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    const v4i kf[2] = {B::columns(lds, 32 * kt + 16 * st, d, lane, 0), B::columns(lds, 32 * kt + 16 * st, d, lane, 1)};
+                    const v4i kf[2] = {B::columns(tile, column_place, 16 * st, d, 0), B::columns(tile, column_place, 16 * st, d, 1)};
                     acc[d] = mfma_cut(kf, df, acc[d]);
                 }
             }
@@ -317,7 +306,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
                 v4f out;
 #pragma unroll
                 for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * down * a.scale : 0.0f;
-                if (a.dk == DK || col < a.dk) *reinterpret_cast<v4f *>(dq + col) = out;
+                if (!PAD || col < a.dk) *reinterpret_cast<v4f *>(dq + col) = out;
             }
     }
     for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) {
@@ -338,7 +327,7 @@ struct DkvGeom {
 };
 
 // KW waves side by side along the keys, 32 each; the others take the other tile of each block's rows, and their sums are added in the end
-template <int DK, int KW>
+template <int DK, int KW, bool PAD>
 __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dkv(AttnArgs a, BwdGrid grid) {
     using G = DkvGeom<DK>;
     using B = typename G::B;
@@ -406,8 +395,8 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
     AttnRow r_row = {0, 0, -1, 0.0f};
     auto load = [&](Place p) {
         const int head = hk * a.G + p.g, i0 = p.blk * ROWS, end = rows_end - 1 - i0;
-        qs.load(a.Q + ((int64_t)b * a.Sq + i0) * a.ldq + (int64_t)head * a.dk, a.ldq, end, wave, lane, a.dk);
-        os.load(a.dO + ((int64_t)b * a.Sq + i0) * a.lddo + (int64_t)head * a.dk, a.lddo, end, wave, lane, a.dk);
+        qs.template load<PAD>(a.Q + ((int64_t)b * a.Sq + i0) * a.ldq + (int64_t)head * a.dk, a.ldq, end, wave, lane, a.dk);
+        os.template load<PAD>(a.dO + ((int64_t)b * a.Sq + i0) * a.lddo + (int64_t)head * a.dk, a.lddo, end, wave, lane, a.dk);
         if (threadIdx.x < ROWS) {
             const int i = i0 + threadIdx.x;
             r_row.end = 0;
@@ -454,9 +443,9 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
     float k_down, v_down;
     {
         float x[KS][8];
-        load_row(x, a.K + ((int64_t)b * a.kv_rows + key) * a.ldk + (int64_t)hk * a.dk, live, fhalf, a.dk);
+        load_row<PAD>(x, a.K + ((int64_t)b * a.kv_rows + key) * a.ldk + (int64_t)hk * a.dk, live, fhalf, a.dk);
         k_down = cut_row(x, kf);
-        load_row(x, a.V + ((int64_t)b * a.kv_rows + key) * a.ldv + (int64_t)hk * a.dk, live, fhalf, a.dk);
+        load_row<PAD>(x, a.V + ((int64_t)b * a.kv_rows + key) * a.ldv + (int64_t)hk * a.dk, live, fhalf, a.dk);
         v_down = cut_row(x, vf);
     }
     if (at.g < a.G) stage();
@@ -470,6 +459,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
     // acc_k is 2^(BIAS + d_up) times the sum of ds q, acc_v 2^(BIAS + p_up) times that of P dO: running exponents of ds and P times their rows' factors
     int d_up = MOST_UP, p_up = MOST_UP;
 
+    const unsigned row_at = B::row_place(lane), column_at = B::column_place(lane);
     auto attend = [&](int qt) {
         const v4i whole = *reinterpret_cast<const v4i *>(lds + G::TILE_AT + 16 * qt);
         const int t_last = __builtin_amdgcn_readfirstlane(whole[0]), t_sure = __builtin_amdgcn_readfirstlane(whole[1]);
@@ -480,17 +470,19 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
             if (t_high < d_low || t_low > d_high) return;
             partly = true;
         }
+        const unsigned char *tile = lds + 32 * qt * B::PITCH;
+        const unsigned row_place = afresh(row_at), column_place = afresh(column_at);
         v16f s, dp, slope;
 #pragma unroll
         for (int v = 0; v < 16; v++) s[v] = dp[v] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            const v4i qf[2] = {B::rows(lds, 32 * qt, k, lane, 0), B::rows(lds, 32 * qt, k, lane, 1)};
+            const v4i qf[2] = {B::rows(tile, row_place, 0, k, 0), B::rows(tile, row_place, 0, k, 1)};
             s = mfma_cut(qf, kf[k], s);
         }
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            const v4i of[2] = {B::rows(lds + B::BYTES, 32 * qt, k, lane, 0), B::rows(lds + B::BYTES, 32 * qt, k, lane, 1)};
+            const v4i of[2] = {B::rows(tile + B::BYTES, row_place, 0, k, 0), B::rows(tile + B::BYTES, row_place, 0, k, 1)};
             dp = mfma_cut(of, vf[k], dp);
         }
         const unsigned char *mine = lds + G::ROW_AT + 4 * (32 * qt + 4 * fhalf);     // rows 8 g + 0..3 from here: 16 bytes at 32 g
@@ -563,9 +555,9 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
             cut_result(dp, st, two_to(d_up), df);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const v4i of[2] = {B::columns(lds + B::BYTES, 32 * qt + 16 * st, d, lane, 0), B::columns(lds + B::BYTES, 32 * qt + 16 * st, d, lane, 1)};
+                const v4i of[2] = {B::columns(tile + B::BYTES, column_place, 16 * st, d, 0), B::columns(tile + B::BYTES, column_place, 16 * st, d, 1)};
                 acc_v[d] = mfma_cut(of, pf, acc_v[d]);
-                const v4i qf[2] = {B::columns(lds, 32 * qt + 16 * st, d, lane, 0), B::columns(lds, 32 * qt + 16 * st, d, lane, 1)};
+                const v4i qf[2] = {B::columns(tile, column_place, 16 * st, d, 0), B::columns(tile, column_place, 16 * st, d, 1)};
                 acc_k[d] = mfma_cut(qf, df, acc_k[d]);
             }
         }
@@ -641,7 +633,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
                     ok[e] = live ? acc_k[d][4 * g + e] : 0.0f;
                     ov[e] = live ? acc_v[d][4 * g + e] : 0.0f;
                 }
-                if (a.dk == DK || col < a.dk) {
+                if (!PAD || col < a.dk) {
                     *reinterpret_cast<v4f *>(dk + col) = ok;
                     *reinterpret_cast<v4f *>(dv + col) = ov;
                 }
@@ -661,29 +653,29 @@ int launch_tiles(Kernel kernel, int smem, const AttnArgs &a, BwdGrid grid, const
     return AXHIP_OK;
 }
 
-template <int DK>
+template <int DK, bool PAD>
 int launch_bwd(const AttnArgs &a, BwdGrid grid) {
     constexpr int SHARED_KEYS = 2 * DkvGeom<DK>::JOIN > DkvGeom<DK>::SMEM ? 2 * DkvGeom<DK>::JOIN : DkvGeom<DK>::SMEM;
     static bool attr_set = false;
     if (!attr_set) {
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_dq<DK>), hipFuncAttributeMaxDynamicSharedMemorySize, DqGeom<DK>::SMEM), "hipFuncSetAttribute");
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_dkv<DK, 4>), hipFuncAttributeMaxDynamicSharedMemorySize, DkvGeom<DK>::SMEM), "hipFuncSetAttribute");
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_dkv<DK, 2>), hipFuncAttributeMaxDynamicSharedMemorySize, SHARED_KEYS), "hipFuncSetAttribute");
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>((k_attn_dq<DK, PAD>)), hipFuncAttributeMaxDynamicSharedMemorySize, DqGeom<DK>::SMEM), "hipFuncSetAttribute");
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>((k_attn_dkv<DK, 4, PAD>)), hipFuncAttributeMaxDynamicSharedMemorySize, DkvGeom<DK>::SMEM), "hipFuncSetAttribute");
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>((k_attn_dkv<DK, 2, PAD>)), hipFuncAttributeMaxDynamicSharedMemorySize, SHARED_KEYS), "hipFuncSetAttribute");
         attr_set = true;
     }
     if (a.Sq > 0) {
         grid.units = (int64_t)a.B * a.H;
         grid.tiles = (a.Sq + 32 * WAVES - 1) / (32 * WAVES);
-        if (int rc = launch_tiles(k_attn_dq<DK>, DqGeom<DK>::SMEM, a, grid, "attn_bwd queries")) return rc;
+        if (int rc = launch_tiles(k_attn_dq<DK, PAD>, DqGeom<DK>::SMEM, a, grid, "attn_bwd queries")) return rc;
     }
     grid.units = (int64_t)a.B * a.Hkv;
     const int64_t wide = (a.Sk + 127) / 128 * grid.units;
     if (wide > 2 * cu_count()) {
         grid.tiles = (a.Sk + 127) / 128;
-        return launch_tiles(k_attn_dkv<DK, 4>, DkvGeom<DK>::SMEM, a, grid, "attn_bwd keys");
+        return launch_tiles(k_attn_dkv<DK, 4, PAD>, DkvGeom<DK>::SMEM, a, grid, "attn_bwd keys");
     }
     grid.tiles = (a.Sk + 63) / 64;
-    return launch_tiles(k_attn_dkv<DK, 2>, SHARED_KEYS, a, grid, "attn_bwd keys");
+    return launch_tiles(k_attn_dkv<DK, 2, PAD>, SHARED_KEYS, a, grid, "attn_bwd keys");
 }
 
 }  // namespace
@@ -709,10 +701,14 @@ int attn_bwd_tiles(AttnArgs &a) {
         if (int rc = doc_ranges(a.doc_q, a.B, a.Sq, ws + deltas + (size_t)a.B * grid.key_tiles * 8)) return rc;
     }
     note_kernel("attn_grad_tiles");
-    if (a.dk <= 32) return launch_bwd<32>(a, grid);
-    if (a.dk <= 64) return launch_bwd<64>(a, grid);
-    if (a.dk <= 96) return launch_bwd<96>(a, grid);
-    return launch_bwd<128>(a, grid);
+    auto run = [&](auto width) {
+        constexpr int DK = decltype(width)::value;
+        return a.dk < DK ? launch_bwd<DK, true>(a, grid) : launch_bwd<DK, false>(a, grid);
+    };
+    if (a.dk <= 32) return run(std::integral_constant<int, 32>());
+    if (a.dk <= 64) return run(std::integral_constant<int, 64>());
+    if (a.dk <= 96) return run(std::integral_constant<int, 96>());
+    return run(std::integral_constant<int, 128>());
 }
 
 }  // namespace axhip

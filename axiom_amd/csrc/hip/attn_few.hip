@@ -26,7 +26,7 @@ struct FewGeom {
     static constexpr int PART = PIECES * 64 * 4 + 64;            // floats that a range leaves in memory
 };
 
-template <int DK>
+template <int DK, bool PAD>
 __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(AttnArgs a, FewGrid grid) {
     using G = FewGeom<DK>;
     using B = typename G::B;
@@ -66,8 +66,8 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     auto load = [&](int t) {
         const int64_t k0 = (int64_t)t * 32;
         const int end = last - 1 - (int)k0;          // rows past it are read as it
-        ks.load(Kb + k0 * a.ldk, a.ldk, end, 0, lane, a.dk);
-        vs.load(Vb + k0 * a.ldv, a.ldv, end, 0, lane, a.dk);
+        ks.template load<PAD>(Kb + k0 * a.ldk, a.ldk, end, 0, lane, a.dk);
+        vs.template load<PAD>(Vb + k0 * a.ldv, a.ldv, end, 0, lane, a.dk);
         if (docs) doc_here = frow <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + frow] : -1;
     };
     int t = t_begin + wave;
@@ -77,16 +77,11 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     {
         const float *q = a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk;
         float x[KS][8];
+        load_row<PAD>(x, q, live, fhalf, a.dk);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int col = 16 * s + 8 * fhalf + 4 * h;
-                v4f v = {0.f, 0.f, 0.f, 0.f};
-                if (live && (a.dk == DK || col < a.dk)) v = *reinterpret_cast<const v4f *>(q + col);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[s][4 * h + e] = v[e] * a.q_up;
-            }
+            for (int e = 0; e < 8; e++) x[s][e] *= a.q_up;
         q_down = cut_row(x, qf);
     }
     v16f acc[DT];
@@ -97,6 +92,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     float m_run = ATTN_LOWEST, l_run = 0.0f;
     int p_up = MOST_UP;                              // acc is 2^(BIAS + p_up) times the sum: the running exponent of p times its value row's factor
 
+    const unsigned row_at = B::row_place(lane), column_at = B::column_place(lane);
     for (; t < t_end; t += WAVES) {
         const int kt0 = t * 32;
         bool partly = kt0 + 32 > sure, meets = true;
@@ -113,12 +109,13 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
         order_in_wave();
         if (t + WAVES < t_end) load(t + WAVES);
         if (!meets) continue;
+        const unsigned row_place = afresh(row_at), column_place = afresh(column_at);
         v16f s;
 #pragma unroll
         for (int v = 0; v < 16; v++) s[v] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            const v4i kf[2] = {B::rows(at, 0, k, lane, 0), B::rows(at, 0, k, lane, 1)};
+            const v4i kf[2] = {B::rows(at, row_place, 0, k, 0), B::rows(at, row_place, 0, k, 1)};
             s = mfma_cut(kf, qf[k], s);
         }
         auto factors = [&](int what, int g) { return *reinterpret_cast<const v4f *>(row_factors + what * 32 + 8 * g + 4 * fhalf); };
@@ -200,7 +197,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
             cut_result(s, st, two_to(p_up), pf);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const v4i vf[2] = {B::columns(at + B::BYTES, 16 * st, d, lane, 0), B::columns(at + B::BYTES, 16 * st, d, lane, 1)};
+                const v4i vf[2] = {B::columns(at + B::BYTES, column_place, 16 * st, d, 0), B::columns(at + B::BYTES, column_place, 16 * st, d, 1)};
                 acc[d] = mfma_cut(vf, pf, acc[d]);
             }
         }
@@ -298,7 +295,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
 #pragma unroll
         for (int n = 0; n < DT; n++) {
             const int col = 32 * n + 8 * wave + 4 * fhalf;
-            if (a.dk == DK || col < a.dk) *reinterpret_cast<v4f *>(o + col) = live ? out[n] * inv : v4f{0.f, 0.f, 0.f, 0.f};
+            if (!PAD || col < a.dk) *reinterpret_cast<v4f *>(o + col) = live ? out[n] * inv : v4f{0.f, 0.f, 0.f, 0.f};
         }
         if (a.L && wave == 0 && fhalf == 0) a.L[((int64_t)b * a.H + head) * a.Sq + i] = live ? (m_all + __builtin_amdgcn_logf(l_all)) * LN2 : -INFINITY;
     }
@@ -309,12 +306,12 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     }
 }
 
-template <int DK>
+template <int DK, bool PAD>
 int launch_few(const AttnArgs &a, FewGrid grid) {
     using G = FewGeom<DK>;
     static bool attr_set = false;
     if (!attr_set) {
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_few<DK>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>((k_attn_few<DK, PAD>)), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
         attr_set = true;
     }
     const int64_t units = (int64_t)a.B * a.Hkv * grid.row_tiles;
@@ -324,7 +321,7 @@ int launch_few(const AttnArgs &a, FewGrid grid) {
         if (!grid.parts || !grid.arrivals) return AXHIP_ERR_ALLOC;
     }
     note_kernel(grid.splits > 1 ? "attn_few_ranges" : "attn_few");
-    hipLaunchKernelGGL(k_attn_few<DK>, dim3((unsigned)(units * grid.splits)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
+    hipLaunchKernelGGL((k_attn_few<DK, PAD>), dim3((unsigned)(units * grid.splits)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
     return check_launch("attn_fwd");
 }
 
@@ -344,7 +341,12 @@ bool attn_fwd_few(const AttnArgs &a, int &rc) {
     if (splits > 64) splits = 64;
     if (splits < 1) splits = 1;
     grid.splits = (int)splits;
-    rc = a.dk <= 32 ? launch_few<32>(a, grid) : a.dk <= 64 ? launch_few<64>(a, grid) : a.dk <= 96 ? launch_few<96>(a, grid) : launch_few<128>(a, grid);
+    auto run = [&](auto width) {
+        constexpr int DK = decltype(width)::value;
+        return a.dk < DK ? launch_few<DK, true>(a, grid) : launch_few<DK, false>(a, grid);
+    };
+    rc = a.dk <= 32 ? run(std::integral_constant<int, 32>()) : a.dk <= 64 ? run(std::integral_constant<int, 64>()) : a.dk <= 96 ? run(std::integral_constant<int, 96>())
+                                                                                                                  : run(std::integral_constant<int, 128>());
     return true;
 }
 

@@ -25,12 +25,13 @@ struct FwdGeom {
     static constexpr int DOCS_AT = FACTORS_AT + BKV * 8;         // documents of the keys, then the ranges of their two tiles
     static constexpr int STAGE = DOCS_AT + BKV * 4 + 2 * 8;
     static constexpr int META_AT = (DOUBLE ? 2 : 1) * STAGE;     // a row of four ints a wave
+    static constexpr int PER_SIMD = DK >= 96 && WAVES == 4 ? 1 : 2;      // waves: with two, registers would go to memory
     static constexpr int SMEM = META_AT + 16 * WAVES;
     static_assert(STAGE % 16 == 0 && SMEM * (DOUBLE ? 1 : 2) <= 160 * 1024, "eight waves a CU");
 };
 
-template <int DK, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid grid) {
+template <int DK, int WAVES, bool PAD>
+__global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_attn_fwd(AttnArgs a, FwdGrid grid) {
     using G = FwdGeom<DK, WAVES>;
     using B = typename G::B;
     constexpr int KS = DK / 16, DT = DK / 32, BKV = G::BKV;
@@ -110,15 +111,17 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     auto load = [&](int blk) {
         const int64_t k0 = (int64_t)blk * BKV;
         const int end = wg_last - 1 - (int)k0;       // rows past it are read as it
-        ks.load(Kb + k0 * a.ldk, a.ldk, end, wave, lane, a.dk);
-        vs.load(Vb + k0 * a.ldv, a.ldv, end, wave, lane, a.dk);
+        const int l = (int)afresh(lane);
+        ks.template load<PAD>(Kb + k0 * a.ldk, a.ldk, end, wave, l, a.dk);
+        vs.template load<PAD>(Vb + k0 * a.ldv, a.ldv, end, wave, l, a.dk);
         if (docs && threadIdx.x < BKV) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
         if (docs && threadIdx.x < 2) range_here = 2 * blk + (int)threadIdx.x < grid.range_tiles ? ranges[2 * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
     };
     auto stage = [&](unsigned char *at) {
         float *factors = reinterpret_cast<float *>(at + G::FACTORS_AT);
-        ks.put(at, factors, wave, lane, 1.0f);
-        vs.put(at + B::BYTES, factors + BKV, wave, lane, 1.0f);
+        const int l = (int)afresh(lane);
+        ks.put(at, factors, wave, l, 1.0f);
+        vs.put(at + B::BYTES, factors + BKV, wave, l, 1.0f);
         if (docs && threadIdx.x < BKV) reinterpret_cast<int *>(at + G::DOCS_AT)[threadIdx.x] = doc_here;
         if (docs && threadIdx.x < 2) reinterpret_cast<DocRange *>(at + G::DOCS_AT + BKV * 4)[threadIdx.x] = range_here;
     };
@@ -130,16 +133,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     {
         const float *q = a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk;
         float x[KS][8];
+        load_row<PAD>(x, q, live, fhalf, a.dk);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int col = 16 * s + 8 * fhalf + 4 * h;
-                v4f v = {0.f, 0.f, 0.f, 0.f};
-                if (live && (a.dk == DK || col < a.dk)) v = *reinterpret_cast<const v4f *>(q + col);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[s][4 * h + e] = v[e] * a.q_up;
-            }
+            for (int e = 0; e < 8; e++) x[s][e] *= a.q_up;
         q_down = cut_row(x, qf);
     }
     if (blk < nblocks) {
@@ -157,6 +155,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     float m_run = ATTN_LOWEST, l_run = 0.0f;         // l_run: this lane half's share of the row sum
     int p_up = MOST_UP;                              // acc is 2^(BIAS + p_up) times the sum: the running exponent of p times its value row's factor
 
+    const unsigned row_at = B::row_place(lane), column_at = B::column_place(lane);
     auto attend = [&](int blk, const unsigned char *at) {
 #pragma unroll 1
         for (int kt = 0; kt < BKV / 32; kt++) {
@@ -169,6 +168,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 if (!here.meets(d_low, d_high)) continue;
                 partly |= here.low != here.high || here.low != d_low || d_low != d_high;
             }
+            const unsigned char *tile = at + 32 * kt * B::PITCH;
+            const unsigned row_place = afresh(row_at), column_place = afresh(column_at);
             // ---- scores ----
             v16f s;
 #pragma unroll
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
             __builtin_amdgcn_s_setprio(1);           // matrix phases go ahead of the co-resident wave's vector work
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const v4i kf[2] = {B::rows(at, 32 * kt, k, lane, 0), B::rows(at, 32 * kt, k, lane, 1)};
+                const v4i kf[2] = {B::rows(tile, row_place, 0, k, 0), B::rows(tile, row_place, 0, k, 1)};
                 s = mfma_cut(kf, qf[k], s);
             }
             __builtin_amdgcn_s_setprio(0);
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 cut_result(s, st, two_to(p_up), pf);
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
-                    const v4i vf[2] = {B::columns(at + B::BYTES, 32 * kt + 16 * st, d, lane, 0), B::columns(at + B::BYTES, 32 * kt + 16 * st, d, lane, 1)};
+                    const v4i vf[2] = {B::columns(tile + B::BYTES, column_place, 16 * st, d, 0), B::columns(tile + B::BYTES, column_place, 16 * st, d, 1)};
                     acc[d] = mfma_cut(vf, pf, acc[d]);
                 }
             }
@@ -337,13 +338,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 v4f out;
 #pragma unroll
                 for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * p_down * inv : 0.0f;
-                if (a.dk == DK || col < a.dk) *reinterpret_cast<v4f *>(o + col) = out;
+                if (!PAD || col < a.dk) *reinterpret_cast<v4f *>(o + col) = out;
             }
         if (a.L && fhalf == 0) a.L[((int64_t)b * a.H + head) * a.Sq + i] = live ? (m_run + __builtin_amdgcn_logf(l_tot)) * LN2 : -INFINITY;
     }
     for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) {
         const int n = __builtin_ctz(rest);
-        attn_fwd_row(a, b, __builtin_amdgcn_readlane(head, n), __builtin_amdgcn_readlane(i, n), lane);
+        attn_fwd_row(a, b, __builtin_amdgcn_readlane(head, n), __builtin_amdgcn_readlane(i, n), (int)afresh(lane));
     }
 }
 
@@ -365,12 +366,12 @@ __global__ void __launch_bounds__(256) k_doc_ranges(const int32_t *ids, int64_t 
     if ((threadIdx.x & 31) == 0) out[n] = high < 0 ? DocRange{0x7fffffff, -1} : DocRange{none ? ~low : low, high};
 }
 
-template <int DK, int WAVES>
+template <int DK, int WAVES, bool PAD>
 int launch_fwd(const AttnArgs &a, FwdGrid grid) {
     using G = FwdGeom<DK, WAVES>;
     static bool attr_set = false;
     if (!attr_set) {
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_fwd<DK, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_fwd<DK, WAVES, PAD>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
         attr_set = true;
     }
     grid.tiles = (int)(((int64_t)grid.pack * a.Sq + G::BQ - 1) / G::BQ);
@@ -378,10 +379,18 @@ int launch_fwd(const AttnArgs &a, FwdGrid grid) {
     note_kernel(WAVES == 8 ? "attn_tiles_w8" : "attn_tiles");
     for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
         const int64_t left = all - grid.first;
-        hipLaunchKernelGGL((k_attn_fwd<DK, WAVES>), dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
+        hipLaunchKernelGGL((k_attn_fwd<DK, WAVES, PAD>), dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
         if (int rc = check_launch("attn_fwd")) return rc;
     }
     return AXHIP_OK;
+}
+
+template <int DK>
+int launch_fwd(const AttnArgs &a, const FwdGrid &grid, bool eight) {
+    const bool pad = a.dk < DK;
+    if constexpr (DK > 32)
+        if (eight) return pad ? launch_fwd<DK, 8, true>(a, grid) : launch_fwd<DK, 8, false>(a, grid);
+    return pad ? launch_fwd<DK, 4, true>(a, grid) : launch_fwd<DK, 4, false>(a, grid);
 }
 
 }  // namespace
@@ -410,10 +419,10 @@ int attn_fwd_tiles(const AttnArgs &a) {
     }
     const int64_t rows = (int64_t)grid.pack * a.Sq, wide = (rows + 255) / 256 * grid.units;
     const bool eight = wide >= cu_count();
-    if (a.dk <= 32) return launch_fwd<32, 4>(a, grid);
-    if (a.dk <= 64) return eight ? launch_fwd<64, 8>(a, grid) : launch_fwd<64, 4>(a, grid);
-    if (a.dk <= 96) return eight ? launch_fwd<96, 8>(a, grid) : launch_fwd<96, 4>(a, grid);
-    return eight ? launch_fwd<128, 8>(a, grid) : launch_fwd<128, 4>(a, grid);
+    if (a.dk <= 32) return launch_fwd<32>(a, grid, eight);
+    if (a.dk <= 64) return launch_fwd<64>(a, grid, eight);
+    if (a.dk <= 96) return launch_fwd<96>(a, grid, eight);
+    return launch_fwd<128>(a, grid, eight);
 }
 
 }  // namespace axhip

@@ -16,18 +16,33 @@ struct Block {
         const int key = DK == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : DK == 64 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : (row >> 2) & 3;
         return (unsigned)(row * PITCH + ((chunk ^ key) << 4));
     }
-    // rows r0 .. r0 + 31 as the rows of an operand, columns 16 ks + 8 * half ..
-    __device__ static v4i rows(const unsigned char *base, int r0, int ks, int lane, int term) {
-        return *reinterpret_cast<const v4i *>(base + at(r0 + (lane & 31), 2 * ks + (lane >> 5)) + term * PLANE);
+    // A lane's place for rows(): row (lane & 31), chunk (lane >> 5); and for columns(): see read_columns.  Other rows and chunks are a distance and an exchange
+    // of bits away (the bits of MASK are those that rows leave free), so a lane holds two addresses and not one for every fragment.
+    static constexpr unsigned MASK = DK == 96 ? 63 : PITCH - 1;
+    __device__ static unsigned row_place(int lane) { return at(lane & 31, lane >> 5); }
+    __device__ static unsigned column_place(int lane) {
+        const int l = lane & 15;
+        return at(4 * (lane >> 5) + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) + 8 * (l & 1);
     }
-    // columns 32 d .. 32 d + 31 as the rows of an operand; its eight k are rows r0 + 4 * half + 0..3 and 8 more on: those that registers 8 s .. 8 s + 7
-    // of a result tile hold
-    __device__ static v4i columns(const unsigned char *base, int r0, int d, int lane, int term) {
-        const int l = lane & 15, row = r0 + 4 * (lane >> 5) + (l >> 2), chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1);
-        const v2i32 a = read_columns(base + at(row, chunk) + 8 * (l & 1) + term * PLANE), b = read_columns(base + at(row + 8, chunk) + 8 * (l & 1) + term * PLANE);
+    __device__ static unsigned moved(unsigned place, unsigned by) { return (place ^ (by & MASK)) + (by & ~MASK); }
+    // rows r0 .. r0 + 31 as the rows of an operand, columns 16 k + 8 * half ..
+    __device__ static v4i rows(const unsigned char *base, unsigned place, int r0, int k, int term) {
+        return *reinterpret_cast<const v4i *>(base + moved(place, 32 * k) + r0 * PITCH + term * PLANE);
+    }
+    // columns 32 d .. 32 d + 31 as the rows of an operand; its eight k are rows r0 + 4 * half + 0..3 and 8 more on (r0 a multiple of 16): those that registers
+    // 8 s .. 8 s + 7 of a result tile hold
+    __device__ static v4i columns(const unsigned char *base, unsigned place, int r0, int d, int term) {
+        const unsigned near = moved(place, 64 * d);
+        const v2i32 a = read_columns(base + near + r0 * PITCH + term * PLANE), b = read_columns(base + (near ^ 32) + (r0 + 8) * PITCH + term * PLANE);
         return v4i{a[0], a[1], b[0], b[1]};
     }
 };
+
+// A value that the compiler may not carry through a loop in other forms
+__device__ __forceinline__ unsigned afresh(unsigned v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 // How the waves of a workgroup bring a block from memory: wave w rows RPW w .. RPW w + RPW - 1, eight columns a lane and piece, LANES lanes a row.
 template <int DK, int ROWS, int WAVES>
@@ -37,7 +52,8 @@ struct Stage {
     using B = Block<DK, ROWS>;
     float x[PIECES][8];
     __device__ static int row_of(int piece, int wave, int lane) { return wave * RPW + piece * (64 / LANES) + lane / LANES; }
-    // row r of the block is at base + min(r, last) * pitch; columns from dk on are zero
+    // row r of the block is at base + min(r, last) * pitch.  PAD: the head is dk < DK columns wide, those from dk on are zero
+    template <bool PAD>
     __device__ __forceinline__ void load(const float *base, int64_t pitch, int last, int wave, int lane, int dk) {
         const int col = lane % LANES * 8;
 #pragma unroll
@@ -46,10 +62,10 @@ struct Stage {
             const float *p = base + (int64_t)(row < last ? row : last) * pitch + col;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                v4f a = {0.f, 0.f, 0.f, 0.f};
-                if ((dk == DK && DK == 8 * LANES) || col + 4 * h < dk) a = *reinterpret_cast<const v4f *>(p + 4 * h);
+                const bool in = !(PAD || DK != 8 * LANES) || col + 4 * h < dk;       // (other lanes read column 0 on)
+                const v4f a = *reinterpret_cast<const v4f *>(in ? p + 4 * h : p - col);
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[i][4 * h + e] = a[e];
+                for (int e = 0; e < 4; e++) x[i][4 * h + e] = in ? a[e] : 0.0f;
             }
         }
     }
@@ -77,6 +93,21 @@ struct Stage {
         }
     }
 };
+
+// A lane's half of a row: columns 16 s + 8 * half .. + 7 for step s.  Rows that are not live are zero, and not read.
+template <bool PAD, int KS>
+__device__ __forceinline__ void load_row(float (&x)[KS][8], const float *row, bool live, int fhalf, int dk) {
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int col = 16 * s + 8 * fhalf + 4 * h;
+            v4f v = {0.f, 0.f, 0.f, 0.f};
+            if (live && (!PAD || col < dk)) v = *reinterpret_cast<const v4f *>(row + col);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[s][4 * h + e] = v[e];
+        }
+}
 
 // The documents of 32 keys (or rows): the lowest and highest id there, -1 and below not counted; `low` is ~lowest where some are not
 // counted, so that one document all over is low == high.  No id at all: (INT_MAX, -1).
