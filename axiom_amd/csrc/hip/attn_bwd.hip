@@ -86,7 +86,7 @@ struct DqGeom {
     static constexpr int DOCS_AT = FACTORS_AT + ROWS * 8;
     static constexpr int META_AT = DOCS_AT + ROWS * 4 + 2 * 8;
     static constexpr int SMEM = META_AT + 16 * WAVES;
-    static constexpr int PER_SIMD = DK <= 64 ? 2 : 1;
+    static constexpr int PER_SIMD = DK <= 32 ? 2 : 1;
 };
 
 template <int DK, bool PAD>
@@ -189,8 +189,10 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
 #pragma unroll
         for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
     int d_up = MOST_UP;                              // acc is 2^(BIAS + d_up) times the sum: the running exponent of ds times its key row's factor
+    float o_times = o_down * two_to(d_up), delta_times = delta * two_to(d_up);
+    const float one = hidden_one();
 
-    const unsigned row_at = B::row_place(lane), column_at = B::column_place(lane);
+    const unsigned row_at = B::row_place(lane) + lds_address(lds), column_at = B::column_place(lane) + lds_address(lds);
     auto attend = [&](int blk) {
 #pragma unroll 1
         for (int kt = 0; kt < 2; kt++) {
@@ -203,21 +205,19 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
                 if (!here.meets(d_low, d_high)) continue;
                 partly |= here.low != here.high || here.low != d_low || d_low != d_high;
             }
-            const unsigned char *tile = lds + 32 * kt * B::PITCH;
-            const unsigned row_place = afresh(row_at), column_place = afresh(column_at);
+            const unsigned row_place = afresh(row_at) + 32 * kt * B::PITCH, column_place = afresh(column_at) + 32 * kt * B::PITCH;
             v16f s, dp, slope;
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = dp[v] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const v4i kf[2] = {B::rows(tile, row_place, 0, k, 0), B::rows(tile, row_place, 0, k, 1)};
-                s = mfma_cut(kf, qf[k], s);
-            }
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const v4i vf[2] = {B::rows(tile + B::BYTES, row_place, 0, k, 0), B::rows(tile + B::BYTES, row_place, 0, k, 1)};
-                dp = mfma_cut(vf, of[k], dp);
-            }
+            products<2 * KS>(
+                [&](int n, v4i (&f)[2]) {
+                    f[1] = B::rows(row_place + n / KS * B::BYTES, n % KS, 1);
+                    f[0] = B::rows(row_place + n / KS * B::BYTES, n % KS, 0);
+                },
+                [&](int n, const v4i (&f)[2]) {
+                    if (n < KS) s = mfma_cut(f, qf[n % KS], s);
+                    else dp = mfma_cut(f, of[n % KS], dp);
+                });
             auto factors = [&](int what, int g) {    // of keys 8 g + 4 * half + 0..3 of the tile
                 return *reinterpret_cast<const v4f *>(lds + G::FACTORS_AT + what * ROWS * 4 + 4 * (32 * kt + 8 * g + 4 * fhalf));
             };
@@ -244,36 +244,49 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
                     }
                 }
             }
-            float most = 0.0f;
+            // ds times its key row's factor and 2^d_up, which is in o_times and delta_times
+            v16f x;
+            float most;
+            auto form = [&]() {
+                most = 0.0f;
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const v4f kf = factors(0, g), vf = factors(1, g);
+                for (int g = 0; g < 4; g++) {
+                    const v4f kf = factors(0, g), vf = factors(1, g);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int v = 4 * g + e;
-                    const float p = __builtin_amdgcn_exp2f(s[v] - lse2);
-                    s[v] = p * __builtin_fmaf(dp[v] * vf[e], o_down, -delta);
-                    if (a.cap2 > 0.0f) s[v] *= slope[v];
-                    s[v] *= kf[e];
-                    most = fmaxf(most, __builtin_fabsf(s[v]));
+                    for (int e = 0; e < 4; e++) {
+                        const int v = 4 * g + e;
+                        x[v] = __builtin_amdgcn_exp2f(s[v] - lse2) * __builtin_fmaf(dp[v] * vf[e], o_times, -delta_times);
+                        if (a.cap2 > 0.0f) x[v] *= slope[v];
+                        x[v] *= kf[e];
+                        most = fmaxf(most, __builtin_fabsf(x[v]));
+                    }
                 }
+                most = fmaxf(most, __shfl_xor(most, 32, 64));
+            };
+            form();
+            if (__builtin_amdgcn_ballot_w64(most > ROOM)) {      // (always for the first that are not zero)
+                const int before = d_up;
+                const bool over = most > ROOM;
+                if (over) d_up -= MOST_UP;                       // a scale at which they are floats, then the right one
+                o_times = o_down * two_to(d_up);
+                delta_times = delta * two_to(d_up);
+                form();
+                if (over) d_up += LARGEST - __builtin_amdgcn_frexp_expf(most);
+                if (d_up > MOST_UP) d_up = MOST_UP;
+                o_times = o_down * two_to(d_up);
+                delta_times = delta * two_to(d_up);
+                times(acc, two_to(d_up - before));
+                form();
             }
-            most = fmaxf(most, __shfl_xor(most, 32, 64));
-            if (__builtin_amdgcn_ballot_w64(outgrown(most, d_up))) {
-                const int grown = regrown(most, d_up);
-                times(acc, two_to(grown - d_up));
-                d_up = grown;
-            }
-#pragma unroll
-            for (int st = 0; st < 2; st++) {
-                v4i df[2];
-                cut_result(s, st, two_to(d_up), df);
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const v4i kf[2] = {B::columns(tile, column_place, 16 * st, d, 0), B::columns(tile, column_place, 16 * st, d, 1)};
-                    acc[d] = mfma_cut(kf, df, acc[d]);
-                }
-            }
+            v4i df[2][2];
+            cut_scaled(x, 0, one, df[0]);
+            cut_scaled(x, 1, one, df[1]);
+            products<2 * DT>(
+                [&](int n, v4i (&f)[2]) {
+                    f[1] = B::columns(column_place, 16 * (n / DT), n % DT, 1);
+                    f[0] = B::columns(column_place, 16 * (n / DT), n % DT, 0);
+                },
+                [&](int n, const v4i (&f)[2]) { acc[n % DT] = mfma_cut(f, df[n / DT], acc[n % DT]); });
         }
     };
     while (blk < blocks.n) {
@@ -321,7 +334,7 @@ struct DkvGeom {
     static constexpr int ROW_AT = 2 * B::BYTES;                  // of each row: factors of Q and dO, lse, delta, slope (floats), end, position, document (ints)
     static constexpr int TILE_AT = ROW_AT + ROWS * 32;           // of each 32 rows: last end, first end, range of documents
     static constexpr int SMEM = TILE_AT + 2 * 16;
-    static constexpr int PER_SIMD = DK <= 64 ? 2 : 1;
+    static constexpr int PER_SIMD = DK <= 32 ? 2 : 1;
     // the sums of the waves that share keys: [2 DT][64 lanes][16]
     static constexpr int JOIN = 2 * (DK / 32) * 64 * 64;
 };
@@ -459,7 +472,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
     // acc_k is 2^(BIAS + d_up) times the sum of ds q, acc_v 2^(BIAS + p_up) times that of P dO: running exponents of ds and P times their rows' factors
     int d_up = MOST_UP, p_up = MOST_UP;
 
-    const unsigned row_at = B::row_place(lane), column_at = B::column_place(lane);
+    const unsigned row_at = B::row_place(lane) + lds_address(lds), column_at = B::column_place(lane) + lds_address(lds);
     auto attend = [&](int qt) {
         const v4i whole = *reinterpret_cast<const v4i *>(lds + G::TILE_AT + 16 * qt);
         const int t_last = __builtin_amdgcn_readfirstlane(whole[0]), t_sure = __builtin_amdgcn_readfirstlane(whole[1]);
@@ -470,21 +483,19 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
             if (t_high < d_low || t_low > d_high) return;
             partly = true;
         }
-        const unsigned char *tile = lds + 32 * qt * B::PITCH;
-        const unsigned row_place = afresh(row_at), column_place = afresh(column_at);
+        const unsigned row_place = afresh(row_at) + 32 * qt * B::PITCH, column_place = afresh(column_at) + 32 * qt * B::PITCH;
         v16f s, dp, slope;
 #pragma unroll
         for (int v = 0; v < 16; v++) s[v] = dp[v] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const v4i qf[2] = {B::rows(tile, row_place, 0, k, 0), B::rows(tile, row_place, 0, k, 1)};
-            s = mfma_cut(qf, kf[k], s);
-        }
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const v4i of[2] = {B::rows(tile + B::BYTES, row_place, 0, k, 0), B::rows(tile + B::BYTES, row_place, 0, k, 1)};
-            dp = mfma_cut(of, vf[k], dp);
-        }
+        products<2 * KS>(
+            [&](int n, v4i (&f)[2]) {
+                f[1] = B::rows(row_place + n / KS * B::BYTES, n % KS, 1);
+                f[0] = B::rows(row_place + n / KS * B::BYTES, n % KS, 0);
+            },
+            [&](int n, const v4i (&f)[2]) {
+                if (n < KS) s = mfma_cut(f, kf[n % KS], s);
+                else dp = mfma_cut(f, vf[n % KS], dp);
+            });
         const unsigned char *mine = lds + G::ROW_AT + 4 * (32 * qt + 4 * fhalf);     // rows 8 g + 0..3 from here: 16 bytes at 32 g
         auto of_rows = [&](int what, int g) { return *reinterpret_cast<const v4i *>(mine + what * ROWS * 4 + 32 * g); };
         auto floats = [&](int what, int g) { return __builtin_bit_cast(v4f, of_rows(what, g)); };
@@ -548,19 +559,22 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
             times(acc_v, two_to(grown - p_up));
             p_up = grown;
         }
+        v4i pf[2][2], df[2][2];
 #pragma unroll
         for (int st = 0; st < 2; st++) {
-            v4i pf[2], df[2];
-            cut_result(s, st, two_to(p_up), pf);
-            cut_result(dp, st, two_to(d_up), df);
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const v4i of[2] = {B::columns(tile + B::BYTES, column_place, 16 * st, d, 0), B::columns(tile + B::BYTES, column_place, 16 * st, d, 1)};
-                acc_v[d] = mfma_cut(of, pf, acc_v[d]);
-                const v4i qf[2] = {B::columns(tile, column_place, 16 * st, d, 0), B::columns(tile, column_place, 16 * st, d, 1)};
-                acc_k[d] = mfma_cut(qf, df, acc_k[d]);
-            }
+            cut_result(s, st, two_to(p_up), pf[st]);
+            cut_result(dp, st, two_to(d_up), df[st]);
         }
+        products<4 * DT>(
+            [&](int n, v4i (&f)[2]) {
+                const unsigned at = column_place + (n < 2 * DT ? B::BYTES : 0);
+                f[1] = B::columns(at, 16 * (n / DT % 2), n % DT, 1);
+                f[0] = B::columns(at, 16 * (n / DT % 2), n % DT, 0);
+            },
+            [&](int n, const v4i (&f)[2]) {
+                if (n < 2 * DT) acc_v[n % DT] = mfma_cut(f, pf[n / DT % 2], acc_v[n % DT]);
+                else acc_k[n % DT] = mfma_cut(f, df[n / DT % 2], acc_k[n % DT]);
+            });
     };
     while (at.g < a.G) {
         const Place ahead = settle({at.g, at.blk + 1});

@@ -17,12 +17,12 @@ template <int DK>
 struct FewGeom {
     using B = Block<DK, 32>;
     static constexpr int DT = DK / 32, PIECES = 4 * DT;          // a lane's output in pieces of four
-    static constexpr int FACTORS_AT = 2 * B::BYTES, DOCS_AT = FACTORS_AT + 256, BLOCK = DOCS_AT + 128;
+    static constexpr int FACTORS_AT = 2 * B::BYTES, DOCS_AT = FACTORS_AT + 256, BLOCK = DOCS_AT + 256;
     static constexpr int JOIN_AT = 0, ML_AT = WAVES * PIECES * 1024;   // of the waves: pieces [64] v4f, then maxima and sums [2][32]
     static constexpr int BLOCKS = WAVES * BLOCK, JOINED = ML_AT + WAVES * 256;
     static constexpr int FLAGS_AT = BLOCKS > JOINED ? BLOCKS : JOINED;   // a word a wave: the rows whose sums are not finite; then who is last
     static constexpr int SMEM = FLAGS_AT + 4 * WAVES + 16;
-    static_assert(BLOCK % 16 == 0 && SMEM <= 160 * 1024, "LDS");
+    static_assert(BLOCK % 256 == 0 && SMEM <= 160 * 1024, "LDS");
     static constexpr int PART = PIECES * 64 * 4 + 64;            // floats that a range leaves in memory
 };
 
@@ -89,10 +89,10 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
-    float m_run = ATTN_LOWEST, l_run = 0.0f;
-    int p_up = MOST_UP;                              // acc is 2^(BIAS + p_up) times the sum: the running exponent of p times its value row's factor
+    float ref = ATTN_LOWEST, l_run = 0.0f;           // as in the tile kernel: acc is 2^BIAS times the sum
+    const float one = hidden_one();
 
-    const unsigned row_at = B::row_place(lane), column_at = B::column_place(lane);
+    const unsigned row_at = B::row_place(lane) + lds_address(at), column_at = B::column_place(lane) + lds_address(at) + B::BYTES;
     for (; t < t_end; t += WAVES) {
         const int kt0 = t * 32;
         bool partly = kt0 + 32 > sure, meets = true;
@@ -113,11 +113,12 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
         v16f s;
 #pragma unroll
         for (int v = 0; v < 16; v++) s[v] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const v4i kf[2] = {B::rows(at, row_place, 0, k, 0), B::rows(at, row_place, 0, k, 1)};
-            s = mfma_cut(kf, qf[k], s);
-        }
+        products<KS>(
+            [&](int k, v4i (&f)[2]) {
+                f[1] = B::rows(row_place, k, 1);
+                f[0] = B::rows(row_place, k, 0);
+            },
+            [&](int k, const v4i (&f)[2]) { s = mfma_cut(f, qf[k], s); });
         auto factors = [&](int what, int g) { return *reinterpret_cast<const v4f *>(row_factors + what * 32 + 8 * g + 4 * fhalf); };
 #pragma unroll
         for (int g = 0; g < 4; g++) {
@@ -155,66 +156,67 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
                         if (d[e] != row.doc) s[4 * g + e] = -INFINITY;
                 }
         }
-        float m_blk = s[0];
+        v16f x;
+        float most, l_blk;
+        auto weigh = [&]() {
+            most = l_blk = 0.0f;
 #pragma unroll
-        for (int v = 1; v < 16; v++) m_blk = fmaxf(m_blk, s[v]);
-        m_blk = fmaxf(m_blk, __shfl_xor(m_blk, 32, 64));
-        if (__builtin_amdgcn_ballot_w64(m_blk > m_run + 8.0f)) {
-            const float m_new = fmaxf(m_run, m_blk), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            for (int g = 0; g < 4; g++) {
+                const v4f f = factors(1, g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int v = 4 * g + e;
+                    const float p = __builtin_amdgcn_exp2f(s[v] - ref);
+                    l_blk += p;
+                    x[v] = p * f[e];
+                    most = fmaxf(most, x[v]);
+                }
+            }
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+        };
+        weigh();
+        if (__builtin_amdgcn_ballot_w64(most > ROOM)) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const v4f f = factors(1, g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = fmaxf(top, s[4 * g + e] + __builtin_amdgcn_logf(f[e]));
+            }
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) - (float)LARGEST;
+            const float next = most > ROOM ? fmaxf(ref, top) : ref, alpha = __builtin_amdgcn_exp2f(ref - next);
+            ref = next;
             l_run *= alpha;
-            m_run = m_new;
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) acc[d][v] *= alpha;
-        }
-        float l_blk = 0.0f, most = 0.0f;
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const v4f f = factors(1, g);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float p = __builtin_amdgcn_exp2f(s[4 * g + e] - m_run);
-                l_blk += p;
-                s[4 * g + e] = p * f[e];
-                most = fmaxf(most, s[4 * g + e]);
-            }
+            weigh();
         }
         l_run += l_blk;
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        if (__builtin_amdgcn_ballot_w64(outgrown(most, p_up))) {
-            const int grown = regrown(most, p_up);
-            const float by = two_to(grown - p_up);
-            p_up = grown;
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) acc[d][v] *= by;
-        }
-#pragma unroll
-        for (int st = 0; st < 2; st++) {
-            v4i pf[2];
-            cut_result(s, st, two_to(p_up), pf);
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const v4i vf[2] = {B::columns(at + B::BYTES, column_place, 16 * st, d, 0), B::columns(at + B::BYTES, column_place, 16 * st, d, 1)};
-                acc[d] = mfma_cut(vf, pf, acc[d]);
-            }
-        }
+        v4i pf[2][2];
+        cut_scaled(x, 0, one, pf[0]);
+        cut_scaled(x, 1, one, pf[1]);
+        products<2 * DT>(
+            [&](int n, v4i (&f)[2]) {
+                f[1] = B::columns(column_place, 16 * (n / DT), n % DT, 1);
+                f[0] = B::columns(column_place, 16 * (n / DT), n % DT, 0);
+            },
+            [&](int n, const v4i (&f)[2]) { acc[n % DT] = mfma_cut(f, pf[n / DT], acc[n % DT]); });
     }
 
     // ---- the waves' parts together ----
     __syncthreads();                                 // the blocks have been read
     v4f *const part = reinterpret_cast<v4f *>(lds + G::JOIN_AT);
     float *const ml = reinterpret_cast<float *>(lds + G::ML_AT);
-    const float p_down = two_to(-p_up - BIAS), l_wave = l_run + __shfl_xor(l_run, 32, 64);
+    const float l_wave = l_run + __shfl_xor(l_run, 32, 64);
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int g = 0; g < 4; g++)
-            part[(wave * PIECES + 4 * d + g) * 64 + lane] = v4f{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]} * p_down;
+            part[(wave * PIECES + 4 * d + g) * 64 + lane] = v4f{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]} * two_to(-BIAS);
     if (fhalf == 0) {
-        ml[wave * 64 + frow] = m_run;
+        ml[wave * 64 + frow] = ref;
         ml[wave * 64 + 32 + frow] = l_wave;
     }
     __syncthreads();

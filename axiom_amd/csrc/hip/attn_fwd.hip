@@ -1,49 +1,55 @@
 // Attention forward under score rules: tiles of queries on the f16 matrix core.
 //
-// A workgroup of four or eight waves owns 128 or 256 rows of queries, a wave 32 of them; the rows are those of one query head, or, where a head has
-// few, of all heads that share keys, one after the other.  Keys and values stream through LDS in blocks of 64, cut into f16 terms on the way (f16x2.h; a
-// query's row once, a probability when it is used).  As in plain attention (sdpa.hip) a lane owns query (l & 31) in the score tile and in the output:
+// A workgroup of eight waves owns 256 rows of queries, a wave 32 of them, or 128, two waves 32 of them and half of the keys each; the rows are those of one query head, or,
+// where a head has few, of all heads that share keys, one after the other.  Keys and values stream through LDS in blocks of 64 (128 of narrow heads), cut into f16 terms on the
+// way (f16x2.h; a query's row once, a probability when it is used).  As in plain attention (sdpa.hip) a lane owns query (l & 31) in the score tile and in the output:
 //   S^T tile   A = keys' rows, B = the wave's queries; register v of a lane is key 8 (v >> 2) + 4 (l >> 5) + (v & 3)
-//   softmax    online, in log2 units; the reference point moves only when a maximum exceeds it by 2^8
+//   softmax    online, in log2 units; the reference point moves only when a probability times its value row's factor no longer fits an operand
 //   O^T tile   A = V^T, read from the rows by transposing LDS reads, B = the probabilities where the score tile left them
 // What a query sees is the keys before `end` that have its document (AttnRow).  Blocks that no row of the workgroup sees are not fetched, 32-key tiles that no row of a
 // wave sees not computed, and only tiles that some row sees in part pay for the mask; with documents the ranges of ids of each 32 keys, formed by a first
 // launch, decide that.  A row whose sums are not finite (infinities or NaNs that it sees, or that a masked key of a tile holds) is formed again with fp32
 // instructions by its wave.
+#include <algorithm>
+
 #include "attn_launch.h"
 #include "attn_tiles.h"
 
 namespace {
 using namespace axhip;
 
-template <int DK, int WAVES>
+constexpr int WAVES = 8;
+
+// SETS waves side by side along the queries, 32 each; with four, the others take the other half of each block's keys
+template <int DK, int SETS>
 struct FwdGeom {
-    static constexpr int BQ = 32 * WAVES, BKV = 64;
+    static constexpr int BQ = 32 * SETS, BKV = DK == 32 ? 128 : 64, SHARES = WAVES / SETS;
     using B = Block<DK, BKV>;
-    static constexpr bool DOUBLE = WAVES == 8;   // two blocks in LDS, or two workgroups a CU
     static constexpr int FACTORS_AT = 2 * B::BYTES;              // of each key row, then of each value row
-    static constexpr int DOCS_AT = FACTORS_AT + BKV * 8;         // documents of the keys, then the ranges of their two tiles
-    static constexpr int STAGE = DOCS_AT + BKV * 4 + 2 * 8;
-    static constexpr int META_AT = (DOUBLE ? 2 : 1) * STAGE;     // a row of four ints a wave
-    static constexpr int PER_SIMD = DK >= 96 && WAVES == 4 ? 1 : 2;      // waves: with two, registers would go to memory
+    static constexpr int DOCS_AT = FACTORS_AT + BKV * 8;         // documents of the keys, then the ranges of their tiles
+    static constexpr int STAGE = (DOCS_AT + BKV * 4 + BKV / 32 * 8 + 255) / 256 * 256;
+    static constexpr int META_AT = 2 * STAGE;                    // a row of four ints a wave
+    // the other share's sums: a wave's pieces [64] v4f, then maxima and sums [2][32]
+    static constexpr int PART = DK / 8 * 1024 + 256;
     static constexpr int SMEM = META_AT + 16 * WAVES;
-    static_assert(STAGE % 16 == 0 && SMEM * (DOUBLE ? 1 : 2) <= 160 * 1024, "eight waves a CU");
+    static_assert(SMEM <= 160 * 1024 && (SHARES == 1 || SETS * PART <= META_AT), "LDS");
 };
 
-template <int DK, int WAVES, bool PAD>
-__global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_attn_fwd(AttnArgs a, FwdGrid grid) {
-    using G = FwdGeom<DK, WAVES>;
+template <int DK, int SETS, bool PAD>
+__global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid grid) {
+    using G = FwdGeom<DK, SETS>;
     using B = typename G::B;
-    constexpr int KS = DK / 16, DT = DK / 32, BKV = G::BKV;
+    constexpr int KS = DK / 16, DT = DK / 32, BKV = G::BKV, TILES = BKV / 32;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
 
-    // Eight units (heads, or groups of heads) go to the eight XCDs in turn; a unit's tiles to one, causal ones from the last, the longest, on.
+    // Workgroups go to the eight XCDs in turn.  A unit's tiles (a head's, or a group of heads') go to one: eight units at a time, or, causal, the last and longest tile of every
+    // unit first, so that the short ones fill up what the long ones leave.
     const int64_t lin = grid.first + blockIdx.x, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
-    const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8, unit = group * 8 + r8 % width;
-    const int tile = a.causal ? grid.tiles - 1 - (int)(r8 / width) : (int)(r8 / width);
+    const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8, unit = a.causal ? lin % grid.units : group * 8 + r8 % width;
+    const int tile = a.causal ? grid.tiles - 1 - (int)(lin / grid.units) : (int)(r8 / width);
     const int per_b = a.H / grid.pack, b = (int)(unit / per_b), h0 = (int)(unit - (int64_t)b * per_b) * grid.pack, hk = h0 / a.G;
-    const int rows = grid.pack * a.Sq, r = tile * G::BQ + wave * 32 + frow;
+    const int rows = grid.pack * a.Sq, r = tile * G::BQ + wave % SETS * 32 + frow;
     const bool valid = r < rows;
     const int over = grid.pack == 1 ? 0 : (valid ? r : rows - 1) / a.Sq, head = h0 + over, i = (valid ? r : rows - 1) - over * a.Sq;
     AttnRow row = attn_row(a, b, head, i);
@@ -92,8 +98,9 @@ __global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_
                 const int mine = window_at + lane;
                 bool meets = false;
                 if (mine < nblocks) {
-                    meets = ranges[2 * mine].meets(wg_low, wg_high);
-                    if (2 * mine + 1 < grid.range_tiles) meets |= ranges[2 * mine + 1].meets(wg_low, wg_high);
+#pragma unroll
+                    for (int kt = 0; kt < TILES; kt++)
+                        if (TILES * mine + kt < grid.range_tiles) meets |= ranges[TILES * mine + kt].meets(wg_low, wg_high);
                 }
                 window = __builtin_amdgcn_ballot_w64(meets);
             }
@@ -115,7 +122,7 @@ __global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_
         ks.template load<PAD>(Kb + k0 * a.ldk, a.ldk, end, wave, l, a.dk);
         vs.template load<PAD>(Vb + k0 * a.ldv, a.ldv, end, wave, l, a.dk);
         if (docs && threadIdx.x < BKV) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
-        if (docs && threadIdx.x < 2) range_here = 2 * blk + (int)threadIdx.x < grid.range_tiles ? ranges[2 * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
+        if (docs && threadIdx.x < TILES) range_here = TILES * blk + (int)threadIdx.x < grid.range_tiles ? ranges[TILES * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
     };
     auto stage = [&](unsigned char *at) {
         float *factors = reinterpret_cast<float *>(at + G::FACTORS_AT);
@@ -123,7 +130,7 @@ __global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_
         ks.put(at, factors, wave, l, 1.0f);
         vs.put(at + B::BYTES, factors + BKV, wave, l, 1.0f);
         if (docs && threadIdx.x < BKV) reinterpret_cast<int *>(at + G::DOCS_AT)[threadIdx.x] = doc_here;
-        if (docs && threadIdx.x < 2) reinterpret_cast<DocRange *>(at + G::DOCS_AT + BKV * 4)[threadIdx.x] = range_here;
+        if (docs && threadIdx.x < TILES) reinterpret_cast<DocRange *>(at + G::DOCS_AT + BKV * 4)[threadIdx.x] = range_here;
     };
 
     int blk = next(0), ahead = nblocks;
@@ -143,7 +150,7 @@ __global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_
     if (blk < nblocks) {
         stage(lds);
         ahead = next(blk + 1);
-        if (G::DOUBLE && ahead < nblocks) load(ahead);
+        if (ahead < nblocks) load(ahead);
     }
     __syncthreads();
 
@@ -152,13 +159,16 @@ __global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
-    float m_run = ATTN_LOWEST, l_run = 0.0f;         // l_run: this lane half's share of the row sum
-    int p_up = MOST_UP;                              // acc is 2^(BIAS + p_up) times the sum: the running exponent of p times its value row's factor
+    // Probabilities are 2^(x - ref), l_run this lane half's share of their sum, acc 2^BIAS times that of their products.  The running reference keeps not the probabilities but
+    // their products with the factors of the value rows, which go to the matrix core, below ROOM.
+    float ref = ATTN_LOWEST, l_run = 0.0f;
+    const float one = hidden_one();
 
-    const unsigned row_at = B::row_place(lane), column_at = B::column_place(lane);
-    auto attend = [&](int blk, const unsigned char *at) {
+    const unsigned row_at = B::row_place(lane) + lds_address(lds), column_at = B::column_place(lane) + lds_address(lds) + B::BYTES;
+    auto attend = [&](int blk, unsigned cur) {
+        const unsigned char *at = lds + cur;
 #pragma unroll 1
-        for (int kt = 0; kt < BKV / 32; kt++) {
+        for (int kt = wave / SETS; kt < TILES; kt += G::SHARES) {
             const int kt0 = blk * BKV + 32 * kt;
             if (kt0 >= last) break;
             bool partly = kt0 + 32 > sure;
@@ -168,18 +178,18 @@ __global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_
                 if (!here.meets(d_low, d_high)) continue;
                 partly |= here.low != here.high || here.low != d_low || d_low != d_high;
             }
-            const unsigned char *tile = at + 32 * kt * B::PITCH;
-            const unsigned row_place = afresh(row_at), column_place = afresh(column_at);
+            const unsigned tile_at = cur + 32 * kt * B::PITCH, row_place = afresh(row_at) + tile_at, column_place = afresh(column_at) + tile_at;
             // ---- scores ----
             v16f s;
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = 0.0f;
             __builtin_amdgcn_s_setprio(1);           // matrix phases go ahead of the co-resident wave's vector work
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const v4i kf[2] = {B::rows(tile, row_place, 0, k, 0), B::rows(tile, row_place, 0, k, 1)};
-                s = mfma_cut(kf, qf[k], s);
-            }
+            products<KS>(
+                [&](int k, v4i (&f)[2]) {
+                    f[1] = B::rows(row_place, k, 1);
+                    f[0] = B::rows(row_place, k, 0);
+                },
+                [&](int k, const v4i (&f)[2]) { s = mfma_cut(f, qf[k], s); });
             __builtin_amdgcn_s_setprio(0);
             auto factors = [&](int what, int g) {    // of keys 8 g + 4 * half + 0..3 of the tile
                 return *reinterpret_cast<const v4f *>(at + G::FACTORS_AT + what * BKV * 4 + 4 * (32 * kt + 8 * g + 4 * fhalf));
@@ -228,106 +238,119 @@ __global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_
                 }
             }
             // ---- online softmax ----
-            float m_blk = s[0];
+            v16f x;
+            float most, l_blk;
+            auto weigh = [&]() {
+                most = l_blk = 0.0f;
 #pragma unroll
-            for (int v = 1; v < 16; v++) m_blk = fmaxf(m_blk, s[v]);
-            m_blk = fmaxf(m_blk, __shfl_xor(m_blk, 32, 64)) * down;
-            if (__builtin_amdgcn_ballot_w64(m_blk > m_run + 8.0f)) {
-                const float m_new = fmaxf(m_run, m_blk), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+                for (int g = 0; g < 4; g++) {
+                    const v4f f = factors(1, g);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int v = 4 * g + e;
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], down, -ref));
+                        l_blk += p;
+                        x[v] = p * f[e];
+                        most = fmaxf(most, x[v]);
+                    }
+                }
+                most = fmaxf(most, __shfl_xor(most, 32, 64));
+            };
+            weigh();
+            if (__builtin_amdgcn_ballot_w64(most > ROOM)) {      // (always for the first finite scores)
+                float top = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const v4f f = factors(1, g);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = fmaxf(top, __builtin_fmaf(s[4 * g + e], down, __builtin_amdgcn_logf(f[e])));
+                }
+                top = fmaxf(top, __shfl_xor(top, 32, 64)) - (float)LARGEST;
+                const float next = most > ROOM ? fmaxf(ref, top) : ref, alpha = __builtin_amdgcn_exp2f(ref - next);
+                ref = next;
                 l_run *= alpha;
-                m_run = m_new;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
                     for (int v = 0; v < 16; v++) acc[d][v] *= alpha;
-            }
-            float l_blk = 0.0f;
-#pragma unroll
-            for (int v = 0; v < 16; v++) {
-                s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], down, -m_run));
-                l_blk += s[v];
+                weigh();
             }
             l_run += l_blk;
             // ---- O^T += V^T P^T ----
-            float most = 0.0f;
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const v4f f = factors(1, g);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    s[4 * g + e] *= f[e];
-                    most = fmaxf(most, s[4 * g + e]);
-                }
-            }
-            most = fmaxf(most, __shfl_xor(most, 32, 64));
-            if (__builtin_amdgcn_ballot_w64(outgrown(most, p_up))) {
-                const int grown = regrown(most, p_up);
-                const float by = two_to(grown - p_up);
-                p_up = grown;
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int v = 0; v < 16; v++) acc[d][v] *= by;
-            }
-#pragma unroll
-            for (int st = 0; st < 2; st++) {
-                v4i pf[2];
-                cut_result(s, st, two_to(p_up), pf);
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const v4i vf[2] = {B::columns(tile + B::BYTES, column_place, 16 * st, d, 0), B::columns(tile + B::BYTES, column_place, 16 * st, d, 1)};
-                    acc[d] = mfma_cut(vf, pf, acc[d]);
-                }
-            }
+            v4i pf[2][2];
+            cut_scaled(x, 0, one, pf[0]);
+            cut_scaled(x, 1, one, pf[1]);
+            __builtin_amdgcn_s_setprio(1);
+            products<2 * DT>(
+                [&](int n, v4i (&f)[2]) {
+                    f[1] = B::columns(column_place, 16 * (n / DT), n % DT, 1);
+                    f[0] = B::columns(column_place, 16 * (n / DT), n % DT, 0);
+                },
+                [&](int n, const v4i (&f)[2]) { acc[n % DT] = mfma_cut(f, pf[n / DT], acc[n % DT]); });
+            __builtin_amdgcn_s_setprio(0);
         }
     };
-    if constexpr (G::DOUBLE) {
-        // Two blocks in LDS and the next in registers.  The two waves of a SIMD (w, w + 4) put it beside the current block before and after that is
-        // multiplied, so that one cuts while the other's products run.
-        unsigned cur = 0;
-        while (blk < nblocks) {
-            const bool more = ahead < nblocks;
-            int after = nblocks;
-            auto bring = [&]() {
-                stage(lds + (cur ^ G::STAGE));
-                after = next(ahead + 1);
-                if (after < nblocks) load(after);
-            };
-            if (more && wave >= 4) bring();
-            attend(blk, lds + cur);
-            if (more && wave < 4) bring();
-            __syncthreads();
-            blk = ahead;
-            ahead = after;
-            cur ^= G::STAGE;
-        }
-    } else {
-        while (blk < nblocks) {
-            const bool more = ahead < nblocks;
-            if (more) load(ahead);
-            attend(blk, lds);
-            __syncthreads();                         // the block has been read
-            if (more) {
-                stage(lds);
-                __syncthreads();
+    // Two blocks in LDS and the next in registers.  The two waves of a SIMD (w, w + 4) put it beside the current block before and after that is
+    // multiplied, so that one cuts while the other's products run.
+    unsigned cur = 0;
+    while (blk < nblocks) {
+        const bool more = ahead < nblocks;
+        int after = nblocks;
+        auto bring = [&]() {
+            stage(lds + (cur ^ G::STAGE));
+            after = next(ahead + 1);
+            if (after < nblocks) load(after);
+        };
+        if (more && wave >= 4) bring();
+        attend(blk, cur);
+        if (more && wave < 4) bring();
+        __syncthreads();
+        blk = ahead;
+        ahead = after;
+        cur ^= G::STAGE;
+    }
+
+    float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+    if constexpr (G::SHARES == 2) {                  // the other share's keys (the last barrier has passed: no block is read any more)
+        unsigned char *part = lds + wave % SETS * G::PART;
+        v4f *sums = reinterpret_cast<v4f *>(part) + lane;
+        float *of_row = reinterpret_cast<float *>(part + G::PART - 256) + frow;
+        if (wave >= SETS) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) sums[64 * (4 * d + g)] = v4f{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+            if (fhalf == 0) {
+                of_row[0] = ref;
+                of_row[32] = l_tot;
             }
-            blk = ahead;
-            ahead = more ? next(ahead + 1) : nblocks;
         }
+        __syncthreads();
+        if (wave >= SETS) return;
+        const float other = of_row[0], both = fmaxf(ref, other), mine = __builtin_amdgcn_exp2f(ref - both), theirs = __builtin_amdgcn_exp2f(other - both);
+        l_tot = l_tot * mine + of_row[32] * theirs;
+        ref = both;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const v4f sum = sums[64 * (4 * d + g)];
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[d][4 * g + e] = __builtin_fmaf(acc[d][4 * g + e], mine, sum[e] * theirs);
+            }
     }
 
     // ---- normalise and write: a lane owns its query's columns 32 d + 8 g + 4 * half .. + 3 ----
-    float seen = l_run * 0.0f;
+    float seen = l_tot * 0.0f;
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int v = 0; v < 16; v++) seen = __builtin_fmaf(acc[d][v], 0.0f, seen);
-    const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
     const bool unfit = live && (!(seen == 0.0f) || l_tot == 0.0f);
     uint64_t again = __builtin_amdgcn_ballot_w64(unfit);
     again |= again >> 32;
     const bool fit = !((again >> frow) & 1);
-    const float inv = 1.0f / l_tot, p_down = two_to(-p_up - BIAS);
+    const float inv = 1.0f / l_tot;
     if (valid && fit) {
         float *o = a.O + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk;
 #pragma unroll
@@ -337,10 +360,10 @@ __global__ void __launch_bounds__(64 * WAVES, (FwdGeom<DK, WAVES>::PER_SIMD)) k_
                 const int col = 32 * d + 8 * g + 4 * fhalf;
                 v4f out;
 #pragma unroll
-                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * p_down * inv : 0.0f;
+                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * two_to(-BIAS) * inv : 0.0f;
                 if (!PAD || col < a.dk) *reinterpret_cast<v4f *>(o + col) = out;
             }
-        if (a.L && fhalf == 0) a.L[((int64_t)b * a.H + head) * a.Sq + i] = live ? (m_run + __builtin_amdgcn_logf(l_tot)) * LN2 : -INFINITY;
+        if (a.L && fhalf == 0) a.L[((int64_t)b * a.H + head) * a.Sq + i] = live ? (ref + __builtin_amdgcn_logf(l_tot)) * LN2 : -INFINITY;
     }
     for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) {
         const int n = __builtin_ctz(rest);
@@ -366,31 +389,29 @@ __global__ void __launch_bounds__(256) k_doc_ranges(const int32_t *ids, int64_t 
     if ((threadIdx.x & 31) == 0) out[n] = high < 0 ? DocRange{0x7fffffff, -1} : DocRange{none ? ~low : low, high};
 }
 
-template <int DK, int WAVES, bool PAD>
+template <int DK, int SETS, bool PAD>
 int launch_fwd(const AttnArgs &a, FwdGrid grid) {
-    using G = FwdGeom<DK, WAVES>;
+    using G = FwdGeom<DK, SETS>;
     static bool attr_set = false;
     if (!attr_set) {
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_fwd<DK, WAVES, PAD>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_attn_fwd<DK, SETS, PAD>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
         attr_set = true;
     }
     grid.tiles = (int)(((int64_t)grid.pack * a.Sq + G::BQ - 1) / G::BQ);
     const int64_t all = grid.units * grid.tiles;
-    note_kernel(WAVES == 8 ? "attn_tiles_w8" : "attn_tiles");
+    note_kernel(SETS == 8 ? "attn_tiles_256" : "attn_tiles_128");
     for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
         const int64_t left = all - grid.first;
-        hipLaunchKernelGGL((k_attn_fwd<DK, WAVES, PAD>), dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
+        hipLaunchKernelGGL((k_attn_fwd<DK, SETS, PAD>), dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
         if (int rc = check_launch("attn_fwd")) return rc;
     }
     return AXHIP_OK;
 }
 
 template <int DK>
-int launch_fwd(const AttnArgs &a, const FwdGrid &grid, bool eight) {
-    const bool pad = a.dk < DK;
-    if constexpr (DK > 32)
-        if (eight) return pad ? launch_fwd<DK, 8, true>(a, grid) : launch_fwd<DK, 8, false>(a, grid);
-    return pad ? launch_fwd<DK, 4, true>(a, grid) : launch_fwd<DK, 4, false>(a, grid);
+int launch_fwd(const AttnArgs &a, const FwdGrid &grid, bool wide) {
+    if (a.dk < DK) return wide ? launch_fwd<DK, 8, true>(a, grid) : launch_fwd<DK, 4, true>(a, grid);
+    return wide ? launch_fwd<DK, 8, false>(a, grid) : launch_fwd<DK, 4, false>(a, grid);
 }
 
 }  // namespace
@@ -417,12 +438,23 @@ int attn_fwd_tiles(const AttnArgs &a) {
         if (int rc = doc_ranges(a.doc_k, a.B, a.Sk, ranges)) return rc;
         grid.ranges = static_cast<DocRange *>(ranges);
     }
-    const int64_t rows = (int64_t)grid.pack * a.Sq, wide = (rows + 255) / 256 * grid.units;
-    const bool eight = wide >= cu_count();
-    if (a.dk <= 32) return launch_fwd<32>(a, grid, eight);
-    if (a.dk <= 64) return launch_fwd<64>(a, grid, eight);
-    if (a.dk <= 96) return launch_fwd<96>(a, grid, eight);
-    return launch_fwd<128>(a, grid, eight);
+    // Tiles of 256 or 128 rows: the wide ones, which cut keys and values half as often, take one and a half times as long and not twice, but there are half as many to share out.
+    // Rounds of tiles over the CUs, or, causal, the longest tile or all of them evenly, whichever is more (us, 128 -> 256: 64 heads of [1024, 128] 139 -> 113, causal 88 and 91, 32
+    // causal ones of [3000, 96] 260 -> 224, but 36 causal ones of [777, 80] 54 -> 78, 8 of [2048, 64] 68 -> 110).
+    const int64_t rows = (int64_t)grid.pack * a.Sq, wide_tiles = (rows + 255) / 256, tiles = (rows + 127) / 128, cus = cu_count();
+    int64_t wide_time, time;
+    if (a.causal) {
+        wide_time = std::max(6 * cus, 3 * grid.units * (wide_tiles + 1));
+        time = std::max(4 * cus, 2 * grid.units * (tiles + 1));
+    } else {
+        wide_time = 3 * ((grid.units * wide_tiles + cus - 1) / cus);
+        time = 2 * ((grid.units * tiles + cus - 1) / cus);
+    }
+    const bool wide = wide_time <= time;
+    if (a.dk <= 32) return launch_fwd<32>(a, grid, wide);
+    if (a.dk <= 64) return launch_fwd<64>(a, grid, wide);
+    if (a.dk <= 96) return launch_fwd<96>(a, grid, wide);
+    return launch_fwd<128>(a, grid, wide);
 }
 
 }  // namespace axhip

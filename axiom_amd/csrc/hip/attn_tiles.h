@@ -25,15 +25,14 @@ struct Block {
         return at(4 * (lane >> 5) + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) + 8 * (l & 1);
     }
     __device__ static unsigned moved(unsigned place, unsigned by) { return (place ^ (by & MASK)) + (by & ~MASK); }
+    // `place` with the block's address added (a multiple of 256, which leaves the bits of MASK free).
     // rows r0 .. r0 + 31 as the rows of an operand, columns 16 k + 8 * half ..
-    __device__ static v4i rows(const unsigned char *base, unsigned place, int r0, int k, int term) {
-        return *reinterpret_cast<const v4i *>(base + moved(place, 32 * k) + r0 * PITCH + term * PLANE);
-    }
+    __device__ static v4i rows(unsigned place, int k, int term) { return read_chunk(moved(place, 32 * k) + term * PLANE); }
     // columns 32 d .. 32 d + 31 as the rows of an operand; its eight k are rows r0 + 4 * half + 0..3 and 8 more on (r0 a multiple of 16): those that registers
     // 8 s .. 8 s + 7 of a result tile hold
-    __device__ static v4i columns(const unsigned char *base, unsigned place, int r0, int d, int term) {
+    __device__ static v4i columns(unsigned place, int r0, int d, int term) {
         const unsigned near = moved(place, 64 * d);
-        const v2i32 a = read_columns(base + near + r0 * PITCH + term * PLANE), b = read_columns(base + (near ^ 32) + (r0 + 8) * PITCH + term * PLANE);
+        const v2i32 a = read_columns(near + r0 * PITCH + term * PLANE), b = read_columns((near ^ 32) + (r0 + 8) * PITCH + term * PLANE);
         return v4i{a[0], a[1], b[0], b[1]};
     }
 };
@@ -69,7 +68,7 @@ struct Stage {
             }
         }
     }
-    // to LDS, times `by`, cut; the rows' factors beside them
+    // to LDS, cut; the rows' factors, times `by`, beside them
     __device__ __forceinline__ void put(unsigned char *block, float *factors, int wave, int lane, float by) {
         const int chunk = lane % LANES;
 #pragma unroll
@@ -78,18 +77,15 @@ struct Stage {
             float most = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) most = fmaxf(most, __builtin_fabsf(x[i][e]));
-            const int up = up_of(most_of_lanes<LANES>(most * __builtin_fabsf(by)));
+            const float up = row_up(most_of_lanes<LANES>(most));
             v4i t[2];
-            if (by != 1.0f)
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[i][e] *= by;
-            cut_halves(x[i], two_to(up), t);
+            cut_halves(x[i], up, t);
             if (8 * LANES == DK || 8 * chunk < DK) {
                 unsigned char *to = block + B::at(row, chunk);
                 *reinterpret_cast<v4i *>(to) = t[0];
                 *reinterpret_cast<v4i *>(to + B::PLANE) = t[1];
             }
-            if (chunk == 0) factors[row] = factor_of(up);
+            if (chunk == 0) factors[row] = row_factor(up) * by;
         }
     }
 };
@@ -107,6 +103,24 @@ __device__ __forceinline__ void load_row(float (&x)[KS][8], const float *row, bo
 #pragma unroll
             for (int e = 0; e < 4; e++) x[s][4 * h + e] = v[e];
         }
+}
+
+// STEPS steps of products: fetch(i, f) reads the operand of step i from LDS, multiply(i, f) uses it.  Reads go out two steps ahead, so that no product waits for a
+// read that was only just asked for; left alone, the compiler saves registers, asks for each operand right before its use, and the matrix core
+// idles for the LDS's latency at every step.
+template <int STEPS, typename Fetch, typename Multiply>
+__device__ __forceinline__ void products(Fetch fetch, Multiply multiply) {
+    constexpr int ALU = 0x6;                         // vector and scalar instructions may pass from step to step, memory and matrix ones not
+    v4i f[3][2];
+    fetch(0, f[0]);
+    if (STEPS > 1) fetch(1, f[1]);
+    __builtin_amdgcn_sched_barrier(ALU);
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+        if (s + 2 < STEPS) fetch(s + 2, f[(s + 2) % 3]);
+        multiply(s, f[s % 3]);
+        __builtin_amdgcn_sched_barrier(ALU);
+    }
 }
 
 // The documents of 32 keys (or rows): the lowest and highest id there, -1 and below not counted; `low` is ~lowest where some are not

@@ -6,7 +6,7 @@
 // subnormals exactly (measured), so what a value below 2^-17 of its row's largest loses is an absolute 2^-40 of that.
 // Every row has a power of its own, and not a block: a row of 1e30 that a mask hides would otherwise take the bits of its neighbours.  Where rows are summed over
 // (P V), their powers go to the other operand, whose largest so far a running exponent holds.
-// Cutting a pair: two products, two conversions of pairs, two mixed multiply-adds.
+// Cutting a pair: two products (none where the values come scaled), two conversions of pairs, two mixed multiply-adds.
 // (Sums of products of split operands: Dekker, "A floating-point technique for extending the available precision", 1971.)
 #pragma once
 #include "common.h"
@@ -14,22 +14,25 @@
 namespace axhip {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef int v2i32 __attribute__((ext_vector_type(2)));
 
-// N values (4 or 8) times `up`, as two terms
-template <int N> using Half = std::conditional_t<N == 8, v4i, v2i32>;
-template <int N>
-__device__ __forceinline__ void cut_halves(const float (&x)[N], float up, Half<N> (&t)[2]) {
+// Eight values times `up`, as two terms.  (`hi` passes through a register that the compiler cannot see through: it would convert twice, once for
+// the pair and once for each value.)
+__device__ __forceinline__ void cut_pair(float x, float y, float up, int &first, int &second) {
     typedef float v2f __attribute__((ext_vector_type(2)));
+    first = __builtin_bit_cast(int, __builtin_convertvector(v2f{x * up, y * up}, v2h));
+    asm("" : "+v"(first));
+    const v2h hi = __builtin_bit_cast(v2h, first);
+    second = __builtin_bit_cast(int, __builtin_convertvector(v2f{__builtin_fmaf(x, up, -(float)hi[0]), __builtin_fmaf(y, up, -(float)hi[1])}, v2h));
+}
+__device__ __forceinline__ void cut_halves(const float (&x)[8], float up, v4i (&t)[2]) {
 #pragma unroll
-    for (int e = 0; e < N; e += 2) {
-        const v2h hi = __builtin_convertvector(v2f{x[e] * up, x[e + 1] * up}, v2h);
-        const float ra = __builtin_fmaf(x[e], up, -(float)hi[0]), rb = __builtin_fmaf(x[e + 1], up, -(float)hi[1]);
-        const v2h lo = __builtin_convertvector(v2f{ra, rb}, v2h);
-        t[0][e / 2] = __builtin_bit_cast(int, hi);
-        t[1][e / 2] = __builtin_bit_cast(int, lo);
+    for (int e = 0; e < 8; e += 2) {
+        int a, b;
+        cut_pair(x[e], x[e + 1], up, a, b);
+        t[0][e / 2] = a;
+        t[1][e / 2] = b;
     }
 }
 
@@ -45,14 +48,15 @@ __device__ __forceinline__ v16f mfma_cut(const v4i (&a)[2], const v4i (&b)[2], v
 
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigned)((e < -126 ? -126 : e) + 127) << 23); }
 
-// The exponent e of a row whose largest magnitude is `most`: at most MOST_UP, which a row of zeros gets.  The factor kept with a row is 2^(BIAS - e): times it, what
-// small rows are multiplied by does not run out of exponents.  (Rows past 2^100 get an infinite factor, and what it meets is formed again.)
+// What a row whose largest magnitude is `most` is taken times, 2^e, e at most MOST_UP (rows of zeros); and the factor kept with it, 2^(BIAS - e): times that, what small rows
+// are multiplied by does not run out of exponents.  (Rows past 2^100 get an infinite factor, and what it meets is formed again.)  Both straight from the exponent
+// field E of `most`, which is 2^(E - 127) to twice that: e = 141 - E.
 constexpr int MOST_UP = 100, BIAS = 24;
-__device__ __forceinline__ int up_of(float most) {
-    const int e = 15 - __builtin_amdgcn_frexp_expf(most);
-    return most == 0.0f || e > MOST_UP ? MOST_UP : e;
+__device__ __forceinline__ float row_up(float most) {
+    const unsigned bits = ((127u + 141u) << 23) - (__float_as_uint(most) & 0x7f800000u);
+    return __uint_as_float(min(bits, (127u + MOST_UP) << 23));
 }
-__device__ __forceinline__ float factor_of(int e) { return BIAS - e > 127 ? INFINITY : two_to(BIAS - e); }
+__device__ __forceinline__ float row_factor(float up) { return __uint_as_float(min(((254u + BIAS) << 23) - __float_as_uint(up), 0x7f800000u)); }
 
 // The largest of each LANES neighbouring lanes' values (4, 8 or 16), in all of them
 template <int LANES>
@@ -66,11 +70,14 @@ __device__ __forceinline__ float most_of_lanes(float v) {
     return v;
 }
 
-// A running exponent `up` for sums over what has no scale of its own: `most`, the largest factor yet, may not exceed 2^15 times it; it starts at MOST_UP and
-// falls so that the largest lies at 2^10, which leaves room for others.
+// What an operand may reach, and where a running reference puts the largest so far when it has gone past that: the room between is for others.
+constexpr float ROOM = 32768.0f;
+constexpr int LARGEST = 10;
+
+// A running exponent `up` for sums over what has no scale of its own: it starts at MOST_UP and falls when the largest so far, `most`, times 2^up is past ROOM
 __device__ __forceinline__ bool outgrown(float most, int up) { return most > two_to(15 - up); }
 __device__ __forceinline__ int regrown(float most, int up) {
-    const int e = 10 - __builtin_amdgcn_frexp_expf(most);
+    const int e = LARGEST - __builtin_amdgcn_frexp_expf(most);
     return outgrown(most, up) ? (e < MOST_UP ? e : MOST_UP) : up;
 }
 
@@ -79,8 +86,26 @@ __device__ __forceinline__ void cut_result(const v16f &x, int s, float up, v4i (
     const float part[8] = {x[8 * s], x[8 * s + 1], x[8 * s + 2], x[8 * s + 3], x[8 * s + 4], x[8 * s + 5], x[8 * s + 6], x[8 * s + 7]};
     cut_halves(part, up, t);
 }
+// 1.0f that the compiler does not know: times it, a mixed multiply-add is one instruction and not a conversion and a subtraction
+__device__ __forceinline__ float hidden_one() {
+    float one = 1.0f;
+    asm("" : "+s"(one));
+    return one;
+}
+__device__ __forceinline__ void cut_scaled(const v16f &x, int s, float one, v4i (&t)[2]) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        int hi = __builtin_bit_cast(int, __builtin_convertvector(v2f{x[8 * s + e], x[8 * s + e + 1]}, v2h));
+        asm("" : "+v"(hi));
+        const v2h h = __builtin_bit_cast(v2h, hi);
+        t[0][e / 2] = hi;
+        t[1][e / 2] = __builtin_bit_cast(
+            int, __builtin_convertvector(v2f{__builtin_fmaf(x[8 * s + e], one, -(float)h[0]), __builtin_fmaf(x[8 * s + e + 1], one, -(float)h[1])}, v2h));
+    }
+}
 
-// A lane's row (its other half in lane ^ 32) as operand terms, columns 16 s + 8 * half .. + 7 for step s; gives back the 2^-e that its products are taken times, less BIAS
+// A lane's row (its other half in lane ^ 32) as operand terms, columns 16 s + 8 * half .. + 7 for step s; gives back what its products are taken times, 2^(-e - BIAS)
 template <int KS>
 __device__ __forceinline__ float cut_row(float (&x)[KS][8], v4i (&t)[KS][2]) {
     float most = 0.0f;
@@ -88,17 +113,22 @@ __device__ __forceinline__ float cut_row(float (&x)[KS][8], v4i (&t)[KS][2]) {
     for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int e = 0; e < 8; e++) most = fmaxf(most, __builtin_fabsf(x[s][e]));
-    const int up = up_of(fmaxf(most, __shfl_xor(most, 32, 64)));
+    const float up = row_up(fmaxf(most, __shfl_xor(most, 32, 64)));
 #pragma unroll
-    for (int s = 0; s < KS; s++) cut_halves(x[s], two_to(up), t[s]);
-    return two_to(-up - BIAS);
+    for (int s = 0; s < KS; s++) cut_halves(x[s], up, t[s]);
+    return 1.0f / up * two_to(-BIAS);
 }
+
+// LDS by its address in it
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+__device__ __forceinline__ unsigned lds_address(const unsigned char *p) { return (unsigned)(uintptr_t)(const lds_byte *)p; }
+__device__ __forceinline__ v4i read_chunk(unsigned at) { return *reinterpret_cast<const __attribute__((address_space(3))) v4i *>(at); }
 
 // Four rows of one column each from LDS: lane l of a group of 16 lanes gives the address of four columns of one row (rows go with l / 4, columns with
 // l % 4) and gets column l of the four rows.
-__device__ __forceinline__ v2i32 read_columns(const unsigned char *at) {
+__device__ __forceinline__ v2i32 read_columns(unsigned at) {
     typedef short v4s __attribute__((ext_vector_type(4)));
-    return __builtin_bit_cast(v2i32, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)at));
+    return __builtin_bit_cast(v2i32, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) v4s *>(at)));
 }
 
 }  // namespace axhip
