@@ -6,6 +6,8 @@
 // far at 2^10 to 2^15, and the sum is rescaled when it moves, as an online softmax does.  In k_attn_dkv the key is on the lane side: a lane owns key (l & 31), its
 // registers are 16 rows, and what these need (lse, delta, end, document) lies in LDS beside the block.  Rows (keys) whose sums are not finite are formed again
 // with fp32 instructions.
+#include <algorithm>
+
 #include "attn_launch.h"
 #include "attn_tiles.h"
 
@@ -47,7 +49,8 @@ __device__ __forceinline__ void score_tile(const AttnArgs &a, v16f &s, v16f &slo
         for (int v = 0; v < 16; v++) s[v] -= distance(v);
 }
 
-// The next 64-row block from `blk` on, below n, of which some tile's documents meet [low, high]: 64 blocks at a time, a lane each
+// The next block of TILES tiles from `blk` on, below n, of which some tile's documents meet [low, high]: 64 blocks at a time, a lane each
+template <int TILES>
 struct Blocks {
     const DocRange *ranges;                      // NULL: every block
     int n, tiles, low, high, at;
@@ -61,8 +64,9 @@ struct Blocks {
                 const int mine = at + lane;
                 bool meets = false;
                 if (mine < n) {
-                    meets = ranges[2 * mine].meets(low, high);
-                    if (2 * mine + 1 < tiles) meets |= ranges[2 * mine + 1].meets(low, high);
+#pragma unroll
+                    for (int i = 0; i < TILES; i++)
+                        if (TILES * mine + i < tiles) meets |= ranges[TILES * mine + i].meets(low, high);
                 }
                 window = __builtin_amdgcn_ballot_w64(meets);
             }
@@ -77,30 +81,48 @@ struct Blocks {
     }
 };
 
-constexpr int WAVES = 4, ROWS = 64;              // rows of a block
+// Workgroups go to the eight XCDs in turn: a unit's tiles (a head's, a group of heads') to one, eight units at a time, or, causal, the longest tile of every unit first
+__device__ __forceinline__ void work_of(const AttnArgs &a, const BwdGrid &grid, int64_t &unit, int &tile) {
+    const int64_t lin = grid.first + blockIdx.x, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
+    const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8;
+    unit = a.causal ? lin % grid.units : group * 8 + r8 % width;
+    tile = (int)(a.causal ? lin / grid.units : r8 / width);
+}
 
+// Eight waves, two a SIMD, where their registers allow it, and rows of a block
 template <int DK>
-struct DqGeom {
+struct BwdGeom {
+    static constexpr int WAVES = DK <= 64 ? 8 : 4, ROWS = DK <= 32 ? 128 : 64, TILES = ROWS / 32;
     using B = Block<DK, ROWS>;
-    static constexpr int FACTORS_AT = 2 * B::BYTES;              // of each key row, then of each value row
-    static constexpr int DOCS_AT = FACTORS_AT + ROWS * 8;
-    static constexpr int META_AT = DOCS_AT + ROWS * 4 + 2 * 8;
-    static constexpr int SMEM = META_AT + 16 * WAVES;
-    static constexpr int PER_SIMD = DK <= 32 ? 2 : 1;
+    static constexpr int PER_SIMD = WAVES / 4;
 };
 
-template <int DK, bool PAD>
-__global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(AttnArgs a, BwdGrid grid) {
+template <int DK>
+struct DqGeom : BwdGeom<DK> {
+    using typename BwdGeom<DK>::B;
+    using BwdGeom<DK>::WAVES, BwdGeom<DK>::ROWS, BwdGeom<DK>::TILES;
+    static constexpr int FACTORS_AT = 2 * B::BYTES;              // of each key row, then of each value row
+    static constexpr int DOCS_AT = FACTORS_AT + ROWS * 8;
+    static constexpr int META_AT = DOCS_AT + ROWS * 4 + TILES * 8;
+    static constexpr int SMEM = META_AT + 16 * WAVES;
+    // the other share's sums: [DT][4][64 lanes] v4f a wave
+    static constexpr int JOIN = DK / 32 * 4096;
+};
+
+// SETS waves side by side along the queries, 32 rows each; where those are half of the waves, the others take the other tiles of each block
+template <int DK, int SETS, bool PAD>
+__global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIMD)) k_attn_dq(AttnArgs a, BwdGrid grid) {
     using G = DqGeom<DK>;
     using B = typename G::B;
-    constexpr int KS = DK / 16, DT = DK / 32;
+    constexpr int KS = DK / 16, DT = DK / 32, WAVES = G::WAVES, ROWS = G::ROWS, TILES = G::TILES, SHARES = WAVES / SETS;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
-    const int64_t lin = grid.first + blockIdx.x, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
-    const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8, unit = group * 8 + r8 % width;
-    const int tile = a.causal ? grid.tiles - 1 - (int)(r8 / width) : (int)(r8 / width);
+    int64_t unit;
+    int tile;
+    work_of(a, grid, unit, tile);
+    if (a.causal) tile = grid.tiles - 1 - tile;
     const int b = (int)(unit / a.H), head = (int)(unit - (int64_t)b * a.H), hk = head / a.G;
-    const int r = tile * 32 * WAVES + wave * 32 + frow, i = r < a.Sq ? r : a.Sq - 1;
+    const int r = tile * 32 * SETS + wave % SETS * 32 + frow, i = r < a.Sq ? r : a.Sq - 1;
     const bool valid = r < a.Sq;
     AttnRow row = attn_row(a, b, head, i);
     if (!valid) row.end = 0;
@@ -132,7 +154,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
     wg_low = __builtin_amdgcn_readfirstlane(wg_low);
     wg_high = __builtin_amdgcn_readfirstlane(wg_high);
     const DocRange *ranges = docs ? grid.key_ranges + (int64_t)b * grid.key_tiles : nullptr;
-    Blocks blocks(ranges, (wg_last + ROWS - 1) / ROWS, grid.key_tiles, wg_low, wg_high);
+    Blocks<TILES> blocks(ranges, (wg_last + ROWS - 1) / ROWS, grid.key_tiles, wg_low, wg_high);
 
     const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;
     Stage<DK, ROWS, WAVES> ks, vs;
@@ -144,14 +166,14 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
         ks.template load<PAD>(Kb + k0 * a.ldk, a.ldk, end, wave, lane, a.dk);
         vs.template load<PAD>(Vb + k0 * a.ldv, a.ldv, end, wave, lane, a.dk);
         if (docs && threadIdx.x < ROWS) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
-        if (docs && threadIdx.x < 2) range_here = 2 * blk + (int)threadIdx.x < grid.key_tiles ? ranges[2 * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
+        if (docs && threadIdx.x < TILES) range_here = TILES * blk + (int)threadIdx.x < grid.key_tiles ? ranges[TILES * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
     };
     auto stage = [&]() {
         float *factors = reinterpret_cast<float *>(lds + G::FACTORS_AT);
         ks.put(lds, factors, wave, lane, 1.0f);
         vs.put(lds + B::BYTES, factors + ROWS, wave, lane, 1.0f);
         if (docs && threadIdx.x < ROWS) reinterpret_cast<int *>(lds + G::DOCS_AT)[threadIdx.x] = doc_here;
-        if (docs && threadIdx.x < 2) reinterpret_cast<DocRange *>(lds + G::DOCS_AT + ROWS * 4)[threadIdx.x] = range_here;
+        if (docs && threadIdx.x < TILES) reinterpret_cast<DocRange *>(lds + G::DOCS_AT + ROWS * 4)[threadIdx.x] = range_here;
     };
 
     int blk = blocks.next(0, lane);
@@ -195,7 +217,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
     const unsigned row_at = B::row_place(lane) + lds_address(lds), column_at = B::column_place(lane) + lds_address(lds);
     auto attend = [&](int blk) {
 #pragma unroll 1
-        for (int kt = 0; kt < 2; kt++) {
+        for (int kt = wave / SETS; kt < TILES; kt += SHARES) {
             const int kt0 = blk * ROWS + 32 * kt;
             if (kt0 >= last) break;
             bool partly = kt0 + 32 > sure;
@@ -301,6 +323,25 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
         blk = ahead;
     }
 
+    times(acc, two_to(-d_up - BIAS));
+    if constexpr (SHARES == 2) {                     // the other share's keys (the last barrier has passed: no block is read any more)
+        v4f *sums = reinterpret_cast<v4f *>(lds + wave % SETS * G::JOIN) + lane;
+        if (wave >= SETS)
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) sums[64 * (4 * d + g)] = v4f{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+        __syncthreads();
+        if (wave >= SETS) return;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const v4f sum = sums[64 * (4 * d + g)];
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[d][4 * g + e] += sum[e];
+            }
+    }
     float seen = 0.0f;
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -309,7 +350,6 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
     uint64_t again = __builtin_amdgcn_ballot_w64(live && !(seen == 0.0f));
     again |= again >> 32;
     if (valid && !((again >> frow) & 1)) {
-        const float down = two_to(-d_up - BIAS);
         float *dq = a.dQ + ((int64_t)b * a.Sq + i) * a.lddq + (int64_t)head * a.dk;
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -318,7 +358,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
                 const int col = 32 * d + 8 * g + 4 * fhalf;
                 v4f out;
 #pragma unroll
-                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * down * a.scale : 0.0f;
+                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * a.scale : 0.0f;
                 if (!PAD || col < a.dk) *reinterpret_cast<v4f *>(dq + col) = out;
             }
     }
@@ -329,27 +369,26 @@ __global__ void __launch_bounds__(64 * WAVES, (DqGeom<DK>::PER_SIMD)) k_attn_dq(
 }
 
 template <int DK>
-struct DkvGeom {
-    using B = Block<DK, ROWS>;
+struct DkvGeom : BwdGeom<DK> {
+    using typename BwdGeom<DK>::B;
+    using BwdGeom<DK>::WAVES, BwdGeom<DK>::ROWS, BwdGeom<DK>::TILES;
     static constexpr int ROW_AT = 2 * B::BYTES;                  // of each row: factors of Q and dO, lse, delta, slope (floats), end, position, document (ints)
     static constexpr int TILE_AT = ROW_AT + ROWS * 32;           // of each 32 rows: last end, first end, range of documents
-    static constexpr int SMEM = TILE_AT + 2 * 16;
-    static constexpr int PER_SIMD = DK <= 32 ? 2 : 1;
-    // the sums of the waves that share keys: [2 DT][64 lanes][16]
-    static constexpr int JOIN = 2 * (DK / 32) * 64 * 64;
+    static constexpr int SMEM = TILE_AT + TILES * 16;
+    static constexpr int JOIN = DK / 32 * 8192;      // the other share's sums, of both gradients
 };
 
-// KW waves side by side along the keys, 32 each; the others take the other tile of each block's rows, and their sums are added in the end
+// KW waves side by side along the keys, 32 each, and the tiles of rows shared out as above
 template <int DK, int KW, bool PAD>
-__global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dkv(AttnArgs a, BwdGrid grid) {
+__global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIMD)) k_attn_dkv(AttnArgs a, BwdGrid grid) {
     using G = DkvGeom<DK>;
     using B = typename G::B;
-    constexpr int KS = DK / 16, DT = DK / 32;
+    constexpr int KS = DK / 16, DT = DK / 32, WAVES = G::WAVES, ROWS = G::ROWS, TILES = G::TILES, SHARES = WAVES / KW;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
-    const int64_t lin = grid.first + blockIdx.x, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
-    const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8, unit = group * 8 + r8 % width;
-    const int tile = (int)(r8 / width);              // causal: the first keys, which most rows see, go out first
+    int64_t unit;
+    int tile;                                        // (causal: the first keys are those that most rows see)
+    work_of(a, grid, unit, tile);
     const int b = (int)(unit / a.Hkv), hk = (int)(unit - (int64_t)b * a.Hkv);
     const int k0 = tile * 32 * KW, kw0 = k0 + wave % KW * 32, key = kw0 + frow;
     const int len = attn_len(a, b), start = attn_start(a, b);
@@ -388,7 +427,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
     first = __builtin_amdgcn_readfirstlane(first);
     rows_end = __builtin_amdgcn_readfirstlane(rows_end);
     const DocRange *row_ranges = docs ? grid.row_ranges + (int64_t)b * grid.row_tiles : nullptr;
-    Blocks blocks(row_ranges, rows_end > 0 ? (rows_end + ROWS - 1) / ROWS : 0, grid.row_tiles, wg_low, wg_high);
+    Blocks<TILES> blocks(row_ranges, rows_end > 0 ? (rows_end + ROWS - 1) / ROWS : 0, grid.row_tiles, wg_low, wg_high);
 
     // head `g` of the group, block `blk` of it: the place of the work, and the next one
     struct Place {
@@ -446,7 +485,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
                 low = min(low, __shfl_xor(low, off, 64));
                 high = max(high, __shfl_xor(high, off, 64));
             }
-            if (frow == 0) *reinterpret_cast<v4i *>(lds + G::TILE_AT + 16 * fhalf) = v4i{last, sure, low, high};
+            if (frow == 0) *reinterpret_cast<v4i *>(lds + G::TILE_AT + 16 * (threadIdx.x >> 5)) = v4i{last, sure, low, high};
         }
     };
 
@@ -579,12 +618,8 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
     while (at.g < a.G) {
         const Place ahead = settle({at.g, at.blk + 1});
         if (ahead.g < a.G) load(ahead);
-        if (KW == WAVES) {
 #pragma unroll 1
-            for (int qt = 0; qt < 2; qt++) attend(qt);
-        } else {
-            attend(wave / KW);
-        }
+        for (int qt = wave / KW; qt < TILES; qt += SHARES) attend(qt);
         __syncthreads();                             // the block has been read
         if (ahead.g < a.G) {
             stage();
@@ -601,8 +636,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
             acc_k[d][v] = acc_k[d][v] * two_to(-d_up - BIAS) * k_out;
             acc_v[d][v] = acc_v[d][v] * two_to(-p_up - BIAS);
         }
-    if constexpr (KW < WAVES) {
-        static_assert(WAVES == 2 * KW, "two waves share keys");
+    if constexpr (SHARES == 2) {
         v4f *part = reinterpret_cast<v4f *>(lds + wave % KW * G::JOIN) + lane;
         if (wave >= KW)
 #pragma unroll
@@ -656,40 +690,48 @@ __global__ void __launch_bounds__(64 * WAVES, (DkvGeom<DK>::PER_SIMD)) k_attn_dk
     for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) attn_dkv_row(a, b, hk, kw0 + __builtin_ctz(rest), lane);
 }
 
-template <typename Kernel>
-int launch_tiles(Kernel kernel, int smem, const AttnArgs &a, BwdGrid grid, const char *what) {
+template <auto KERNEL>
+int launch_tiles(int smem, int waves, const AttnArgs &a, BwdGrid grid, const char *what) {
+    static bool attr_set = false;
+    if (!attr_set) {
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, smem), "hipFuncSetAttribute");
+        attr_set = true;
+    }
     const int64_t all = grid.units * grid.tiles;
     for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
         const int64_t left = all - grid.first;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), smem, kStream, a, grid);
+        hipLaunchKernelGGL(KERNEL, dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * waves), smem, kStream, a, grid);
         if (int rc = check_launch(what)) return rc;
     }
     return AXHIP_OK;
 }
 
+// Whether all waves go side by side over `length` rows (or keys) of each unit, or half of them: as for the tiles of the forward pass (attn_fwd.hip)
+bool all_abreast(const AttnArgs &a, int64_t units, int64_t length, int waves) {
+    const int64_t wide_tiles = (length + 32 * waves - 1) / (32 * waves), tiles = (length + 16 * waves - 1) / (16 * waves), cus = cu_count();
+    if (a.causal) return std::max(6 * cus, 3 * units * (wide_tiles + 1)) <= std::max(4 * cus, 2 * units * (tiles + 1));
+    return 3 * ((units * wide_tiles + cus - 1) / cus) <= 2 * ((units * tiles + cus - 1) / cus);
+}
+
 template <int DK, bool PAD>
 int launch_bwd(const AttnArgs &a, BwdGrid grid) {
-    constexpr int SHARED_KEYS = 2 * DkvGeom<DK>::JOIN > DkvGeom<DK>::SMEM ? 2 * DkvGeom<DK>::JOIN : DkvGeom<DK>::SMEM;
-    static bool attr_set = false;
-    if (!attr_set) {
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>((k_attn_dq<DK, PAD>)), hipFuncAttributeMaxDynamicSharedMemorySize, DqGeom<DK>::SMEM), "hipFuncSetAttribute");
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>((k_attn_dkv<DK, 4, PAD>)), hipFuncAttributeMaxDynamicSharedMemorySize, DkvGeom<DK>::SMEM), "hipFuncSetAttribute");
-        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>((k_attn_dkv<DK, 2, PAD>)), hipFuncAttributeMaxDynamicSharedMemorySize, SHARED_KEYS), "hipFuncSetAttribute");
-        attr_set = true;
-    }
+    constexpr int WAVES = BwdGeom<DK>::WAVES, HALF = WAVES / 2, DQ = DqGeom<DK>::SMEM, DKV = DkvGeom<DK>::SMEM;
+    constexpr int DQ_HALF = std::max(DQ, HALF * DqGeom<DK>::JOIN), DKV_HALF = std::max(DKV, HALF * DkvGeom<DK>::JOIN);
     if (a.Sq > 0) {
         grid.units = (int64_t)a.B * a.H;
-        grid.tiles = (a.Sq + 32 * WAVES - 1) / (32 * WAVES);
-        if (int rc = launch_tiles(k_attn_dq<DK, PAD>, DqGeom<DK>::SMEM, a, grid, "attn_bwd queries")) return rc;
+        const bool wide = all_abreast(a, grid.units, a.Sq, WAVES);
+        const int rows = 32 * (wide ? WAVES : HALF);
+        grid.tiles = (a.Sq + rows - 1) / rows;
+        if (int rc = wide ? launch_tiles<k_attn_dq<DK, WAVES, PAD>>(DQ, WAVES, a, grid, "attn_bwd queries")
+                          : launch_tiles<k_attn_dq<DK, HALF, PAD>>(DQ_HALF, WAVES, a, grid, "attn_bwd queries"))
+            return rc;
     }
     grid.units = (int64_t)a.B * a.Hkv;
-    const int64_t wide = (a.Sk + 127) / 128 * grid.units;
-    if (wide > 2 * cu_count()) {
-        grid.tiles = (a.Sk + 127) / 128;
-        return launch_tiles(k_attn_dkv<DK, 4, PAD>, DkvGeom<DK>::SMEM, a, grid, "attn_bwd keys");
-    }
-    grid.tiles = (a.Sk + 63) / 64;
-    return launch_tiles(k_attn_dkv<DK, 2, PAD>, SHARED_KEYS, a, grid, "attn_bwd keys");
+    const bool wide = all_abreast(a, grid.units, a.Sk, WAVES);
+    const int keys = 32 * (wide ? WAVES : HALF);
+    grid.tiles = (a.Sk + keys - 1) / keys;
+    return wide ? launch_tiles<k_attn_dkv<DK, WAVES, PAD>>(DKV, WAVES, a, grid, "attn_bwd keys")
+                : launch_tiles<k_attn_dkv<DK, HALF, PAD>>(DKV_HALF, WAVES, a, grid, "attn_bwd keys");
 }
 
 }  // namespace
