@@ -127,18 +127,8 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     AttnRow row = attn_row(a, b, head, i);
     if (!valid) row.end = 0;
     const bool live = row.end > 0, docs = a.doc_q != nullptr;
-    int last = row.end, sure = live ? row.end : 0x7fffffff, d_low = live ? row.doc : 0x7fffffff, d_high = live ? row.doc : -1;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        last = max(last, __shfl_xor(last, off, 64));
-        sure = min(sure, __shfl_xor(sure, off, 64));
-        d_low = min(d_low, __shfl_xor(d_low, off, 64));
-        d_high = max(d_high, __shfl_xor(d_high, off, 64));
-    }
-    last = __builtin_amdgcn_readfirstlane(last);
-    sure = __builtin_amdgcn_readfirstlane(sure);
-    d_low = __builtin_amdgcn_readfirstlane(d_low);
-    d_high = __builtin_amdgcn_readfirstlane(d_high);
+    const RowsSeen mine = same_for_wave(rows_seen(row));
+    const int last = mine.last, sure = mine.sure, d_low = mine.low, d_high = mine.high;
     int *meta = reinterpret_cast<int *>(lds + G::META_AT);
     if (lane == 0) *reinterpret_cast<v4i *>(meta + 4 * wave) = v4i{last, 0, d_low, d_high};
     __syncthreads();
@@ -391,7 +381,8 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     work_of(a, grid, unit, tile);
     const int b = (int)(unit / a.Hkv), hk = (int)(unit - (int64_t)b * a.Hkv);
     const int k0 = tile * 32 * KW, kw0 = k0 + wave % KW * 32, key = kw0 + frow;
-    const int len = attn_len(a, b), start = attn_start(a, b);
+    const AttnSeq seq = attn_seq(a, b);
+    const int len = seq.len, start = seq.start;
     const bool valid = key < a.Sk, live = key < len, docs = a.doc_q != nullptr;
     int doc = 0, d_low = 0, d_high = 0, wg_low = 0, wg_high = 0;
     if (docs) {
@@ -420,7 +411,7 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     // rows of a head that may see the workgroup's keys
     int first = 0, rows_end = a.Sq;
     if (a.causal) {
-        if (!(a.prefix && a.prefix[b] > k0)) first = k0 - start > 0 ? k0 - start : 0;
+        if (seq.prefix <= k0) first = k0 - start > 0 ? k0 - start : 0;
         if (len - start < rows_end) rows_end = len - start;
     }
     if (k0 >= len || first >= rows_end) rows_end = 0;
@@ -443,49 +434,39 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
         return p;
     };
     Stage<DK, ROWS, WAVES> qs, os;
-    float r_lse = INFINITY, r_delta = 0.0f, r_slope = 0.0f;
-    AttnRow r_row = {0, 0, -1, 0.0f};
+    float r_lse = 0.0f, r_delta = 0.0f;
+    int r_doc = 0;
     auto load = [&](Place p) {
         const int head = hk * a.G + p.g, i0 = p.blk * ROWS, end = rows_end - 1 - i0;
         qs.template load<PAD>(a.Q + ((int64_t)b * a.Sq + i0) * a.ldq + (int64_t)head * a.dk, a.ldq, end, wave, lane, a.dk);
         os.template load<PAD>(a.dO + ((int64_t)b * a.Sq + i0) * a.lddo + (int64_t)head * a.dk, a.lddo, end, wave, lane, a.dk);
         if (threadIdx.x < ROWS) {
-            const int i = i0 + threadIdx.x;
-            r_row.end = 0;
-            r_lse = INFINITY;
-            r_delta = 0.0f;
-            if (i < rows_end) {
-                r_row = attn_row(a, b, head, i);
-                const int64_t at = ((int64_t)b * a.H + head) * a.Sq + i;
-                r_lse = a.Lin[at] * LOG2E;
-                if (r_lse == -INFINITY) r_lse = INFINITY;
-                r_delta = a.delta[at];
-            }
-            r_slope = r_row.slope2;
+            const int i = min(i0 + (int)threadIdx.x, rows_end - 1);
+            const int64_t at = ((int64_t)b * a.H + head) * a.Sq + i;
+            r_lse = a.Lin[at];
+            r_delta = a.delta[at];
+            if (docs) r_doc = a.doc_q[(int64_t)b * a.Sq + i];
         }
     };
-    auto stage = [&]() {
+    auto stage = [&](Place p) {
         float *of_rows = reinterpret_cast<float *>(lds + G::ROW_AT);
         qs.put(lds, of_rows, wave, lane, a.q_up);
         os.put(lds + B::BYTES, of_rows + ROWS, wave, lane, 1.0f);
         if (threadIdx.x < ROWS) {
+            const int i = p.blk * ROWS + threadIdx.x;
+            AttnRow row = attn_row(a, seq, i, r_doc, a.slopes ? a.slopes[hk * a.G + p.g] : 0.0f);
+            if (i >= rows_end) row.end = 0;
             float *at = of_rows + threadIdx.x;
             int *ints = reinterpret_cast<int *>(at);
-            at[2 * ROWS] = r_lse;
-            at[3 * ROWS] = r_delta;
-            at[4 * ROWS] = r_slope;
-            ints[5 * ROWS] = r_row.end;
-            ints[6 * ROWS] = r_row.p;
-            ints[7 * ROWS] = r_row.doc;
-            int last = r_row.end, sure = r_row.end, low = r_row.end > 0 ? r_row.doc : 0x7fffffff, high = r_row.end > 0 ? r_row.doc : -1;
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) {
-                last = max(last, __shfl_xor(last, off, 64));
-                sure = min(sure, __shfl_xor(sure, off, 64));
-                low = min(low, __shfl_xor(low, off, 64));
-                high = max(high, __shfl_xor(high, off, 64));
-            }
-            if (frow == 0) *reinterpret_cast<v4i *>(lds + G::TILE_AT + 16 * (threadIdx.x >> 5)) = v4i{last, sure, low, high};
+            at[2 * ROWS] = r_lse == -INFINITY ? INFINITY : r_lse * LOG2E;     // a row that saw nothing: no probability
+            at[3 * ROWS] = row.end > 0 ? r_delta : 0.0f;
+            at[4 * ROWS] = row.slope2;
+            ints[5 * ROWS] = row.end;
+            ints[6 * ROWS] = row.p;
+            ints[7 * ROWS] = row.doc;
+            RowsSeen seen = rows_seen(row);
+            if (of_half_wave(row.end, [](int x, int y) { return min(x, y); }) == 0) seen.sure = 0;
+            if (frow == 0) *reinterpret_cast<v4i *>(lds + G::TILE_AT + 16 * (threadIdx.x >> 5)) = v4i{seen.last, seen.sure, seen.low, seen.high};
         }
     };
 
@@ -500,7 +481,7 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
         load_row<PAD>(x, a.V + ((int64_t)b * a.kv_rows + key) * a.ldv + (int64_t)hk * a.dk, live, fhalf, a.dk);
         v_down = cut_row(x, vf);
     }
-    if (at.g < a.G) stage();
+    if (at.g < a.G) stage(at);
     __syncthreads();
 
     v16f acc_k[DT], acc_v[DT];
@@ -622,7 +603,7 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
         for (int qt = wave / KW; qt < TILES; qt += SHARES) attend(qt);
         __syncthreads();                             // the block has been read
         if (ahead.g < a.G) {
-            stage();
+            stage(ahead);
             __syncthreads();
         }
         at = ahead;

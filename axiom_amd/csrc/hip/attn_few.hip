@@ -44,18 +44,8 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     AttnRow row = attn_row(a, b, head, i);
     if (!valid) row.end = 0;
     const bool live = row.end > 0;
-    int last = row.end, sure = live ? row.end : 0x7fffffff, d_low = live ? row.doc : 0x7fffffff, d_high = live ? row.doc : -1;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        last = max(last, __shfl_xor(last, off, 64));
-        sure = min(sure, __shfl_xor(sure, off, 64));
-        d_low = min(d_low, __shfl_xor(d_low, off, 64));
-        d_high = max(d_high, __shfl_xor(d_high, off, 64));
-    }
-    last = __builtin_amdgcn_readfirstlane(last);
-    sure = __builtin_amdgcn_readfirstlane(sure);
-    d_low = __builtin_amdgcn_readfirstlane(d_low);
-    d_high = __builtin_amdgcn_readfirstlane(d_high);
+    const RowsSeen mine = same_for_wave(rows_seen(row));
+    const int last = mine.last, sure = mine.sure, d_low = mine.low, d_high = mine.high;
     const int all = (last + 31) / 32, t_begin = (int)((int64_t)all * split / grid.splits), t_end = (int)((int64_t)all * (split + 1) / grid.splits);
 
     const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;

@@ -57,18 +57,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     const bool live = row.end > 0;
 
     // what the wave sees, and what the workgroup does: the last end, the first end of rows that see anything, the range of documents
-    int last = row.end, sure = live ? row.end : 0x7fffffff, d_low = live ? row.doc : 0x7fffffff, d_high = live ? row.doc : -1;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        last = max(last, __shfl_xor(last, off, 64));
-        sure = min(sure, __shfl_xor(sure, off, 64));
-        d_low = min(d_low, __shfl_xor(d_low, off, 64));
-        d_high = max(d_high, __shfl_xor(d_high, off, 64));
-    }
-    last = __builtin_amdgcn_readfirstlane(last);
-    sure = __builtin_amdgcn_readfirstlane(sure);
-    d_low = __builtin_amdgcn_readfirstlane(d_low);
-    d_high = __builtin_amdgcn_readfirstlane(d_high);
+    const RowsSeen mine = same_for_wave(rows_seen(row));
+    const int last = mine.last, sure = mine.sure, d_low = mine.low, d_high = mine.high;
     int *meta = reinterpret_cast<int *>(lds + G::META_AT);
     if (lane == 0) *reinterpret_cast<v4i *>(meta + 4 * wave) = v4i{last, 0, d_low, d_high};
     __syncthreads();

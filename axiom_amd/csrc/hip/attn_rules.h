@@ -27,34 +27,34 @@ struct AttnRow {
     float slope2;                                // log2 units
 };
 
-__device__ __forceinline__ int attn_len(const AttnArgs &a, int b) {
-    if (!a.lens) return a.Sk;
-    const int n = a.lens[b];
-    return n < 0 ? 0 : n > a.Sk ? a.Sk : n;
-}
-__device__ __forceinline__ int attn_start(const AttnArgs &a, int b) {
-    if (!a.start) return a.Sk - a.Sq;
+// What all rows of a sequence share: its keys, the position of its first query, its prefix
+struct AttnSeq {
+    int len, start, prefix;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b) {
     constexpr int FAR = 1 << 24;
-    const int s = a.start[b];
-    return s < -FAR ? -FAR : s > FAR ? FAR : s;
+    AttnSeq s = {a.Sk, a.Sk - a.Sq, 0};
+    if (a.lens) s.len = min(max(a.lens[b], 0), a.Sk);
+    if (a.start) s.start = min(max(a.start[b], -FAR), FAR);
+    if (a.prefix) s.prefix = a.prefix[b];
+    return s;
+}
+// doc: of the row, where there are documents
+__device__ __forceinline__ AttnRow attn_row(const AttnArgs &a, const AttnSeq &s, int i, int doc, float slope) {
+    AttnRow r;
+    r.p = s.start + i;
+    r.end = s.len;
+    if (a.causal) {
+        const int e = max(r.p + 1, s.prefix);
+        r.end = r.p >= s.len || e <= 0 ? 0 : min(e, s.len);
+    }
+    r.doc = a.doc_q ? doc : 0;
+    if (r.doc < 0) r.end = 0;
+    r.slope2 = slope * a.bias2;
+    return r;
 }
 __device__ __forceinline__ AttnRow attn_row(const AttnArgs &a, int b, int head, int i) {
-    AttnRow r;
-    r.p = attn_start(a, b) + i;
-    const int len = attn_len(a, b);
-    r.end = len;
-    if (a.causal) {
-        int e = r.p + 1;
-        if (a.prefix && a.prefix[b] > e) e = a.prefix[b];
-        r.end = r.p >= len || e <= 0 ? 0 : e < len ? e : len;
-    }
-    r.doc = 0;
-    if (a.doc_q) {
-        r.doc = a.doc_q[(int64_t)b * a.Sq + i];
-        if (r.doc < 0) r.end = 0;
-    }
-    r.slope2 = a.slopes ? a.slopes[head] * a.bias2 : 0.0f;
-    return r;
+    return attn_row(a, attn_seq(a, b), i, a.doc_q ? a.doc_q[(int64_t)b * a.Sq + i] : 0, a.slopes ? a.slopes[head] : 0.0f);
 }
 
 // tanh and its derivative.  Near zero x (1 + x^2 p(x^2)), a minimax fit of degree 4 on |x| < 0.6 (relative error 3e-9 before rounding); beyond, with

@@ -105,6 +105,30 @@ __device__ __forceinline__ void load_row(float (&x)[KS][8], const float *row, bo
         }
 }
 
+// The least or most of the values of 32 lanes (each half of a wave), in all of them
+template <typename Pick>
+__device__ __forceinline__ int of_half_wave(int v, Pick pick) {
+    v = pick(v, __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true));
+    v = pick(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));
+    v = pick(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true));
+    v = pick(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true));
+    const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    return pick((int)r[0], (int)r[1]);
+}
+// What 32 rows see together: the last end, the first end of those that see anything, the range of their documents
+struct RowsSeen {
+    int last, sure, low, high;
+};
+__device__ __forceinline__ RowsSeen rows_seen(const AttnRow &row) {
+    auto least = [](int a, int b) { return min(a, b); };
+    auto most = [](int a, int b) { return max(a, b); };
+    const bool live = row.end > 0;
+    return {of_half_wave(row.end, most), of_half_wave(live ? row.end : 0x7fffffff, least), of_half_wave(live ? row.doc : 0x7fffffff, least), of_half_wave(live ? row.doc : -1, most)};
+}
+__device__ __forceinline__ RowsSeen same_for_wave(const RowsSeen &s) {
+    return {__builtin_amdgcn_readfirstlane(s.last), __builtin_amdgcn_readfirstlane(s.sure), __builtin_amdgcn_readfirstlane(s.low), __builtin_amdgcn_readfirstlane(s.high)};
+}
+
 // STEPS steps of products: fetch(i, f) reads the operand of step i from LDS, multiply(i, f) uses it.  Reads go out two steps ahead, so that no product waits for a
 // read that was only just asked for; left alone, the compiler saves registers, asks for each operand right before its use, and the matrix core
 // idles for the LDS's latency at every step.
