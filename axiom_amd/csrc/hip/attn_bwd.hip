@@ -147,21 +147,25 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     Blocks<TILES> blocks(ranges, (wg_last + ROWS - 1) / ROWS, grid.key_tiles, wg_low, wg_high);
 
     const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;
-    Stage<DK, ROWS, WAVES> ks, vs;
+    using S = Stage<DK, ROWS, WAVES, PAD>;
+    S ks, vs;
+    const unsigned base = lds_address(lds);
     int doc_here = -1;
     DocRange range_here = {0, 0};
     auto load = [&](int blk) {
         const int64_t k0 = (int64_t)blk * ROWS;
         const int end = wg_last - 1 - (int)k0;
-        ks.template load<PAD>(Kb + k0 * a.ldk, a.ldk, end, wave, lane, a.dk);
-        vs.template load<PAD>(Vb + k0 * a.ldv, a.ldv, end, wave, lane, a.dk);
+        const int l = (int)afresh(lane);             // (places of lanes are formed anew: registers are dearer)
+        ks.load(Kb + k0 * a.ldk, a.ldk, end, S::place(wave, l, a.ldk), l, a.dk);
+        vs.load(Vb + k0 * a.ldv, a.ldv, end, S::place(wave, l, a.ldv), l, a.dk);
         if (docs && threadIdx.x < ROWS) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
         if (docs && threadIdx.x < TILES) range_here = TILES * blk + (int)threadIdx.x < grid.key_tiles ? ranges[TILES * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
     };
     auto stage = [&]() {
-        float *factors = reinterpret_cast<float *>(lds + G::FACTORS_AT);
-        ks.put(lds, factors, wave, lane, 1.0f);
-        vs.put(lds + B::BYTES, factors + ROWS, wave, lane, 1.0f);
+        const int l = (int)afresh(lane);
+        const typename S::Place place = S::place(wave, l, 0);
+        ks.put(base, base + G::FACTORS_AT, place, l, 1.0f, a.dk);
+        vs.put(base + B::BYTES, base + G::FACTORS_AT + 4 * ROWS, place, l, 1.0f, a.dk);
         if (docs && threadIdx.x < ROWS) reinterpret_cast<int *>(lds + G::DOCS_AT)[threadIdx.x] = doc_here;
         if (docs && threadIdx.x < TILES) reinterpret_cast<DocRange *>(lds + G::DOCS_AT + ROWS * 4)[threadIdx.x] = range_here;
     };
@@ -204,7 +208,7 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     float o_times = o_down * two_to(d_up), delta_times = delta * two_to(d_up);
     const float one = hidden_one();
 
-    const unsigned row_at = B::row_place(lane) + lds_address(lds), column_at = B::column_place(lane) + lds_address(lds);
+    const unsigned row_at = B::row_place(lane) + base, column_at = B::column_place(lane) + base;
     auto attend = [&](int blk) {
 #pragma unroll 1
         for (int kt = wave / SETS; kt < TILES; kt += SHARES) {
@@ -433,13 +437,16 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
         }
         return p;
     };
-    Stage<DK, ROWS, WAVES> qs, os;
+    using S = Stage<DK, ROWS, WAVES, PAD>;
+    S qs, os;
+    const unsigned base = lds_address(lds);
     float r_lse = 0.0f, r_delta = 0.0f;
     int r_doc = 0;
     auto load = [&](Place p) {
         const int head = hk * a.G + p.g, i0 = p.blk * ROWS, end = rows_end - 1 - i0;
-        qs.template load<PAD>(a.Q + ((int64_t)b * a.Sq + i0) * a.ldq + (int64_t)head * a.dk, a.ldq, end, wave, lane, a.dk);
-        os.template load<PAD>(a.dO + ((int64_t)b * a.Sq + i0) * a.lddo + (int64_t)head * a.dk, a.lddo, end, wave, lane, a.dk);
+        const int l = (int)afresh(lane);
+        qs.load(a.Q + ((int64_t)b * a.Sq + i0) * a.ldq + (int64_t)head * a.dk, a.ldq, end, S::place(wave, l, a.ldq), l, a.dk);
+        os.load(a.dO + ((int64_t)b * a.Sq + i0) * a.lddo + (int64_t)head * a.dk, a.lddo, end, S::place(wave, l, a.lddo), l, a.dk);
         if (threadIdx.x < ROWS) {
             const int i = min(i0 + (int)threadIdx.x, rows_end - 1);
             const int64_t at = ((int64_t)b * a.H + head) * a.Sq + i;
@@ -450,8 +457,10 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     };
     auto stage = [&](Place p) {
         float *of_rows = reinterpret_cast<float *>(lds + G::ROW_AT);
-        qs.put(lds, of_rows, wave, lane, a.q_up);
-        os.put(lds + B::BYTES, of_rows + ROWS, wave, lane, 1.0f);
+        const int l = (int)afresh(lane);
+        const typename S::Place place = S::place(wave, l, 0);
+        qs.put(base, base + G::ROW_AT, place, l, a.q_up, a.dk);
+        os.put(base + B::BYTES, base + G::ROW_AT + 4 * ROWS, place, l, 1.0f, a.dk);
         if (threadIdx.x < ROWS) {
             const int i = p.blk * ROWS + threadIdx.x;
             AttnRow row = attn_row(a, seq, i, r_doc, a.slopes ? a.slopes[hk * a.G + p.g] : 0.0f);
@@ -492,7 +501,7 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     // acc_k is 2^(BIAS + d_up) times the sum of ds q, acc_v 2^(BIAS + p_up) times that of P dO: running exponents of ds and P times their rows' factors
     int d_up = MOST_UP, p_up = MOST_UP;
 
-    const unsigned row_at = B::row_place(lane) + lds_address(lds), column_at = B::column_place(lane) + lds_address(lds);
+    const unsigned row_at = B::row_place(lane) + base, column_at = B::column_place(lane) + base;
     auto attend = [&](int qt) {
         const v4i whole = *reinterpret_cast<const v4i *>(lds + G::TILE_AT + 16 * qt);
         const int t_last = __builtin_amdgcn_readfirstlane(whole[0]), t_sure = __builtin_amdgcn_readfirstlane(whole[1]);

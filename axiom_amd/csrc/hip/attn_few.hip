@@ -51,13 +51,16 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;
     unsigned char *const at = lds + wave * G::BLOCK;
     float *const row_factors = reinterpret_cast<float *>(at + G::FACTORS_AT);
-    Stage<DK, 32, 1> ks, vs;
+    const unsigned base = lds_address(at);
+    using S = Stage<DK, 32, 1, PAD>;
+    S ks, vs;
     int doc_here = -1;
     auto load = [&](int t) {
         const int64_t k0 = (int64_t)t * 32;
         const int end = last - 1 - (int)k0;          // rows past it are read as it
-        ks.template load<PAD>(Kb + k0 * a.ldk, a.ldk, end, 0, lane, a.dk);
-        vs.template load<PAD>(Vb + k0 * a.ldv, a.ldv, end, 0, lane, a.dk);
+        const int l = (int)afresh(lane);
+        ks.load(Kb + k0 * a.ldk, a.ldk, end, S::place(0, l, a.ldk), l, a.dk);
+        vs.load(Vb + k0 * a.ldv, a.ldv, end, S::place(0, l, a.ldv), l, a.dk);
         if (docs) doc_here = frow <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + frow] : -1;
     };
     int t = t_begin + wave;
@@ -82,7 +85,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     float ref = ATTN_LOWEST, l_run = 0.0f;           // as in the tile kernel: acc is 2^BIAS times the sum
     const float one = hidden_one();
 
-    const unsigned row_at = B::row_place(lane) + lds_address(at), column_at = B::column_place(lane) + lds_address(at) + B::BYTES;
+    const unsigned row_at = B::row_place(lane) + base, column_at = B::column_place(lane) + base + B::BYTES;
     for (; t < t_end; t += WAVES) {
         const int kt0 = t * 32;
         bool partly = kt0 + 32 > sure, meets = true;
@@ -92,8 +95,10 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
         }
         order_in_wave();                             // the last tile has been read
         if (meets) {
-            ks.put(at, row_factors, 0, lane, 1.0f);
-            vs.put(at + B::BYTES, row_factors + 32, 0, lane, 1.0f);
+            const int l = (int)afresh(lane);
+            const typename S::Place place = S::place(0, l, 0);
+            ks.put(base, base + G::FACTORS_AT, place, l, 1.0f, a.dk);
+            vs.put(base + B::BYTES, base + G::FACTORS_AT + 128, place, l, 1.0f, a.dk);
             if (docs && lane < 32) reinterpret_cast<int *>(at + G::DOCS_AT)[lane] = doc_here;
         }
         order_in_wave();

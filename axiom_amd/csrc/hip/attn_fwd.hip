@@ -102,23 +102,26 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     };
 
     const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;
-    Stage<DK, BKV, WAVES> ks, vs;
+    using S = Stage<DK, BKV, WAVES, PAD>;
+    S ks, vs;
+    const unsigned base = lds_address(lds);
     int doc_here = -1;
     DocRange range_here = {0, 0};
     auto load = [&](int blk) {
         const int64_t k0 = (int64_t)blk * BKV;
         const int end = wg_last - 1 - (int)k0;       // rows past it are read as it
-        const int l = (int)afresh(lane);
-        ks.template load<PAD>(Kb + k0 * a.ldk, a.ldk, end, wave, l, a.dk);
-        vs.template load<PAD>(Vb + k0 * a.ldv, a.ldv, end, wave, l, a.dk);
+        const int l = (int)afresh(lane);             // (places of lanes are formed anew: registers are dearer)
+        ks.load(Kb + k0 * a.ldk, a.ldk, end, S::place(wave, l, a.ldk), l, a.dk);
+        vs.load(Vb + k0 * a.ldv, a.ldv, end, S::place(wave, l, a.ldv), l, a.dk);
         if (docs && threadIdx.x < BKV) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
         if (docs && threadIdx.x < TILES) range_here = TILES * blk + (int)threadIdx.x < grid.range_tiles ? ranges[TILES * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
     };
-    auto stage = [&](unsigned char *at) {
-        float *factors = reinterpret_cast<float *>(at + G::FACTORS_AT);
+    auto stage = [&](unsigned cur) {
+        unsigned char *at = lds + cur;
         const int l = (int)afresh(lane);
-        ks.put(at, factors, wave, l, 1.0f);
-        vs.put(at + B::BYTES, factors + BKV, wave, l, 1.0f);
+        const typename S::Place place = S::place(wave, l, 0);
+        ks.put(base + cur, base + cur + G::FACTORS_AT, place, l, 1.0f, a.dk);
+        vs.put(base + cur + B::BYTES, base + cur + G::FACTORS_AT + 4 * BKV, place, l, 1.0f, a.dk);
         if (docs && threadIdx.x < BKV) reinterpret_cast<int *>(at + G::DOCS_AT)[threadIdx.x] = doc_here;
         if (docs && threadIdx.x < TILES) reinterpret_cast<DocRange *>(at + G::DOCS_AT + BKV * 4)[threadIdx.x] = range_here;
     };
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
         q_down = cut_row(x, qf);
     }
     if (blk < nblocks) {
-        stage(lds);
+        stage(0);
         ahead = next(blk + 1);
         if (ahead < nblocks) load(ahead);
     }
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     float ref = ATTN_LOWEST, l_run = 0.0f;
     const float one = hidden_one();
 
-    const unsigned row_at = B::row_place(lane) + lds_address(lds), column_at = B::column_place(lane) + lds_address(lds) + B::BYTES;
+    const unsigned row_at = B::row_place(lane) + base, column_at = B::column_place(lane) + base + B::BYTES;
     auto attend = [&](int blk, unsigned cur) {
         const unsigned char *at = lds + cur;
 #pragma unroll 1
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
         const bool more = ahead < nblocks;
         int after = nblocks;
         auto bring = [&]() {
-            stage(lds + (cur ^ G::STAGE));
+            stage(cur ^ G::STAGE);
             after = next(ahead + 1);
             if (after < nblocks) load(after);
         };

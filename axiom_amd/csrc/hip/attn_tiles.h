@@ -43,37 +43,54 @@ __device__ __forceinline__ unsigned afresh(unsigned v) {
     return v;
 }
 
-// How the waves of a workgroup bring a block from memory: wave w rows RPW w .. RPW w + RPW - 1, eight columns a lane and piece, LANES lanes a row.
-template <int DK, int ROWS, int WAVES>
+// How the waves of a workgroup bring a block from memory: wave w rows RPW w .. RPW w + RPW - 1, eight columns a lane and piece, LANES lanes a row, STEP rows a piece.
+template <int DK, int ROWS, int WAVES, bool PAD>
 struct Stage {
-    static constexpr int RPW = ROWS / WAVES, LANES = DK <= 32 ? 4 : DK <= 64 ? 8 : 16, PIECES = RPW * LANES / 64;
-    static_assert(PIECES * 64 == RPW * LANES, "a block divides over the lanes");
+    static constexpr int RPW = ROWS / WAVES, LANES = DK <= 32 ? 4 : DK <= 64 ? 8 : 16, STEP = 64 / LANES, PIECES = RPW / STEP;
+    static_assert(PIECES * STEP == RPW && RPW % 8 == 0, "a block divides over the lanes");
+    static constexpr bool SOME = PAD || DK != 8 * LANES;         // some lanes have columns past the head
     using B = Block<DK, ROWS>;
     float x[PIECES][8];
-    __device__ static int row_of(int piece, int wave, int lane) { return wave * RPW + piece * (64 / LANES) + lane / LANES; }
-    // row r of the block is at base + min(r, last) * pitch.  PAD: the head is dk < DK columns wide, those from dk on are zero
-    template <bool PAD>
-    __device__ __forceinline__ void load(const float *base, int64_t pitch, int last, int wave, int lane, int dk) {
+    // Of a lane: its row and column in the first piece in memory (bytes) and in LDS
+    struct Place {
+        unsigned from, to, row;
+    };
+    __device__ static Place place(int wave, int lane, int64_t pitch) {
+        const unsigned row = wave * RPW + lane / LANES, chunk = lane % LANES;
+        return {row * (unsigned)pitch * 4 + 32 * chunk, B::at(row, chunk), row};
+    }
+    // Row r of the block is at base + min(r, last) * pitch (below 2^32 bytes: pitches are up to 2^24 bytes).  Lanes past the head read its first columns.
+    __device__ __forceinline__ void load(const float *base, int64_t pitch, int last, const Place &at, int lane, int dk) {
+        const char *from = reinterpret_cast<const char *>(base);
         const int col = lane % LANES * 8;
+        const unsigned step = (unsigned)pitch * 4 * STEP;
+        unsigned off[PIECES];
+        if (last >= ROWS - 1) {
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const int row = row_of(i, wave, lane);
-            const float *p = base + (int64_t)(row < last ? row : last) * pitch + col;
+            for (int i = 0; i < PIECES; i++) off[i] = at.from + i * step;
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) off[i] = (unsigned)min((int)at.row + i * STEP, last) * (unsigned)pitch * 4 + 4 * col;
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; i++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const bool in = !(PAD || DK != 8 * LANES) || col + 4 * h < dk;       // (other lanes read column 0 on)
-                const v4f a = *reinterpret_cast<const v4f *>(in ? p + 4 * h : p - col);
+                const unsigned there = !SOME || col + 4 * h < dk ? off[i] + 16 * h : off[i] - 4 * col;
+                const v4f a = *reinterpret_cast<const v4f *>(from + (uint64_t)there);
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[i][4 * h + e] = in ? a[e] : 0.0f;
+                for (int e = 0; e < 4; e++) x[i][4 * h + e] = a[e];
             }
-        }
     }
-    // to LDS, cut; the rows' factors, times `by`, beside them
-    __device__ __forceinline__ void put(unsigned char *block, float *factors, int wave, int lane, float by) {
+    // to LDS at `block`, cut; the rows' factors, times `by`, beside them.  A piece further on is STEP rows and an exchange of chunks away.
+    __device__ __forceinline__ void put(unsigned block, unsigned factors, const Place &at, int lane, float by, int dk) {
         const int chunk = lane % LANES;
+        const unsigned to = at.to + block;
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            const int row = row_of(i, wave, lane);
+            if (PAD)                                 // columns from dk on are zero
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] = 8 * chunk + (e & 4) < dk ? x[i][e] : 0.0f;
             float most = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) most = fmaxf(most, __builtin_fabsf(x[i][e]));
@@ -81,11 +98,11 @@ struct Stage {
             v4i t[2];
             cut_halves(x[i], up, t);
             if (8 * LANES == DK || 8 * chunk < DK) {
-                unsigned char *to = block + B::at(row, chunk);
-                *reinterpret_cast<v4i *>(to) = t[0];
-                *reinterpret_cast<v4i *>(to + B::PLANE) = t[1];
+                const unsigned there = (to ^ ((i * STEP >> 2 & 3) << 4)) + i * STEP * B::PITCH;
+                write_chunk(there, t[0]);
+                write_chunk(there + B::PLANE, t[1]);
             }
-            if (chunk == 0) factors[row] = row_factor(up) * by;
+            if (chunk == 0) write_float(factors + 4 * (at.row + i * STEP), row_factor(up) * by);
         }
     }
 };

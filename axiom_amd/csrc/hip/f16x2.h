@@ -123,6 +123,8 @@ __device__ __forceinline__ float cut_row(float (&x)[KS][8], v4i (&t)[KS][2]) {
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 __device__ __forceinline__ unsigned lds_address(const unsigned char *p) { return (unsigned)(uintptr_t)(const lds_byte *)p; }
 __device__ __forceinline__ v4i read_chunk(unsigned at) { return *reinterpret_cast<const __attribute__((address_space(3))) v4i *>(at); }
+__device__ __forceinline__ void write_chunk(unsigned at, const v4i &v) { *reinterpret_cast<__attribute__((address_space(3))) v4i *>(at) = v; }
+__device__ __forceinline__ void write_float(unsigned at, float v) { *reinterpret_cast<__attribute__((address_space(3))) float *>(at) = v; }
 
 // Four rows of one column each from LDS: lane l of a group of 16 lanes gives the address of four columns of one row (rows go with l / 4, columns with
 // l % 4) and gets column l of the four rows.
