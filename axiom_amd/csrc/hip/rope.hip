@@ -262,22 +262,27 @@ __global__ void __launch_bounds__(64) k_heads_any(HeadsArgs p) {
     }
 }
 
-// dgamma from the workgroups' sums: 64 columns a workgroup, its 16 waves take rows of sums in turn
+// dgamma from the workgroups' sums: 16 columns a workgroup, its 64 parts take the sums in turn, sixteen loads of each under way
 __global__ void __launch_bounds__(1024) k_gamma_sums(const float *partial, int n, int dk, float *dgq, float *dgk) {
-    __shared__ float part[16][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+    __shared__ float parts[64][16];
+    const int here = threadIdx.x & 15, col = blockIdx.x * 16 + here, part = threadIdx.x >> 4;
     float sum = 0.0f;
-    if (col < 2 * dk)
-        for (int b = wave; b < n; b += 16) sum += partial[(int64_t)b * 2 * dk + col];
-    part[wave][threadIdx.x & 63] = sum;
+    if (col < 2 * dk) {
+#pragma unroll 16
+        for (int b = part; b < n; b += 64) sum += partial[(int64_t)b * 2 * dk + col];
+    }
+    parts[part][here] = sum;
     __syncthreads();
-    if (wave != 0 || col >= 2 * dk) return;
-    for (int w = 1; w < 16; w++) sum += part[w][threadIdx.x];
+    for (int half = 32; half > 0; half >>= 1) {
+        if (part < half) parts[part][here] += parts[part + half][here];
+        __syncthreads();
+    }
+    if (part != 0 || col >= 2 * dk) return;
     float *out = col < dk ? dgq : dgk;
-    if (out) out[col < dk ? col : col - dk] = sum;
+    if (out) out[col < dk ? col : col - dk] = parts[0][here];
 }
 
-constexpr int64_t GRAD_GROUPS = 1024;            // workgroups at most whose sums are joined by k_gamma_sums
+constexpr int64_t GRAD_GROUPS = 1024;            // workgroups of four waves at most whose sums are joined by k_gamma_sums (of one: four times as many)
 
 template <Mode MODE, int LANES>
 int launch_heads(HeadsArgs &p, unsigned grid) {
@@ -297,18 +302,17 @@ int run_heads(HeadsArgs &p, float *dgq, float *dgk) {
     if (units) {
         while (8 * lanes < p.dk) lanes *= 2;
         const int64_t groups = 256 / lanes;
-        // Heads of a row are shared out until there are some eight waves a CU; with more rows than that a group walks a whole row, so that its angles
-        // are formed once.
+        // A group of lanes takes four heads of a row, what it has under way at a time, so that its angles serve four; fewer where that leaves less than eight waves a
+        // CU.  (us, whole rows -> four heads: 16000 rows of 24 heads of 128 89 -> 78, but one head each 80; 2000 rows of 20 heads of 64, two each 6.2, one each 7.5.)
         const int64_t want = (int64_t)cu_count() * 8 * 64 / lanes;
-        int64_t chunks = p.rows >= want ? 1 : (want + p.rows - 1) / p.rows;
-        if (chunks > p.heads) chunks = p.heads;
-        p.chunk = (int)((p.heads + chunks - 1) / chunks);
+        p.chunk = 4;
+        while (p.chunk > 1 && p.rows * ((p.heads + p.chunk - 1) / p.chunk) < want) p.chunk /= 2;
         p.chunks = (p.heads + p.chunk - 1) / p.chunk;
         grid = (p.rows * p.chunks + groups - 1) / groups;
     } else {
         grid = p.rows * p.heads;
     }
-    const int64_t most = sums_wanted ? GRAD_GROUPS : 1 << 22;
+    const int64_t most = !sums_wanted ? 1 << 22 : units ? GRAD_GROUPS : 4 * GRAD_GROUPS;
     if (grid > most) grid = most;
     if (sums_wanted && !(p.partial = static_cast<float *>(workspace((size_t)grid * 2 * p.dk * sizeof(float))))) return AXHIP_ERR_ALLOC;
     int rc;
@@ -322,7 +326,7 @@ int run_heads(HeadsArgs &p, float *dgq, float *dgk) {
     else if (lanes == 32) rc = launch_heads<MODE, 32>(p, (unsigned)grid);
     else rc = launch_heads<MODE, 64>(p, (unsigned)grid);
     if (rc || !sums_wanted) return rc;
-    hipLaunchKernelGGL(k_gamma_sums, dim3((unsigned)((2 * p.dk + 63) / 64)), dim3(1024), 0, kStream, p.partial, (int)grid, p.dk, dgq, dgk);
+    hipLaunchKernelGGL(k_gamma_sums, dim3((unsigned)((2 * p.dk + 15) / 16)), dim3(1024), 0, kStream, p.partial, (int)grid, p.dk, dgq, dgk);
     return check_launch("rope gamma sums");
 }
 
