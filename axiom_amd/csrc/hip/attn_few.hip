@@ -326,18 +326,34 @@ int launch_few(const AttnArgs &a, FewGrid grid) {
 
 namespace axhip {
 
-// Whether the few-rows form takes the call, and in how many ranges of keys.  Ranges: until there are two workgroups a CU, each wave with a tile or more.
+// Whether the few-rows form takes the call, and in how many ranges of keys: until there are two workgroups a CU, each wave with a tile or more.
+// Which form: by what each takes, in us.  Tiles: 128 rows a CU, as long as their keys.  Few rows: a step of 32 rows and 32 keys costs the chip so much (the
+// wider heads have one workgroup a CU and twice the work), and every further round of workgroups its start.  Within a few per cent where it is close (us, tiles -> this: 1 token
+// of 8 sequences over 1000 keys, 8 heads of 32 25.0 -> 13.4, 4 x 4 of [512, 64] causal 22.5 -> 11.8, 16 queries of 4 heads over 16000 keys, 8 heads of 128 711 -> 94, 4 x 2 x 8 of
+// [2048, 32] causal 47 -> 34; the other side 32 of [1024, 96] causal 53 -> 146, 64 of [400, 128] 38 -> 93, 128 of [512, 64] 43 -> 70).  Over 135 random calls it chose
+// the slower one 7 times, by 1.8 times at most.
 bool attn_fwd_few(const AttnArgs &a, int &rc) {
     const int64_t rows = (int64_t)a.G * a.Sq, cus = cu_count();
     FewGrid grid = {};
     grid.row_tiles = (int)((rows + 31) / 32);
     const int64_t units = (int64_t)a.B * a.Hkv * grid.row_tiles, tiles = ((int64_t)a.Sk + 31) / 32;
-    if (rows > 32 || units > GRID_MOST / 64) return false;
+    if (units > GRID_MOST / 64) return false;
     int64_t splits = (2 * cus + units - 1) / units;
     if (splits > (tiles + WAVES - 1) / WAVES) splits = (tiles + WAVES - 1) / WAVES;
     if (splits > 64) splits = 64;
     if (splits < 1) splits = 1;
     grid.splits = (int)splits;
+    if (rows > 32) {
+        const int width = (a.dk + 31) / 32 - 1, pack = a.G > 1 && a.Sq <= 64 ? a.G : 1;
+        constexpr double TILE_STEP[] = {0.65, 0.95, 1.5, 1.5}, FEW_STEP[] = {1.1e-3, 1.8e-3, 8e-3, 8e-3};
+        const int64_t big = (int64_t)a.B * (a.H / pack) * (((int64_t)pack * a.Sq + 127) / 128);
+        const int64_t room = cus * (width < 2 ? 2 : 1), few_rounds = (units * splits + room - 1) / room;
+        if (big > cus || a.doc_k) return false;      // (more tiles than CUs never lost to this form; and it fetches what a document hides)
+        const double loaded = (double)big / (double)cus, seen = a.causal && a.Sq == a.Sk ? 0.5 : 1.0;
+        const double tile_time = 6.0 + (double)tiles * TILE_STEP[width] * (1.0 + 0.45 * loaded);
+        const double few_time = 5.5 + (splits > 1 ? 1.5 : 0.0) + 6.0 * (double)(few_rounds - 1) + (double)(units * tiles) * seen * FEW_STEP[width];
+        if (few_time >= tile_time) return false;
+    }
     auto run = [&](auto width) {
         constexpr int DK = decltype(width)::value;
         return a.dk < DK ? launch_few<DK, true>(a, grid) : launch_few<DK, false>(a, grid);
