@@ -322,3 +322,97 @@ def test_large_rows_beside_ordinary_ones(hip, dk):
     want = attention(q, k, v, dk ** -0.5, rules, d_o)
     # what the large value and gradient add to others is in their bounds, as in any fp32 sum
     check(hip, q, k, v, dk ** -0.5, rules, d_o, want=want)
+
+
+def some_heads(rules, b, heads):
+    """The rules of one sequence and some query heads"""
+    cut = {n: None if getattr(rules, n) is None else np.asarray(getattr(rules, n))[heads if n == "slopes" else slice(b, b + 1)] for n in Rules.ARRAYS}
+    return Rules(cap=rules.cap, causal=rules.causal, **cut)
+
+
+@pytest.mark.parametrize("dk", [20, 32, 48, 64, 80, 96, 100, 128])
+@pytest.mark.parametrize("kind", ["plain", "capped", "documents", "everything"])
+def test_many_heads(hip, dk, kind):
+    """Enough tiles for the wide ones, forward and backward; a few heads of the first and last sequence are compared, keys shared by two heads."""
+    say("attn many", dk, kind)
+    B, S, H, Hkv = 8, 500, 64, 32
+    rng, q, k, v, d_o = draw(dk, B, S, S, H, Hkv, dk)
+    rules = rules_of(kind, rng, B, S, S, H)
+    if rules.lens is not None:
+        rules.lens[[0, -1]] = [S, 170]
+        rules.start = None
+    if kind == "documents":
+        rules.causal = 0
+    r, held = device_rules(hip, rules)
+    ld, ldk = H * dk, Hkv * dk
+    dq, dk_, dv, do, o, lse = hip.array(q), hip.array(k), hip.array(v), hip.array(d_o), hip.empty(q.shape), hip.empty((B, H, S))
+    grads = [hip.empty(x.shape) for x in (q, k, v)]
+    hip.check(hip.L.axhip_attn_fwd(dq.ptr, ld, dk_.ptr, ldk, dv.ptr, ldk, S, o.ptr, ld, lse.ptr, B, H, Hkv, S, S, dk, 0.1, C.byref(r)))
+    assert hip.last_kernel() == "attn_tiles_256"
+    hip.check(hip.L.axhip_attn_bwd(dq.ptr, ld, dk_.ptr, ldk, dv.ptr, ldk, S, o.ptr, ld, lse.ptr, do.ptr, ld, grads[0].ptr, ld, grads[1].ptr, ldk, grads[2].ptr, ldk,
+                                   B, H, Hkv, S, S, dk, 0.1, C.byref(r)))
+    assert hip.last_kernel() == "attn_grad_tiles"
+    o, lse, grads = o.numpy(), lse.numpy(), [g.numpy() for g in grads]
+    for b, h in ((0, 0), (0, 62), (B - 1, 34)):
+        heads, kv = slice(h, h + 2), slice(h // 2, h // 2 + 1)
+        part = some_heads(rules, b, heads)
+        want = attention(q[b:b + 1, :, heads], k[b:b + 1, :, kv], v[b:b + 1, :, kv], 0.1, part, d_o[b:b + 1, :, heads])
+        empty = np.isneginf(want["lse"])
+        assert np.array_equal(np.isneginf(lse[b:b + 1, heads]), empty)
+        within(o[b:b + 1, :, heads], want, "o")
+        within(np.where(empty, 0, lse[b:b + 1, heads]), dict(want, lse=np.where(empty, 0, want["lse"])), "lse")
+        for n, g, hh in (("dq", grads[0], heads), ("dk", grads[1], kv), ("dv", grads[2], kv)):
+            # the gradient from the kernel's own O and log-sum-exp, off by their bounds: twice each bound holds both
+            within(g[b:b + 1, :, hh], {n: want[n], "tol_" + n: 2 * want["tol_" + n]}, n)
+
+
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk,dk,form", [(1, 8, 1, 4, 4000, 64, "attn_few_ranges"), (1, 8, 1, 5, 4000, 64, "attn_few_ranges"), (4, 4, 4, 512, 512, 64, "attn_few"),
+                                                   (4, 16, 16, 400, 400, 64, "attn_tiles_128"), (32, 16, 2, 40, 200, 96, "attn_tiles_128"), (1, 64, 1, 1, 3000, 128, "attn_few_ranges"),
+                                                   (2, 2, 2, 33, 100, 36, "attn_few")])
+@pytest.mark.parametrize("kind", ["plain", "distance"])
+def test_which_form_takes_it(hip, B, H, Hkv, Sq, Sk, dk, form, kind):
+    """Both sides of the rules, several tiles of rows in the form for few rows among them (256 CUs)."""
+    say("attn forms", B, H, Hkv, Sq, Sk, dk)
+    rng, q, k, v, _ = draw(Sq + Sk, B, Sq, Sk, H, Hkv, dk)
+    r = Rules() if kind == "plain" else Rules(slopes=(2.0 ** -rng.uniform(1, 6, H)).astype(np.float32))
+    rules, held = device_rules(hip, r)
+    dq, dk_, dv, o, lse = hip.array(q), hip.array(k), hip.array(v), hip.empty(q.shape), hip.empty((B, H, Sq))
+    hip.check(hip.L.axhip_attn_fwd(dq.ptr, H * dk, dk_.ptr, Hkv * dk, dv.ptr, Hkv * dk, Sk, o.ptr, H * dk, lse.ptr, B, H, Hkv, Sq, Sk, dk, 0.2, C.byref(rules)))
+    assert hip.last_kernel().startswith(form), hip.last_kernel()
+    o, lse = o.numpy(), lse.numpy()
+    for b, h in ((0, 0), (B - 1, H - 1)):
+        want = attention(q[b:b + 1, :, h:h + 1], k[b:b + 1, :, h * Hkv // H][:, :, None], v[b:b + 1, :, h * Hkv // H][:, :, None], 0.2, some_heads(r, b, slice(h, h + 1)))
+        within(o[b:b + 1, :, h:h + 1], want, "o")
+        within(lse[b:b + 1, h:h + 1], want, "lse")
+
+
+def test_caches_past_32_bits(hip):
+    """Rows of a sequence, and sequences, that lie more than 2^32 bytes behind the pointer: 2 sequences of 1.2 million rows of 8 heads of 128, 4.9 GB each.  Keys are zero,
+    so every probability is one over their number."""
+    B, rows, Hkv, G, dk = 2, 1200000, 8, 2, 128
+    ld, H = Hkv * dk, Hkv * G
+    k, v = hip.empty((B * rows, ld)), hip.empty((B * rows, ld))      # zeroes
+    rng = np.random.default_rng(15)
+    tail = rng.normal(size=(B, 7, Hkv, dk)).astype(np.float32) * np.float32(rows)
+    for b in range(B):
+        piece = np.ascontiguousarray(tail[b])
+        hip.check(hip.L.axhip_memcpy_h2d(v.ptr + 4 * ld * (b * rows + rows - 7), piece.ctypes.data, piece.nbytes))
+    q, d_o = (rng.normal(size=(B, 3, H, dk)).astype(np.float32) for _ in range(2))
+    dq, o, lse = hip.array(q), hip.empty(q.shape), hip.empty((B, H, 3))
+    for Sq in (1, 3):
+        hip.check(hip.L.axhip_attn_fwd(dq.ptr, H * dk, k.ptr, ld, v.ptr, ld, rows, o.ptr, H * dk, lse.ptr, B, H, Hkv, Sq, rows, dk, 0.1, None))
+        want = tail.astype(np.float64).sum(1) / rows                 # [B, Hkv, dk]
+        got = o.numpy().reshape(-1)[:B * Sq * H * dk].reshape(B, Sq, Hkv, G, dk)
+        # seven terms of a size of one, each probability off by the sums' roundings over 37500 tiles at most
+        assert np.abs(got - want[:, None, :, None]).max() <= 1e-5 * np.abs(want).max() + 1e-5
+    k_grad, v_grad = hip.empty((B * rows, ld)), hip.empty((B * rows, ld))
+    do, dqg = hip.array(d_o), hip.empty(q.shape)
+    hip.check(hip.L.axhip_attn_bwd(dq.ptr, H * dk, k.ptr, ld, v.ptr, ld, rows, o.ptr, H * dk, lse.ptr, do.ptr, H * dk, dqg.ptr, H * dk, k_grad.ptr, ld, v_grad.ptr, ld,
+                                   B, H, Hkv, 3, rows, dk, 0.1, None))
+    want = d_o.astype(np.float64).reshape(B, 3, Hkv, G, dk).sum((1, 3)) / rows
+    for b in range(B):
+        for at in (0, 40000, rows - 1):
+            row = np.empty((Hkv, dk), np.float32)
+            hip.check(hip.L.axhip_memcpy_d2h(row.ctypes.data, v_grad.ptr + 4 * ld * (b * rows + at), row.nbytes))
+            assert np.abs(row - want[b]).max() <= 1e-5 * np.abs(want).max()
+    assert (dqg.numpy() == 0).all()                                  # keys of zero
