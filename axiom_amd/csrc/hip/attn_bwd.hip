@@ -3,9 +3,14 @@
 //   dQ = scale ds K (k_attn_dq, a tile of queries over the keys that it sees), dK = scale ds^T Q and dV = P^T dO (k_attn_dkv, a tile of keys over the rows that see
 //   it, of all query heads that share it).  Scores and dP are formed by both: seven products a pair where five would do, for sums in a fixed order.
 // Operands are cut into f16 terms as in the forward pass (f16x2.h).  ds and P have no scale of their own: a running exponent for each row (or key) keeps the largest so
-// far at 2^10 to 2^15, and the sum is rescaled when it moves, as an online softmax does.  In k_attn_dkv the key is on the lane side: a lane owns key (l & 31), its
-// registers are 16 rows, and what these need (lse, delta, end, document) lies in LDS beside the block.  Rows (keys) whose sums are not finite are formed again
-// with fp32 instructions.
+// far, times the factors of what it is multiplied by, at 2^10 to 2^15, and the sum is rescaled when it moves, as an online softmax does.
+//
+// A wave owns 16 rows (or keys): two operands of them and two sums are half as many registers as for 32, so two waves share a SIMD at every head size, and one's vector
+// instructions run beside the other's products.  (32 rows a wave had one wave a SIMD from heads of 96 on, its matrix core idle two thirds of the time; what 16 cost is twice the reads from LDS
+// for a product.)  A lane owns row (l & 15) of the wave in the tiles of 32 keys: its eight values are keys 16 t + 4 (l / 16) + 0..3, t = 0, 1.  In
+// k_attn_dkv the key is on the lane side and the eight are rows, and what these need (lse, delta, end, document) lies in LDS beside the block.  Blocks are double in
+// LDS and staged by the two waves of a SIMD at different times, as in the forward pass.  Rows (keys) whose sums are not finite are formed again with fp32
+// instructions.
 #include <algorithm>
 
 #include "attn_launch.h"
@@ -14,31 +19,32 @@
 namespace {
 using namespace axhip;
 
-template <int DT>
-__device__ __forceinline__ void times(v16f (&acc)[DT], float by) {
+constexpr int WAVES = 8;
+typedef float Eight[8];
+
+template <int N>
+__device__ __forceinline__ void times(v4f (&acc)[N], float by) {
 #pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) acc[d][v] *= by;
+    for (int n = 0; n < N; n++) acc[n] *= by;
 }
 
-// Scores of a tile (products already scaled) after cap and distance; `slope` the cap's derivative.  from[v]: position less key of register v.
+// Scores of a lane (products already scaled) after cap and distance; `slope` the cap's derivative
 template <typename Distance>
-__device__ __forceinline__ void score_tile(const AttnArgs &a, v16f &s, v16f &slope, Distance distance) {
+__device__ __forceinline__ void score_tile(const AttnArgs &a, Eight &s, Eight &slope, Distance distance) {
     if (a.cap2 > 0.0f) {
         float big = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 16; v++) big = fmaxf(big, __builtin_fabsf(s[v]));
+        for (int v = 0; v < 8; v++) big = fmaxf(big, __builtin_fabsf(s[v]));
         if (__builtin_amdgcn_ballot_w64(!(big < TANH_NEAR)))
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
+            for (int v = 0; v < 8; v++) {
                 const Tanh t = tanh_of(s[v]);
                 s[v] = a.cap2 * t.value;
                 slope[v] = t.slope;
             }
         else
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
+            for (int v = 0; v < 8; v++) {
                 const float t = tanh_near(s[v]);
                 s[v] = a.cap2 * t;
                 slope[v] = __builtin_fmaf(-t, t, 1.0f);
@@ -46,7 +52,7 @@ __device__ __forceinline__ void score_tile(const AttnArgs &a, v16f &s, v16f &slo
     }
     if (a.slopes)
 #pragma unroll
-        for (int v = 0; v < 16; v++) s[v] -= distance(v);
+        for (int v = 0; v < 8; v++) s[v] -= distance(v);
 }
 
 // The next block of TILES tiles from `blk` on, below n, of which some tile's documents meet [low, high]: 64 blocks at a time, a lane each
@@ -89,40 +95,38 @@ __device__ __forceinline__ void work_of(const AttnArgs &a, const BwdGrid &grid, 
     tile = (int)(a.causal ? lin / grid.units : r8 / width);
 }
 
-// Eight waves, two a SIMD, where their registers allow it, and rows of a block
-template <int DK>
+// SETS waves side by side, 16 rows (or keys) each; where those are half of the waves, the others take the other tiles of each block
+template <int DK, int SETS>
 struct BwdGeom {
-    static constexpr int WAVES = DK <= 64 ? 8 : 4, ROWS = DK <= 32 ? 128 : 64, TILES = ROWS / 32;
+    static constexpr int ROWS = DK <= 32 ? 128 : 64, TILES = ROWS / 32, SHARES = WAVES / SETS;
     using B = Block<DK, ROWS>;
-    static constexpr int PER_SIMD = WAVES / 4;
 };
 
-template <int DK>
-struct DqGeom : BwdGeom<DK> {
-    using typename BwdGeom<DK>::B;
-    using BwdGeom<DK>::WAVES, BwdGeom<DK>::ROWS, BwdGeom<DK>::TILES;
-    static constexpr int FACTORS_AT = 2 * B::BYTES;              // of each key row, then of each value row
-    static constexpr int DOCS_AT = FACTORS_AT + ROWS * 8;
-    static constexpr int META_AT = DOCS_AT + ROWS * 4 + TILES * 8;
+template <int DK, int SETS>
+struct DqGeom : BwdGeom<DK, SETS> {
+    using Base = BwdGeom<DK, SETS>;
+    static constexpr int FACTORS_AT = 2 * Base::B::BYTES;        // of each key row, then of each value row
+    static constexpr int DOCS_AT = FACTORS_AT + Base::ROWS * 8;  // documents of the keys, then the ranges of their tiles
+    static constexpr int STAGE = (DOCS_AT + Base::ROWS * 4 + Base::TILES * 8 + 255) / 256 * 256;
+    static constexpr int META_AT = 2 * STAGE;
+    static constexpr int JOIN = DK / 16 * 1024;                  // the other share's sums: [DK / 16][64 lanes] v4f a wave
     static constexpr int SMEM = META_AT + 16 * WAVES;
-    // the other share's sums: [DT][4][64 lanes] v4f a wave
-    static constexpr int JOIN = DK / 32 * 4096;
+    static_assert(SMEM <= 160 * 1024 && SETS * JOIN <= META_AT, "LDS");
 };
 
-// SETS waves side by side along the queries, 32 rows each; where those are half of the waves, the others take the other tiles of each block
 template <int DK, int SETS, bool PAD>
-__global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIMD)) k_attn_dq(AttnArgs a, BwdGrid grid) {
-    using G = DqGeom<DK>;
+__global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid grid) {
+    using G = DqGeom<DK, SETS>;
     using B = typename G::B;
-    constexpr int KS = DK / 16, DT = DK / 32, WAVES = G::WAVES, ROWS = G::ROWS, TILES = G::TILES, SHARES = WAVES / SETS;
+    constexpr int KS = DK / 32, NT = DK / 16, ROWS = G::ROWS, TILES = G::TILES;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, part = lane >> 4;
     int64_t unit;
     int tile;
     work_of(a, grid, unit, tile);
     if (a.causal) tile = grid.tiles - 1 - tile;
     const int b = (int)(unit / a.H), head = (int)(unit - (int64_t)b * a.H), hk = head / a.G;
-    const int r = tile * 32 * SETS + wave % SETS * 32 + frow, i = r < a.Sq ? r : a.Sq - 1;
+    const int r = tile * 16 * SETS + wave % SETS * 16 + col, i = r < a.Sq ? r : a.Sq - 1;
     const bool valid = r < a.Sq;
     AttnRow row = attn_row(a, b, head, i);
     if (!valid) row.end = 0;
@@ -154,23 +158,23 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     DocRange range_here = {0, 0};
     auto load = [&](int blk) {
         const int64_t k0 = (int64_t)blk * ROWS;
-        const int end = wg_last - 1 - (int)k0;
-        const int l = (int)afresh(lane);             // (places of lanes are formed anew: registers are dearer)
+        const int end = wg_last - 1 - (int)k0, l = (int)afresh(lane);        // (places of lanes are formed anew: registers are dearer)
         ks.load(Kb + k0 * a.ldk, a.ldk, end, S::place(wave, l, a.ldk), l, a.dk);
         vs.load(Vb + k0 * a.ldv, a.ldv, end, S::place(wave, l, a.ldv), l, a.dk);
         if (docs && threadIdx.x < ROWS) doc_here = (int)threadIdx.x <= end ? a.doc_k[(int64_t)b * a.Sk + k0 + threadIdx.x] : -1;
         if (docs && threadIdx.x < TILES) range_here = TILES * blk + (int)threadIdx.x < grid.key_tiles ? ranges[TILES * blk + threadIdx.x] : DocRange{0x7fffffff, -1};
     };
-    auto stage = [&]() {
+    auto stage = [&](unsigned cur) {
+        unsigned char *at = lds + cur;
         const int l = (int)afresh(lane);
         const typename S::Place place = S::place(wave, l, 0);
-        ks.put(base, base + G::FACTORS_AT, place, l, 1.0f, a.dk);
-        vs.put(base + B::BYTES, base + G::FACTORS_AT + 4 * ROWS, place, l, 1.0f, a.dk);
-        if (docs && threadIdx.x < ROWS) reinterpret_cast<int *>(lds + G::DOCS_AT)[threadIdx.x] = doc_here;
-        if (docs && threadIdx.x < TILES) reinterpret_cast<DocRange *>(lds + G::DOCS_AT + ROWS * 4)[threadIdx.x] = range_here;
+        ks.put(base + cur, base + cur + G::FACTORS_AT, place, l, 1.0f, a.dk);
+        vs.put(base + cur + B::BYTES, base + cur + G::FACTORS_AT + 4 * ROWS, place, l, 1.0f, a.dk);
+        if (docs && threadIdx.x < ROWS) reinterpret_cast<int *>(at + G::DOCS_AT)[threadIdx.x] = doc_here;
+        if (docs && threadIdx.x < TILES) reinterpret_cast<DocRange *>(at + G::DOCS_AT + ROWS * 4)[threadIdx.x] = range_here;
     };
 
-    int blk = blocks.next(0, lane);
+    int blk = blocks.next(0, lane), ahead = blocks.n;
     if (blk < blocks.n) load(blk);
     // ---- the row: query, gradient, delta ----
     const int64_t at = ((int64_t)b * a.H + head) * a.Sq + i;
@@ -178,106 +182,111 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     float q_down, o_down, delta = 0.0f;
     {
         float x[KS][8], y[KS][8];
-        load_row<PAD>(x, a.Oin + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk, live, fhalf, a.dk);
-        load_row<PAD>(y, a.dO + ((int64_t)b * a.Sq + i) * a.lddo + (int64_t)head * a.dk, live, fhalf, a.dk);
+        load_row<PAD, 4>(x, a.Oin + ((int64_t)b * a.Sq + i) * a.ldo + (int64_t)head * a.dk, live, part, a.dk);
+        load_row<PAD, 4>(y, a.dO + ((int64_t)b * a.Sq + i) * a.lddo + (int64_t)head * a.dk, live, part, a.dk);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) delta = __builtin_fmaf(x[s][e], y[s][e], delta);
-        delta += __shfl_xor(delta, 32, 64);
-        o_down = cut_row(y, of);
-        load_row<PAD>(x, a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk, live, fhalf, a.dk);
+        delta = over_parts(delta, [](float p, float q) { return p + q; });
+        o_down = cut_row(y, most_of_parts(most_of(y)), of);
+        load_row<PAD, 4>(x, a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk, live, part, a.dk);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) x[s][e] *= a.q_up;
-        q_down = cut_row(x, qf);
+        q_down = cut_row(x, most_of_parts(most_of(x)), qf);
     }
-    if (valid && fhalf == 0) a.delta[at] = delta;
+    if (valid && part == 0 && wave < SETS) a.delta[at] = delta;
     float lse2 = live ? a.Lin[at] * LOG2E : INFINITY;
     if (lse2 == -INFINITY) lse2 = INFINITY;          // a row that saw nothing: no probability
-    if (blk < blocks.n) stage();
+    if (blk < blocks.n) {
+        stage(0);
+        ahead = blocks.next(blk + 1, lane);
+        if (ahead < blocks.n) load(ahead);
+    }
     __syncthreads();
 
-    v16f acc[DT];
+    v4f acc[NT];
 #pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) acc[d][v] = 0.0f;
+    for (int n = 0; n < NT; n++) acc[n] = v4f{0.f, 0.f, 0.f, 0.f};
     int d_up = MOST_UP;                              // acc is 2^(BIAS + d_up) times the sum: the running exponent of ds times its key row's factor
     float o_times = o_down * two_to(d_up), delta_times = delta * two_to(d_up);
     const float one = hidden_one();
 
-    const unsigned row_at = B::row_place(lane) + base, column_at = B::column_place(lane) + base;
-    auto attend = [&](int blk) {
+    const unsigned row_at = B::row_place16(lane) + base, column_at = B::column_place16(lane) + base;
+    auto attend = [&](int blk, unsigned cur) {
+        const unsigned char *here = lds + cur;
 #pragma unroll 1
-        for (int kt = wave / SETS; kt < TILES; kt += SHARES) {
+        for (int kt = wave / SETS; kt < TILES; kt += G::SHARES) {
             const int kt0 = blk * ROWS + 32 * kt;
             if (kt0 >= last) break;
             bool partly = kt0 + 32 > sure;
             if (docs) {
-                const v2i32 range = *reinterpret_cast<const v2i32 *>(lds + G::DOCS_AT + ROWS * 4 + 8 * kt);
-                const DocRange here = {__builtin_amdgcn_readfirstlane(range[0]), __builtin_amdgcn_readfirstlane(range[1])};
-                if (!here.meets(d_low, d_high)) continue;
-                partly |= here.low != here.high || here.low != d_low || d_low != d_high;
+                const v2i32 range = *reinterpret_cast<const v2i32 *>(here + G::DOCS_AT + ROWS * 4 + 8 * kt);
+                const DocRange of_keys = {__builtin_amdgcn_readfirstlane(range[0]), __builtin_amdgcn_readfirstlane(range[1])};
+                if (!of_keys.meets(d_low, d_high)) continue;
+                partly |= of_keys.low != of_keys.high || of_keys.low != d_low || d_low != d_high;
             }
-            const unsigned row_place = afresh(row_at) + 32 * kt * B::PITCH, column_place = afresh(column_at) + 32 * kt * B::PITCH;
-            v16f s, dp, slope;
-#pragma unroll
-            for (int v = 0; v < 16; v++) s[v] = dp[v] = 0.0f;
-            products<2 * KS>(
+            const unsigned tile_at = cur + 32 * kt * B::PITCH, row_place = afresh(row_at) + tile_at, column_place = afresh(column_at) + tile_at;
+            v4f sc[2], pr[2];
+            sc[0] = sc[1] = pr[0] = pr[1] = v4f{0.f, 0.f, 0.f, 0.f};
+            __builtin_amdgcn_s_setprio(1);
+            products<4 * KS>(                        // scores of both halves of the keys, then their dP
                 [&](int n, v4i (&f)[2]) {
-                    f[1] = B::rows(row_place + n / KS * B::BYTES, n % KS, 1);
-                    f[0] = B::rows(row_place + n / KS * B::BYTES, n % KS, 0);
+                    const unsigned from = row_place + n / (2 * KS) * B::BYTES;
+                    f[1] = B::rows16(from, 16 * (n & 1), n / 2 % KS, 1);
+                    f[0] = B::rows16(from, 16 * (n & 1), n / 2 % KS, 0);
                 },
                 [&](int n, const v4i (&f)[2]) {
-                    if (n < KS) s = mfma_cut(f, qf[n % KS], s);
-                    else dp = mfma_cut(f, of[n % KS], dp);
+                    if (n < 2 * KS) sc[n & 1] = mfma_cut16(f, qf[n / 2 % KS], sc[n & 1]);
+                    else pr[n & 1] = mfma_cut16(f, of[n / 2 % KS], pr[n & 1]);
                 });
-            auto factors = [&](int what, int g) {    // of keys 8 g + 4 * half + 0..3 of the tile
-                return *reinterpret_cast<const v4f *>(lds + G::FACTORS_AT + what * ROWS * 4 + 4 * (32 * kt + 8 * g + 4 * fhalf));
+            __builtin_amdgcn_s_setprio(0);
+            auto factors = [&](int what, int t) {    // of keys 16 t + 4 part + 0..3 of the tile
+                return *reinterpret_cast<const v4f *>(here + G::FACTORS_AT + what * ROWS * 4 + 4 * (32 * kt + 16 * t + 4 * part));
             };
+            Eight s, slope;
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const v4f f = factors(0, g);
+            for (int t = 0; t < 2; t++) {
+                const v4f f = factors(0, t);
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e] * q_down;
+                for (int e = 0; e < 4; e++) s[4 * t + e] = sc[t][e] * f[e] * q_down;
             }
-            const float from = (float)(row.p - kt0 - 4 * fhalf);
-            score_tile(a, s, slope, [&](int v) { return row.slope2 * __builtin_fabsf(from - (float)(8 * (v >> 2) + (v & 3))); });
+            const float from = (float)(row.p - kt0 - 4 * part);
+            score_tile(a, s, slope, [&](int v) { return row.slope2 * __builtin_fabsf(from - (float)(16 * (v >> 2) + (v & 3))); });
             if (partly) {
-                const int end = row.end - kt0 - 4 * fhalf;
+                const int end = row.end - kt0 - 4 * part;
 #pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (8 * (v >> 2) + (v & 3) >= end) s[v] = -INFINITY;
-                if (docs) {
+                for (int v = 0; v < 8; v++)
+                    if (16 * (v >> 2) + (v & 3) >= end) s[v] = -INFINITY;
+                if (docs)
 #pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        const v4i d = *reinterpret_cast<const v4i *>(lds + G::DOCS_AT + 4 * (32 * kt + 8 * g + 4 * fhalf));
+                    for (int t = 0; t < 2; t++) {
+                        const v4i d = *reinterpret_cast<const v4i *>(here + G::DOCS_AT + 4 * (32 * kt + 16 * t + 4 * part));
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (d[e] != row.doc) s[4 * g + e] = -INFINITY;
+                            if (d[e] != row.doc) s[4 * t + e] = -INFINITY;
                     }
-                }
             }
             // ds times its key row's factor and 2^d_up, which is in o_times and delta_times
-            v16f x;
+            Eight x;
             float most;
             auto form = [&]() {
                 most = 0.0f;
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const v4f kf = factors(0, g), vf = factors(1, g);
+                for (int t = 0; t < 2; t++) {
+                    const v4f kf = factors(0, t), vf = factors(1, t);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int v = 4 * g + e;
-                        x[v] = __builtin_amdgcn_exp2f(s[v] - lse2) * __builtin_fmaf(dp[v] * vf[e], o_times, -delta_times);
+                        const int v = 4 * t + e;
+                        x[v] = __builtin_amdgcn_exp2f(s[v] - lse2) * __builtin_fmaf(pr[t][e] * vf[e], o_times, -delta_times);
                         if (a.cap2 > 0.0f) x[v] *= slope[v];
                         x[v] *= kf[e];
                         most = fmaxf(most, __builtin_fabsf(x[v]));
                     }
                 }
-                most = fmaxf(most, __shfl_xor(most, 32, 64));
+                most = most_of_parts(most);
             };
             form();
             if (__builtin_amdgcn_ballot_w64(most > ROOM)) {      // (always for the first that are not zero)
@@ -294,97 +303,92 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
                 times(acc, two_to(d_up - before));
                 form();
             }
-            v4i df[2][2];
-            cut_scaled(x, 0, one, df[0]);
-            cut_scaled(x, 1, one, df[1]);
-            products<2 * DT>(
+            v4i df[2];
+            cut_scaled(x, one, df);
+            __builtin_amdgcn_s_setprio(1);
+            products<NT>(
                 [&](int n, v4i (&f)[2]) {
-                    f[1] = B::columns(column_place, 16 * (n / DT), n % DT, 1);
-                    f[0] = B::columns(column_place, 16 * (n / DT), n % DT, 0);
+                    f[1] = B::columns16(column_place, n, 1);
+                    f[0] = B::columns16(column_place, n, 0);
                 },
-                [&](int n, const v4i (&f)[2]) { acc[n % DT] = mfma_cut(f, df[n / DT], acc[n % DT]); });
+                [&](int n, const v4i (&f)[2]) { acc[n] = mfma_cut16(f, df, acc[n]); });
+            __builtin_amdgcn_s_setprio(0);
         }
     };
+    unsigned cur = 0;
     while (blk < blocks.n) {
-        const int ahead = blocks.next(blk + 1, lane);
-        if (ahead < blocks.n) load(ahead);
-        attend(blk);
-        __syncthreads();                             // the block has been read
-        if (ahead < blocks.n) {
-            stage();
-            __syncthreads();
-        }
+        const bool more = ahead < blocks.n;
+        int after = blocks.n;
+        auto bring = [&]() {
+            stage(cur ^ G::STAGE);
+            after = blocks.next(ahead + 1, lane);
+            if (after < blocks.n) load(after);
+        };
+        if (more && wave >= 4) bring();
+        attend(blk, cur);
+        if (more && wave < 4) bring();
+        __syncthreads();
         blk = ahead;
+        ahead = after;
+        cur ^= G::STAGE;
     }
 
     times(acc, two_to(-d_up - BIAS));
-    if constexpr (SHARES == 2) {                     // the other share's keys (the last barrier has passed: no block is read any more)
+    if constexpr (G::SHARES == 2) {                  // the other share's keys (the last barrier has passed: no block is read any more)
         v4f *sums = reinterpret_cast<v4f *>(lds + wave % SETS * G::JOIN) + lane;
         if (wave >= SETS)
 #pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) sums[64 * (4 * d + g)] = v4f{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+            for (int n = 0; n < NT; n++) sums[64 * n] = acc[n];
         __syncthreads();
         if (wave >= SETS) return;
 #pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const v4f sum = sums[64 * (4 * d + g)];
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[d][4 * g + e] += sum[e];
-            }
+        for (int n = 0; n < NT; n++) acc[n] += sums[64 * n];
     }
     float seen = 0.0f;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int v = 0; v < 16; v++) seen = __builtin_fmaf(acc[d][v], 0.0f, seen);
+        for (int e = 0; e < 4; e++) seen = __builtin_fmaf(acc[n][e], 0.0f, seen);
     uint64_t again = __builtin_amdgcn_ballot_w64(live && !(seen == 0.0f));
     again |= again >> 32;
-    if (valid && !((again >> frow) & 1)) {
+    again = (again | again >> 16) & 0xffff;
+    if (valid && !((again >> col) & 1)) {
         float *dq = a.dQ + ((int64_t)b * a.Sq + i) * a.lddq + (int64_t)head * a.dk;
 #pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int col = 32 * d + 8 * g + 4 * fhalf;
-                v4f out;
-#pragma unroll
-                for (int e = 0; e < 4; e++) out[e] = live ? acc[d][4 * g + e] * a.scale : 0.0f;
-                if (!PAD || col < a.dk) *reinterpret_cast<v4f *>(dq + col) = out;
-            }
+        for (int n = 0; n < NT; n++) {
+            const int c = 16 * n + 4 * part;
+            if (!PAD || c < a.dk) *reinterpret_cast<v4f *>(dq + c) = live ? acc[n] * a.scale : v4f{0.f, 0.f, 0.f, 0.f};
+        }
     }
     for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) {
         const int n = __builtin_ctz(rest);
-        attn_dq_row(a, b, head, __builtin_amdgcn_readlane(i, n), lane);
+        attn_dq_row(a, b, head, __builtin_amdgcn_readlane(i, n), (int)afresh(lane));
     }
 }
 
-template <int DK>
-struct DkvGeom : BwdGeom<DK> {
-    using typename BwdGeom<DK>::B;
-    using BwdGeom<DK>::WAVES, BwdGeom<DK>::ROWS, BwdGeom<DK>::TILES;
-    static constexpr int ROW_AT = 2 * B::BYTES;                  // of each row: factors of Q and dO, lse, delta, slope (floats), end, position, document (ints)
-    static constexpr int TILE_AT = ROW_AT + ROWS * 32;           // of each 32 rows: last end, first end, range of documents
-    static constexpr int SMEM = TILE_AT + TILES * 16;
-    static constexpr int JOIN = DK / 32 * 8192;      // the other share's sums, of both gradients
+template <int DK, int SETS>
+struct DkvGeom : BwdGeom<DK, SETS> {
+    using Base = BwdGeom<DK, SETS>;
+    static constexpr int ROW_AT = 2 * Base::B::BYTES;            // of each row: factors of Q and dO, lse, delta, slope (floats), end, position, document (ints)
+    static constexpr int TILE_AT = ROW_AT + Base::ROWS * 32;     // of each 32 rows: last end, first end, range of documents
+    static constexpr int STAGE = (TILE_AT + Base::TILES * 16 + 255) / 256 * 256;
+    static constexpr int JOIN = DK / 16 * 2048;                  // the other share's sums, of both gradients
+    static constexpr int SMEM = 2 * STAGE;
+    static_assert(SMEM <= 160 * 1024 && SETS * JOIN <= SMEM, "LDS");
 };
 
-// KW waves side by side along the keys, 32 each, and the tiles of rows shared out as above
-template <int DK, int KW, bool PAD>
-__global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIMD)) k_attn_dkv(AttnArgs a, BwdGrid grid) {
-    using G = DkvGeom<DK>;
+template <int DK, int SETS, bool PAD>
+__global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid grid) {
+    using G = DkvGeom<DK, SETS>;
     using B = typename G::B;
-    constexpr int KS = DK / 16, DT = DK / 32, WAVES = G::WAVES, ROWS = G::ROWS, TILES = G::TILES, SHARES = WAVES / KW;
+    constexpr int KS = DK / 32, NT = DK / 16, ROWS = G::ROWS, TILES = G::TILES;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, part = lane >> 4;
     int64_t unit;
     int tile;                                        // (causal: the first keys are those that most rows see)
     work_of(a, grid, unit, tile);
     const int b = (int)(unit / a.Hkv), hk = (int)(unit - (int64_t)b * a.Hkv);
-    const int k0 = tile * 32 * KW, kw0 = k0 + wave % KW * 32, key = kw0 + frow;
+    const int k0 = tile * 16 * SETS, kw0 = k0 + wave % SETS * 16, key = kw0 + col;
     const AttnSeq seq = attn_seq(a, b);
     const int len = seq.len, start = seq.start;
     const bool valid = key < a.Sk, live = key < len, docs = a.doc_q != nullptr;
@@ -396,13 +400,13 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
         d_low = wg_low = 0x7fffffff;
         d_high = wg_high = -1;
 #pragma unroll
-        for (int w = 0; w < KW; w++)
+        for (int w = 0; w < SETS / 2; w++)
             if (k0 / 32 + w < grid.key_tiles) {
                 const DocRange range = ranges[k0 / 32 + w];
                 const int low = range.low < 0 ? ~range.low : range.low;
                 wg_low = min(wg_low, low);
                 wg_high = max(wg_high, range.high);
-                if (w == wave % KW) {
+                if (w == wave % SETS / 2) {
                     d_low = low;
                     d_high = range.high;
                 }
@@ -424,7 +428,7 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     const DocRange *row_ranges = docs ? grid.row_ranges + (int64_t)b * grid.row_tiles : nullptr;
     Blocks<TILES> blocks(row_ranges, rows_end > 0 ? (rows_end + ROWS - 1) / ROWS : 0, grid.row_tiles, wg_low, wg_high);
 
-    // head `g` of the group, block `blk` of it: the place of the work, and the next one
+    // head `g` of the group, block `blk` of it: the place of the work
     struct Place {
         int g, blk;
     };
@@ -443,8 +447,7 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
     float r_lse = 0.0f, r_delta = 0.0f;
     int r_doc = 0;
     auto load = [&](Place p) {
-        const int head = hk * a.G + p.g, i0 = p.blk * ROWS, end = rows_end - 1 - i0;
-        const int l = (int)afresh(lane);
+        const int head = hk * a.G + p.g, i0 = p.blk * ROWS, end = rows_end - 1 - i0, l = (int)afresh(lane);
         qs.load(a.Q + ((int64_t)b * a.Sq + i0) * a.ldq + (int64_t)head * a.dk, a.ldq, end, S::place(wave, l, a.ldq), l, a.dk);
         os.load(a.dO + ((int64_t)b * a.Sq + i0) * a.lddo + (int64_t)head * a.dk, a.lddo, end, S::place(wave, l, a.lddo), l, a.dk);
         if (threadIdx.x < ROWS) {
@@ -455,17 +458,16 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
             if (docs) r_doc = a.doc_q[(int64_t)b * a.Sq + i];
         }
     };
-    auto stage = [&](Place p) {
-        float *of_rows = reinterpret_cast<float *>(lds + G::ROW_AT);
+    auto stage = [&](Place p, unsigned cur) {
         const int l = (int)afresh(lane);
         const typename S::Place place = S::place(wave, l, 0);
-        qs.put(base, base + G::ROW_AT, place, l, a.q_up, a.dk);
-        os.put(base + B::BYTES, base + G::ROW_AT + 4 * ROWS, place, l, 1.0f, a.dk);
+        qs.put(base + cur, base + cur + G::ROW_AT, place, l, a.q_up, a.dk);
+        os.put(base + cur + B::BYTES, base + cur + G::ROW_AT + 4 * ROWS, place, l, 1.0f, a.dk);
         if (threadIdx.x < ROWS) {
             const int i = p.blk * ROWS + threadIdx.x;
             AttnRow row = attn_row(a, seq, i, r_doc, a.slopes ? a.slopes[hk * a.G + p.g] : 0.0f);
             if (i >= rows_end) row.end = 0;
-            float *at = of_rows + threadIdx.x;
+            float *at = reinterpret_cast<float *>(lds + cur + G::ROW_AT) + threadIdx.x;
             int *ints = reinterpret_cast<int *>(at);
             at[2 * ROWS] = r_lse == -INFINITY ? INFINITY : r_lse * LOG2E;     // a row that saw nothing: no probability
             at[3 * ROWS] = row.end > 0 ? r_delta : 0.0f;
@@ -475,100 +477,105 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
             ints[7 * ROWS] = row.doc;
             RowsSeen seen = rows_seen(row);
             if (of_half_wave(row.end, [](int x, int y) { return min(x, y); }) == 0) seen.sure = 0;
-            if (frow == 0) *reinterpret_cast<v4i *>(lds + G::TILE_AT + 16 * (threadIdx.x >> 5)) = v4i{seen.last, seen.sure, seen.low, seen.high};
+            if ((lane & 31) == 0) *reinterpret_cast<v4i *>(lds + cur + G::TILE_AT + 16 * (threadIdx.x >> 5)) = v4i{seen.last, seen.sure, seen.low, seen.high};
         }
     };
 
-    Place at = settle({0, first / ROWS});
+    Place at = settle({0, first / ROWS}), ahead = {a.G, 0};
     if (at.g < a.G) load(at);
     v4i kf[KS][2], vf[KS][2];                        // this lane's key and value rows
     float k_down, v_down;
     {
         float x[KS][8];
-        load_row<PAD>(x, a.K + ((int64_t)b * a.kv_rows + key) * a.ldk + (int64_t)hk * a.dk, live, fhalf, a.dk);
-        k_down = cut_row(x, kf);
-        load_row<PAD>(x, a.V + ((int64_t)b * a.kv_rows + key) * a.ldv + (int64_t)hk * a.dk, live, fhalf, a.dk);
-        v_down = cut_row(x, vf);
+        load_row<PAD, 4>(x, a.K + ((int64_t)b * a.kv_rows + key) * a.ldk + (int64_t)hk * a.dk, live, part, a.dk);
+        k_down = cut_row(x, most_of_parts(most_of(x)), kf);
+        load_row<PAD, 4>(x, a.V + ((int64_t)b * a.kv_rows + key) * a.ldv + (int64_t)hk * a.dk, live, part, a.dk);
+        v_down = cut_row(x, most_of_parts(most_of(x)), vf);
     }
-    if (at.g < a.G) stage(at);
+    if (at.g < a.G) {
+        stage(at, 0);
+        ahead = settle({at.g, at.blk + 1});
+        if (ahead.g < a.G) load(ahead);
+    }
     __syncthreads();
 
-    v16f acc_k[DT], acc_v[DT];
+    v4f acc_k[NT], acc_v[NT];
 #pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) acc_k[d][v] = acc_v[d][v] = 0.0f;
+    for (int n = 0; n < NT; n++) acc_k[n] = acc_v[n] = v4f{0.f, 0.f, 0.f, 0.f};
     // acc_k is 2^(BIAS + d_up) times the sum of ds q, acc_v 2^(BIAS + p_up) times that of P dO: running exponents of ds and P times their rows' factors
     int d_up = MOST_UP, p_up = MOST_UP;
 
-    const unsigned row_at = B::row_place(lane) + base, column_at = B::column_place(lane) + base;
-    auto attend = [&](int qt) {
-        const v4i whole = *reinterpret_cast<const v4i *>(lds + G::TILE_AT + 16 * qt);
+    const unsigned row_at = B::row_place16(lane) + base, column_at = B::column_place16(lane) + base;
+    auto attend = [&](int qt, unsigned cur) {
+        const v4i whole = *reinterpret_cast<const v4i *>(lds + cur + G::TILE_AT + 16 * qt);
         const int t_last = __builtin_amdgcn_readfirstlane(whole[0]), t_sure = __builtin_amdgcn_readfirstlane(whole[1]);
         if (t_last <= kw0) return;
-        bool partly = t_sure < kw0 + 32;
+        bool partly = t_sure < kw0 + 16;
         if (docs) {
             const int t_low = __builtin_amdgcn_readfirstlane(whole[2]), t_high = __builtin_amdgcn_readfirstlane(whole[3]);
             if (t_high < d_low || t_low > d_high) return;
             partly = true;
         }
-        const unsigned row_place = afresh(row_at) + 32 * qt * B::PITCH, column_place = afresh(column_at) + 32 * qt * B::PITCH;
-        v16f s, dp, slope;
-#pragma unroll
-        for (int v = 0; v < 16; v++) s[v] = dp[v] = 0.0f;
-        products<2 * KS>(
+        const unsigned tile_at = cur + 32 * qt * B::PITCH, row_place = afresh(row_at) + tile_at, column_place = afresh(column_at) + tile_at;
+        v4f sc[2], pr[2];
+        sc[0] = sc[1] = pr[0] = pr[1] = v4f{0.f, 0.f, 0.f, 0.f};
+        __builtin_amdgcn_s_setprio(1);
+        products<4 * KS>(
             [&](int n, v4i (&f)[2]) {
-                f[1] = B::rows(row_place + n / KS * B::BYTES, n % KS, 1);
-                f[0] = B::rows(row_place + n / KS * B::BYTES, n % KS, 0);
+                const unsigned from = row_place + n / (2 * KS) * B::BYTES;
+                f[1] = B::rows16(from, 16 * (n & 1), n / 2 % KS, 1);
+                f[0] = B::rows16(from, 16 * (n & 1), n / 2 % KS, 0);
             },
             [&](int n, const v4i (&f)[2]) {
-                if (n < KS) s = mfma_cut(f, kf[n % KS], s);
-                else dp = mfma_cut(f, vf[n % KS], dp);
+                if (n < 2 * KS) sc[n & 1] = mfma_cut16(f, kf[n / 2 % KS], sc[n & 1]);
+                else pr[n & 1] = mfma_cut16(f, vf[n / 2 % KS], pr[n & 1]);
             });
-        const unsigned char *mine = lds + G::ROW_AT + 4 * (32 * qt + 4 * fhalf);     // rows 8 g + 0..3 from here: 16 bytes at 32 g
-        auto of_rows = [&](int what, int g) { return *reinterpret_cast<const v4i *>(mine + what * ROWS * 4 + 32 * g); };
-        auto floats = [&](int what, int g) { return __builtin_bit_cast(v4f, of_rows(what, g)); };
+        __builtin_amdgcn_s_setprio(0);
+        const unsigned char *of_tile = lds + cur + G::ROW_AT + 4 * (32 * qt + 4 * part);     // rows 16 t + 0..3 from here: 16 bytes at 64 t
+        auto of_rows = [&](int what, int t) { return *reinterpret_cast<const v4i *>(of_tile + what * ROWS * 4 + 64 * t); };
+        auto floats = [&](int what, int t) { return __builtin_bit_cast(v4f, of_rows(what, t)); };
+        Eight s, dp, slope;
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const v4f f = floats(0, g);
+        for (int t = 0; t < 2; t++) {
+            const v4f f = floats(0, t);
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e] * k_down;
+            for (int e = 0; e < 4; e++) s[4 * t + e] = sc[t][e] * f[e] * k_down;
         }
         if (a.cap2 > 0.0f || a.slopes) {
-            v16f far;
+            Eight far;
             if (a.slopes)
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const v4f sl = floats(4, g);
-                    const v4i p = of_rows(6, g);
+                for (int t = 0; t < 2; t++) {
+                    const v4f sl = floats(4, t);
+                    const v4i p = of_rows(6, t);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) far[4 * g + e] = sl[e] * __builtin_fabsf((float)(p[e] - key));
+                    for (int e = 0; e < 4; e++) far[4 * t + e] = sl[e] * __builtin_fabsf((float)(p[e] - key));
                 }
             score_tile(a, s, slope, [&](int v) { return far[v]; });
         }
         if (partly)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const v4i end = of_rows(5, g);
+            for (int t = 0; t < 2; t++) {
+                const v4i end = of_rows(5, t);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (key >= end[e]) s[4 * g + e] = -INFINITY;
+                    if (key >= end[e]) s[4 * t + e] = -INFINITY;
                 if (docs) {
-                    const v4i d = of_rows(7, g);
+                    const v4i d = of_rows(7, t);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        if (d[e] != doc) s[4 * g + e] = -INFINITY;
+                        if (d[e] != doc) s[4 * t + e] = -INFINITY;
                 }
             }
         float most_d = 0.0f, most_p = 0.0f;
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const v4f qf = floats(0, g), of = floats(1, g), lse = floats(2, g), delta = floats(3, g);
+        for (int t = 0; t < 2; t++) {
+            const v4f qf = floats(0, t), of = floats(1, t), lse = floats(2, t), delta = floats(3, t);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int v = 4 * g + e;
+                const int v = 4 * t + e;
                 const float p = __builtin_amdgcn_exp2f(s[v] - lse[e]);
-                dp[v] = p * __builtin_fmaf(dp[v] * of[e], v_down, -delta[e]);
+                dp[v] = p * __builtin_fmaf(pr[t][e] * of[e], v_down, -delta[e]);
                 if (a.cap2 > 0.0f) dp[v] *= slope[v];
                 dp[v] *= qf[e];
                 s[v] = p * of[e];
@@ -576,112 +583,93 @@ __global__ void __launch_bounds__(64 * BwdGeom<DK>::WAVES, (BwdGeom<DK>::PER_SIM
                 most_d = fmaxf(most_d, __builtin_fabsf(dp[v]));
             }
         }
-        most_p = fmaxf(most_p, __shfl_xor(most_p, 32, 64));
-        most_d = fmaxf(most_d, __shfl_xor(most_d, 32, 64));
-        if (__builtin_amdgcn_ballot_w64(outgrown(most_d, d_up))) {
-            const int grown = regrown(most_d, d_up);
-            times(acc_k, two_to(grown - d_up));
-            d_up = grown;
+        most_p = most_of_parts(most_p);
+        most_d = most_of_parts(most_d);
+        if (__builtin_amdgcn_ballot_w64(outgrown(most_d, d_up) || outgrown(most_p, p_up))) {
+            const int d_grown = regrown(most_d, d_up), p_grown = regrown(most_p, p_up);
+            times(acc_k, two_to(d_grown - d_up));
+            times(acc_v, two_to(p_grown - p_up));
+            d_up = d_grown;
+            p_up = p_grown;
         }
-        if (__builtin_amdgcn_ballot_w64(outgrown(most_p, p_up))) {
-            const int grown = regrown(most_p, p_up);
-            times(acc_v, two_to(grown - p_up));
-            p_up = grown;
-        }
-        v4i pf[2][2], df[2][2];
-#pragma unroll
-        for (int st = 0; st < 2; st++) {
-            cut_result(s, st, two_to(p_up), pf[st]);
-            cut_result(dp, st, two_to(d_up), df[st]);
-        }
-        products<4 * DT>(
+        v4i pf[2], df[2];
+        cut_halves(s, two_to(p_up), pf);
+        cut_halves(dp, two_to(d_up), df);
+        __builtin_amdgcn_s_setprio(1);
+        products<2 * NT>(
             [&](int n, v4i (&f)[2]) {
-                const unsigned at = column_place + (n < 2 * DT ? B::BYTES : 0);
-                f[1] = B::columns(at, 16 * (n / DT % 2), n % DT, 1);
-                f[0] = B::columns(at, 16 * (n / DT % 2), n % DT, 0);
+                const unsigned from = column_place + (n < NT ? B::BYTES : 0);
+                f[1] = B::columns16(from, n % NT, 1);
+                f[0] = B::columns16(from, n % NT, 0);
             },
             [&](int n, const v4i (&f)[2]) {
-                if (n < 2 * DT) acc_v[n % DT] = mfma_cut(f, pf[n / DT % 2], acc_v[n % DT]);
-                else acc_k[n % DT] = mfma_cut(f, df[n / DT % 2], acc_k[n % DT]);
+                if (n < NT) acc_v[n % NT] = mfma_cut16(f, pf, acc_v[n % NT]);
+                else acc_k[n % NT] = mfma_cut16(f, df, acc_k[n % NT]);
             });
+        __builtin_amdgcn_s_setprio(0);
     };
+    unsigned cur = 0;
     while (at.g < a.G) {
-        const Place ahead = settle({at.g, at.blk + 1});
-        if (ahead.g < a.G) load(ahead);
+        const bool more = ahead.g < a.G;
+        Place after = {a.G, 0};
+        auto bring = [&]() {
+            stage(ahead, cur ^ G::STAGE);
+            after = settle({ahead.g, ahead.blk + 1});
+            if (after.g < a.G) load(after);
+        };
+        if (more && wave >= 4) bring();
 #pragma unroll 1
-        for (int qt = wave / KW; qt < TILES; qt += SHARES) attend(qt);
-        __syncthreads();                             // the block has been read
-        if (ahead.g < a.G) {
-            stage(ahead);
-            __syncthreads();
-        }
+        for (int qt = wave / SETS; qt < TILES; qt += G::SHARES) attend(qt, cur);
+        if (more && wave < 4) bring();
+        __syncthreads();
         at = ahead;
+        ahead = after;
+        cur ^= G::STAGE;
     }
 
-    const float k_out = a.cap2 > 0.0f ? a.cap2 * LN2 : LN2;      // scale over what the rows of Q were taken times
+    times(acc_k, two_to(-d_up - BIAS) * (a.cap2 > 0.0f ? a.cap2 * LN2 : LN2));      // (scale over what the rows of Q were taken times)
+    times(acc_v, two_to(-p_up - BIAS));
+    if constexpr (G::SHARES == 2) {
+        v4f *sums = reinterpret_cast<v4f *>(lds + wave % SETS * G::JOIN) + lane;
+        if (wave >= SETS)
 #pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
-            acc_k[d][v] = acc_k[d][v] * two_to(-d_up - BIAS) * k_out;
-            acc_v[d][v] = acc_v[d][v] * two_to(-p_up - BIAS);
-        }
-    if constexpr (SHARES == 2) {
-        v4f *part = reinterpret_cast<v4f *>(lds + wave % KW * G::JOIN) + lane;
-        if (wave >= KW)
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    part[64 * (8 * d + g)] = v4f{acc_k[d][4 * g], acc_k[d][4 * g + 1], acc_k[d][4 * g + 2], acc_k[d][4 * g + 3]};
-                    part[64 * (8 * d + 4 + g)] = v4f{acc_v[d][4 * g], acc_v[d][4 * g + 1], acc_v[d][4 * g + 2], acc_v[d][4 * g + 3]};
-                }
-        __syncthreads();
-        if (wave >= KW) return;
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const v4f pk = part[64 * (8 * d + g)], pv = part[64 * (8 * d + 4 + g)];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    acc_k[d][4 * g + e] += pk[e];
-                    acc_v[d][4 * g + e] += pv[e];
-                }
+            for (int n = 0; n < NT; n++) {
+                sums[128 * n] = acc_k[n];
+                sums[128 * n + 64] = acc_v[n];
             }
+        __syncthreads();
+        if (wave >= SETS) return;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            acc_k[n] += sums[128 * n];
+            acc_v[n] += sums[128 * n + 64];
+        }
     }
     float seen = 0.0f;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int v = 0; v < 16; v++) seen = __builtin_fmaf(acc_v[d][v], 0.0f, __builtin_fmaf(acc_k[d][v], 0.0f, seen));
+        for (int e = 0; e < 4; e++) seen = __builtin_fmaf(acc_v[n][e], 0.0f, __builtin_fmaf(acc_k[n][e], 0.0f, seen));
     uint64_t again = __builtin_amdgcn_ballot_w64(live && !(seen == 0.0f));
     again |= again >> 32;
-    if (valid && !((again >> frow) & 1)) {
+    again = (again | again >> 16) & 0xffff;
+    if (valid && !((again >> col) & 1)) {
         const int64_t row = (int64_t)b * a.kv_rows + key;
         float *dk = a.dK + row * a.lddk + (int64_t)hk * a.dk, *dv = a.dV + row * a.lddv + (int64_t)hk * a.dk;
 #pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int col = 32 * d + 8 * g + 4 * fhalf;
-                v4f ok, ov;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    ok[e] = live ? acc_k[d][4 * g + e] : 0.0f;
-                    ov[e] = live ? acc_v[d][4 * g + e] : 0.0f;
-                }
-                if (!PAD || col < a.dk) {
-                    *reinterpret_cast<v4f *>(dk + col) = ok;
-                    *reinterpret_cast<v4f *>(dv + col) = ov;
-                }
+        for (int n = 0; n < NT; n++) {
+            const int c = 16 * n + 4 * part;
+            if (!PAD || c < a.dk) {
+                *reinterpret_cast<v4f *>(dk + c) = live ? acc_k[n] : v4f{0.f, 0.f, 0.f, 0.f};
+                *reinterpret_cast<v4f *>(dv + c) = live ? acc_v[n] : v4f{0.f, 0.f, 0.f, 0.f};
             }
+        }
     }
-    for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) attn_dkv_row(a, b, hk, kw0 + __builtin_ctz(rest), lane);
+    for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) attn_dkv_row(a, b, hk, kw0 + __builtin_ctz(rest), (int)afresh(lane));
 }
 
 template <auto KERNEL>
-int launch_tiles(int smem, int waves, const AttnArgs &a, BwdGrid grid, const char *what) {
+int launch_tiles(int smem, const AttnArgs &a, BwdGrid grid, const char *what) {
     static bool attr_set = false;
     if (!attr_set) {
         AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, smem), "hipFuncSetAttribute");
@@ -690,38 +678,34 @@ int launch_tiles(int smem, int waves, const AttnArgs &a, BwdGrid grid, const cha
     const int64_t all = grid.units * grid.tiles;
     for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
         const int64_t left = all - grid.first;
-        hipLaunchKernelGGL(KERNEL, dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * waves), smem, kStream, a, grid);
+        hipLaunchKernelGGL(KERNEL, dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), smem, kStream, a, grid);
         if (int rc = check_launch(what)) return rc;
     }
     return AXHIP_OK;
 }
 
 // Whether all waves go side by side over `length` rows (or keys) of each unit, or half of them: as for the tiles of the forward pass (attn_fwd.hip)
-bool all_abreast(const AttnArgs &a, int64_t units, int64_t length, int waves) {
-    const int64_t wide_tiles = (length + 32 * waves - 1) / (32 * waves), tiles = (length + 16 * waves - 1) / (16 * waves), cus = cu_count();
+bool all_abreast(const AttnArgs &a, int64_t units, int64_t length) {
+    const int64_t wide_tiles = (length + 127) / 128, tiles = (length + 63) / 64, cus = cu_count();
     if (a.causal) return std::max(6 * cus, 3 * units * (wide_tiles + 1)) <= std::max(4 * cus, 2 * units * (tiles + 1));
     return 3 * ((units * wide_tiles + cus - 1) / cus) <= 2 * ((units * tiles + cus - 1) / cus);
 }
 
 template <int DK, bool PAD>
 int launch_bwd(const AttnArgs &a, BwdGrid grid) {
-    constexpr int WAVES = BwdGeom<DK>::WAVES, HALF = WAVES / 2, DQ = DqGeom<DK>::SMEM, DKV = DkvGeom<DK>::SMEM;
-    constexpr int DQ_HALF = std::max(DQ, HALF * DqGeom<DK>::JOIN), DKV_HALF = std::max(DKV, HALF * DkvGeom<DK>::JOIN);
     if (a.Sq > 0) {
         grid.units = (int64_t)a.B * a.H;
-        const bool wide = all_abreast(a, grid.units, a.Sq, WAVES);
-        const int rows = 32 * (wide ? WAVES : HALF);
-        grid.tiles = (a.Sq + rows - 1) / rows;
-        if (int rc = wide ? launch_tiles<k_attn_dq<DK, WAVES, PAD>>(DQ, WAVES, a, grid, "attn_bwd queries")
-                          : launch_tiles<k_attn_dq<DK, HALF, PAD>>(DQ_HALF, WAVES, a, grid, "attn_bwd queries"))
+        const bool wide = all_abreast(a, grid.units, a.Sq);
+        grid.tiles = wide ? (a.Sq + 127) / 128 : (a.Sq + 63) / 64;
+        if (int rc = wide ? launch_tiles<k_attn_dq<DK, 8, PAD>>(DqGeom<DK, 8>::SMEM, a, grid, "attn_bwd queries")
+                          : launch_tiles<k_attn_dq<DK, 4, PAD>>(DqGeom<DK, 4>::SMEM, a, grid, "attn_bwd queries"))
             return rc;
     }
     grid.units = (int64_t)a.B * a.Hkv;
-    const bool wide = all_abreast(a, grid.units, a.Sk, WAVES);
-    const int keys = 32 * (wide ? WAVES : HALF);
-    grid.tiles = (a.Sk + keys - 1) / keys;
-    return wide ? launch_tiles<k_attn_dkv<DK, WAVES, PAD>>(DKV, WAVES, a, grid, "attn_bwd keys")
-                : launch_tiles<k_attn_dkv<DK, HALF, PAD>>(DKV_HALF, WAVES, a, grid, "attn_bwd keys");
+    const bool wide = all_abreast(a, grid.units, a.Sk);
+    grid.tiles = wide ? (a.Sk + 127) / 128 : (a.Sk + 63) / 64;
+    return wide ? launch_tiles<k_attn_dkv<DK, 8, PAD>>(DkvGeom<DK, 8>::SMEM, a, grid, "attn_bwd keys")
+                : launch_tiles<k_attn_dkv<DK, 4, PAD>>(DkvGeom<DK, 4>::SMEM, a, grid, "attn_bwd keys");
 }
 
 }  // namespace

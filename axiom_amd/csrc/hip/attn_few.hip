@@ -70,12 +70,13 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
     {
         const float *q = a.Q + ((int64_t)b * a.Sq + i) * a.ldq + (int64_t)head * a.dk;
         float x[KS][8];
-        load_row<PAD>(x, q, live, fhalf, a.dk);
+        load_row<PAD, 2>(x, q, live, fhalf, a.dk);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) x[s][e] *= a.q_up;
-        q_down = cut_row(x, qf);
+        const float most = most_of(x);
+        q_down = cut_row(x, fmaxf(most, __shfl_xor(most, 32, 64)), qf);
     }
     v16f acc[DT];
 #pragma unroll

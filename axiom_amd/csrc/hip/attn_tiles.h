@@ -6,14 +6,15 @@
 namespace axhip {
 
 // A block of ROWS rows of DK columns: two planes of terms, rows of 2 DK bytes whose 16-byte chunks are exchanged by row, so that both ways
-// of reading it touch every bank once: 16 lanes with one chunk of 16 rows (operands whose rows are these rows), and 32 lanes with four
-// columns of four rows each (read_columns: operands whose rows are these columns).
+// of reading it touch every bank once: 16 lanes with one chunk of 16 rows (operands whose rows are these rows), and 32 lanes with 32 columns of four rows, or 16
+// columns of eight (read_columns: operands whose rows are these columns).
 template <int DK, int ROWS>
 struct Block {
     static_assert(DK == 32 || DK == 64 || DK == 96 || DK == 128, "head dimension");
     static constexpr int PITCH = DK * 2, PLANE = ROWS * PITCH, BYTES = 2 * PLANE;
+    __device__ static constexpr int low_key(int row) { return ((row >> 2) & 1) << 1 | ((row >> 3) & 1); }
     __device__ static unsigned at(int row, int chunk) {
-        const int key = DK == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : DK == 64 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : (row >> 2) & 3;
+        const int key = low_key(row) | (DK == 128 ? (row & 3) << 2 : DK == 64 ? ((row >> 1) & 1) << 2 : 0);
         return (unsigned)(row * PITCH + ((chunk ^ key) << 4));
     }
     // A lane's place for rows(): row (lane & 31), chunk (lane >> 5); and for columns(): see read_columns.  Other rows and chunks are a distance and an exchange
@@ -32,7 +33,20 @@ struct Block {
     // 8 s .. 8 s + 7 of a result tile hold
     __device__ static v4i columns(unsigned place, int r0, int d, int term) {
         const unsigned near = moved(place, 64 * d);
-        const v2i32 a = read_columns(near + r0 * PITCH + term * PLANE), b = read_columns((near ^ 32) + (r0 + 8) * PITCH + term * PLANE);
+        const v2i32 a = read_columns(near + r0 * PITCH + term * PLANE), b = read_columns((near ^ 16) + (r0 + 8) * PITCH + term * PLANE);
+        return v4i{a[0], a[1], b[0], b[1]};
+    }
+    // The same for operands of 16 rows and 32 k: rows r0 .. r0 + 15, columns 32 k + 8 * (lane / 16) ..; and columns 16 n .. 16 n + 15, whose eight k are rows
+    // r0 + 4 * (lane / 16) + 0..3 and 16 more on: those that a lane's two result tiles hold
+    __device__ static unsigned row_place16(int lane) { return at(lane & 15, lane >> 4); }
+    __device__ static unsigned column_place16(int lane) {
+        const int l = lane & 15;
+        return at(4 * (lane >> 4) + (l >> 2), (l & 3) >> 1) + 8 * (l & 1);
+    }
+    __device__ static v4i rows16(unsigned place, int r0, int k, int term) { return read_chunk(moved(place, 64 * k) + r0 * PITCH + term * PLANE); }
+    __device__ static v4i columns16(unsigned place, int n, int term) {
+        const unsigned near = moved(place, 32 * n) + term * PLANE;
+        const v2i32 a = read_columns(near), b = read_columns(near + 16 * PITCH);
         return v4i{a[0], a[1], b[0], b[1]};
     }
 };
@@ -98,7 +112,7 @@ struct Stage {
             v4i t[2];
             cut_halves(x[i], up, t);
             if (8 * LANES == DK || 8 * chunk < DK) {
-                const unsigned there = (to ^ ((i * STEP >> 2 & 3) << 4)) + i * STEP * B::PITCH;
+                const unsigned there = (to ^ (B::low_key(i * STEP) << 4)) + i * STEP * B::PITCH;
                 write_chunk(there, t[0]);
                 write_chunk(there + B::PLANE, t[1]);
             }
@@ -107,14 +121,14 @@ struct Stage {
     }
 };
 
-// A lane's half of a row: columns 16 s + 8 * half .. + 7 for step s.  Rows that are not live are zero, and not read.
-template <bool PAD, int KS>
-__device__ __forceinline__ void load_row(float (&x)[KS][8], const float *row, bool live, int fhalf, int dk) {
+// A lane's part of a row, of PARTS: columns 8 (PARTS s + part) .. + 7 for step s.  Rows that are not live are zero, and not read.
+template <bool PAD, int PARTS, int KS>
+__device__ __forceinline__ void load_row(float (&x)[KS][8], const float *row, bool live, int part, int dk) {
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int col = 16 * s + 8 * fhalf + 4 * h;
+            const int col = 8 * (PARTS * s + part) + 4 * h;
             v4f v = {0.f, 0.f, 0.f, 0.f};
             if (live && (!PAD || col < dk)) v = *reinterpret_cast<const v4f *>(row + col);
 #pragma unroll

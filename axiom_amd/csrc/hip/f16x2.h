@@ -48,6 +48,15 @@ __device__ __forceinline__ v16f mfma_cut(const v4i (&a)[2], const v4i (&b)[2], v
 
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigned)((e < -126 ? -126 : e) + 127) << 23); }
 
+// Tiles of 16 x 16 and 32 k
+__device__ __forceinline__ v4f mfma_cut16(const v4i (&a)[2], const v4i (&b)[2], v4f c) {
+    auto one = [&](const v4i &x, const v4i &y) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0); };
+    one(a[1], b[0]);
+    one(a[0], b[1]);
+    one(a[0], b[0]);
+    return c;
+}
+
 // What a row whose largest magnitude is `most` is taken times, 2^e, e at most MOST_UP (rows of zeros); and the factor kept with it, 2^(BIAS - e): times that, what small rows
 // are multiplied by does not run out of exponents.  (Rows past 2^100 get an infinite factor, and what it meets is formed again.)  Both straight from the exponent
 // field E of `most`, which is 2^(E - 127) to twice that: e = 141 - E.
@@ -81,42 +90,58 @@ __device__ __forceinline__ int regrown(float most, int up) {
     return outgrown(most, up) ? (e < MOST_UP ? e : MOST_UP) : up;
 }
 
-// Registers 8 s .. 8 s + 7 of a result tile as an operand, times `up`
-__device__ __forceinline__ void cut_result(const v16f &x, int s, float up, v4i (&t)[2]) {
-    const float part[8] = {x[8 * s], x[8 * s + 1], x[8 * s + 2], x[8 * s + 3], x[8 * s + 4], x[8 * s + 5], x[8 * s + 6], x[8 * s + 7]};
-    cut_halves(part, up, t);
-}
 // 1.0f that the compiler does not know: times it, a mixed multiply-add is one instruction and not a conversion and a subtraction
 __device__ __forceinline__ float hidden_one() {
     float one = 1.0f;
     asm("" : "+s"(one));
     return one;
 }
-__device__ __forceinline__ void cut_scaled(const v16f &x, int s, float one, v4i (&t)[2]) {
+// Eight values that come scaled, as two terms
+__device__ __forceinline__ void cut_scaled(const float (&x)[8], float one, v4i (&t)[2]) {
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
         typedef float v2f __attribute__((ext_vector_type(2)));
-        int hi = __builtin_bit_cast(int, __builtin_convertvector(v2f{x[8 * s + e], x[8 * s + e + 1]}, v2h));
+        int hi = __builtin_bit_cast(int, __builtin_convertvector(v2f{x[e], x[e + 1]}, v2h));
         asm("" : "+v"(hi));
         const v2h h = __builtin_bit_cast(v2h, hi);
         t[0][e / 2] = hi;
-        t[1][e / 2] = __builtin_bit_cast(
-            int, __builtin_convertvector(v2f{__builtin_fmaf(x[8 * s + e], one, -(float)h[0]), __builtin_fmaf(x[8 * s + e + 1], one, -(float)h[1])}, v2h));
+        t[1][e / 2] = __builtin_bit_cast(int, __builtin_convertvector(v2f{__builtin_fmaf(x[e], one, -(float)h[0]), __builtin_fmaf(x[e + 1], one, -(float)h[1])}, v2h));
     }
 }
+// Registers 8 s .. 8 s + 7 of a result tile, scaled, as an operand
+__device__ __forceinline__ void cut_scaled(const v16f &x, int s, float one, v4i (&t)[2]) {
+    const float part[8] = {x[8 * s], x[8 * s + 1], x[8 * s + 2], x[8 * s + 3], x[8 * s + 4], x[8 * s + 5], x[8 * s + 6], x[8 * s + 7]};
+    cut_scaled(part, one, t);
+}
 
-// A lane's row (its other half in lane ^ 32) as operand terms, columns 16 s + 8 * half .. + 7 for step s; gives back what its products are taken times, 2^(-e - BIAS)
+// Over the four lanes that hold the parts of a row in 16-wide tiles (lane, lane ^ 16, lane ^ 32, lane ^ 48)
+template <typename Join>
+__device__ __forceinline__ float over_parts(float v, Join join) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = join(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return join(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
+__device__ __forceinline__ float most_of_parts(float v) {
+    return over_parts(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
+// A lane's part of a row as operand terms, whose largest value over all parts is `most`; gives back what its products are taken times, 2^(-e - BIAS)
 template <int KS>
-__device__ __forceinline__ float cut_row(float (&x)[KS][8], v4i (&t)[KS][2]) {
+__device__ __forceinline__ float cut_row(const float (&x)[KS][8], float most, v4i (&t)[KS][2]) {
+    const float up = row_up(most);
+#pragma unroll
+    for (int s = 0; s < KS; s++) cut_halves(x[s], up, t[s]);
+    return 1.0f / up * two_to(-BIAS);
+}
+template <int KS>
+__device__ __forceinline__ float most_of(const float (&x)[KS][8]) {
     float most = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int e = 0; e < 8; e++) most = fmaxf(most, __builtin_fabsf(x[s][e]));
-    const float up = row_up(fmaxf(most, __shfl_xor(most, 32, 64)));
-#pragma unroll
-    for (int s = 0; s < KS; s++) cut_halves(x[s], up, t[s]);
-    return 1.0f / up * two_to(-BIAS);
+    return most;
 }
 
 // LDS by its address in it
