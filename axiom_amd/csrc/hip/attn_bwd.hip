@@ -98,7 +98,7 @@ __device__ __forceinline__ void work_of(const AttnArgs &a, const BwdGrid &grid, 
 // SETS waves side by side, 16 rows (or keys) each; where those are half of the waves, the others take the other tiles of each block
 template <int DK, int SETS>
 struct BwdGeom {
-    static constexpr int ROWS = DK <= 32 ? 128 : 64, TILES = ROWS / 32, SHARES = WAVES / SETS;
+    static constexpr int ROWS = DK <= 64 ? 128 : 64, TILES = ROWS / 32, SHARES = WAVES / SETS;
     using B = Block<DK, ROWS>;
 };
 
@@ -231,7 +231,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
             const unsigned tile_at = cur + 32 * kt * B::PITCH, row_place = afresh(row_at) + tile_at, column_place = afresh(column_at) + tile_at;
             v4f sc[2], pr[2];
             sc[0] = sc[1] = pr[0] = pr[1] = v4f{0.f, 0.f, 0.f, 0.f};
-            __builtin_amdgcn_s_setprio(1);
             products<4 * KS>(                        // scores of both halves of the keys, then their dP
                 [&](int n, v4i (&f)[2]) {
                     const unsigned from = row_place + n / (2 * KS) * B::BYTES;
@@ -242,7 +241,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
                     if (n < 2 * KS) sc[n & 1] = mfma_cut16(f, qf[n / 2 % KS], sc[n & 1]);
                     else pr[n & 1] = mfma_cut16(f, of[n / 2 % KS], pr[n & 1]);
                 });
-            __builtin_amdgcn_s_setprio(0);
             auto factors = [&](int what, int t) {    // of keys 16 t + 4 part + 0..3 of the tile
                 return *reinterpret_cast<const v4f *>(here + G::FACTORS_AT + what * ROWS * 4 + 4 * (32 * kt + 16 * t + 4 * part));
             };
@@ -305,14 +303,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
             }
             v4i df[2];
             cut_scaled(x, one, df);
-            __builtin_amdgcn_s_setprio(1);
             products<NT>(
                 [&](int n, v4i (&f)[2]) {
                     f[1] = B::columns16(column_place, n, 1);
                     f[0] = B::columns16(column_place, n, 0);
                 },
                 [&](int n, const v4i (&f)[2]) { acc[n] = mfma_cut16(f, df, acc[n]); });
-            __builtin_amdgcn_s_setprio(0);
         }
     };
     unsigned cur = 0;
@@ -519,7 +515,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
         const unsigned tile_at = cur + 32 * qt * B::PITCH, row_place = afresh(row_at) + tile_at, column_place = afresh(column_at) + tile_at;
         v4f sc[2], pr[2];
         sc[0] = sc[1] = pr[0] = pr[1] = v4f{0.f, 0.f, 0.f, 0.f};
-        __builtin_amdgcn_s_setprio(1);
         products<4 * KS>(
             [&](int n, v4i (&f)[2]) {
                 const unsigned from = row_place + n / (2 * KS) * B::BYTES;
@@ -530,7 +525,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
                 if (n < 2 * KS) sc[n & 1] = mfma_cut16(f, kf[n / 2 % KS], sc[n & 1]);
                 else pr[n & 1] = mfma_cut16(f, vf[n / 2 % KS], pr[n & 1]);
             });
-        __builtin_amdgcn_s_setprio(0);
         const unsigned char *of_tile = lds + cur + G::ROW_AT + 4 * (32 * qt + 4 * part);     // rows 16 t + 0..3 from here: 16 bytes at 64 t
         auto of_rows = [&](int what, int t) { return *reinterpret_cast<const v4i *>(of_tile + what * ROWS * 4 + 64 * t); };
         auto floats = [&](int what, int t) { return __builtin_bit_cast(v4f, of_rows(what, t)); };
@@ -595,7 +589,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
         v4i pf[2], df[2];
         cut_halves(s, two_to(p_up), pf);
         cut_halves(dp, two_to(d_up), df);
-        __builtin_amdgcn_s_setprio(1);
         products<2 * NT>(
             [&](int n, v4i (&f)[2]) {
                 const unsigned from = column_place + (n < NT ? B::BYTES : 0);
@@ -606,7 +599,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
                 if (n < NT) acc_v[n % NT] = mfma_cut16(f, pf, acc_v[n % NT]);
                 else acc_k[n % NT] = mfma_cut16(f, df, acc_k[n % NT]);
             });
-        __builtin_amdgcn_s_setprio(0);
     };
     unsigned cur = 0;
     while (at.g < a.G) {

@@ -12,7 +12,7 @@ template <int DK, int ROWS>
 struct Block {
     static_assert(DK == 32 || DK == 64 || DK == 96 || DK == 128, "head dimension");
     static constexpr int PITCH = DK * 2, PLANE = ROWS * PITCH, BYTES = 2 * PLANE;
-    __device__ static constexpr int low_key(int row) { return ((row >> 2) & 1) << 1 | ((row >> 3) & 1); }
+    __device__ static constexpr int low_key(int row) { return ((row >> 2 ^ row >> 3) & 1) << 1 | (row >> 3 & 1); }
     __device__ static unsigned at(int row, int chunk) {
         const int key = low_key(row) | (DK == 128 ? (row & 3) << 2 : DK == 64 ? ((row >> 1) & 1) << 2 : 0);
         return (unsigned)(row * PITCH + ((chunk ^ key) << 4));
@@ -33,7 +33,7 @@ struct Block {
     // 8 s .. 8 s + 7 of a result tile hold
     __device__ static v4i columns(unsigned place, int r0, int d, int term) {
         const unsigned near = moved(place, 64 * d);
-        const v2i32 a = read_columns(near + r0 * PITCH + term * PLANE), b = read_columns((near ^ 16) + (r0 + 8) * PITCH + term * PLANE);
+        const v2i32 a = read_columns(near + r0 * PITCH + term * PLANE), b = read_columns((near ^ 48) + (r0 + 8) * PITCH + term * PLANE);
         return v4i{a[0], a[1], b[0], b[1]};
     }
     // The same for operands of 16 rows and 32 k: rows r0 .. r0 + 15, columns 32 k + 8 * (lane / 16) ..; and columns 16 n .. 16 n + 15, whose eight k are rows
