@@ -213,6 +213,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
     int d_up = MOST_UP;                              // acc is 2^(BIAS + d_up) times the sum: the running exponent of ds times its key row's factor
     float o_times = o_down * two_to(d_up), delta_times = delta * two_to(d_up);
     const float one = hidden_one();
+    // what is left to a score: q_down, where more is done to it before, in the exponential's multiply-add otherwise
+    const bool plain = a.cap2 == 0.0f && !a.slopes;
+    const float down = plain ? q_down : 1.0f;
 
     const unsigned row_at = B::row_place16(lane) + base, column_at = B::column_place16(lane) + base;
     auto attend = [&](int blk, unsigned cur) {
@@ -249,8 +252,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
             for (int t = 0; t < 2; t++) {
                 const v4f f = factors(0, t);
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[4 * t + e] = sc[t][e] * f[e] * q_down;
+                for (int e = 0; e < 4; e++) s[4 * t + e] = sc[t][e] * f[e];
             }
+            if (!plain)
+#pragma unroll
+                for (int v = 0; v < 8; v++) s[v] *= q_down;
             const float from = (float)(row.p - kt0 - 4 * part);
             score_tile(a, s, slope, [&](int v) { return row.slope2 * __builtin_fabsf(from - (float)(16 * (v >> 2) + (v & 3))); });
             if (partly) {
@@ -278,22 +284,22 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int v = 4 * t + e;
-                        x[v] = __builtin_amdgcn_exp2f(s[v] - lse2) * __builtin_fmaf(pr[t][e] * vf[e], o_times, -delta_times);
+                        x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], down, -lse2)) * __builtin_fmaf(pr[t][e] * vf[e], o_times, -delta_times);
                         if (a.cap2 > 0.0f) x[v] *= slope[v];
                         x[v] *= kf[e];
                         most = fmaxf(most, __builtin_fabsf(x[v]));
                     }
                 }
-                most = most_of_parts(most);
             };
             form();
             if (__builtin_amdgcn_ballot_w64(most > ROOM)) {      // (always for the first that are not zero)
                 const int before = d_up;
-                const bool over = most > ROOM;
+                const bool over = most_of_parts(most) > ROOM;
                 if (over) d_up -= MOST_UP;                       // a scale at which they are floats, then the right one
                 o_times = o_down * two_to(d_up);
                 delta_times = delta * two_to(d_up);
                 form();
+                most = most_of_parts(most);
                 if (over) d_up += LARGEST - __builtin_amdgcn_frexp_expf(most);
                 if (d_up > MOST_UP) d_up = MOST_UP;
                 o_times = o_down * two_to(d_up);
@@ -498,8 +504,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
     v4f acc_k[NT], acc_v[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) acc_k[n] = acc_v[n] = v4f{0.f, 0.f, 0.f, 0.f};
-    // acc_k is 2^(BIAS + d_up) times the sum of ds q, acc_v 2^(BIAS + p_up) times that of P dO: running exponents of ds and P times their rows' factors
-    int d_up = MOST_UP, p_up = MOST_UP;
+    // acc_k is 2^BIAS d_scale times the sum of ds q, acc_v 2^BIAS p_scale times that of P dO: running scales of ds and P times their rows' factors
+    float d_scale = two_to(MOST_UP), p_scale = d_scale;
+    const bool plain = a.cap2 == 0.0f && !a.slopes;  // (as for the rows' gradient)
+    const float down = plain ? k_down : 1.0f;
 
     const unsigned row_at = B::row_place16(lane) + base, column_at = B::column_place16(lane) + base;
     auto attend = [&](int qt, unsigned cur) {
@@ -533,8 +541,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
         for (int t = 0; t < 2; t++) {
             const v4f f = floats(0, t);
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[4 * t + e] = sc[t][e] * f[e] * k_down;
+            for (int e = 0; e < 4; e++) s[4 * t + e] = sc[t][e] * f[e];
         }
+        if (!plain)
+#pragma unroll
+            for (int v = 0; v < 8; v++) s[v] *= k_down;
         if (a.cap2 > 0.0f || a.slopes) {
             Eight far;
             if (a.slopes)
@@ -568,7 +579,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int v = 4 * t + e;
-                const float p = __builtin_amdgcn_exp2f(s[v] - lse[e]);
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], down, -lse[e]));
                 dp[v] = p * __builtin_fmaf(pr[t][e] * of[e], v_down, -delta[e]);
                 if (a.cap2 > 0.0f) dp[v] *= slope[v];
                 dp[v] *= qf[e];
@@ -577,18 +588,16 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
                 most_d = fmaxf(most_d, __builtin_fabsf(dp[v]));
             }
         }
-        most_p = most_of_parts(most_p);
-        most_d = most_of_parts(most_d);
-        if (__builtin_amdgcn_ballot_w64(outgrown(most_d, d_up) || outgrown(most_p, p_up))) {
-            const int d_grown = regrown(most_d, d_up), p_grown = regrown(most_p, p_up);
-            times(acc_k, two_to(d_grown - d_up));
-            times(acc_v, two_to(p_grown - p_up));
-            d_up = d_grown;
-            p_up = p_grown;
+        if (__builtin_amdgcn_ballot_w64(most_d * d_scale > ROOM || most_p * p_scale > ROOM)) {
+            const float d_next = regrown(most_of_parts(most_d), d_scale), p_next = regrown(most_of_parts(most_p), p_scale);
+            times(acc_k, d_next / d_scale);
+            times(acc_v, p_next / p_scale);
+            d_scale = d_next;
+            p_scale = p_next;
         }
         v4i pf[2], df[2];
-        cut_halves(s, two_to(p_up), pf);
-        cut_halves(dp, two_to(d_up), df);
+        cut_halves(s, p_scale, pf);
+        cut_halves(dp, d_scale, df);
         products<2 * NT>(
             [&](int n, v4i (&f)[2]) {
                 const unsigned from = column_place + (n < NT ? B::BYTES : 0);
@@ -619,8 +628,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
         cur ^= G::STAGE;
     }
 
-    times(acc_k, two_to(-d_up - BIAS) * (a.cap2 > 0.0f ? a.cap2 * LN2 : LN2));      // (scale over what the rows of Q were taken times)
-    times(acc_v, two_to(-p_up - BIAS));
+    times(acc_k, two_to(-BIAS) / d_scale * (a.cap2 > 0.0f ? a.cap2 * LN2 : LN2));      // (scale over what the rows of Q were taken times)
+    times(acc_v, two_to(-BIAS) / p_scale);
     if constexpr (G::SHARES == 2) {
         v4f *sums = reinterpret_cast<v4f *>(lds + wave % SETS * G::JOIN) + lane;
         if (wave >= SETS)

@@ -168,10 +168,10 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
                     most = fmaxf(most, x[v]);
                 }
             }
-            most = fmaxf(most, __shfl_xor(most, 32, 64));
         };
         weigh();
         if (__builtin_amdgcn_ballot_w64(most > ROOM)) {
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
             float top = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; g++) {

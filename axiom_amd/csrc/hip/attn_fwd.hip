@@ -248,10 +248,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                         most = fmaxf(most, x[v]);
                     }
                 }
-                most = fmaxf(most, __shfl_xor(most, 32, 64));
             };
             weigh();
             if (__builtin_amdgcn_ballot_w64(most > ROOM)) {      // (always for the first finite scores)
+                most = fmaxf(most, __shfl_xor(most, 32, 64));
                 float top = -INFINITY;
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
