@@ -685,7 +685,9 @@ int launch_tiles(int smem, const AttnArgs &a, BwdGrid grid, const char *what) {
     return AXHIP_OK;
 }
 
-// Whether all waves go side by side over `length` rows (or keys) of each unit, or half of them: as for the tiles of the forward pass (attn_fwd.hip)
+// Whether all waves go side by side over `length` rows (or keys) of each unit, or half of them, with twice the workgroups to share out: as for the tiles of the forward pass
+// (attn_fwd.hip; us, 64 rows -> 128: 64 heads of [2048, 64] 1038 -> 836, 32 of [1000, 128] 243 -> 188, 16 of [1500, 96] 297 -> 218, 32 causal ones of [2048, 128] 491 -> 388, but 32
+// causal ones of [600, 128] 84 -> 113, 16 of [2048, 64] 154 -> 204)
 bool all_abreast(const AttnArgs &a, int64_t units, int64_t length) {
     const int64_t wide_tiles = (length + 127) / 128, tiles = (length + 63) / 64, cus = cu_count();
     if (a.causal) return std::max(6 * cus, 3 * units * (wide_tiles + 1)) <= std::max(4 * cus, 2 * units * (tiles + 1));

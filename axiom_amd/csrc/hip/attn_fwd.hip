@@ -10,6 +10,11 @@
 // wave sees not computed, and only tiles that some row sees in part pay for the mask; with documents the ranges of ids of each 32 keys, formed by a first
 // launch, decide that.  A row whose sums are not finite (infinities or NaNs that it sees, or that a masked key of a tile holds) is formed again with fp32
 // instructions by its wave.
+//
+// What bounds it: three f16 products for each fp32 one, and vector instructions beside them.  A tile of 32 x 32 scores of heads of 128 is 48 matrix instructions, 1536 cycles
+// of a SIMD, and 290 vector ones (a quarter of them cut keys and values), which the two waves of a SIMD overlap in part: the matrix core is busy 53 % of the time, 39 % with
+// heads of 64.  64 heads of [1024, 128] without a mask take 107 to 115 us, about 310 TFLOP/s of fp32 products (a large library product in bf16 does a third of
+// 1255), 512 heads of [512, 64] 146 us, 235 TFLOP/s; 64 causal heads of [1024, 128] under a cap 92 us.
 #include <algorithm>
 
 #include "attn_launch.h"
@@ -433,8 +438,8 @@ int attn_fwd_tiles(const AttnArgs &a) {
         grid.ranges = static_cast<DocRange *>(ranges);
     }
     // Tiles of 256 or 128 rows: the wide ones, which cut keys and values half as often, take one and a half times as long and not twice, but there are half as many to share out.
-    // Rounds of tiles over the CUs, or, causal, the longest tile or all of them evenly, whichever is more (us, 128 -> 256: 64 heads of [1024, 128] 139 -> 113, causal 88 and 91, 32
-    // causal ones of [3000, 96] 260 -> 224, but 36 causal ones of [777, 80] 54 -> 78, 8 of [2048, 64] 68 -> 110).
+    // Rounds of tiles over the CUs, or, causal, the longest tile or all of them evenly, whichever is more (us, 128 -> 256: 64 heads of [1024, 128] 142 -> 115, causal 84 and 88, 32
+    // causal ones of [3000, 96] 236 -> 206, but 36 causal ones of [777, 80] 42 -> 57).
     const int64_t rows = (int64_t)grid.pack * a.Sq, wide_tiles = (rows + 255) / 256, tiles = (rows + 127) / 128, cus = cu_count();
     int64_t wide_time, time;
     if (a.causal) {
