@@ -9,8 +9,12 @@
 // instructions run beside the other's products.  (32 rows a wave had one wave a SIMD from heads of 96 on, its matrix core idle two thirds of the time; what 16 cost is twice the reads from LDS
 // for a product.)  A lane owns row (l & 15) of the wave in the tiles of 32 keys: its eight values are keys 16 t + 4 (l / 16) + 0..3, t = 0, 1.  In
 // k_attn_dkv the key is on the lane side and the eight are rows, and what these need (lse, delta, end, document) lies in LDS beside the block.  Blocks are double in
-// LDS and staged by the two waves of a SIMD at different times, as in the forward pass.  Rows (keys) whose sums are not finite are formed again with fp32
-// instructions.
+// LDS and staged by the two waves of a SIMD at different times, as in the forward pass.  Where there are few tiles, what each runs over is shared out to several workgroups, which
+// meet in memory (plan_of, met).  Rows (keys) whose sums are not finite are formed again with fp32 instructions.
+//
+// What bounds it: as in the forward pass the matrix core and the vector instructions in turn, which two waves overlap in part; the matrix core is busy 45 % of the time with heads of
+// 128, 36 % with heads of 64 (tiles of 32 rows by 16 keys: 96 matrix and 220 vector instructions, 48 and 250).  2 x 16 heads, 8 of keys, [2048, 128] without a mask take 700 us,
+// 245 TFLOP/s counted as five products, 343 of the seven that are formed; causal and under a cap 455 to 475; 4 x 16 of [2048, 64] 838 and 470.
 #include <algorithm>
 
 #include "attn_launch.h"
@@ -88,11 +92,59 @@ struct Blocks {
 };
 
 // Workgroups go to the eight XCDs in turn: a unit's tiles (a head's, a group of heads') to one, eight units at a time, or, causal, the longest tile of every unit first
-__device__ __forceinline__ void work_of(const AttnArgs &a, const BwdGrid &grid, int64_t &unit, int &tile) {
-    const int64_t lin = grid.first + blockIdx.x, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
+struct Work {
+    int64_t lin;                                 // the tile of the launch
+    int split;
+};
+__device__ __forceinline__ Work work_of(const AttnArgs &a, const BwdGrid &grid, int64_t &unit, int &tile) {
+    const int64_t at = grid.first + blockIdx.x, lin = at / grid.splits, group = lin / (8 * (int64_t)grid.tiles), r8 = lin - group * 8 * grid.tiles;
     const int64_t left = grid.units - group * 8, width = left < 8 ? left : 8;
     unit = a.causal ? lin % grid.units : group * 8 + r8 % width;
     tile = (int)(a.causal ? lin / grid.units : r8 / width);
+    return {lin, (int)(at - lin * grid.splits)};
+}
+
+// The splits of a tile meet in memory: each leaves the sums of its `mine` waves (wave w, `part` floats a split), the last to arrive adds them, in order, and true is
+// what it gets.  Parts, counter and reads are device-scope accesses (the workgroups run on XCDs with an L2 each); the wait completes a thread's stores before the
+// barrier, the barrier orders them before thread 0's increment.  `flag`: a word of LDS that is no longer read.
+template <int N>
+__device__ __forceinline__ bool met(const BwdGrid &grid, const Work &work, int part, bool mine, int w, int lane, int *flag, v4f *(&&sums)[N], int each) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    const int64_t of_tile = work.lin * grid.splits * part;
+    const int at = w * N * each * 256 + lane * 4;
+    if (mine) {
+        float *to = grid.parts + of_tile + (int64_t)work.split * part + at;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < each; i++) {
+                const v4f v = sums[n][i];
+                int64_t *there = reinterpret_cast<int64_t *>(to + (n * each + i) * 256);
+                __hip_atomic_store(there, __builtin_bit_cast(int64_t, v2f{v[0], v[1]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(there + 1, __builtin_bit_cast(int64_t, v2f{v[2], v[3]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                sums[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
+            }
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) *flag = __hip_atomic_fetch_add(grid.arrivals + work.lin, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == grid.splits - 1;
+    __syncthreads();
+    if (!*flag) return false;
+    if (mine)
+        for (int s = 0; s < grid.splits; s++) {
+            const float *from = grid.parts + of_tile + (int64_t)s * part + at;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int i = 0; i < each; i++) {
+                    const int64_t *there = reinterpret_cast<const int64_t *>(from + (n * each + i) * 256);
+                    const v2f x = __builtin_bit_cast(v2f, __hip_atomic_load(there, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                    const v2f y = __builtin_bit_cast(v2f, __hip_atomic_load(there + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                    sums[n][i] += v4f{x[0], x[1], y[0], y[1]};
+                }
+        }
+    if (threadIdx.x == 0) __hip_atomic_store(grid.arrivals + work.lin, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);       // ready for the next launch
+    return true;
 }
 
 // SETS waves side by side, 16 rows (or keys) each; where those are half of the waves, the others take the other tiles of each block
@@ -123,7 +175,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, part = lane >> 4;
     int64_t unit;
     int tile;
-    work_of(a, grid, unit, tile);
+    const Work work = work_of(a, grid, unit, tile);
     if (a.causal) tile = grid.tiles - 1 - tile;
     const int b = (int)(unit / a.H), head = (int)(unit - (int64_t)b * a.H), hk = head / a.G;
     const int r = tile * 16 * SETS + wave % SETS * 16 + col, i = r < a.Sq ? r : a.Sq - 1;
@@ -148,7 +200,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
     wg_low = __builtin_amdgcn_readfirstlane(wg_low);
     wg_high = __builtin_amdgcn_readfirstlane(wg_high);
     const DocRange *ranges = docs ? grid.key_ranges + (int64_t)b * grid.key_tiles : nullptr;
-    Blocks<TILES> blocks(ranges, (wg_last + ROWS - 1) / ROWS, grid.key_tiles, wg_low, wg_high);
+    const int64_t all_blocks = (wg_last + ROWS - 1) / ROWS;
+    Blocks<TILES> blocks(ranges, (int)(all_blocks * (work.split + 1) / grid.splits), grid.key_tiles, wg_low, wg_high);
 
     const float *Kb = a.K + (int64_t)b * a.kv_rows * a.ldk + (int64_t)hk * a.dk, *Vb = a.V + (int64_t)b * a.kv_rows * a.ldv + (int64_t)hk * a.dk;
     using S = Stage<DK, ROWS, WAVES, PAD>;
@@ -174,7 +227,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
         if (docs && threadIdx.x < TILES) reinterpret_cast<DocRange *>(at + G::DOCS_AT + ROWS * 4)[threadIdx.x] = range_here;
     };
 
-    int blk = blocks.next(0, lane), ahead = blocks.n;
+    int blk = blocks.next((int)(all_blocks * work.split / grid.splits), lane), ahead = blocks.n;
     if (blk < blocks.n) load(blk);
     // ---- the row: query, gradient, delta ----
     const int64_t at = ((int64_t)b * a.H + head) * a.Sq + i;
@@ -197,7 +250,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
             for (int e = 0; e < 8; e++) x[s][e] *= a.q_up;
         q_down = cut_row(x, most_of_parts(most_of(x)), qf);
     }
-    if (valid && part == 0 && wave < SETS) a.delta[at] = delta;
+    if (valid && part == 0 && wave < SETS && work.split == 0) a.delta[at] = delta;
     float lse2 = live ? a.Lin[at] * LOG2E : INFINITY;
     if (lse2 == -INFINITY) lse2 = INFINITY;          // a row that saw nothing: no probability
     if (blk < blocks.n) {
@@ -342,10 +395,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
 #pragma unroll
             for (int n = 0; n < NT; n++) sums[64 * n] = acc[n];
         __syncthreads();
-        if (wave >= SETS) return;
+        if (wave < SETS)
 #pragma unroll
-        for (int n = 0; n < NT; n++) acc[n] += sums[64 * n];
+            for (int n = 0; n < NT; n++) acc[n] += sums[64 * n];
     }
+    if (grid.splits > 1 && !met(grid, work, SETS * NT * 256, wave < SETS, wave, lane, reinterpret_cast<int *>(lds), {acc}, NT)) return;
+    if (wave >= SETS) return;
     float seen = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -388,7 +443,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, part = lane >> 4;
     int64_t unit;
     int tile;                                        // (causal: the first keys are those that most rows see)
-    work_of(a, grid, unit, tile);
+    const Work work = work_of(a, grid, unit, tile);
     const int b = (int)(unit / a.Hkv), hk = (int)(unit - (int64_t)b * a.Hkv);
     const int k0 = tile * 16 * SETS, kw0 = k0 + wave % SETS * 16, key = kw0 + col;
     const AttnSeq seq = attn_seq(a, b);
@@ -434,13 +489,16 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
     struct Place {
         int g, blk;
     };
+    const int first_blk = first / ROWS, of_head = blocks.n > 0 ? blocks.n - first_blk : 0;
+    const int64_t stop = (int64_t)a.G * of_head * (work.split + 1) / grid.splits;
     auto settle = [&](Place p) -> Place {            // the first place from p on with work
         while (p.g < a.G) {
             p.blk = blocks.next(p.blk, lane);
-            if (p.blk < blocks.n) return p;
-            p.g = blocks.n > 0 ? p.g + 1 : a.G;
-            p.blk = first / ROWS;
+            if (p.blk < blocks.n) break;
+            p.g++;
+            p.blk = first_blk;
         }
+        if ((int64_t)p.g * of_head + p.blk - first_blk >= stop) p.g = a.G;
         return p;
     };
     using S = Stage<DK, ROWS, WAVES, PAD>;
@@ -483,7 +541,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
         }
     };
 
-    Place at = settle({0, first / ROWS}), ahead = {a.G, 0};
+    Place at = {a.G, 0}, ahead = at;
+    if (of_head > 0) {
+        const int64_t from = (int64_t)a.G * of_head * work.split / grid.splits;
+        at = settle({(int)(from / of_head), first_blk + (int)(from % of_head)});
+    }
     if (at.g < a.G) load(at);
     v4i kf[KS][2], vf[KS][2];                        // this lane's key and value rows
     float k_down, v_down;
@@ -639,13 +701,15 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
                 sums[128 * n + 64] = acc_v[n];
             }
         __syncthreads();
-        if (wave >= SETS) return;
+        if (wave < SETS)
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            acc_k[n] += sums[128 * n];
-            acc_v[n] += sums[128 * n + 64];
-        }
+            for (int n = 0; n < NT; n++) {
+                acc_k[n] += sums[128 * n];
+                acc_v[n] += sums[128 * n + 64];
+            }
     }
+    if (grid.splits > 1 && !met(grid, work, SETS * NT * 512, wave < SETS, wave, lane, reinterpret_cast<int *>(lds), {acc_k, acc_v}, NT)) return;
+    if (wave >= SETS) return;
     float seen = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -676,7 +740,7 @@ int launch_tiles(int smem, const AttnArgs &a, BwdGrid grid, const char *what) {
         AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, smem), "hipFuncSetAttribute");
         attr_set = true;
     }
-    const int64_t all = grid.units * grid.tiles;
+    const int64_t all = grid.units * grid.tiles * grid.splits;
     for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
         const int64_t left = all - grid.first;
         hipLaunchKernelGGL(KERNEL, dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), smem, kStream, a, grid);
@@ -694,21 +758,54 @@ bool all_abreast(const AttnArgs &a, int64_t units, int64_t length) {
     return 3 * ((units * wide_tiles + cus - 1) / cus) <= 2 * ((units * tiles + cus - 1) / cus);
 }
 
+// How the `length` rows (or keys) of each unit are shared out, each tile over `blocks` blocks of the other side.  Where there are fewer tiles than CUs, or the longest causal one would
+// keep the others waiting, what they run over is split.  Time is counted in blocks, a workgroup's start and end as START of them: rounds of workgroups, or, causal, the longest or all of
+// them evenly.  (us, in one -> split: 8 heads, 2 of keys, of [500, 64] 96 -> 43, 16, 4 of keys, of [1000, 128] 281 -> 129, 32, 8 of keys, of [1024, 96] 270 -> 150, 4 of [2048, 128]
+// without a mask 218 -> 143; with workgroups for two rounds it would be 182, and 8 of [777, 80] 85 where they take 69.)
+struct Plan {
+    bool wide;
+    int64_t units;
+    int tiles, splits;
+    size_t part;                                     // floats that a split leaves, for each column of a sum
+};
+Plan plan_of(const AttnArgs &a, int64_t units, int64_t length, int64_t blocks) {
+    Plan p = {all_abreast(a, units, length), units, 0, 1, 0};
+    const int rows = p.wide ? 128 : 64;
+    p.tiles = (int)((length + rows - 1) / rows);
+    const int64_t work = units * p.tiles, cus = cu_count();
+    constexpr double START = 8.0;
+    auto time = [&](int64_t s) {
+        const double each = (double)blocks / (double)s;
+        if (a.causal) return std::max(START + each, (double)(work * s) / (double)cus * (START + 0.5 * each));
+        return (double)((work * s + cus - 1) / cus) * (START + each);
+    };
+    double best = time(1);
+    if (work < 2 * cus)
+        for (int64_t s = 2; s <= std::min<int64_t>(blocks, 32); s++)
+            if (time(s) < 0.97 * best) {
+                p.splits = (int)s;
+                best = time(s);
+            }
+    if (p.splits > 1) p.part = (size_t)work * p.splits * rows;
+    return p;
+}
+
 template <int DK, bool PAD>
-int launch_bwd(const AttnArgs &a, BwdGrid grid) {
+int launch_bwd(const AttnArgs &a, BwdGrid grid, const Plan &of_rows, const Plan &of_keys) {
+    auto set = [&](const Plan &p) {
+        grid.units = p.units;
+        grid.tiles = p.tiles;
+        grid.splits = p.splits;
+    };
     if (a.Sq > 0) {
-        grid.units = (int64_t)a.B * a.H;
-        const bool wide = all_abreast(a, grid.units, a.Sq);
-        grid.tiles = wide ? (a.Sq + 127) / 128 : (a.Sq + 63) / 64;
-        if (int rc = wide ? launch_tiles<k_attn_dq<DK, 8, PAD>>(DqGeom<DK, 8>::SMEM, a, grid, "attn_bwd queries")
-                          : launch_tiles<k_attn_dq<DK, 4, PAD>>(DqGeom<DK, 4>::SMEM, a, grid, "attn_bwd queries"))
+        set(of_rows);
+        if (int rc = of_rows.wide ? launch_tiles<k_attn_dq<DK, 8, PAD>>(DqGeom<DK, 8>::SMEM, a, grid, "attn_bwd queries")
+                                  : launch_tiles<k_attn_dq<DK, 4, PAD>>(DqGeom<DK, 4>::SMEM, a, grid, "attn_bwd queries"))
             return rc;
     }
-    grid.units = (int64_t)a.B * a.Hkv;
-    const bool wide = all_abreast(a, grid.units, a.Sk);
-    grid.tiles = wide ? (a.Sk + 127) / 128 : (a.Sk + 63) / 64;
-    return wide ? launch_tiles<k_attn_dkv<DK, 8, PAD>>(DkvGeom<DK, 8>::SMEM, a, grid, "attn_bwd keys")
-                : launch_tiles<k_attn_dkv<DK, 4, PAD>>(DkvGeom<DK, 4>::SMEM, a, grid, "attn_bwd keys");
+    set(of_keys);
+    return of_keys.wide ? launch_tiles<k_attn_dkv<DK, 8, PAD>>(DkvGeom<DK, 8>::SMEM, a, grid, "attn_bwd keys")
+                        : launch_tiles<k_attn_dkv<DK, 4, PAD>>(DkvGeom<DK, 4>::SMEM, a, grid, "attn_bwd keys");
 }
 
 }  // namespace
@@ -724,9 +821,20 @@ int attn_bwd_tiles(AttnArgs &a) {
         grid.row_tiles = (int)(((int64_t)a.Sq + 31) / 32);
         bytes += (size_t)a.B * (grid.key_tiles + grid.row_tiles) * 8;
     }
+    const int width = (a.dk + 31) / 32 * 32;
+    const int64_t rows = width <= 64 ? 128 : 64;     // of a block
+    const Plan of_rows = plan_of(a, (int64_t)a.B * a.H, a.Sq, (a.Sk + rows - 1) / rows), of_keys = plan_of(a, (int64_t)a.B * a.Hkv, a.Sk, a.G * ((a.Sq + rows - 1) / rows));
+    const size_t parts_at = (bytes + 15) & ~size_t(15), parts = std::max(of_rows.part, 2 * of_keys.part) * width * sizeof(float);
+    if (parts) {
+        bytes = parts_at + parts;
+        auto tiles = [](const Plan &p) { return p.splits > 1 ? p.units * p.tiles : 0; };
+        grid.arrivals = strip_counters((size_t)std::max(tiles(of_rows), tiles(of_keys)));
+        if (!grid.arrivals) return AXHIP_ERR_ALLOC;
+    }
     char *ws = static_cast<char *>(workspace(bytes));
     if (!ws) return AXHIP_ERR_ALLOC;
     a.delta = reinterpret_cast<float *>(ws);
+    grid.parts = reinterpret_cast<float *>(ws + parts_at);
     if (a.doc_k) {
         grid.key_ranges = reinterpret_cast<DocRange *>(ws + deltas);
         grid.row_ranges = reinterpret_cast<DocRange *>(ws + deltas + (size_t)a.B * grid.key_tiles * 8);
@@ -736,7 +844,7 @@ int attn_bwd_tiles(AttnArgs &a) {
     note_kernel("attn_grad_tiles");
     auto run = [&](auto width) {
         constexpr int DK = decltype(width)::value;
-        return a.dk < DK ? launch_bwd<DK, true>(a, grid) : launch_bwd<DK, false>(a, grid);
+        return a.dk < DK ? launch_bwd<DK, true>(a, grid, of_rows, of_keys) : launch_bwd<DK, false>(a, grid, of_rows, of_keys);
     };
     if (a.dk <= 32) return run(std::integral_constant<int, 32>());
     if (a.dk <= 64) return run(std::integral_constant<int, 64>());

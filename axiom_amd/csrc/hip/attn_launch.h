@@ -22,9 +22,11 @@ struct FewGrid {
 
 struct BwdGrid {
     int64_t first, units;                        // units: query heads, or heads of keys
-    int tiles;
+    int tiles, splits;                           // splits: of what a tile runs over, each a workgroup's
     const DocRange *key_ranges, *row_ranges;     // [B, key_tiles], [B, row_tiles], with documents
     int key_tiles, row_tiles;
+    float *parts;                                // what the splits leave
+    int *arrivals;
 };
 
 // The ranges of ids [B, S] in each 32 (8 bytes each)

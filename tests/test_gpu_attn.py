@@ -330,6 +330,18 @@ def some_heads(rules, b, heads):
     return Rules(cap=rules.cap, causal=rules.causal, **cut)
 
 
+@pytest.mark.parametrize("kind", ["plain", "causal", "documents", "everything"])
+@pytest.mark.parametrize("B,Sq,Sk,H,Hkv,dk", [(1, 500, 500, 8, 2, 64), (1, 700, 40, 4, 4, 128), (1, 40, 1500, 2, 1, 96), (1, 1100, 1100, 1, 1, 32), (1, 333, 333, 4, 1, 80), (1, 1, 700, 2, 2, 64)])
+def test_gradients_of_few_tiles(hip, B, Sq, Sk, H, Hkv, dk, kind):
+    """Few tiles of rows or keys: workgroups share what each runs over and meet in memory; the same bits whoever comes last."""
+    rng, q, k, v, d_o = draw(29, B, Sq, Sk, H, Hkv, dk)
+    rules = rules_of(kind, rng, B, Sq, Sk, H)
+    want = attention(q, k, v, 1 / dk ** 0.5, rules, d_o)
+    first, second = (check(hip, q, k, v, 1 / dk ** 0.5, rules, d_o, want=want) for _ in range(2))
+    for n in ("dq", "dk", "dv"):
+        assert first[n].tobytes() == second[n].tobytes(), n
+
+
 @pytest.mark.parametrize("dk", [20, 32, 48, 64, 80, 96, 100, 128])
 @pytest.mark.parametrize("kind", ["plain", "capped", "documents", "everything"])
 def test_many_heads(hip, dk, kind):
