@@ -13,7 +13,7 @@
 // meet in memory (plan_of, met).  Rows (keys) whose sums are not finite are formed again with fp32 instructions.
 //
 // What bounds it: as in the forward pass the matrix core and the vector instructions in turn, which two waves overlap in part; the matrix core is busy 45 % of the time with heads of
-// 128, 36 % with heads of 64 (tiles of 32 rows by 16 keys: 96 matrix and 220 vector instructions, 48 and 250).  2 x 16 heads, 8 of keys, [2048, 128] without a mask take 700 us,
+// 128, 36 % with heads of 64 (32 rows by 16 keys: 96 matrix and 320 vector instructions, 48 and 254).  2 x 16 heads, 8 of keys, [2048, 128] without a mask take 700 us,
 // 245 TFLOP/s counted as five products, 343 of the seven that are formed; causal and under a cap 455 to 475; 4 x 16 of [2048, 64] 838 and 470.
 #include <algorithm>
 
@@ -285,6 +285,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
                 partly |= of_keys.low != of_keys.high || of_keys.low != d_low || d_low != d_high;
             }
             const unsigned tile_at = cur + 32 * kt * B::PITCH, row_place = afresh(row_at) + tile_at, column_place = afresh(column_at) + tile_at;
+            v4f of_k[2], of_v[2];                    // factors of keys 16 t + 4 part + 0..3 of the tile and of their values
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const v4f *from = reinterpret_cast<const v4f *>(here + G::FACTORS_AT + 4 * (32 * kt + 16 * t + 4 * part));
+                of_k[t] = from[0];
+                of_v[t] = from[ROWS / 4];
+            }
             v4f sc[2], pr[2];
             sc[0] = sc[1] = pr[0] = pr[1] = v4f{0.f, 0.f, 0.f, 0.f};
             products<4 * KS>(                        // scores of both halves of the keys, then their dP
@@ -297,13 +304,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
                     if (n < 2 * KS) sc[n & 1] = mfma_cut16(f, qf[n / 2 % KS], sc[n & 1]);
                     else pr[n & 1] = mfma_cut16(f, of[n / 2 % KS], pr[n & 1]);
                 });
-            auto factors = [&](int what, int t) {    // of keys 16 t + 4 part + 0..3 of the tile
-                return *reinterpret_cast<const v4f *>(here + G::FACTORS_AT + what * ROWS * 4 + 4 * (32 * kt + 16 * t + 4 * part));
-            };
             Eight s, slope;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const v4f f = factors(0, t);
+                const v4f f = of_k[t];
 #pragma unroll
                 for (int e = 0; e < 4; e++) s[4 * t + e] = sc[t][e] * f[e];
             }
@@ -333,7 +337,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
                 most = 0.0f;
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    const v4f kf = factors(0, t), vf = factors(1, t);
+                    const v4f kf = of_k[t], vf = of_v[t];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int v = 4 * t + e;
@@ -439,6 +443,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
     using G = DkvGeom<DK, SETS>;
     using B = typename G::B;
     constexpr int KS = DK / 32, NT = DK / 16, ROWS = G::ROWS, TILES = G::TILES;
+    constexpr bool EARLY = DK <= 96;                // registers for what rows need before the products are formed
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, part = lane >> 4;
     int64_t unit;
@@ -583,6 +588,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
             partly = true;
         }
         const unsigned tile_at = cur + 32 * qt * B::PITCH, row_place = afresh(row_at) + tile_at, column_place = afresh(column_at) + tile_at;
+        const unsigned char *of_tile = lds + cur + G::ROW_AT + 4 * (32 * qt + 4 * part);     // rows 16 t + 0..3 from here: 16 bytes at 64 t
+        auto of_rows = [&](int what, int t) { return *reinterpret_cast<const v4i *>(of_tile + what * ROWS * 4 + 64 * t); };
+        auto floats = [&](int what, int t) { return __builtin_bit_cast(v4f, of_rows(what, t)); };
+        v4f ahead[4][2];
+        if (EARLY)
+#pragma unroll
+            for (int n = 0; n < 8; n++) ahead[n / 2][n % 2] = floats(n / 2, n % 2);
+        auto of_q = [&](int t) { return EARLY ? ahead[0][t] : floats(0, t); };
         v4f sc[2], pr[2];
         sc[0] = sc[1] = pr[0] = pr[1] = v4f{0.f, 0.f, 0.f, 0.f};
         products<4 * KS>(
@@ -595,13 +608,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
                 if (n < 2 * KS) sc[n & 1] = mfma_cut16(f, kf[n / 2 % KS], sc[n & 1]);
                 else pr[n & 1] = mfma_cut16(f, vf[n / 2 % KS], pr[n & 1]);
             });
-        const unsigned char *of_tile = lds + cur + G::ROW_AT + 4 * (32 * qt + 4 * part);     // rows 16 t + 0..3 from here: 16 bytes at 64 t
-        auto of_rows = [&](int what, int t) { return *reinterpret_cast<const v4i *>(of_tile + what * ROWS * 4 + 64 * t); };
-        auto floats = [&](int what, int t) { return __builtin_bit_cast(v4f, of_rows(what, t)); };
         Eight s, dp, slope;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const v4f f = floats(0, t);
+            const v4f f = of_q(t);
 #pragma unroll
             for (int e = 0; e < 4; e++) s[4 * t + e] = sc[t][e] * f[e];
         }
@@ -637,7 +647,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
         float most_d = 0.0f, most_p = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const v4f qf = floats(0, t), of = floats(1, t), lse = floats(2, t), delta = floats(3, t);
+            const v4f qf = of_q(t), of = EARLY ? ahead[1][t] : floats(1, t), lse = EARLY ? ahead[2][t] : floats(2, t), delta = EARLY ? ahead[3][t] : floats(3, t);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int v = 4 * t + e;

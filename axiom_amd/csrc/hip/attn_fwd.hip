@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
     using G = FwdGeom<DK, SETS>;
     using B = typename G::B;
     constexpr int KS = DK / 16, DT = DK / 32, BKV = G::BKV, TILES = BKV / 32;
+    constexpr bool EARLY = DK <= 96;                // registers for what the scores are scaled by before their products are formed
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
 
@@ -179,6 +180,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
             }
             const unsigned tile_at = cur + 32 * kt * B::PITCH, row_place = afresh(row_at) + tile_at, column_place = afresh(column_at) + tile_at;
             // ---- scores ----
+            auto factors = [&](int what, int g) {    // of keys 8 g + 4 * half + 0..3 of the tile
+                return *reinterpret_cast<const v4f *>(at + G::FACTORS_AT + what * BKV * 4 + 4 * (32 * kt + 8 * g + 4 * fhalf));
+            };
+            v4f ahead_k[4], ahead_v[4];
+            if (EARLY)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    ahead_k[g] = factors(0, g);
+                    ahead_v[g] = factors(1, g);
+                }
+            auto of_k = [&](int g) { return EARLY ? ahead_k[g] : factors(0, g); };
+            auto of_v = [&](int g) { return EARLY ? ahead_v[g] : factors(1, g); };
             v16f s;
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = 0.0f;
@@ -190,12 +203,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 },
                 [&](int k, const v4i (&f)[2]) { s = mfma_cut(f, qf[k], s); });
             __builtin_amdgcn_s_setprio(0);
-            auto factors = [&](int what, int g) {    // of keys 8 g + 4 * half + 0..3 of the tile
-                return *reinterpret_cast<const v4f *>(at + G::FACTORS_AT + what * BKV * 4 + 4 * (32 * kt + 8 * g + 4 * fhalf));
-            };
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const v4f f = factors(0, g);
+                const v4f f = of_k(g);
 #pragma unroll
                 for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e];
             }
@@ -243,7 +253,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 most = l_blk = 0.0f;
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
-                    const v4f f = factors(1, g);
+                    const v4f f = of_v(g);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int v = 4 * g + e;
@@ -260,7 +270,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 float top = -INFINITY;
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
-                    const v4f f = factors(1, g);
+                    const v4f f = of_v(g);
 #pragma unroll
                     for (int e = 0; e < 4; e++) top = fmaxf(top, __builtin_fmaf(s[4 * g + e], down, __builtin_amdgcn_logf(f[e])));
                 }
