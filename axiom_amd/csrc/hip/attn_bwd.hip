@@ -16,6 +16,7 @@
 // 128, 36 % with heads of 64 (32 rows by 16 keys: 96 matrix and 320 vector instructions, 48 and 254).  2 x 16 heads, 8 of keys, [2048, 128] without a mask take 700 us,
 // 245 TFLOP/s counted as five products, 343 of the seven that are formed; causal and under a cap 455 to 475; 4 x 16 of [2048, 64] 838 and 470.
 #include <algorithm>
+#include <cmath>
 
 #include "attn_launch.h"
 #include "attn_tiles.h"
@@ -759,19 +760,12 @@ int launch_tiles(int smem, const AttnArgs &a, BwdGrid grid, const char *what) {
     return AXHIP_OK;
 }
 
-// Whether all waves go side by side over `length` rows (or keys) of each unit, or half of them, with twice the workgroups to share out: as for the tiles of the forward pass
-// (attn_fwd.hip; us, 64 rows -> 128: 64 heads of [2048, 64] 1038 -> 836, 32 of [1000, 128] 243 -> 188, 16 of [1500, 96] 297 -> 218, 32 causal ones of [2048, 128] 491 -> 388, but 32
-// causal ones of [600, 128] 84 -> 113, 16 of [2048, 64] 154 -> 204)
-bool all_abreast(const AttnArgs &a, int64_t units, int64_t length) {
-    const int64_t wide_tiles = (length + 127) / 128, tiles = (length + 63) / 64, cus = cu_count();
-    if (a.causal) return std::max(6 * cus, 3 * units * (wide_tiles + 1)) <= std::max(4 * cus, 2 * units * (tiles + 1));
-    return 3 * ((units * wide_tiles + cus - 1) / cus) <= 2 * ((units * tiles + cus - 1) / cus);
-}
-
-// How the `length` rows (or keys) of each unit are shared out, each tile over `blocks` blocks of the other side.  Where there are fewer tiles than CUs, or the longest causal one would
-// keep the others waiting, what they run over is split.  Time is counted in blocks, a workgroup's start and end as START of them: rounds of workgroups, or, causal, the longest or all of
-// them evenly.  (us, in one -> split: 8 heads, 2 of keys, of [500, 64] 96 -> 43, 16, 4 of keys, of [1000, 128] 281 -> 129, 32, 8 of keys, of [1024, 96] 270 -> 150, 4 of [2048, 128]
-// without a mask 218 -> 143; with workgroups for two rounds it would be 182, and 8 of [777, 80] 85 where they take 69.)
+// How the `length` rows (or keys) of each unit are shared out, each tile over `blocks` blocks of the other side: tiles of 128, or of 64 with two shares, and what a tile runs over whole
+// or split to several workgroups.  The least time by a model, in blocks of a tile of 64 (of 128: WIDE each): a workgroup's start and end are START of them, and splits cost MEET and
+// PART each for the last one to add; rounds of workgroups over the CUs, or, causal, the longest, the pairs that fall on one CU, or all of them evenly.  (us:
+//   tiles of 64 -> 128: 64 heads of [2048, 64] 1038 -> 836, 32 of [1000, 128] 243 -> 188, 32 causal ones of [2048, 128] 491 -> 388, but 32 of [600, 128] 84 -> 113, 16 of [2048, 64] 154 -> 204;
+//   whole -> split: causal, 8 heads, 2 of keys, of [500, 64] 96 -> 43, 16, 4 of keys, of [1000, 128] 281 -> 129, 4 heads of [2048, 128] without a mask 218 -> 141, but with splits for two rounds 182;
+//   64 -> 128 and split in two: causal, 2 x 16, 8 of keys, of [2048, 128] under a cap 457 -> 444, of [1500, 96] 254 -> 225.)
 struct Plan {
     bool wide;
     int64_t units;
@@ -779,23 +773,29 @@ struct Plan {
     size_t part;                                     // floats that a split leaves, for each column of a sum
 };
 Plan plan_of(const AttnArgs &a, int64_t units, int64_t length, int64_t blocks) {
-    Plan p = {all_abreast(a, units, length), units, 0, 1, 0};
-    const int rows = p.wide ? 128 : 64;
-    p.tiles = (int)((length + rows - 1) / rows);
-    const int64_t work = units * p.tiles, cus = cu_count();
-    constexpr double START = 8.0;
-    auto time = [&](int64_t s) {
-        const double each = (double)blocks / (double)s;
-        if (a.causal) return std::max(START + each, (double)(work * s) / (double)cus * (START + 0.5 * each));
-        return (double)((work * s + cus - 1) / cus) * (START + each);
-    };
-    double best = time(1);
-    if (work < 2 * cus)
-        for (int64_t s = 2; s <= std::min<int64_t>(blocks, 32); s++)
-            if (time(s) < 0.97 * best) {
+    Plan p = {false, units, 0, 1, 0};
+    if (units == 0 || length == 0) return p;
+    constexpr double START = 8.0, WIDE = 1.75, MEET = 1.0, PART[] = {0.1, 0.6};
+    const int64_t cus = cu_count();
+    double best = INFINITY;
+    for (int wide = 0; wide < 2; wide++) {
+        const int64_t tiles = wide ? (length + 127) / 128 : (length + 63) / 64, work = units * tiles;
+        for (int64_t s = 1; s == 1 || (work < 2 * cus && s <= std::min<int64_t>(blocks, 32)); s++) {
+            const double each = (wide ? WIDE : 1.0) * (double)blocks / (double)s, start = START + (s > 1 ? MEET + PART[wide] * (double)s : 0.0);
+            const double rounds = (double)(work * s) / (double)cus;
+            double time = start + each;
+            if (!a.causal) time *= std::ceil(rounds);
+            else if (rounds > 2.0) time = std::max(time, rounds * (start + 0.5 * each));
+            else if (rounds > 1.0) time = std::max(time, 2.0 * (start + (1.0 - 1.0 / rounds) * each));
+            if (time < 0.98 * best) {
+                best = time;
+                p.wide = wide != 0;
+                p.tiles = (int)tiles;
                 p.splits = (int)s;
-                best = time(s);
             }
+        }
+    }
+    const int64_t work = units * p.tiles, rows = p.wide ? 128 : 64;
     if (p.splits > 1) p.part = (size_t)work * p.splits * rows;
     return p;
 }
