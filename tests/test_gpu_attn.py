@@ -331,7 +331,8 @@ def some_heads(rules, b, heads):
 
 
 @pytest.mark.parametrize("kind", ["plain", "causal", "documents", "everything"])
-@pytest.mark.parametrize("B,Sq,Sk,H,Hkv,dk", [(1, 500, 500, 8, 2, 64), (1, 700, 40, 4, 4, 128), (1, 40, 1500, 2, 1, 96), (1, 1100, 1100, 1, 1, 32), (1, 333, 333, 4, 1, 80), (1, 1, 700, 2, 2, 64)])
+@pytest.mark.parametrize("B,Sq,Sk,H,Hkv,dk", [(1, 500, 500, 8, 2, 64), (1, 700, 40, 4, 4, 128), (1, 40, 1500, 2, 1, 96), (1, 1100, 1100, 1, 1, 32), (1, 333, 333, 4, 1, 80), (1, 1, 700, 2, 2, 64),
+                                               (1, 600, 600, 16, 4, 128), (1, 128, 520, 64, 16, 128)])
 def test_gradients_of_few_tiles(hip, B, Sq, Sk, H, Hkv, dk, kind):
     """Few tiles of rows or keys: workgroups share what each runs over and meet in memory; the same bits whoever comes last."""
     rng, q, k, v, d_o = draw(29, B, Sq, Sk, H, Hkv, dk)
