@@ -164,7 +164,7 @@ __device__ __forceinline__ void attn_pair(const AttnArgs &a, const AttnRow &r, i
     ds = p * (attn_dot(d_o, v, a.dk, 1.0f) - delta) * slope;
 }
 
-// The gradient of query row i; leaves its delta for the keys' side.
+// The gradient of query row i.  (Its delta for the keys' side is left as the matrix kernel wrote it: of splits of a row's keys another workgroup did.)
 __device__ __forceinline__ void attn_dq_row(const AttnArgs &a, int b, int head, int i, int lane) {
     const AttnRow r = attn_row(a, b, head, i);
     const int hk = head / a.G;
@@ -179,7 +179,6 @@ __device__ __forceinline__ void attn_dq_row(const AttnArgs &a, int b, int head, 
         if (lane + 64 < a.dk) delta = __builtin_fmaf(d_o[lane + 64], o[lane + 64], delta);
         delta = wave_sum(delta);
     }
-    if (lane == 0) a.delta[at] = delta;
     for (int k0 = 0; k0 < r.end; k0 += 64) {
         const int key = k0 + lane;
         const bool sees = attn_sees(a, r, b, key);

@@ -140,7 +140,7 @@ def test_against_64_bits(hip, shape, kind):
 @pytest.mark.parametrize("kind", ["causal", "documents", "everything", "lens"])
 @pytest.mark.parametrize("dk", [64, 128])
 def test_garbage_where_nobody_looks(hip, kind, dk):
-    """NaN, infinities and the largest floats in rows that no query sees, and in queries that see nothing: the same bits as with zeros there."""
+    """NaN, infinities and the largest floats in rows that no query sees, and in queries that see nothing: what zeros there give."""
     say("attn garbage", kind, dk)
     B, S, H, Hkv = 2, 150, 4, 2
     rng, q, k, v, d_o = draw(7, B, S, S, H, Hkv, dk)
@@ -338,6 +338,23 @@ def test_gradients_of_few_tiles(hip, B, Sq, Sk, H, Hkv, dk, kind):
     rng, q, k, v, d_o = draw(29, B, Sq, Sk, H, Hkv, dk)
     rules = rules_of(kind, rng, B, Sq, Sk, H)
     want = attention(q, k, v, 1 / dk ** 0.5, rules, d_o)
+    first, second = (check(hip, q, k, v, 1 / dk ** 0.5, rules, d_o, want=want) for _ in range(2))
+    for n in ("dq", "dk", "dv"):
+        assert first[n].tobytes() == second[n].tobytes(), n
+
+
+@pytest.mark.parametrize("dk", [32, 64, 100, 128])
+def test_few_tiles_with_garbage_between(hip, dk):
+    """NaN in keys that no query sees, beside others in their tiles: rows formed again by the last of several workgroups, the same bits each time."""
+    S, H, Hkv = 420, 2, 1
+    rng, q, k, v, d_o = draw(31, 1, S, S, H, Hkv, dk)
+    ids = rng.integers(0, 2, (1, S)).astype(np.int32)
+    ids[0, ::37] = -1
+    rules = Rules(doc_q=ids, doc_k=ids)
+    hidden = ids[0] < 0
+    k[0, hidden] = v[0, hidden] = q[0, hidden] = d_o[0, hidden] = 0
+    want = attention(q, k, v, 1 / dk ** 0.5, rules, d_o)
+    k[0, hidden] = v[0, hidden] = q[0, hidden] = d_o[0, hidden] = np.nan
     first, second = (check(hip, q, k, v, 1 / dk ** 0.5, rules, d_o, want=want) for _ in range(2))
     for n in ("dq", "dk", "dv"):
         assert first[n].tobytes() == second[n].tobytes(), n
