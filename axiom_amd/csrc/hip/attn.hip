@@ -30,6 +30,7 @@ int attn_arguments(const char *who, AttnArgs &a, const Tensor *tensors, int n, i
     axhip_attn_rules r = {};
     if (rules) r = *rules;
     if (!(r.cap >= 0.0f) || isinf(r.cap)) return fail(AXHIP_ERR_SHAPE, "%s: the cap must be zero or positive", who);
+    if (r.cap > 0.0f && isfinite(scale) && isinf(scale / r.cap)) return fail(AXHIP_ERR_SHAPE, "%s: the scale over the cap overflows", who);
     if (r.prefix && !r.causal) return fail(AXHIP_ERR_SHAPE, "%s: a prefix without a causal mask", who);
     if ((r.doc_q == nullptr) != (r.doc_k == nullptr)) return fail(AXHIP_ERR_NULL_ARG, "%s: documents of queries and of keys, or neither", who);
     a.kv_rows = kv_rows;

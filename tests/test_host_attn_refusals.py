@@ -80,7 +80,7 @@ for f in (fwd, bwd):
         assert f(dk=dk, ldq=1024, ldk=1024, ldv=1024, ldo=1024) == 10, dk
     for bad in (dict(B=-1), dict(H=0), dict(Hkv=0), dict(H=3), dict(Sq=-1), dict(Sk=-1), dict(Sq=(1 << 24) + 1), dict(Sk=(1 << 24) + 1, kv_rows=1 << 25), dict(kv_rows=31),
                 dict(ldq=255), dict(ldq=258), dict(ldk=124), dict(ldv=124), dict(ldo=252), dict(ldk=(1 << 22) + 4), dict(B=1 << 23), dict(kv_rows=1 << 41),
-                dict(rules=AttnRules(cap=-1.0)), dict(rules=AttnRules(cap=nan)), dict(rules=AttnRules(cap=inf)), dict(rules=AttnRules(prefix=P[9]))):
+                dict(rules=AttnRules(cap=-1.0)), dict(rules=AttnRules(cap=nan)), dict(rules=AttnRules(cap=inf)), dict(rules=AttnRules(cap=1e-40)), dict(rules=AttnRules(prefix=P[9]))):
         assert f(**bad) == 3, bad
     assert f(rules=AttnRules(doc_q=P[9])) == 1 and f(rules=AttnRules(doc_k=P[9])) == 1
 assert bwd(lse=None) == 1 and bwd(do=None) == 1 and bwd(do=P[5] + 8) == 3
