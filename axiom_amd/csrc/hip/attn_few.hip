@@ -332,7 +332,8 @@ namespace axhip {
 // wider heads have one workgroup a CU and twice the work), and every further round of workgroups its start.  Within a few per cent where it is close (us, tiles -> this: 1 token
 // of 8 sequences over 1000 keys, 8 heads of 32 25.0 -> 13.4, 4 x 4 of [512, 64] causal 22.5 -> 11.8, 16 queries of 4 heads over 16000 keys, 8 heads of 128 711 -> 94, 4 x 2 x 8 of
 // [2048, 32] causal 47 -> 34; the other side 32 of [1024, 96] causal 53 -> 146, 64 of [400, 128] 38 -> 93, 128 of [512, 64] 43 -> 70).  Over 135 random calls it chose
-// the slower one 7 times, by 1.8 times at most.
+// the slower one 7 times, by 1.8 times at most.  Documents hide much of what tiles would walk, which the host cannot know, and cost them a launch; this form fetches what
+// is hidden: it has to be a quarter ahead (42 calls of 2, 7 and 30 documents that it takes by that: 1.34 in the mean, 0.77 to 2.6).
 bool attn_fwd_few(const AttnArgs &a, int &rc) {
     const int64_t rows = (int64_t)a.G * a.Sq, cus = cu_count();
     FewGrid grid = {};
@@ -349,11 +350,11 @@ bool attn_fwd_few(const AttnArgs &a, int &rc) {
         constexpr double TILE_STEP[] = {0.65, 0.95, 1.5, 1.5}, FEW_STEP[] = {1.1e-3, 1.8e-3, 8e-3, 8e-3};
         const int64_t big = (int64_t)a.B * (a.H / pack) * (((int64_t)pack * a.Sq + 127) / 128);
         const int64_t room = cus * (width < 2 ? 2 : 1), few_rounds = (units * splits + room - 1) / room;
-        if (big > cus || a.doc_k) return false;      // (more tiles than CUs never lost to this form; and it fetches what a document hides)
+        if (big > cus) return false;                 // (more tiles than CUs never lost to this form)
         const double loaded = (double)big / (double)cus, seen = a.causal && a.Sq == a.Sk ? 0.5 : 1.0;
         const double tile_time = 6.0 + (double)tiles * TILE_STEP[width] * (1.0 + 0.45 * loaded);
         const double few_time = 5.5 + (splits > 1 ? 1.5 : 0.0) + 6.0 * (double)(few_rounds - 1) + (double)(units * tiles) * seen * FEW_STEP[width];
-        if (few_time >= tile_time) return false;
+        if (few_time >= (a.doc_k ? 0.75 * (tile_time + 5.0) : tile_time)) return false;
     }
     auto run = [&](auto width) {
         constexpr int DK = decltype(width)::value;
