@@ -56,6 +56,7 @@ SIGNATURES = {
     "ax_compute_fill": (C.c_int, [TP, C.c_double]), "ax_compute_copy": (C.c_int, [TP, TP]),
     "ax_hip_sdpa_fwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, i64, i64, i64,
                                  C.c_float, C.c_bool, C.c_void_p]),
+    "ax_hip_sdpa_bwd": (C.c_int, [C.c_void_p] * 9 + [i64, i64, i64, C.c_float, C.c_bool, C.c_void_p]),
     "ax_compute_sum": (C.c_int, [TP, C.c_int, TP]), "ax_compute_axpy": (C.c_int, [TP, C.c_float, TP]),
     **{"ax_compute_" + n: (C.c_int, [TP, TP, TP]) for n in ("add", "sub", "mul", "div", "equal", "greater", "add_relu")},
     **{"ax_compute_" + n: (C.c_int, [TP, TP]) for n in ("neg", "abs", "exp", "log", "sqrt", "square", "sigmoid", "tanh",

@@ -12,9 +12,9 @@
 // instructions by its wave.
 //
 // What bounds it: three f16 products for each fp32 one, and vector instructions beside them.  A tile of 32 x 32 scores of heads of 128 is 48 matrix instructions, 1536 cycles
-// of a SIMD, and 290 vector ones (a quarter of them cut keys and values), which the two waves of a SIMD overlap in part: the matrix core is busy 53 % of the time, 39 % with
+// of a SIMD, and 290 vector ones (a quarter of them cut keys and values), which the two waves of a SIMD overlap in part: the matrix core is busy 53 % of the time, 41 % with
 // heads of 64.  64 heads of [1024, 128] without a mask take 107 to 115 us, about 310 TFLOP/s of fp32 products (a large library product in bf16 does a third of
-// 1255), 512 heads of [512, 64] 146 us, 235 TFLOP/s; 64 causal heads of [1024, 128] under a cap 92 us.
+// 1255), 512 heads of [512, 64] 151 us, 228 TFLOP/s; 64 causal heads of [1024, 128] under a cap 91 us.
 #include <algorithm>
 
 #include "attn_launch.h"

@@ -572,6 +572,18 @@ ax_status_t ax_hip_sdpa_fwd(const float *Q, const float *K, const float *V, floa
     return lift(axhip_sdpa_fwd(Q, K, V, out, L, BH, S, dk, scale, causal ? 1 : 0), "hip sdpa_fwd");
 }
 
+/* Its gradient, with the signature of the `sdpa_bwd` member, from O and the log-sum-exp L; the probabilities are formed again,
+ * whether P_saved is given or not.  The extension table does not carry it, since its other backward members are not provided either. */
+ax_status_t ax_hip_sdpa_bwd(const float *Q, const float *K, const float *V, const float *O, const float *dO, const float *L,
+                            float *dQ, float *dK, float *dV, int64_t BH, int64_t S, int64_t dk, float scale, bool causal,
+                            const float *P_saved) {
+    (void)P_saved;
+    axhip_attn_rules rules = {0};
+    rules.causal = causal ? 1 : 0;
+    return lift(axhip_attn_bwd(Q, dk, K, dk, V, dk, S, O, dk, L, dO, dk, dQ, dk, dK, dk, dV, dk, BH, 1, 1, S, S, dk, scale, &rules),
+                "hip sdpa_bwd");
+}
+
 static ax_status_t ext_sdpa_fwd_rows(const float *Q, const float *K, const float *V, int64_t ld, float *out, int64_t ldo,
                                      float *L, int64_t B, int64_t H, int64_t S, int64_t dk, float scale, bool causal) {
     return lift(axhip_sdpa_fwd_rows(Q, K, V, ld, out, ldo, L, B, H, S, dk, scale, causal ? 1 : 0), "hip sdpa_fwd_rows");

@@ -139,6 +139,10 @@ const ax_backend_ops_t *ax_hip_ops_for_device(ax_device_t as_device);
  * out are [BH, S, dk] fp32, L is [BH, S] or NULL; P_save must be NULL. */
 ax_status_t ax_hip_sdpa_fwd(const float *Q, const float *K, const float *V, float *out, float *L,
                             int64_t BH, int64_t S, int64_t dk, float scale, bool causal, float *P_save);
+/* Its gradient, with the arguments of the sdpa_bwd member: from O and L as the forward pass gave them; P_saved is not read. */
+ax_status_t ax_hip_sdpa_bwd(const float *Q, const float *K, const float *V, const float *O, const float *dO, const float *L,
+                            float *dQ, float *dK, float *dV, int64_t BH, int64_t S, int64_t dk, float scale, bool causal,
+                            const float *P_saved);
 
 #ifdef __cplusplus
 }

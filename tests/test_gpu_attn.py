@@ -416,6 +416,28 @@ def test_which_form_takes_it(hip, B, H, Hkv, Sq, Sk, dk, form, kind):
         within(lse[b:b + 1, h:h + 1], want, "lse")
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_backward_with_the_extension_signature(hip, causal):
+    """ax_hip_sdpa_fwd and ax_hip_sdpa_bwd, one after the other, on device memory"""
+    from axiom_amd.axiom import Axiom
+    ax = Axiom()
+    assert ax.L.ax_init() == 0, ax.err()
+    BH, S, dk = 6, 150, 64
+    rng, q, k, v, d_o = draw(41, BH, S, S, 1, 1, dk)
+    want = attention(q, k, v, 0.125, Rules(causal=int(causal)), d_o)
+    dq, dk_, dv, do = (hip.array(x.reshape(BH, S, dk)) for x in (q, k, v, d_o))
+    o, lse, *grads = (hip.array(np.full(s, 7, np.float32)) for s in ((BH, S, dk), (BH, S)) + ((BH, S, dk),) * 3)
+    assert ax.L.ax_hip_sdpa_fwd(dq.ptr, dk_.ptr, dv.ptr, o.ptr, lse.ptr, BH, S, dk, 0.125, causal, None) == 0
+    # the gradient's bounds hold for an O and L that are rounded once
+    o, lse = hip.array(want["o"].astype(np.float32).reshape(BH, S, dk)), hip.array(want["lse"].astype(np.float32).reshape(BH, S))
+    args = [dq.ptr, dk_.ptr, dv.ptr, o.ptr, do.ptr, lse.ptr, *(g.ptr for g in grads), BH, S, dk, 0.125, causal, None]
+    assert ax.L.ax_hip_sdpa_bwd(*args) == 0
+    for n, g, x in zip(("dq", "dk", "dv"), grads, (q, k, v)):
+        within(g.numpy().reshape(x.shape), want, n)
+    args[5] = None
+    assert ax.L.ax_hip_sdpa_bwd(*args) == 1
+
+
 def test_caches_past_32_bits(hip):
     """Rows of a sequence, and sequences, that lie more than 2^32 bytes behind the pointer: 2 sequences of 1.2 million rows of 8 heads of 128, 4.9 GB each.  Keys are zero,
     so every probability is one over their number."""
