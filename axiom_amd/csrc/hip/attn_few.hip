@@ -6,15 +6,15 @@
 // the tile kernel does (attn_fwd.hip).  Maxima, sums and outputs of the waves meet in LDS, those of the ranges in memory, where the last workgroup of the rows to arrive adds
 // them, in order: one launch, and the same bits whoever is last.
 //
-// A token of each of 32 sequences over 2048 to 4096 keys, 32 heads, 8 of keys, of 128 takes 184 us, 4.4 TB/s of cache; the matrix core is busy 11 % of the cycles, vector instructions 37 %.  One
-// token over 500 keys, 16 heads, 4 of keys, of 64: 10.7 us, latency of lengths, keys and the join (15.3 in one range).
+// A token of each of 32 sequences over 2048 to 4096 keys, 32 heads, 8 of keys, of 128 takes 167 us, 4.9 TB/s of cache; the matrix core is busy a tenth of the cycles, vector instructions two fifths.
+// One token over 500 keys, 16 heads, 4 of keys, of 64: 10.2 us, latency of lengths, keys and the join (15.3 in one range).
 #include "attn_launch.h"
 #include "attn_tiles.h"
 
 namespace {
 using namespace axhip;
 
-constexpr int WAVES = 4;
+constexpr int WAVES = 4, SPLITS_MOST = 64;
 
 template <int DK>
 struct FewGeom {
@@ -257,21 +257,48 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
         auto read = [&](int64_t from) {
             return __builtin_bit_cast(v2f, __hip_atomic_load(reinterpret_cast<const int64_t *>(theirs + from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
         };
+        // Every read is a trip to memory, so they go out together: maxima and sums by eight groups of 32 lanes, then AHEAD ranges' outputs at a time.  (5 tokens of 4 sequences over 9578
+        // keys, 2 heads of keys of 32, in 64 ranges: 39 us with four at a time and the maxima one after the other, 23 so.)
+        static_assert(SPLITS_MOST == 64 && G::JOINED >= 64 * 256, "LDS for the maxima and sums of all ranges");
+        v2f *const both = reinterpret_cast<v2f *>(lds + G::JOIN_AT) + frow;
+        v2f here[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int s = (int)(threadIdx.x >> 5) + 8 * k;
+            if (s < grid.splits) here[k] = read((int64_t)s * G::PART + PIECES * 256 + 2 * frow);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int s = (int)(threadIdx.x >> 5) + 8 * k;
+            if (s < grid.splits) both[32 * s] = here[k];
+        }
+        __syncthreads();
         m_all = ATTN_LOWEST;
-        for (int s = 0; s < grid.splits; s++) m_all = fmaxf(m_all, read((int64_t)s * G::PART + PIECES * 256 + 2 * frow)[0]);
+        for (int s = 0; s < grid.splits; s++) m_all = fmaxf(m_all, both[32 * s][0]);
         l_all = 0.0f;
 #pragma unroll
         for (int n = 0; n < DT; n++) out[n] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int s = 0; s < grid.splits; s++) {
-            const v2f both = read((int64_t)s * G::PART + PIECES * 256 + 2 * frow);
-            const float w = __builtin_amdgcn_exp2f(both[0] - m_all);
-            l_all = __builtin_fmaf(both[1], w, l_all);
+        constexpr int AHEAD = 8;
+        for (int s0 = 0; s0 < grid.splits; s0 += AHEAD) {
+            v4f x[AHEAD][DT];
 #pragma unroll
-            for (int n = 0; n < DT; n++) {
-                const int64_t from = (int64_t)s * G::PART + ((wave + 4 * n) * 64 + lane) * 4;
-                const v2f x = read(from), y = read(from + 2);
-                out[n] += v4f{x[0], x[1], y[0], y[1]} * w;
+            for (int k = 0; k < AHEAD; k++) {
+                if (s0 + k >= grid.splits) break;
+#pragma unroll
+                for (int n = 0; n < DT; n++) {
+                    const int64_t from = (int64_t)(s0 + k) * G::PART + ((wave + 4 * n) * 64 + lane) * 4;
+                    const v2f p = read(from), q = read(from + 2);
+                    x[k][n] = v4f{p[0], p[1], q[0], q[1]};
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) {
+                if (s0 + k >= grid.splits) break;
+                const v2f ml_here = both[32 * (s0 + k)];
+                const float w = __builtin_amdgcn_exp2f(ml_here[0] - m_all);
+                l_all = __builtin_fmaf(ml_here[1], w, l_all);
+#pragma unroll
+                for (int n = 0; n < DT; n++) out[n] += x[k][n] * w;
             }
         }
         if (threadIdx.x == 0) __hip_atomic_store(grid.arrivals + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);       // ready for the next launch
@@ -330,7 +357,8 @@ int launch_few(const AttnArgs &a, FewGrid grid) {
 
 namespace axhip {
 
-// Whether the few-rows form takes the call, and in how many ranges of keys: until there are two workgroups a CU, each wave with a tile or more.
+// Whether the few-rows form takes the call, and in how many ranges of keys: until there are two workgroups a CU, or one of heads past 64, which hold a CU alone (us, two -> one: 5 tokens of 2
+// sequences over 6000 keys, 16 heads, 8 of keys, of 112 52 -> 34, a token of 8 over 4000, 16, 4 of keys, of 96 44 -> 31), each wave with a tile or more.
 // Which form: by what each takes, in us.  Tiles: 128 rows a CU, as long as their keys.  Few rows: a step of 32 rows and 32 keys costs the chip so much (the
 // wider heads have one workgroup a CU and twice the work), and every further round of workgroups its start.  Within a few per cent where it is close (us, tiles -> this: 1 token
 // of 8 sequences over 1000 keys, 8 heads of 32 25.0 -> 13.4, 4 x 4 of [512, 64] causal 22.5 -> 11.8, 16 queries of 4 heads over 16000 keys, 8 heads of 128 711 -> 94, 4 x 2 x 8 of
@@ -343,9 +371,9 @@ bool attn_fwd_few(const AttnArgs &a, int &rc) {
     grid.row_tiles = (int)((rows + 31) / 32);
     const int64_t units = (int64_t)a.B * a.Hkv * grid.row_tiles, tiles = ((int64_t)a.Sk + 31) / 32;
     if (units > GRID_MOST / 64) return false;
-    int64_t splits = (2 * cus + units - 1) / units;
+    int64_t splits = ((a.dk > 64 ? 1 : 2) * cus + units - 1) / units;
     if (splits > (tiles + WAVES - 1) / WAVES) splits = (tiles + WAVES - 1) / WAVES;
-    if (splits > 64) splits = 64;
+    if (splits > SPLITS_MOST) splits = SPLITS_MOST;
     if (splits < 1) splits = 1;
     grid.splits = (int)splits;
     if (rows > 32) {
