@@ -30,7 +30,8 @@ int attn_arguments(const char *who, AttnArgs &a, const Tensor *tensors, int n, i
     axhip_attn_rules r = {};
     if (rules) r = *rules;
     if (!(r.cap >= 0.0f) || isinf(r.cap)) return fail(AXHIP_ERR_SHAPE, "%s: the cap must be zero or positive", who);
-    if (r.cap > 0.0f && isfinite(scale) && isinf(scale / r.cap)) return fail(AXHIP_ERR_SHAPE, "%s: the scale over the cap overflows", who);
+    if (r.cap > 0.0f && isinf(1.0f / (r.cap * LOG2E))) return fail(AXHIP_ERR_SHAPE, "%s: the cap must be zero or at least 2.1e-39", who);
+    if (isfinite(scale) && isinf(scale * LOG2E)) return fail(AXHIP_ERR_SHAPE, "%s: the scale must be below 2.35e38", who);
     if (r.prefix && !r.causal) return fail(AXHIP_ERR_SHAPE, "%s: a prefix without a causal mask", who);
     if ((r.doc_q == nullptr) != (r.doc_k == nullptr)) return fail(AXHIP_ERR_NULL_ARG, "%s: documents of queries and of keys, or neither", who);
     a.kv_rows = kv_rows;
@@ -42,8 +43,10 @@ int attn_arguments(const char *who, AttnArgs &a, const Tensor *tensors, int n, i
     a.Sk = (int)Sk;
     a.dk = (int)dk;
     a.scale = scale;
-    a.q_up = r.cap > 0.0f ? scale / r.cap : scale * LOG2E;
-    a.cap2 = r.cap * LOG2E;
+    a.q_up = scale * LOG2E;
+    a.cap = r.cap;
+    a.cap_down = r.cap > 0.0f ? (float)(1.0 / ((double)r.cap * LOG2E)) : 0.0f;
+    a.cap_near = (float)((double)r.cap * LOG2E * TANH_NEAR);
     a.bias2 = LOG2E;
     a.slopes = r.slopes;
     a.prefix = r.prefix;

@@ -36,23 +36,23 @@ __device__ __forceinline__ void times(v4f (&acc)[N], float by) {
 // Scores of a lane (products already scaled) after cap and distance; `slope` the cap's derivative
 template <typename Distance>
 __device__ __forceinline__ void score_tile(const AttnArgs &a, Eight &s, Eight &slope, Distance distance) {
-    if (a.cap2 > 0.0f) {
+    if (a.cap > 0.0f) {
         float big = 0.0f;
 #pragma unroll
         for (int v = 0; v < 8; v++) big = fmaxf(big, __builtin_fabsf(s[v]));
-        if (__builtin_amdgcn_ballot_w64(!(big < TANH_NEAR)))
+        if (__builtin_amdgcn_ballot_w64(!(big < a.cap_near)))
 #pragma unroll
             for (int v = 0; v < 8; v++) {
-                const Tanh t = tanh_of(s[v]);
-                s[v] = a.cap2 * t.value;
-                slope[v] = t.slope;
+                const Capped c = capped(a, s[v]);
+                s[v] = c.score;
+                slope[v] = c.slope;
             }
         else
 #pragma unroll
             for (int v = 0; v < 8; v++) {
-                const float t = tanh_near(s[v]);
-                s[v] = a.cap2 * t;
-                slope[v] = __builtin_fmaf(-t, t, 1.0f);
+                const Capped c = capped_near(a, s[v]);
+                s[v] = c.score;
+                slope[v] = c.slope;
             }
     }
     if (a.slopes)
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
     float o_times = o_down * two_to(d_up), delta_times = delta * two_to(d_up);
     const float one = hidden_one();
     // what is left to a score: q_down, where more is done to it before, in the exponential's multiply-add otherwise
-    const bool plain = a.cap2 == 0.0f && !a.slopes;
+    const bool plain = a.cap == 0.0f && !a.slopes;
     const float down = plain ? q_down : 1.0f;
 
     const unsigned row_at = B::row_place16(lane) + base, column_at = B::column_place16(lane) + base;
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
                     for (int e = 0; e < 4; e++) {
                         const int v = 4 * t + e;
                         x[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], down, -lse2)) * __builtin_fmaf(pr[t][e] * vf[e], o_times, -delta_times);
-                        if (a.cap2 > 0.0f) x[v] *= slope[v];
+                        if (a.cap > 0.0f) x[v] *= slope[v];
                         x[v] *= kf[e];
                         most = fmaxf(most, __builtin_fabsf(x[v]));
                     }
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
     for (int n = 0; n < NT; n++) acc_k[n] = acc_v[n] = v4f{0.f, 0.f, 0.f, 0.f};
     // acc_k is 2^BIAS d_scale times the sum of ds q, acc_v 2^BIAS p_scale times that of P dO: running scales of ds and P times their rows' factors
     float d_scale = two_to(MOST_UP), p_scale = d_scale;
-    const bool plain = a.cap2 == 0.0f && !a.slopes;  // (as for the rows' gradient)
+    const bool plain = a.cap == 0.0f && !a.slopes;  // (as for the rows' gradient)
     const float down = plain ? k_down : 1.0f;
 
     const unsigned row_at = B::row_place16(lane) + base, column_at = B::column_place16(lane) + base;
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
         if (!plain)
 #pragma unroll
             for (int v = 0; v < 8; v++) s[v] *= k_down;
-        if (a.cap2 > 0.0f || a.slopes) {
+        if (a.cap > 0.0f || a.slopes) {
             Eight far;
             if (a.slopes)
 #pragma unroll
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
                 const int v = 4 * t + e;
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], down, -lse[e]));
                 dp[v] = p * __builtin_fmaf(pr[t][e] * of[e], v_down, -delta[e]);
-                if (a.cap2 > 0.0f) dp[v] *= slope[v];
+                if (a.cap > 0.0f) dp[v] *= slope[v];
                 dp[v] *= qf[e];
                 s[v] = p * of[e];
                 most_p = fmaxf(most_p, s[v]);
@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
         cur ^= G::STAGE;
     }
 
-    times(acc_k, two_to(-BIAS) / d_scale * (a.cap2 > 0.0f ? a.cap2 * LN2 : LN2));      // (scale over what the rows of Q were taken times)
+    times(acc_k, two_to(-BIAS) / d_scale * LN2);                // (scale over what the rows of Q were taken times)
     times(acc_v, two_to(-BIAS) / p_scale);
     if constexpr (G::SHARES == 2) {
         v4f *sums = reinterpret_cast<v4f *>(lds + wave % SETS * G::JOIN) + lane;

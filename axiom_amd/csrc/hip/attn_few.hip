@@ -125,16 +125,16 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
 #pragma unroll
             for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e] * q_down;
         }
-        if (a.cap2 > 0.0f) {
+        if (a.cap > 0.0f) {
             float big = 0.0f;
 #pragma unroll
             for (int v = 0; v < 16; v++) big = fmaxf(big, __builtin_fabsf(s[v]));
-            if (__builtin_amdgcn_ballot_w64(!(big < TANH_NEAR)))
+            if (__builtin_amdgcn_ballot_w64(!(big < a.cap_near)))
 #pragma unroll
-                for (int v = 0; v < 16; v++) s[v] = a.cap2 * tanh_of(s[v]).value;
+                for (int v = 0; v < 16; v++) s[v] = capped(a, s[v]).score;
             else
 #pragma unroll
-                for (int v = 0; v < 16; v++) s[v] = a.cap2 * tanh_near(s[v]);
+                for (int v = 0; v < 16; v++) s[v] = capped_near(a, s[v]).score;
         }
         if (a.slopes) {
             const float from = (float)(row.p - kt0 - 4 * fhalf);

@@ -11,8 +11,9 @@ struct AttnArgs {
     int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv, kv_rows;
     int B, H, Hkv, G, Sq, Sk, dk;                // G: query heads to a head of keys
     float scale;                                 // gradients of q and k are sums of ds * scale
-    float q_up;                                  // a query is taken times this: its products are scores in log2 units, or over the cap
-    float cap2, bias2;                           // the cap in log2 units (0: none); log2(e) for the slopes
+    float q_up;                                  // a query is taken times this: its products are scores in log2 units
+    float cap, cap_down, cap_near;               // the cap (0: none); one over it in log2 units; how far scores are near zero for it, in log2 units
+    float bias2;                                 // log2(e) for the slopes
     const float *slopes;
     const int32_t *prefix, *start, *lens, *doc_q, *doc_k;
     int causal;
@@ -57,35 +58,36 @@ __device__ __forceinline__ AttnRow attn_row(const AttnArgs &a, int b, int head, 
     return attn_row(a, attn_seq(a, b), i, a.doc_q ? a.doc_q[(int64_t)b * a.Sq + i] : 0, a.slopes ? a.slopes[head] : 0.0f);
 }
 
-// tanh and its derivative.  Near zero x (1 + x^2 p(x^2)), a minimax fit of degree 4 on |x| < 0.6 (relative error 3e-9 before rounding); beyond, with
-// r = 2 / (e^(2|x|) + 1), 1 - r and r (2 - r), neither of which cancels.
-struct Tanh {
-    float value, slope;
-};
-__device__ __forceinline__ float tanh_near(float x) {
-    const float u = x * x;
-    float p = __builtin_fmaf(u, -0.005895156413316727f, 0.020795969292521477f);
-    p = __builtin_fmaf(u, p, -0.053783830255270004f);
-    p = __builtin_fmaf(u, p, 0.13331924378871918f);
-    p = __builtin_fmaf(u, p, -0.33333298563957214f);
-    return __builtin_fmaf(x, u * p, x);
-}
+// A score x in log2 units under a cap c in the same units, c tanh(u) with u = x / c, and its derivative.  Near zero tanh(u) is u (1 + w), w = u^2 p(u^2) a minimax fit
+// of degree 4 on |u| < 0.6 (relative error 5e-9 before rounding), and the score is x + x w: as precise as x under any cap, though u may have lost its bits.
+// Beyond, with r = 2 / (e^(2|u|) + 1), they are c (1 - r) and r (2 - r), neither of which cancels; c may be past the largest float, the cap itself is not.
 constexpr float TANH_NEAR = 0.6f;
-__device__ __forceinline__ Tanh tanh_of(float x) {
-    const float e = __builtin_amdgcn_exp2f(__builtin_fabsf(x) * 2.8853900817779268f);
-    const float r = 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
-    const bool near = __builtin_fabsf(x) < TANH_NEAR;
-    const float n = tanh_near(x);
-    return {near ? n : __builtin_copysignf(1.0f - r, x), near ? __builtin_fmaf(-n, n, 1.0f) : r * (2.0f - r)};
+struct Capped {
+    float score, slope;
+};
+__device__ __forceinline__ Capped capped_near(const AttnArgs &a, float x) {
+    const float u = x * a.cap_down, uu = u * u;
+    float p = __builtin_fmaf(uu, -0.005895156413316727f, 0.020795969292521477f);
+    p = __builtin_fmaf(uu, p, -0.053783830255270004f);
+    p = __builtin_fmaf(uu, p, 0.13331924378871918f);
+    p = __builtin_fmaf(uu, p, -0.33333298563957214f);
+    const float w = uu * p, t = __builtin_fmaf(u, w, u);
+    return {__builtin_fmaf(x, w, x), __builtin_fmaf(-t, t, 1.0f)};
+}
+__device__ __forceinline__ Capped capped(const AttnArgs &a, float x) {
+    const float u = __builtin_fabsf(x * a.cap_down);
+    const float r = 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * 2.8853900817779268f) + 1.0f);
+    const Capped near = capped_near(a, x);
+    return u < TANH_NEAR ? near : Capped{__builtin_copysignf(__builtin_fmaf(-a.cap, r, a.cap) * LOG2E, x), r * (2.0f - r)};
 }
 
 // A score in log2 units from a product of q (times q_up) and k
 __device__ __forceinline__ float attn_score(const AttnArgs &a, float product, const AttnRow &r, int key, float &slope) {
     slope = 1.0f;
-    if (a.cap2 > 0.0f) {
-        const Tanh t = tanh_of(product);
-        product = a.cap2 * t.value;
-        slope = t.slope;
+    if (a.cap > 0.0f) {
+        const Capped c = capped(a, product);
+        product = c.score;
+        slope = c.slope;
     }
     return a.slopes ? __builtin_fmaf(-r.slope2, (float)(r.p > key ? r.p - key : key - r.p), product) : product;
 }

@@ -403,7 +403,8 @@ typedef struct {
  * h reads head h / (H / Hkv)).  Query i of sequence b is row b * Sq + i of Q and O, its key j row b * kv_rows + j of K and V (kv_rows >= Sk:
  * rows that a cache holds for each sequence).  L [B, H, Sq] is the log-sum-exp of each row of scores, or NULL.  For prompts, training and, with Sq = 1 or a
  * few, single tokens over a cache.  dk a multiple of 4 up to 128 (AXHIP_ERR_NOT_IMPLEMENTED otherwise), pitches multiples of 4 floats up to
- * 2^22, Q, K, V, O 16-byte aligned, Sq and Sk up to 2^24.  scale / cap must be finite.  `rules` is read before
+ * 2^22, Q, K, V, O 16-byte aligned, Sq and Sk up to 2^24.  cap is zero or any float from 2.1e-39 on (one far above all scores leaves
+ * them as they are), scale below 2.35e38.  `rules` is read before
  * the call returns; what it points to when the kernels run.  Outputs must not overlap inputs or each other. */
 int axhip_attn_fwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, const float *V, int64_t ldv, int64_t kv_rows, float *O, int64_t ldo,
                    float *L, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t dk, float scale, const axhip_attn_rules *rules);

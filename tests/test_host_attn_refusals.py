@@ -106,3 +106,24 @@ if H * dk <= 1 << 22:
         hip.check(bwd(None, B, H, Hkv, Sq, Sk, dk, kv_rows=Sk, rules=rules, ldd=(H * dk, H * dk, Hkv * dk, Hkv * dk), **ld))
     assert len(launched()) >= (9 if Sk else 6)
 """ % ((B, H, Hkv, Sq, Sk, dk),))
+
+
+def test_which_caps_and_scales_are_taken(stub):  # noqa: F811
+    """Any cap whose reciprocal is a float, the largest ones too, whatever the scale; and scales that are floats in log2 units."""
+    run(stub, ATTN + """
+def with_scale(scale, cap):
+    rules = AttnRules(cap=cap)
+    shape = (2, 4, 2, 16, 32, 64, scale, C.byref(rules))
+    a = L.axhip_attn_fwd(P[0], 256, P[1], 128, P[2], 128, 32, P[3], 256, P[4], *shape)
+    b = L.axhip_attn_bwd(P[0], 256, P[1], 128, P[2], 128, 32, P[3], 256, P[4], P[5], 256, P[6], 256, P[7], 128, P[8], 128, *shape)
+    assert a == b
+    return a
+biggest = 3.4028234663852886e38
+for cap in (0.0, 2.2e-39, 1e-20, 1.0, 1e33, 1e38, biggest):
+    for scale in (1e-30, 0.125, 1e30):
+        assert with_scale(scale, cap) == 0, (scale, cap)
+for cap in (1e-45, 2e-39, float("inf"), float("nan"), -1.0):
+    for scale in (1e-30, 0.125):
+        assert with_scale(scale, cap) == 3, (scale, cap)
+assert with_scale(2.3e38, 0.0) == 0 and with_scale(2.4e38, 0.0) == 3 and with_scale(-biggest, 30.0) == 3
+""")
