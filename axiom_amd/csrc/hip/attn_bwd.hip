@@ -352,16 +352,26 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
             form();
             if (__builtin_amdgcn_ballot_w64(most > ROOM)) {      // (always for the first that are not zero)
                 const int before = d_up;
-                const bool over = most_of_parts(most) > ROOM;
-                if (over) d_up -= MOST_UP;                       // a scale at which they are floats, then the right one
-                o_times = o_down * two_to(d_up);
-                delta_times = delta * two_to(d_up);
-                form();
+                auto take = [&]() {
+                    o_times = __builtin_ldexpf(o_down, d_up);
+                    delta_times = __builtin_ldexpf(delta, d_up);
+                    // A scale at which the products of dO and V have no float left, or that its inverse could not undo: from here on the row is formed again.
+                    if (o_times == 0.0f || d_up < -126) o_down = o_times = NAN;
+                };
                 most = most_of_parts(most);
-                if (over) d_up += LARGEST - __builtin_amdgcn_frexp_expf(most);
-                if (d_up > MOST_UP) d_up = MOST_UP;
-                o_times = o_down * two_to(d_up);
-                delta_times = delta * two_to(d_up);
+                const bool over = most > ROOM, past = most == INFINITY;
+                if (past) {                                      // no float at the scale so far: by what they are at one where they are
+                    d_up -= MOST_UP;
+                    take();
+                }
+                if (__builtin_amdgcn_ballot_w64(past)) {         // (the other rows come out as they were)
+                    form();
+                    most = most_of_parts(most);
+                }
+                if (over) {
+                    d_up = min(d_up + LARGEST - __builtin_amdgcn_frexp_expf(most), before);
+                    take();
+                }
                 times(acc, two_to(d_up - before));
                 form();
             }

@@ -26,3 +26,16 @@ def test_caps_of_any_size(hip, shape, form, cap):
     rng, q, k, v, d_o = draw(51, *shape)
     check(hip, q, k, v, 3 / shape[-1] ** 0.5, Rules(cap=cap), d_o, kernel=form)
     check(hip, q, k, v, 3 / shape[-1] ** 0.5, Rules(cap=cap, slopes=np.full(shape[3], 0.01, np.float32)), d_o)
+
+
+@pytest.mark.parametrize("dk", [32, 64, 96, 128])
+@pytest.mark.parametrize("k_size,v_size", [(1e15, 1.0), (1e20, 1.0), (1e30, 1.0), (1e16, 1e13), (100.0, 1e4), (1e-20, 1.0), (1e25, 1e-25)])
+def test_gradients_that_grow_along_the_keys(hip, dk, k_size, v_size):
+    """Keys and values of any size, values a thousand times larger behind the first 64 keys and again behind 200: the gradient of the queries takes its scale anew, from
+    wherever it was."""
+    say("attn growing", dk, k_size, v_size)
+    rng, q, k, v, d_o = draw(55, 1, 90, 300, 2, 1, dk)
+    v[:, 64:] *= np.float32(1e3)
+    v[:, 200:] *= np.float32(1e3)
+    check(hip, q / np.float32(k_size), k * np.float32(k_size), v * np.float32(v_size), dk ** -0.5, Rules(), d_o)
+    check(hip, q / np.float32(k_size), k * np.float32(k_size), v * np.float32(v_size), dk ** -0.5, Rules(cap=5.0), d_o)
