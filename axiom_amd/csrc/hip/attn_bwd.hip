@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
         q_down = cut_row(x, most_of_parts(most_of(x)), qf);
     }
     if (valid && part == 0 && wave < SETS && work.split == 0) a.delta[at] = delta;
-    float lse2 = live ? a.Lin[at] * LOG2E : INFINITY;
+    // probabilities come times 2^BIAS
+    float lse2 = live ? __builtin_fmaf(a.Lin[at], LOG2E, -(float)BIAS) : INFINITY;
     if (lse2 == -INFINITY) lse2 = INFINITY;          // a row that saw nothing: no probability
     if (blk < blocks.n) {
         stage(0);
@@ -264,8 +265,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dq(AttnArgs a, BwdGrid g
     v4f acc[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) acc[n] = v4f{0.f, 0.f, 0.f, 0.f};
-    int d_up = MOST_UP;                              // acc is 2^(BIAS + d_up) times the sum: the running exponent of ds times its key row's factor
-    float o_times = o_down * two_to(d_up), delta_times = delta * two_to(d_up);
+    // acc is 2^(BIAS + d_up) times the sum: the running exponent of ds times its key row's factor, which starts where products of dO and delta are floats
+    int d_up = MOST_UP - max(0, max(__builtin_amdgcn_frexp_expf(o_down), __builtin_amdgcn_frexp_expf(delta)));
+    float o_times = __builtin_ldexpf(o_down, d_up), delta_times = __builtin_ldexpf(delta, d_up);
     const float one = hidden_one();
     // what is left to a score: q_down, where more is done to it before, in the exponential's multiply-add otherwise
     const bool plain = a.cap == 0.0f && !a.slopes;
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_dkv(AttnArgs a, BwdGrid 
             if (i >= rows_end) row.end = 0;
             float *at = reinterpret_cast<float *>(lds + cur + G::ROW_AT) + threadIdx.x;
             int *ints = reinterpret_cast<int *>(at);
-            at[2 * ROWS] = r_lse == -INFINITY ? INFINITY : r_lse * LOG2E;     // a row that saw nothing: no probability
+            at[2 * ROWS] = r_lse == -INFINITY ? INFINITY : __builtin_fmaf(r_lse, LOG2E, -(float)BIAS);        // a row that saw nothing: no probability
             at[3 * ROWS] = row.end > 0 ? r_delta : 0.0f;
             at[4 * ROWS] = row.slope2;
             ints[5 * ROWS] = row.end;

@@ -59,15 +59,17 @@ __device__ __forceinline__ v4f mfma_cut16(const v4i (&a)[2], const v4i (&b)[2], 
     return c;
 }
 
-// What a row whose largest magnitude is `most` is taken times, 2^e, e at most MOST_UP (rows of zeros); and the factor kept with it, 2^(BIAS - e): times that, what small rows
-// are multiplied by does not run out of exponents.  (Rows past 2^100 get an infinite factor, and what it meets is formed again.)  Both straight from the exponent
-// field E of `most`, which is 2^(E - 127) to twice that: e = 141 - E.
-constexpr int MOST_UP = 100, BIAS = 24;
+// What a row whose largest magnitude is `most` is taken times, 2^e, straight from the exponent field E of `most`, which is 2^(E - 127) to twice that: e = 141 - E, at most MOST_UP (rows of
+// zeros, and rows below 2^-102, which lose bits); and the factor kept with it, 2^-e.  Products of two cut rows times the factor of the one and then the other's pass 2^128 on the way
+// only for results of 2^27 and more.  (Scores so large are off by more than the exponential reaches, and the log-sum-exp that stands against them is.)
+constexpr int MOST_UP = 100;
 __device__ __forceinline__ float row_up(float most) {
     const unsigned bits = ((127u + 141u) << 23) - (__float_as_uint(most) & 0x7f800000u);
     return __uint_as_float(min(bits, (127u + MOST_UP) << 23));
 }
-__device__ __forceinline__ float row_factor(float up) { return __uint_as_float(min(((254u + BIAS) << 23) - __float_as_uint(up), 0x7f800000u)); }
+__device__ __forceinline__ float row_factor(float up) { return __uint_as_float((254u << 23) - __float_as_uint(up)); }
+// What probabilities (in their exponent) or their rows' factors carry beyond that, so that what small rows are multiplied by does not run out of exponents
+constexpr int BIAS = 24;
 
 // The largest of each LANES neighbouring lanes' values (4, 8 or 16), in all of them
 template <int LANES>
@@ -126,13 +128,13 @@ __device__ __forceinline__ float most_of_parts(float v) {
     return over_parts(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// A lane's part of a row as operand terms, whose largest value over all parts is `most`; gives back what its products are taken times, 2^(-e - BIAS)
+// A lane's part of a row as operand terms, whose largest value over all parts is `most`; gives back the row's factor
 template <int KS>
 __device__ __forceinline__ float cut_row(const float (&x)[KS][8], float most, v4i (&t)[KS][2]) {
     const float up = row_up(most);
 #pragma unroll
     for (int s = 0; s < KS; s++) cut_halves(x[s], up, t[s]);
-    return 1.0f / up * two_to(-BIAS);
+    return row_factor(up);
 }
 template <int KS>
 __device__ __forceinline__ float most_of(const float (&x)[KS][8]) {

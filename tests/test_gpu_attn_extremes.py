@@ -28,6 +28,27 @@ def test_caps_of_any_size(hip, shape, form, cap):
     check(hip, q, k, v, 3 / shape[-1] ** 0.5, Rules(cap=cap, slopes=np.full(shape[3], 0.01, np.float32)), d_o)
 
 
+def low_scores(shape, q_size):
+    """Queries of a size of q_size and keys of its inverse; the scores lie around -14, between -4 and -24."""
+    rng, _, _, v, d_o = draw(52, *shape)
+    B, Sq, Sk, H, Hkv, dk = shape
+    q = rng.normal(1, 0.1, size=(B, Sq, H, dk))
+    k = rng.normal(-14 / dk, 3 / dk ** 0.5, size=(B, Sk, Hkv, dk))
+    return (q * q_size).astype(np.float32), (k / q_size).astype(np.float32), v, d_o
+
+
+@pytest.mark.parametrize("shape,form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("q_size", [1e-27, 1e-18, 1e27])
+def test_low_scores_from_small_and_large_factors(hip, shape, form, q_size):
+    """A visible key counts whatever powers of two its score is formed from."""
+    say("attn low scores", shape, q_size)
+    q, k, v, d_o = low_scores(shape, q_size)
+    d_o = d_o * np.float32(1e-3)
+    check(hip, q, k, v, 1.0, Rules(), d_o, kernel=form)
+    check(hip, q, k, v, 1.0, Rules(slopes=np.full(shape[3], 0.01, np.float32)), d_o)
+    check(hip, q, k, v, 1.0, Rules(cap=100.0), d_o)
+
+
 @pytest.mark.parametrize("dk", [32, 64, 96, 128])
 @pytest.mark.parametrize("k_size,v_size", [(1e15, 1.0), (1e20, 1.0), (1e30, 1.0), (1e16, 1e13), (100.0, 1e4), (1e-20, 1.0), (1e25, 1e-25)])
 def test_gradients_that_grow_along_the_keys(hip, dk, k_size, v_size):
