@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
             }
             top = fmaxf(top, __shfl_xor(top, 32, 64)) - (float)LARGEST;
             const float next = most > ROOM ? fmaxf(ref, top) : ref, alpha = __builtin_amdgcn_exp2f(ref - next);
+            l_run = scaled(l_run, ref - next);
             ref = next;
-            l_run *= alpha;
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
 #pragma unroll
     for (int w = 0; w < WAVES; w++) {
         weight[w] = __builtin_amdgcn_exp2f(ml[w * 64 + frow] - m_all);
-        l_all = __builtin_fmaf(ml[w * 64 + 32 + frow], weight[w], l_all);
+        l_all += scaled(ml[w * 64 + 32 + frow], ml[w * 64 + frow] - m_all);
     }
     v4f out[DT];                                     // this wave's pieces: wave, wave + 4, ...
 #pragma unroll
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
                 if (s0 + k >= grid.splits) break;
                 const v2f ml_here = both[32 * (s0 + k)];
                 const float w = __builtin_amdgcn_exp2f(ml_here[0] - m_all);
-                l_all = __builtin_fmaf(ml_here[1], w, l_all);
+                l_all += scaled(ml_here[1], ml_here[0] - m_all);
 #pragma unroll
                 for (int n = 0; n < DT; n++) out[n] += x[k][n] * w;
             }

@@ -276,8 +276,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
                 }
                 top = fmaxf(top, __shfl_xor(top, 32, 64)) - (float)LARGEST;
                 const float next = most > ROOM ? fmaxf(ref, top) : ref, alpha = __builtin_amdgcn_exp2f(ref - next);
+                l_run = scaled(l_run, ref - next);
                 ref = next;
-                l_run *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
         __syncthreads();
         if (wave >= SETS) return;
         const float other = of_row[0], both = fmaxf(ref, other), mine = __builtin_amdgcn_exp2f(ref - both), theirs = __builtin_amdgcn_exp2f(other - both);
-        l_tot = l_tot * mine + of_row[32] * theirs;
+        l_tot = scaled(l_tot, ref - both) + scaled(of_row[32], other - both);
         ref = both;
 #pragma unroll
         for (int d = 0; d < DT; d++)

@@ -87,6 +87,13 @@ __device__ __forceinline__ float most_of_lanes(float v) {
 constexpr float ROOM = 32768.0f;
 constexpr int LARGEST = 10;
 
+// x 2^e for e down to -252, in two steps: the exponential alone gives nothing below 2^-126.  For sums of probabilities, whose references go with the values' factors and may
+// lie further apart than that (values of nothing before one of 1e13) though the probabilities do not.
+__device__ __forceinline__ float scaled(float x, float e) {
+    const float half = __builtin_amdgcn_exp2f(0.5f * e);
+    return x * half * half;
+}
+
 // A running scale for sums over what has none of its own, a power of two: it starts at 2^MOST_UP and falls when the largest so far, `most`, times it is past ROOM
 __device__ __forceinline__ float regrown(float most, float scale) {
     return most * scale > ROOM ? two_to(min(LARGEST - __builtin_amdgcn_frexp_expf(most), MOST_UP)) : scale;

@@ -49,6 +49,23 @@ def test_low_scores_from_small_and_large_factors(hip, shape, form, q_size):
     check(hip, q, k, v, 1.0, Rules(cap=100.0), d_o)
 
 
+# ... over 1000 keys, so that few keys weigh little
+LONG = [((1, 3, 1000, 4, 2, 64), "attn_few_ranges"), ((1, 1, 1000, 600, 600, 32), "attn_few"), ((1, 40, 1000, 300, 300, 32), "attn_tiles_128"), ((1, 200, 1000, 260, 260, 32), "attn_tiles_256")]
+LONG_IDS = [form for _, form in LONG]
+
+
+@pytest.mark.parametrize("shape,form", LONG, ids=LONG_IDS)
+@pytest.mark.parametrize("low,high", [(0.0, 1e13), (1e-20, 1e20), (1e-30, 1e22), (0.0, 1e23)])
+def test_values_of_nothing_and_a_large_one_share_their_weight(hip, shape, form, low, high):
+    """Rows of values of zeros, or small ones, before and behind a large one: as many keys share the probability as there are."""
+    say("attn uneven values", shape, low, high)
+    rng, q, k, v, _ = draw(54, *shape)
+    for at in (10, 500, 999):
+        vv = v * np.float32(low)
+        vv[:, at] = v[:, at] * np.float32(high)
+        check(hip, q, k, vv, 0.05, Rules(), kernel=form)
+
+
 @pytest.mark.parametrize("dk", [32, 64, 96, 128])
 @pytest.mark.parametrize("k_size,v_size", [(1e15, 1.0), (1e20, 1.0), (1e30, 1.0), (1e16, 1e13), (100.0, 1e4), (1e-20, 1.0), (1e25, 1e-25)])
 def test_gradients_that_grow_along_the_keys(hip, dk, k_size, v_size):
