@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(64 * WAVES, (DK <= 64 ? 2 : 1)) k_attn_few(Att
             const int l = (int)afresh(lane);
             const typename S::Place place = S::place(0, l, 0);
             ks.put(base, base + G::FACTORS_AT, place, l, 1.0f, a.dk);
-            vs.put(base + B::BYTES, base + G::FACTORS_AT + 128, place, l, two_to(BIAS), a.dk);
+            vs.put(base + B::BYTES, base + G::FACTORS_AT + 128, place, l, VALUES_UP, a.dk, VALUES_DOWN);
             if (docs && lane < 32) reinterpret_cast<int *>(at + G::DOCS_AT)[lane] = doc_here;
         }
         order_in_wave();

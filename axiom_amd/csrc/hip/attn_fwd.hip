@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_attn_fwd(AttnArgs a, FwdGrid 
         const int l = (int)afresh(lane);
         const typename S::Place place = S::place(wave, l, 0);
         ks.put(base + cur, base + cur + G::FACTORS_AT, place, l, 1.0f, a.dk);
-        vs.put(base + cur + B::BYTES, base + cur + G::FACTORS_AT + 4 * BKV, place, l, two_to(BIAS), a.dk);
+        vs.put(base + cur + B::BYTES, base + cur + G::FACTORS_AT + 4 * BKV, place, l, VALUES_UP, a.dk, VALUES_DOWN);
         if (docs && threadIdx.x < BKV) reinterpret_cast<int *>(at + G::DOCS_AT)[threadIdx.x] = doc_here;
         if (docs && threadIdx.x < TILES) reinterpret_cast<DocRange *>(at + G::DOCS_AT + BKV * 4)[threadIdx.x] = range_here;
     };

@@ -96,8 +96,8 @@ struct Stage {
                 for (int e = 0; e < 4; e++) x[i][4 * h + e] = a[e];
             }
     }
-    // to LDS at `block`, cut; the rows' factors, times `by`, beside them.  A piece further on is STEP rows and an exchange of chunks away.
-    __device__ __forceinline__ void put(unsigned block, unsigned factors, const Place &at, int lane, float by, int dk) {
+    // to LDS at `block`, cut; the rows' factors, times `by` and then `down`, beside them.  A piece further on is STEP rows and an exchange of chunks away.
+    __device__ __forceinline__ void put(unsigned block, unsigned factors, const Place &at, int lane, float by, int dk, float down = 1.0f) {
         const int chunk = lane % LANES;
         const unsigned to = at.to + block;
 #pragma unroll
@@ -116,7 +116,7 @@ struct Stage {
                 write_chunk(there, t[0]);
                 write_chunk(there + B::PLANE, t[1]);
             }
-            if (chunk == 0) write_float(factors + 4 * (at.row + i * STEP), row_factor(up) * by);
+            if (chunk == 0) write_float(factors + 4 * (at.row + i * STEP), row_factor(up) * by * down);
         }
     }
 };

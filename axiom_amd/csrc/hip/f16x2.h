@@ -70,6 +70,10 @@ __device__ __forceinline__ float row_up(float most) {
 __device__ __forceinline__ float row_factor(float up) { return __uint_as_float((254u << 23) - __float_as_uint(up)); }
 // What probabilities (in their exponent) or their rows' factors carry beyond that, so that what small rows are multiplied by does not run out of exponents
 constexpr int BIAS = 24;
+// Values from 2^78 on get an infinite factor, so that what sees them is formed again.  A probability's reference is the largest of the scores and their values' factors: with a value of 2^x the
+// largest probability is 2^-x or more, and one below 2^-126 is taken as nothing.  Below this border 2^24 keys lost like that are less than a rounding of the sum.
+constexpr float VALUES_UP = 0x1p64f, VALUES_DOWN = 0x1p-40f;      // a factor times the one and the other: 2^BIAS, past the largest float from 2^78 on
+static_assert(VALUES_UP * VALUES_DOWN == 1 << BIAS, "as other factors");
 
 // The largest of each LANES neighbouring lanes' values (4, 8 or 16), in all of them
 template <int LANES>

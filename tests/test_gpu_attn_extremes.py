@@ -55,6 +55,22 @@ LONG_IDS = [form for _, form in LONG]
 
 
 @pytest.mark.parametrize("shape,form", LONG, ids=LONG_IDS)
+@pytest.mark.parametrize("size", [1e23, 1e25, 1e32, 1e35])
+def test_a_very_large_value_leaves_the_others_their_weight(hip, shape, form, size):
+    """One value row of any size, seen with a probability of two thirds: the other keys, each 2^-11 of it, keep theirs."""
+    say("attn large value", shape, size)
+    B, Sq, Sk, H, Hkv, dk = shape
+    rng, q, k, v, _ = draw(53, *shape)
+    q[..., 0], k[..., 0] = 1, -11 * np.log(2)
+    for at in (0, 500, 999):
+        kk, vv = k * np.float32(0.01), v.copy()
+        kk[..., 0] = k[..., 0]
+        kk[:, at, :, 0] = 0
+        vv[:, at] *= np.float32(size)
+        check(hip, q, kk, vv, 1.0, Rules(), kernel=form)
+
+
+@pytest.mark.parametrize("shape,form", LONG, ids=LONG_IDS)
 @pytest.mark.parametrize("low,high", [(0.0, 1e13), (1e-20, 1e20), (1e-30, 1e22), (0.0, 1e23)])
 def test_values_of_nothing_and_a_large_one_share_their_weight(hip, shape, form, low, high):
     """Rows of values of zeros, or small ones, before and behind a large one: as many keys share the probability as there are."""
