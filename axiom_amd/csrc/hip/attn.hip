@@ -18,6 +18,7 @@ int attn_arguments(const char *who, AttnArgs &a, const Tensor *tensors, int n, i
         if (!tensors[t].at) return fail(AXHIP_ERR_NULL_ARG, "%s: NULL tensor", who);
     constexpr int64_t LONG = 1 << 24;
     if (B < 0 || H <= 0 || Hkv <= 0 || Sq < 0 || Sk < 0 || Sq > LONG || Sk > LONG) return fail(AXHIP_ERR_SHAPE, "%s: bad extent", who);
+    if (H > (1 << 20)) return fail(AXHIP_ERR_SHAPE, "%s: too many heads", who);        // (more would not fit a row pitch, and their sizes might not fit 64 bits)
     if (H % Hkv != 0) return fail(AXHIP_ERR_SHAPE, "%s: query heads must be a multiple of the heads of keys", who);
     if (dk < 4 || dk > 128 || dk % 4 != 0) return fail(AXHIP_ERR_NOT_IMPLEMENTED, "%s: head size %lld (multiples of 4 up to 128 only)", who, (long long)dk);
     if (kv_rows < Sk) return fail(AXHIP_ERR_SHAPE, "%s: kv_rows must hold Sk rows", who);

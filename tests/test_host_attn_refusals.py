@@ -127,3 +127,15 @@ for cap in (1e-45, 2e-39, float("inf"), float("nan"), -1.0):
         assert with_scale(scale, cap) == 3, (scale, cap)
 assert with_scale(2.3e38, 0.0) == 0 and with_scale(2.4e38, 0.0) == 3 and with_scale(-biggest, 30.0) == 3
 """)
+
+
+@pytest.mark.parametrize("B,H,Hkv", [(4, 1 << 62, 1 << 62), (4, 1 << 62, 1), (1, (1 << 62) + 4, 1), (2, 1 << 61, 1 << 61), (1, (1 << 20) + 1, 1)])
+def test_head_counts_past_64_bits(stub, B, H, Hkv):  # noqa: F811
+    """Heads times their size, or times sequences, that come out small in 64 bits."""
+    run(stub, ATTN + """
+B, H, Hkv = %r
+ld = dict(ldq=1 << 22, ldk=1 << 22, ldv=1 << 22, ldo=1 << 22)
+assert fwd(None, B, H, Hkv, 1, 3, 4, kv_rows=3, **ld) == 3
+assert bwd(None, B, H, Hkv, 1, 3, 4, kv_rows=3, ldd=(1 << 22,) * 4, **ld) == 3
+assert len(launched()) == 0
+""" % ((B, H, Hkv),))
