@@ -35,3 +35,13 @@ def test_planes_keep_their_registers(kernels):
     assert len(mine) == 7
     for name, note in mine.items():
         assert re.search(r"\.private_segment_fixed_size: 0\n", note) and re.search(r"\.vgpr_spill_count: 0\n", note), name
+
+
+def test_attention_under_score_rules_keeps_its_registers(kernels):
+    """All but the forward tiles of heads past 96, which keep seven registers of a lane in memory."""
+    mine = {name: note for name, note in kernels.items() if re.search("k_attn_(fwd|few|dq|dkv)I", name)}
+    assert len(mine) == 56, len(mine)
+    for name, note in mine.items():
+        wide = "k_attn_fwdILi128" in name
+        assert int(re.search(r"\.private_segment_fixed_size: (\d+)\n", note).group(1)) <= (32 if wide else 0), name
+        assert int(re.search(r"\.vgpr_spill_count: (\d+)\n", note).group(1)) <= (7 if wide else 0), name
