@@ -13,8 +13,8 @@
 // meet in memory (plan_of, met).  Rows (keys) whose sums are not finite are formed again with fp32 instructions.
 //
 // What bounds it: as in the forward pass the matrix core and the vector instructions in turn, which two waves overlap in part; the matrix core is busy 46 % of the time with heads of
-// 128, 36 % with heads of 64 (32 rows by 16 keys: 96 matrix and 320 vector instructions, 48 and 254).  2 x 16 heads, 8 of keys, [2048, 128] without a mask take 700 us,
-// 245 TFLOP/s counted as five products, 343 of the seven that are formed; causal and under a cap 445; 4 x 16 of [2048, 64] 838 and 470.
+// 128, 36 % with heads of 64 (32 rows by 16 keys: 96 matrix and 309 vector instructions, 48 and 247).  2 x 16 heads, 8 of keys, [2048, 128] without a mask take 700 us,
+// 245 TFLOP/s counted as five products, 343 of the seven that are formed; causal and under a cap 443 to 474; 4 x 16 of [2048, 64] 838 and 470.
 #include <algorithm>
 #include <cmath>
 

@@ -6,7 +6,7 @@
 // the tile kernel does (attn_fwd.hip).  Maxima, sums and outputs of the waves meet in LDS, those of the ranges in memory, where the last workgroup of the rows to arrive adds
 // them, in order: one launch, and the same bits whoever is last.
 //
-// A token of each of 32 sequences over 2048 to 4096 keys, 32 heads, 8 of keys, of 128 takes 167 us, 4.9 TB/s of cache; the matrix core is busy a tenth of the cycles, vector instructions two fifths.
+// A token of each of 32 sequences over 2048 to 4096 keys, 32 heads, 8 of keys, of 128 takes 169 us, 4.8 TB/s of cache; the matrix core is busy a tenth of the cycles, vector instructions two fifths.
 // One token over 500 keys, 16 heads, 4 of keys, of 64: 10.2 us, latency of lengths, keys and the join (15.3 in one range).
 #include "attn_launch.h"
 #include "attn_tiles.h"

@@ -1,20 +1,24 @@
 // Attention forward under score rules: tiles of queries on the f16 matrix core.
 //
 // A workgroup of eight waves owns 256 rows of queries, a wave 32 of them, or 128, two waves 32 of them and half of the keys each; the rows are those of one query head, or,
-// where a head has few, of all heads that share keys, one after the other.  Keys and values stream through LDS in blocks of 64 (128 of heads up to 64: half the barriers, 3 % less time), cut into f16 terms on the
+// where a head has few, of all heads that share keys, one after the other.  Keys and values stream through LDS in blocks of 64 (128 of heads up to 64, half the barriers), cut into f16 terms on the
 // way (f16x2.h; a query's row once, a probability when it is used).  As in plain attention (sdpa.hip) a lane owns query (l & 31) in the score tile and in the output:
 //   S^T tile   A = keys' rows, B = the wave's queries; register v of a lane is key 8 (v >> 2) + 4 (l >> 5) + (v & 3)
 //   softmax    online, in log2 units; the reference point moves only when a probability times its value row's factor no longer fits an operand
 //   O^T tile   A = V^T, read from the rows by transposing LDS reads, B = the probabilities where the score tile left them
 // What a query sees is the keys before `end` that have its document (AttnRow).  Blocks that no row of the workgroup sees are not fetched, 32-key tiles that no row of a
 // wave sees not computed, and only tiles that some row sees in part pay for the mask; with documents the ranges of ids of each 32 keys, formed by a first
-// launch, decide that.  A row whose sums are not finite (infinities or NaNs that it sees, or that a masked key of a tile holds) is formed again with fp32
+// launch, decide that.  A row whose sums are not finite (infinities, NaNs or values from 2^78 on that it sees, or that a masked key of a tile holds) is formed again with fp32
 // instructions by its wave.
+//
+// Blocks of heads of 64, 64 keys -> 128 (us): 16 causal heads of [4096, 64] 142 -> 139, 128 of [1000, 64] under a cap 96 -> 93.5, 64 of [2048, 64] with 20 documents 74 -> 71.5, 512 of [512, 64] without a
+// mask 145 and 146.
 //
 // What bounds it: three f16 products for each fp32 one, and vector instructions beside them.  A tile of 32 x 32 scores of heads of 128 is 48 matrix instructions, 1536 cycles
 // of a SIMD, and 290 vector ones (a quarter of them cut keys and values), which the two waves of a SIMD overlap in part: the matrix core is busy 53 % of the time, 41 % with
-// heads of 64.  64 heads of [1024, 128] without a mask take 107 to 115 us, about 310 TFLOP/s of fp32 products (a large library product in bf16 does a third of
-// 1255), 512 heads of [512, 64] 151 us, 228 TFLOP/s; 64 causal heads of [1024, 128] under a cap 91 us.
+// heads of 64.  64 heads of [1024, 128] without a mask take 107 to 113 us, about 310 TFLOP/s of fp32 products (a large library product in bf16 does a third of
+// 1255), 512 heads of [512, 64] 146 us, 235 TFLOP/s; 64 causal heads of [1024, 128] under a cap 92 us.
+// Tiles of heads past 96 keep seven registers of a lane in memory.
 #include <algorithm>
 
 #include "attn_launch.h"

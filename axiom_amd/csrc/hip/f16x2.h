@@ -3,7 +3,7 @@
 // A row of a head is taken times 2^e so that its largest value lies in [2^14, 2^15), and each value is cut into hi = f16(x) and lo = f16(x - hi): 11 bits each,
 // so hi + lo is x to 2^-23 of itself.  A product of two values is formed of three products of terms, hi hi + hi lo + lo hi, added in fp32; lo lo, left out,
 // is at most 2^-22 of it.  Half of what six products of bf16 terms cost (bf16x3.h), for one bit of each operand.  The matrix core multiplies f16
-// subnormals exactly (measured), so what a value below 2^-17 of its row's largest loses is an absolute 2^-40 of that.
+// subnormals exactly (measured), so what a value below 2^-17 of its row's largest loses is an absolute 2^-39 of that at most.
 // Every row has a power of its own, and not a block: a row of 1e30 that a mask hides would otherwise take the bits of its neighbours.  Where rows are summed over
 // (P V), their powers go to the other operand, whose largest so far a running exponent holds.
 // Cutting a pair: two products (none where the values come scaled), two conversions of pairs, two mixed multiply-adds, four cycles each.  (Mixed multiply-adds

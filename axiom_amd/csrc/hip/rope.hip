@@ -3,7 +3,8 @@
 //   norm       r = 1 / sqrt(mean x^2 + eps), y = rotation(gamma x r)
 //   gradient   dn = rotation^T dy, dgamma = sum dn x r, dx = r (gamma dn - x r mean(gamma dn x r))
 // HBM-bound: 8 bytes a value (12 backward) against some ten operations.  16000 rows of 24 heads of 128 turned 71 us, 5.5 TB/s; 8192 rows of 40 heads of 128 normed and turned 63 us, 5.35
-// TB/s; the gradient for 4000 rows of 32 heads of 80 26 us, 4.7 TB/s, and 4 for the launch that joins the gammas' sums; 8 or 16 rows 4.5 to 4.8 us, what a launch and one trip to memory take.
+// TB/s; the gradient for 4000 rows of 32 heads of 80 26 us, 4.7 TB/s, and 4 for the launch that joins the gammas' sums
+// (all of them in fp32, in a fixed order: 1.6e-7 of their size there, 0.7e-7 where 64 bits add); 8 or 16 rows 4.5 to 4.8 us, what a launch and one trip to memory take.
 //
 // k_heads: a lane holds a unit of 8 columns of a head (two 16-byte accesses): four pairs, either eight neighbours or four from each half of the
 // rotated part, so a rotation never leaves the lane and a norm is a sum over the 4 to 64 lanes of a head.  The four angles of a

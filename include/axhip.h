@@ -359,8 +359,8 @@ int axhip_rope_frequencies(float *freq, int64_t rot, double theta, int scaling, 
 enum { AXHIP_ROPE_INTERLEAVED = 0, AXHIP_ROPE_HALVES = 1 };
 
 /* Rotary positions: the first rot columns of each of H heads of x [rows, H * dk] turned by a = pos[row] * freq[i] and taken times
- * `amplitude`, the others as they are, to y (the whole heads; y may be x with the same pitch, and must not overlap it otherwise).  The angle is the exact product of the int32 position and the float
- * frequency, reduced in 64 bits.  backward != 0: the transpose, y = amplitude * (turned by -a) of x: the gradient.
+ * `amplitude`, the others as they are, to y (the whole heads; y may be x with the same pitch, and must not overlap it otherwise).  The angle, the int32 position times the float frequency, is formed and
+ * reduced in 64 bits (off by some 2^-53 of its turns); its sine and cosine are taken in 32.  backward != 0: the transpose, y = amplitude * (turned by -a) of x: the gradient.
  * rot even, 0 <= rot <= dk <= 4096 (rot = 0 copies; pos and freq may then be NULL). */
 int axhip_rope_rows(const float *x, int64_t ldx, float *y, int64_t ldy, const int32_t *pos, const float *freq, int64_t rows, int64_t H,
                     int64_t dk, int64_t rot, float amplitude, int layout, int backward);
@@ -405,7 +405,10 @@ typedef struct {
  * few, single tokens over a cache.  dk a multiple of 4 up to 128 (AXHIP_ERR_NOT_IMPLEMENTED otherwise), pitches multiples of 4 floats up to
  * 2^22, Q, K, V, O 16-byte aligned, Sq and Sk up to 2^24.  cap is zero or any float from 2.1e-39 on (one far above all scores leaves
  * them as they are), scale below 2.35e38.  `rules` is read before
- * the call returns; what it points to when the kernels run.  Outputs must not overlap inputs or each other. */
+ * the call returns; what it points to when the kernels run.  Outputs must not overlap inputs or each other.
+ * Precision: products of rows of a head (scores, sums over keys or rows) have operands that are off by at most 2^-23 of themselves, or 2^-39 of the largest magnitude in their row of
+ * the head, whichever is more, and add in fp32; rows below 2^-102 throughout are off by 2^-125.  Values of a size of 2^x cost the probabilities some |x| roundings of theirs.  Sums that
+ * leave the floats on the way, and what sees infinities, NaNs or values of 2^78 and more, are formed again with fp32 instructions, many times slower. */
 int axhip_attn_fwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, const float *V, int64_t ldv, int64_t kv_rows, float *O, int64_t ldo,
                    float *L, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t dk, float scale, const axhip_attn_rules *rules);
 /* Its gradient from dO, with the O and L that the forward pass gave for the same arguments: dQ (rows and columns as Q), dK and dV (as K and

@@ -3,7 +3,7 @@ forward pass and the gradient."""
 import numpy as np
 import pytest
 
-from attn_oracle import Rules
+from attn_oracle import Rules, attention
 from test_gpu_attn import check, draw
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +93,25 @@ def test_gradients_that_grow_along_the_keys(hip, dk, k_size, v_size):
     v[:, 200:] *= np.float32(1e3)
     check(hip, q / np.float32(k_size), k * np.float32(k_size), v * np.float32(v_size), dk ** -0.5, Rules(), d_o)
     check(hip, q / np.float32(k_size), k * np.float32(k_size), v * np.float32(v_size), dk ** -0.5, Rules(cap=5.0), d_o)
+
+
+@pytest.mark.parametrize("shape,form", FORMS, ids=FORM_IDS)
+def test_small_values_beside_large_ones(hip, shape, form):
+    """Columns of values and of output gradients down to 2^-38 of their row: off by 2^-39 of the row's largest more than others, at most."""
+    say("attn small beside large", shape)
+    rng, q, k, v, d_o = draw(56, *shape)
+    B, Sq, Sk, H, Hkv, dk = shape
+    small = (2.0 ** -rng.integers(0, 39, dk)).astype(np.float32)
+    small[0] = 1
+    v, d_o = v * small, d_o * small
+    plain = Rules()
+    want = attention(q, k, v, dk ** -0.5, plain, d_o)
+    # probabilities over the largest of each row: attention of values that are it in every column, and the gradient of values with such output gradients
+    of_v = attention(q, k, np.broadcast_to(np.abs(v).max(-1, keepdims=True), v.shape), dk ** -0.5, plain)["o"]
+    of_o = attention(q, k, v, dk ** -0.5, plain, np.broadcast_to(np.abs(d_o).max(-1, keepdims=True), d_o.shape))["dv"]
+    want["tol_o"] += 2.0 ** -39 * of_v
+    want["tol_dv"] += 2.0 ** -39 * of_o
+    out = check(hip, q, k, v, dk ** -0.5, plain, want=want, kernel=form)
+    # scores' gradients are sums over a row, whose largest decides
+    check(hip, q, k, v, dk ** -0.5, plain, d_o, want=want)
+    assert np.isfinite(out["o"]).all()
