@@ -4,7 +4,7 @@
 //   gradient   dn = rotation^T dy, dgamma = sum dn x r, dx = r (gamma dn - x r mean(gamma dn x r))
 // HBM-bound: 8 bytes a value (12 backward) against some ten operations.  16000 rows of 24 heads of 128 turned 71 us, 5.5 TB/s; 8192 rows of 40 heads of 128 normed and turned 63 us, 5.35
 // TB/s; the gradient for 4000 rows of 32 heads of 80 26 us, 4.7 TB/s, and 4 for the launch that joins the gammas' sums
-// (all of them in fp32, in a fixed order: 1.6e-7 of their size there, 0.7e-7 where 64 bits add); 8 or 16 rows 4.5 to 4.8 us, what a launch and one trip to memory take.
+// (a workgroup's sums in fp32, joined in 64 bits, in a fixed order: 0.9e-7 of their size there; 0.6e-7 would be 64 bits throughout, 1.3e-7 was fp32 throughout); 8 or 16 rows 4.5 to 4.8 us, what a launch and one trip to memory take.
 //
 // k_heads: a lane holds a unit of 8 columns of a head (two 16-byte accesses): four pairs, either eight neighbours or four from each half of the
 // rotated part, so a rotation never leaves the lane and a norm is a sum over the 4 to 64 lanes of a head.  The four angles of a
@@ -262,11 +262,11 @@ __global__ void __launch_bounds__(64) k_heads_any(HeadsArgs p) {
     }
 }
 
-// dgamma from the workgroups' sums: 16 columns a workgroup, its 64 parts take the sums in turn, sixteen loads of each under way
+// dgamma from the workgroups' sums, in 64 bits and rounded once: 16 columns a workgroup, its 64 parts take the sums in turn, sixteen loads of each under way
 __global__ void __launch_bounds__(1024) k_gamma_sums(const float *partial, int n, int dk, float *dgq, float *dgk) {
-    __shared__ float parts[64][16];
+    __shared__ double parts[64][16];
     const int here = threadIdx.x & 15, col = blockIdx.x * 16 + here, part = threadIdx.x >> 4;
-    float sum = 0.0f;
+    double sum = 0.0;
     if (col < 2 * dk) {
 #pragma unroll 16
         for (int b = part; b < n; b += 64) sum += partial[(int64_t)b * 2 * dk + col];
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(1024) k_gamma_sums(const float *partial, int n
     }
     if (part != 0 || col >= 2 * dk) return;
     float *out = col < dk ? dgq : dgk;
-    if (out) out[col < dk ? col : col - dk] = parts[0][here];
+    if (out) out[col < dk ? col : col - dk] = (float)parts[0][here];
 }
 
 constexpr int64_t GRAD_GROUPS = 1024;            // workgroups of four waves at most whose sums are joined by k_gamma_sums (of one: four times as many)
