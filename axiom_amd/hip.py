@@ -19,6 +19,20 @@ class AttnRules(C.Structure):
     _fields_ = [("cap", C.c_float), ("causal", C.c_int32), ("slopes", vp), ("prefix", vp), ("start", vp), ("lens", vp), ("doc_q", vp), ("doc_k", vp)]
 
 
+KV_F16, KV_I8, KV_MX4 = 0, 1, 2
+
+
+class KvCache(C.Structure):
+    """axhip_kv_cache: KvCache(type=KV_I8, page_rows=16, pages=n, heads=8, dk=128, k=ptr, v=ptr, k_scale=ptr, v_scale=ptr, table=ptr, table_ld=n)."""
+    _fields_ = [("type", C.c_int32), ("page_rows", C.c_int32), ("pages", i64), ("heads", i64), ("dk", i64), ("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp),
+                ("table", vp), ("table_ld", i64)]
+
+
+class KvRules(C.Structure):
+    """axhip_kv_rules: KvRules(window=1024, sinks=4)."""
+    _fields_ = [("cap", C.c_float), ("window", C.c_int32), ("sinks", C.c_int32), ("slopes", vp)]
+
+
 # every symbol include/axhip.h declares: (restype, argtypes)
 SIGNATURES = {
     "axhip_init": (C.c_int, []),
@@ -75,6 +89,10 @@ SIGNATURES = {
     "axhip_attn_fwd": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, i64, i64, i64, i64, C.c_float, C.POINTER(AttnRules)]),
     "axhip_attn_bwd": (C.c_int, [vp, i64, vp, i64, vp, i64, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i64, i64, i64, i64,
                                  C.c_float, C.POINTER(AttnRules)]),
+    "axhip_kv_row_bytes": (i64, [C.c_int, i64]),
+    "axhip_kv_write": (C.c_int, [C.POINTER(KvCache), vp, i64, vp, i64, vp, vp, i64, i64, i64]),
+    "axhip_kv_read": (C.c_int, [C.POINTER(KvCache), vp, i64, vp, i64, vp, vp, i64, i64, i64]),
+    "axhip_attn_paged": (C.c_int, [vp, i64, C.POINTER(KvCache), vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, C.c_float, C.POINTER(KvRules)]),
     "axhip_head_split_qkv": (C.c_int, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64]),
     "axhip_head_interleave": (C.c_int, [vp, vp, i64, i64, i64, i64]),
     "axhip_head_deinterleave": (C.c_int, [vp, vp, i64, i64, i64, i64]),

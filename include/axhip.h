@@ -417,6 +417,66 @@ int axhip_attn_bwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, con
                    const float *L, const float *dO, int64_t lddo, float *dQ, int64_t lddq, float *dK, int64_t lddk, float *dV, int64_t lddv,
                    int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t dk, float scale, const axhip_attn_rules *rules);
 
+/* ---- a paged cache of keys and values in few bits, and attention over it ------------------------
+ * For serving: sequences get pages as they grow, their keys and values are quantised as they are written, and the new tokens of all
+ * sequences (chunks of prompts, single tokens, both in one call) attend to what their pages hold.  The reference has no cache.
+ *
+ * A row of a head (dk values x, `top` their largest magnitude) is held as a scale s and dk numbers n of few bits that stand for s n:
+ *   AXHIP_KV_F16   s = 2^e that takes top to [2^14, 2^15), but no less than 2^-100; n = the f16 nearest to x / s (half a step: 2^-11 of x)
+ *   AXHIP_KV_I8    s = top / 127 rounded to fp32, but no less than 2^-100; n = the integer nearest to x / s, within 127
+ *   AXHIP_KV_MX4   a scale for each 32 columns (the last group may be shorter): s = 2^e, e = floor(log2(top of the group)) - 2, but no less than -127;
+ *                  n = the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their opposites (beyond 6: 6)
+ * The nearest to the exact quotient, ties to the even last bit.  A row (for MX4, a group) that holds an infinity or a NaN gets s = NaN and n = 0: all of it is NaN.
+ * In memory, k and v are [pages, heads, page_rows, axhip_kv_row_bytes] bytes: f16; int8; or 4-bit codes, the even column in the low half of a byte (sign, two bits
+ * of exponent, one of mantissa, as the values are listed); zeros behind them.  k_scale and v_scale are 4 bytes a row, [pages, heads, page_rows]: the float s, or a
+ * byte e + 127 (NaN: 255) a group.  All 16-byte aligned device memory, which axhip_malloc gives as zeros; a page may be copied or shared as it is.
+ * Position j of sequence b is row j % page_rows of page table[b * table_ld + j / page_rows]; an entry outside 0 .. pages - 1 is no page: nothing is written to it or read
+ * from it, and its keys are not seen.  No two new rows of a call may be in one place.
+ * page_rows is a power of two up to 2^16; pages * heads * page_rows up to 2^40; dk a multiple of 4 up to 128 (AXHIP_ERR_NOT_IMPLEMENTED otherwise). */
+enum { AXHIP_KV_F16 = 0, AXHIP_KV_I8 = 1, AXHIP_KV_MX4 = 2 };
+typedef struct {
+    int32_t type;
+    int32_t page_rows;
+    int64_t pages;
+    int64_t heads;              /* of keys */
+    int64_t dk;
+    void *k, *v;
+    void *k_scale, *v_scale;
+    const int32_t *table;       /* [B, table_ld] */
+    int64_t table_ld;
+} axhip_kv_cache;
+/* Bytes of a row of a head, a multiple of 16 (0: no such type or head size). */
+int64_t axhip_kv_row_bytes(int type, int64_t dk);
+
+/* The new rows of a call, in all three of the following: those of sequence b are rows first[b] .. first[b + 1] - 1 (at most Sq of them; first NULL: b * Sq .. b * Sq + Sq - 1,
+ * and T = B * Sq) of arrays of T rows, and they are the last of its lens[b] positions: n rows, row i at position p = lens[b] - n + i.  Rows with p < 0 are padding, and
+ * lens[b] is taken as 0 below 0 and as the table's room above it.  first [B + 1] must not fall; lens [B]; Sq, T and positions up to 2^24. */
+
+/* Quantises rows of K and V (heads * dk floats, row pitches ldk and ldv) into their places.  Padding is not written. */
+int axhip_kv_write(const axhip_kv_cache *cache, const float *K, int64_t ldk, const float *V, int64_t ldv, const int32_t *first, const int32_t *lens, int64_t B,
+                   int64_t T, int64_t Sq);
+/* Brings the same rows back as fp32 s n.  Padding, and rows on no page, are left as they were.  With first the sums of lens and Sq the longest, whole sequences. */
+int axhip_kv_read(const axhip_kv_cache *cache, float *K, int64_t ldk, float *V, int64_t ldv, const int32_t *first, const int32_t *lens, int64_t B, int64_t T, int64_t Sq);
+
+/* Rules for the scores of axhip_attn_paged; zeroes, or no rules at all, are plain causal attention.  With x = scale * (q . k):
+ *   cap > 0: x = cap * tanh(x / cap);   slopes: x = x - slopes[h] * (p - j)
+ * and the query at p sees key j if j <= p, and, window > 0, if p - j < window or j < sinks (the first tokens, which stay visible). */
+typedef struct {
+    float cap;
+    int32_t window;
+    int32_t sinks;
+    const float *slopes;        /* [H] */
+} axhip_kv_rules;
+
+/* Attention of new rows over their sequences' pages (the rows' own keys among them: write first), O = softmax(x) V, for H query heads that share the cache's heads (H a
+ * multiple of them: query head h reads head h / (H / heads)).  Rows of Q and O hold H * dk floats; L [T, H] is the log-sum-exp of each row of scores, or NULL.  Sk is the most
+ * positions that any sequence has (lens is taken as Sk above it).  A row that sees no key, padding among them, gets O = 0 and L = -infinity; rows of no sequence are left as they
+ * were.  What a query does not see has no part in its results, whatever it holds.  Pitches multiples of 4 floats up to 2^22, Q and O 16-byte aligned, outputs apart from all
+ * else.  cap and scale as for axhip_attn_fwd; precision too, with what the cache holds taken exactly (of F16 and I8; an MX4 number below 2^-36 of its row's largest loses bits).
+ * The rules are read before the call returns. */
+int axhip_attn_paged(const float *Q, int64_t ldq, const axhip_kv_cache *cache, float *O, int64_t ldo, float *L, const int32_t *first, const int32_t *lens, int64_t B,
+                     int64_t T, int64_t H, int64_t Sq, int64_t Sk, float scale, const axhip_kv_rules *rules);
+
 /* ---- layout transforms around attention (the layout members of the reference's GPU extension
  * table, include/axiom/internal/cuda_extension.h:45-84) ------------------------------------- */
 /* qkv [B*S, 3D] (row = [q | k | v], D = H*dk) -> q, k, v each [B*H, S, dk]; bqkv [3D] is added

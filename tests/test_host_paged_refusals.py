@@ -1,0 +1,90 @@
+"""What the entry points of the paged cache and the attention over it refuse and what they launch, on the host, without a GPU."""
+import pytest
+
+from test_host_runtime import run, stub  # noqa: F401  (stub is a fixture)
+
+PAGED = """
+from axiom_amd.hip import KvCache, KvRules
+hip.check(L.axhip_init())
+P = [1 << n for n in range(45, 57)]
+def cache(type=1, page_rows=16, pages=100, heads=2, dk=64, k=P[0], v=P[1], k_scale=P[2], v_scale=P[3], table=P[4], table_ld=8):
+    return C.byref(KvCache(type=type, page_rows=page_rows, pages=pages, heads=heads, dk=dk, k=k, v=v, k_scale=k_scale, v_scale=v_scale, table=table, table_ld=table_ld))
+def rows(f, c=None, K=P[5], ldk=128, V=P[6], ldv=128, first=P[7], lens=P[8], B=3, T=20, Sq=10, **more):
+    return f(cache(**more) if c is None else c, K, ldk, V, ldv, first, lens, B, T, Sq)
+def write(*a, **more): return rows(L.axhip_kv_write, *a, **more)
+def read(*a, **more): return rows(L.axhip_kv_read, *a, **more)
+def attend(c=None, Q=P[5], ldq=256, O=P[6], ldo=256, lse=P[9], first=P[7], lens=P[8], B=3, T=20, H=4, Sq=10, Sk=128, scale=0.125, rules=None, **more):
+    return L.axhip_attn_paged(Q, ldq, cache(**more) if c is None else c, O, ldo, lse, first, lens, B, T, H, Sq, Sk, scale, C.byref(rules) if rules else None)
+"""
+
+
+def test_refusals(stub):  # noqa: F811
+    run(stub, PAGED + """
+nan, inf = float("nan"), float("inf")
+for f in (write, read, attend):
+    for dk in (0, 2, 6, 132, 63, -4, 1 << 62):
+        assert f(dk=dk) == 10, dk
+    for bad in (dict(type=-1), dict(type=3), dict(page_rows=0), dict(page_rows=3), dict(page_rows=-16), dict(page_rows=1 << 17), dict(heads=0), dict(heads=-2), dict(heads=(1 << 20) + 1),
+                dict(pages=-1), dict(pages=1 << 31), dict(pages=1 << 30, heads=1 << 10), dict(table_ld=-1), dict(table_ld=1 << 41), dict(B=-1), dict(B=1 << 23), dict(T=-1), dict(T=(1 << 24) + 1), dict(Sq=-1),
+                dict(Sq=(1 << 24) + 1), dict(first=None), dict(k=P[0] + 8), dict(v=P[1] + 4), dict(k_scale=P[2] + 4), dict(v_scale=P[3] + 12)):
+        assert f(**bad) == 3, bad
+    for bad in (dict(k=None), dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(table=None), dict(lens=None), dict(c=C.POINTER(KvCache)())):
+        assert f(**bad) == 1, bad
+for f in (write, read):
+    for bad in (dict(ldk=127), dict(ldv=124), dict(ldk=130), dict(ldv=(1 << 22) + 4), dict(K=P[5] + 4), dict(V=P[6] + 8)):
+        assert f(**bad) == 3, bad
+    assert f(K=None) == 1 and f(V=None) == 1
+for bad in (dict(ldq=255), dict(ldq=258), dict(ldo=252), dict(ldo=(1 << 22) + 4), dict(Q=P[5] + 4), dict(O=P[6] + 8), dict(H=0), dict(H=3), dict(H=-2), dict(H=(1 << 20) + 2), dict(H=1 << 62),
+            dict(Sk=-1), dict(Sk=(1 << 24) + 1), dict(B=1 << 22, H=1 << 10, ldq=1 << 16, ldo=1 << 16), dict(rules=KvRules(cap=-1.0)), dict(rules=KvRules(cap=nan)), dict(rules=KvRules(cap=inf)),
+            dict(rules=KvRules(cap=1e-40)), dict(scale=2.4e38), dict(rules=KvRules(window=-1)), dict(rules=KvRules(sinks=-1))):
+    assert attend(**bad) == 3, bad
+assert attend(Q=None) == 1 and attend(O=None) == 1
+assert len(launched()) == 0
+for f in (write, read, attend):
+    assert f(B=0) == 0 and f(T=0) == 0 and f(Sq=0) == 0 and f(first=None, B=2, T=0, Sq=0) == 0
+    assert f(B=0, T=0, lens=None, table=None, k=None) == 0
+assert len(launched()) == 0
+assert write() == 0 and read() == 0 and attend() == 0 and attend(lse=None, rules=KvRules(window=(1 << 31) - 1, sinks=(1 << 31) - 1)) == 0 and attend(first=None, B=2) == 0
+assert len(launched()) > 0
+""")
+
+
+def test_row_bytes(stub):  # noqa: F811
+    run(stub, """
+f = L.axhip_kv_row_bytes
+assert [f(t, 128) for t in (0, 1, 2)] == [256, 128, 64] and [f(t, 80) for t in (0, 1, 2)] == [160, 80, 48] and [f(t, 4) for t in (0, 1, 2)] == [16, 16, 16]
+assert all(f(t, dk) == 0 for t, dk in ((-1, 64), (3, 64), (0, 0), (0, 132), (1, 30), (2, -4)))
+""")
+
+
+def test_which_launches(stub):  # noqa: F811
+    """Few rows of every sequence: one launch; many of every one: tiles alone; unlike ones: both."""
+    run(stub, PAGED + """
+def names(**more):
+    before = stub.stub_launches()
+    assert attend(**more) == 0
+    return [("few" if b"paged_few" in x.kernel else "tiles" if b"paged_tiles" in x.kernel else "join" if b"paged_join" in x.kernel else "?") for x in launched()[before:]]
+assert names(Sq=1, T=3, first=None) == ["few"] and names(Sq=4, T=9) == ["few"] and names(Sq=16, T=9) == ["few"]
+assert names(Sq=100, T=300, first=None, Sk=100)[0] == "tiles" and "few" not in names(Sq=100, T=100, B=1)
+assert names(Sq=100, T=120)[:2] == ["few", "tiles"]
+assert names(Sq=100, T=100, B=1, Sk=100000, table_ld=10000)[-1] == "join"
+""")
+
+
+@pytest.mark.parametrize("B,T,H,heads,Sq,Sk,dk,kind,uniform", [(1, 1, 1, 1, 1, 0, 4, 0, False), (8388607, 1 << 24, 1, 1, 1 << 24, 1 << 24, 128, 1, False), (1, 1 << 24, 8, 1, 1 << 24, 1 << 24, 128, 2, True),
+                                                               (2047, 2047, 1 << 20, 1 << 20, 1, 100, 4, 1, True), (1 << 20, 1 << 20, 8, 8, 1, 1 << 20, 64, 2, True),
+                                                               (1, 3, 1 << 15, 1, 3, 1 << 24, 128, 1, True), (100, 1 << 20, 64, 1, 1 << 20, 1 << 20, 32, 0, False)])
+def test_launches(stub, B, T, H, heads, Sq, Sk, dk, kind, uniform):  # noqa: F811
+    """Any extent is made of launches that the runtime takes, or refused."""
+    run(stub, PAGED + """
+B, T, H, heads, Sq, Sk, dk, kind, uniform = %r
+stub.stub_set_free(C.c_size_t(200 << 30))
+first = None if uniform else P[7]
+more = dict(type=kind, heads=heads, dk=dk, pages=1 << 12, table_ld=1 << 20, B=B, T=T, Sq=Sq, first=first)
+hip.check(write(ldk=heads * dk, ldv=heads * dk, **more))
+hip.check(read(ldk=heads * dk, ldv=heads * dk, **more))
+for rules in (None, KvRules(window=1000, sinks=4, cap=10.0)):
+    hip.check(attend(ldq=H * dk, ldo=H * dk, H=H, Sk=Sk, rules=rules, **more))
+for x in launched():
+    assert 0 < x.grid[0] < 1 << 31 and x.grid[0] * x.block[0] < 1 << 32 and x.block[0] <= 1024 and x.shared <= 160 * 1024, (x.kernel, list(x.grid), list(x.block))
+""" % ((B, T, H, heads, Sq, Sk, dk, kind, uniform),))
