@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(64 * WAVES) k_kv_write(RowsArgs a) {
     for (int i = 0; i < AHEAD; i++) {
         const int task = task0 + i * (64 / LANES);
         const bool of_v = task >= p.heads;
-        const int64_t row = kv_row(p, page, of_v ? task - p.heads : task, pos);
-        unsigned char *const to = (of_v ? p.v : p.k) + row * p.row_bytes, *const scales = (of_v ? p.v_scale : p.k_scale) + row * 4;
+        const int head = of_v ? task - p.heads : task;
+        unsigned char *const to = (of_v ? p.v : p.k) + kv_row_at(p, page, head, pos), *const scales = (of_v ? p.v_scale : p.k_scale) + kv_scale_at(p, page, head, pos);
         float y[8];
         unsigned top = 0;
 #pragma unroll
@@ -143,9 +143,8 @@ __global__ void __launch_bounds__(64 * WAVES) k_kv_read(RowsArgs a) {
         if (task >= tasks || 8 * c >= p.dk) break;
         const bool of_v = task >= p.heads;
         const int head = of_v ? task - p.heads : task;
-        const int64_t row = kv_row(p, page, head, pos);
         float x[8];
-        kv_eight<TYPE>((of_v ? p.v : p.k) + row * p.row_bytes, *reinterpret_cast<const unsigned *>((of_v ? p.v_scale : p.k_scale) + row * 4), c, x);
+        kv_eight<TYPE>((of_v ? p.v : p.k) + kv_row_at(p, page, head, pos), *reinterpret_cast<const unsigned *>((of_v ? p.v_scale : p.k_scale) + kv_scale_at(p, page, head, pos)), c, x);
         float *to = (of_v ? a.v + t * a.ldv : a.k + t * a.ldk) + (int64_t)head * p.dk + 8 * c;
         *reinterpret_cast<v4f *>(to) = v4f{x[0], x[1], x[2], x[3]};
         if (8 * c + 4 < p.dk) *reinterpret_cast<v4f *>(to + 4) = v4f{x[4], x[5], x[6], x[7]};
@@ -196,6 +195,8 @@ int kv_arguments(const char *who, KvPages &a, const axhip_kv_cache *cache, const
         return fail(AXHIP_ERR_SHAPE, "%s: rows of a page must be a power of two up to 2^16", who);
     if (c.heads < 1 || c.heads > (1 << 20)) return fail(AXHIP_ERR_SHAPE, "%s: 1 to 2^20 heads of keys", who);
     if (c.pages < 0 || c.pages > 0x7fffffff || c.pages > (int64_t(1) << 40) / (c.heads * c.page_rows)) return fail(AXHIP_ERR_SHAPE, "%s: bad count of pages", who);
+    const int64_t row_bytes = axhip_kv_row_bytes(c.type, c.dk);
+    if (c.heads * c.page_rows > 0xffffffff / row_bytes) return fail(AXHIP_ERR_SHAPE, "%s: a page of keys must be below 4 GiB", who);
     constexpr int64_t LONG = 1 << 24;
     if (B < 0 || B > 0x7fffff || T < 0 || T > LONG || Sq < 0 || Sq > LONG) return fail(AXHIP_ERR_SHAPE, "%s: bad extent", who);
     if (!first && T != B * Sq) return fail(AXHIP_ERR_SHAPE, "%s: without `first` there are B * Sq rows", who);
@@ -215,7 +216,9 @@ int kv_arguments(const char *who, KvPages &a, const axhip_kv_cache *cache, const
     a.heads = (int)c.heads;
     a.dk = (int)c.dk;
     a.shift = __builtin_ctz((unsigned)c.page_rows);
-    a.row_bytes = (int)axhip_kv_row_bytes(c.type, c.dk);
+    a.row_bytes = (int)row_bytes;
+    a.page_bytes = (uint32_t)(c.heads * c.page_rows * row_bytes);
+    a.page_scales = (uint32_t)(c.heads * c.page_rows * 4);
     a.B = (int)B;
     a.T = (int)T;
     a.Sq = (int)Sq;

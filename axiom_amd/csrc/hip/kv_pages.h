@@ -9,6 +9,7 @@ struct KvPages {
     const int32_t *table, *first, *lens;
     int64_t table_ld, pages;
     int heads, dk, shift, row_bytes;             // page_rows is 2^shift
+    uint32_t page_bytes, page_scales;            // of a page of k or v and of its scales
     int B, T, Sq, room;                          // room: the most positions that a sequence is taken to have
 };
 
@@ -49,14 +50,21 @@ __device__ __forceinline__ int kv_find(const KvPages &a, int lane, Before before
     return b;
 }
 
-// The page of a position below a sequence's length, or -1
+// The table's entry for a position below a sequence's length, and whether it is a page: apart, so that entries can be under way while nothing waits for them
+__device__ __forceinline__ int kv_entry(const KvPages &a, int b, int pos) { return a.table[(int64_t)b * a.table_ld + (pos >> a.shift)]; }
+__device__ __forceinline__ bool kv_is_page(const KvPages &a, int entry) { return (unsigned)entry < (unsigned)a.pages; }
 __device__ __forceinline__ int kv_page(const KvPages &a, int b, int pos) {
-    const int page = a.table[(int64_t)b * a.table_ld + (pos >> a.shift)];
-    return (uint64_t)(int64_t)page < (uint64_t)a.pages ? page : -1;
+    const int entry = kv_entry(a, b, pos);
+    return kv_is_page(a, entry) ? entry : -1;
 }
-// A row of a head, counted over all pages
-__device__ __forceinline__ int64_t kv_row(const KvPages &a, int page, int head, int pos) {
-    return (((int64_t)page * a.heads + head) << a.shift) + (pos & ((1 << a.shift) - 1));
+// Where a row of a head is in k and v, and its scale in k_scale and v_scale, in bytes.  (A page is below 4 GiB, its rows fewer than 2^24 / 256.)
+__device__ __forceinline__ uint64_t kv_row_at(const KvPages &a, int page, int head, int pos) {
+    const unsigned in_page = (unsigned)pos & ((1u << a.shift) - 1);
+    return (uint64_t)(unsigned)page * a.page_bytes + ((unsigned)head << a.shift) * (unsigned)a.row_bytes + __umul24(in_page, (unsigned)a.row_bytes);
+}
+__device__ __forceinline__ uint64_t kv_scale_at(const KvPages &a, int page, int head, int pos) {
+    const unsigned in_page = (unsigned)pos & ((1u << a.shift) - 1);
+    return (uint64_t)(unsigned)page * a.page_scales + (((unsigned)head << a.shift) + in_page) * 4;
 }
 
 typedef _Float16 kv_half2 __attribute__((ext_vector_type(2)));

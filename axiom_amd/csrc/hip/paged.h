@@ -105,19 +105,19 @@ __device__ __forceinline__ void paged_again(const PagedArgs &a, int b, const KvS
         }
         const int key = k0 + lane;
         bool sees = key < r.end && (key >= r.begin || key < a.sinks);
-        int64_t row = 0;
+        int page = 0;
         if (sees) {
-            const int page = kv_page(kv, b, key);
+            page = kv_page(kv, b, key);
             sees = page >= 0;
-            if (sees) row = kv_row(kv, page, hk, key);
         }
         float x = -INFINITY;
         if (sees) {
-            const unsigned scale = *reinterpret_cast<const unsigned *>(kv.k_scale + row * 4);
+            const unsigned scale = *reinterpret_cast<const unsigned *>(kv.k_scale + kv_scale_at(kv, page, hk, key));
+            const unsigned char *row = kv.k + kv_row_at(kv, page, hk, key);
             float sum = 0.0f;
             for (int c = 0; 8 * c < dk; c++) {
                 float k[8];
-                kv_eight<TYPE>(kv.k + row * kv.row_bytes, scale, c, k);
+                kv_eight<TYPE>(row, scale, c, k);
 #pragma unroll
                 for (int e = 0; e < 8; e++)
                     if (8 * c + e < dk) sum = __builtin_fmaf(q[8 * c + e] * a.attn.q_up, k[e], sum);
@@ -137,18 +137,19 @@ __device__ __forceinline__ void paged_again(const PagedArgs &a, int b, const KvS
         for (; seen; seen &= seen - 1) {
             const int j = __builtin_ctzll(seen);
             const float pj = from_lane(p, j);
-            const int64_t vrow = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)row, j) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(row >> 32), j) << 32);
-            const unsigned scale = *reinterpret_cast<const unsigned *>(kv.v_scale + vrow * 4);
+            const int of_j = __builtin_amdgcn_readlane(page, j);
+            const unsigned scale = *reinterpret_cast<const unsigned *>(kv.v_scale + kv_scale_at(kv, of_j, hk, k0 + j));
+            const unsigned char *row = kv.v + kv_row_at(kv, of_j, hk, k0 + j);
             float v[8];
             if (lane < dk) {
-                kv_eight<TYPE>(kv.v + vrow * kv.row_bytes, scale, lane >> 3, v);
+                kv_eight<TYPE>(row, scale, lane >> 3, v);
                 float mine = v[0];
 #pragma unroll
                 for (int e = 1; e < 8; e++) mine = (lane & 7) == e ? v[e] : mine;
                 o0 = __builtin_fmaf(pj, mine, o0);
             }
             if (lane + 64 < dk) {
-                kv_eight<TYPE>(kv.v + vrow * kv.row_bytes, scale, 8 + (lane >> 3), v);
+                kv_eight<TYPE>(row, scale, 8 + (lane >> 3), v);
                 float mine = v[0];
 #pragma unroll
                 for (int e = 1; e < 8; e++) mine = (lane & 7) == e ? v[e] : mine;

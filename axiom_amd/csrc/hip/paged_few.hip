@@ -113,27 +113,27 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
     // keys frow and 16 + frow of a tile
     Quarter<WORDS> kq[2], vq[2];
     unsigned ks[2], vs[2];
-    int page[2], next_page[2];
+    int entry[2];
+    bool here[2];
+    auto pos_of = [&](int n, int t) { return tiles.tile(n) * 32 + 16 * t + frow; };
     auto look = [&](int n) {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const int pos = tiles.tile(n) * 32 + 16 * t + frow;
-            next_page[t] = pos < high.end ? kv_page(kv, b, pos) : -1;
-        }
+        for (int t = 0; t < 2; t++) entry[t] = kv_entry(kv, b, min(pos_of(n, t), high.end - 1));
     };
     auto fetch = [&](int n) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            page[t] = next_page[t];
+            const int pos = pos_of(n, t);
+            here[t] = pos < high.end && kv_is_page(kv, entry[t]);
             kq[t].clear();
             vq[t].clear();
             ks[t] = vs[t] = 0;
-            if (page[t] >= 0) {
-                const int64_t at_row = kv_row(kv, page[t], hk, tiles.tile(n) * 32 + 16 * t + frow);
-                kq[t].template load<PAD>(kv.k + at_row * kv.row_bytes, part, kv.row_bytes);
-                vq[t].template load<PAD>(kv.v + at_row * kv.row_bytes, part, kv.row_bytes);
-                ks[t] = *reinterpret_cast<const unsigned *>(kv.k_scale + at_row * 4);
-                vs[t] = *reinterpret_cast<const unsigned *>(kv.v_scale + at_row * 4);
+            if (here[t]) {
+                const uint64_t at_row = kv_row_at(kv, entry[t], hk, pos), at_scale = kv_scale_at(kv, entry[t], hk, pos);
+                kq[t].template load<PAD>(kv.k + at_row, part, kv.row_bytes);
+                vq[t].template load<PAD>(kv.v + at_row, part, kv.row_bytes);
+                ks[t] = *reinterpret_cast<const unsigned *>(kv.k_scale + at_scale);
+                vs[t] = *reinterpret_cast<const unsigned *>(kv.v_scale + at_scale);
             }
         }
     };
@@ -179,7 +179,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
                 factors[32 + 16 * t + frow] = kv_factor<TYPE>(vs[t]) * T::VALUE_UP * VALUES_DOWN;
             }
         }
-        const bool here[2] = {page[0] >= 0, page[1] >= 0};
         const uint64_t gone0 = __builtin_amdgcn_ballot_w64(!here[0]), gone1 = __builtin_amdgcn_ballot_w64(!here[1]);
         const unsigned gone = ((unsigned)gone0 & 0xffffu) | (unsigned)gone1 << 16;
         v4f s[2];

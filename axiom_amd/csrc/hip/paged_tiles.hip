@@ -93,39 +93,54 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
 
     const unsigned base = lds_address(lds);
     // A pass brings 16 bytes a thread: LANES threads a row, rows of keys and then of values.
+    constexpr int PLACES = PASSES > 1 ? PASSES / 2 : 1;          // with two passes or more, the second half brings the values of the first half's keys
     v4i x[PASSES];
     unsigned scales[PASSES];
-    int page[PASSES], next_page[PASSES];
+    int entry[PLACES];
+    unsigned gone = 0;                               // a bit a place: its key has no page
     auto row_of = [&](int pass) { return (pass * 64 * WAVES + (int)threadIdx.x) / LANES; };      // from BKV on a value's; from 2 BKV on none
+    auto pos_of = [&](int n, int place) { return blocks.tile(n) * BKV + row_of(place) % BKV; };
     auto look = [&](int n) {
 #pragma unroll
-        for (int p = 0; p < PASSES; p++) {
-            const int at_row = row_of(p), pos = blocks.tile(n) * BKV + at_row % BKV;
-            next_page[p] = at_row < 2 * BKV && pos < wg_high.end ? kv_page(kv, b, pos) : -1;
-        }
+        for (int p = 0; p < PLACES; p++) entry[p] = kv_entry(kv, b, min(pos_of(n, p), wg_high.end - 1));
     };
     auto fetch = [&](int n) {
+        const int c = (int)threadIdx.x % LANES;
+        gone = 0;
 #pragma unroll
         for (int p = 0; p < PASSES; p++) {
-            const int at_row = row_of(p), c = (int)threadIdx.x % LANES;
-            page[p] = next_page[p];
             x[p] = v4i{0, 0, 0, 0};
             scales[p] = 0;
-            if (page[p] >= 0) {
-                const int64_t from = kv_row(kv, page[p], hk, blocks.tile(n) * BKV + at_row % BKV);
-                const bool of_v = at_row >= BKV;
-                if ((!PAD && DK != 96) || 16 * c < kv.row_bytes) x[p] = *reinterpret_cast<const v4i *>((of_v ? kv.v : kv.k) + from * kv.row_bytes + 16 * c);
-                scales[p] = *reinterpret_cast<const unsigned *>((of_v ? kv.v_scale : kv.k_scale) + from * 4);
+        }
+#pragma unroll
+        for (int p = 0; p < PLACES; p++) {
+            const int pos = pos_of(n, p);
+            if (pos < wg_high.end && kv_is_page(kv, entry[p]) && (2 * BKV * LANES >= 64 * WAVES || row_of(p) < 2 * BKV)) {
+                const uint64_t at_row = kv_row_at(kv, entry[p], hk, pos) + 16 * c, at_scale = kv_scale_at(kv, entry[p], hk, pos);
+                const bool some = (!PAD && DK != 96) || 16 * c < kv.row_bytes;
+                if (PASSES > 1) {
+                    if (some) {
+                        x[p] = *reinterpret_cast<const v4i *>(kv.k + at_row);
+                        x[(p + PLACES) % PASSES] = *reinterpret_cast<const v4i *>(kv.v + at_row);
+                    }
+                    scales[p] = *reinterpret_cast<const unsigned *>(kv.k_scale + at_scale);
+                    scales[(p + PLACES) % PASSES] = *reinterpret_cast<const unsigned *>(kv.v_scale + at_scale);
+                } else {
+                    const bool of_v = row_of(p) >= BKV;
+                    if (some) x[p] = *reinterpret_cast<const v4i *>((of_v ? kv.v : kv.k) + at_row);
+                    scales[p] = *reinterpret_cast<const unsigned *>((of_v ? kv.v_scale : kv.k_scale) + at_scale);
+                }
+            } else {
+                gone |= 1u << p;
             }
         }
     };
     auto stage = [&](unsigned cur) {
-        bool holes = false;
 #pragma unroll
         for (int p = 0; p < PASSES; p++) {
             const int at_row = row_of(p), c = (int)threadIdx.x % LANES, in_block = at_row % BKV;
             if (2 * BKV * LANES >= 64 * WAVES || at_row < 2 * BKV) {
-                const bool of_v = at_row >= BKV;
+                const bool of_v = PASSES > 1 ? p >= PLACES : at_row >= BKV;
                 const unsigned to = base + cur + (of_v ? G::V_AT : 0);
                 if (DK != 96 || c * COLS < DK) {
                     if constexpr (TYPE == AXHIP_KV_F16) write_chunk(to + B::at(in_block, c), x[p]);
@@ -145,12 +160,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
                 if (c == 0) {
                     const float f = kv_factor<TYPE>(scales[p]);
                     // (the sign of a value's factor says that there is no page)
-                    write_float(base + cur + G::FACTORS_AT + 4 * at_row, !of_v ? f : page[p] < 0 ? -0.0f : f * T::VALUE_UP * VALUES_DOWN);
+                    write_float(base + cur + G::FACTORS_AT + 4 * at_row, !of_v ? f : ((gone >> (p % PLACES)) & 1) ? -0.0f : f * T::VALUE_UP * VALUES_DOWN);
                 }
-                holes |= page[p] < 0;
             }
         }
-        const uint64_t any = __builtin_amdgcn_ballot_w64(holes);
+        const uint64_t any = __builtin_amdgcn_ballot_w64(gone != 0);
         if (lane == 0) *reinterpret_cast<int *>(lds + cur + G::HOLES_AT + 4 * wave) = any != 0;
     };
 

@@ -432,7 +432,7 @@ int axhip_attn_bwd(const float *Q, int64_t ldq, const float *K, int64_t ldk, con
  * byte e + 127 (NaN: 255) a group.  All 16-byte aligned device memory, which axhip_malloc gives as zeros; a page may be copied or shared as it is.
  * Position j of sequence b is row j % page_rows of page table[b * table_ld + j / page_rows]; an entry outside 0 .. pages - 1 is no page: nothing is written to it or read
  * from it, and its keys are not seen.  No two new rows of a call may be in one place.
- * page_rows is a power of two up to 2^16; pages * heads * page_rows up to 2^40; dk a multiple of 4 up to 128 (AXHIP_ERR_NOT_IMPLEMENTED otherwise). */
+ * page_rows is a power of two up to 2^16; a page of k or v below 4 GiB; pages * heads * page_rows up to 2^40; dk a multiple of 4 up to 128 (AXHIP_ERR_NOT_IMPLEMENTED otherwise). */
 enum { AXHIP_KV_F16 = 0, AXHIP_KV_I8 = 1, AXHIP_KV_MX4 = 2 };
 typedef struct {
     int32_t type;

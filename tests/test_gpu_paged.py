@@ -298,7 +298,7 @@ def test_forms(hip, kind, dk, new, lens, kernel):
     """Each form, by the kernel that it says it is."""
     say("forms", kind, dk, kernel)
     heads, G = (23, 1) if kernel == "paged_tiles_256" else (2, 4) if len(new) < 100 else (1, 2)
-    check(hip, kind, heads, G, dk, 64, new, lens, dict(window=500, sinks=70) if dk == 72 else {}, uniform=True, kernel=kernel)
+    check(hip, kind, heads, G, dk, 64, new, lens, dict(window=1500, sinks=70) if dk == 72 else {}, uniform=True, kernel=kernel)
 
 
 @TYPES
