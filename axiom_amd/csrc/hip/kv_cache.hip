@@ -13,7 +13,7 @@ constexpr int64_t GRID_MOST = int64_t(1) << 22;  // workgroups of a launch: a gr
 struct RowsArgs {
     KvPages pages;
     float *k, *v;                                // of the caller
-    int64_t ldk, ldv, first;                     // first: the launch's first workgroup
+    int64_t ldk, ldv, first;                     // first: the launch's first row
     int per_row;                                 // waves to a row
 };
 
@@ -50,9 +50,10 @@ template <int TYPE, int LANES>
 __global__ void __launch_bounds__(64 * WAVES) k_kv_write(RowsArgs a) {
     const KvPages &p = a.pages;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane % LANES;
-    const int64_t item = (a.first + blockIdx.x) * WAVES + wave, t = item / a.per_row;
+    const unsigned item = blockIdx.x * WAVES + wave, row = item / (unsigned)a.per_row;
+    const int64_t t = a.first + row;
     if (t >= p.T) return;
-    const int task0 = (int)(item - t * a.per_row) * (AHEAD * 64 / LANES) + lane / LANES, tasks = 2 * p.heads;
+    const int task0 = (int)(item - row * (unsigned)a.per_row) * (AHEAD * 64 / LANES) + lane / LANES, tasks = 2 * p.heads;
     v4f x[AHEAD][2];
 #pragma unroll
     for (int i = 0; i < AHEAD; i++) {
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(64 * WAVES) k_kv_write(RowsArgs a) {
             if (task < tasks && 8 * c + 4 * h < p.dk) x[i][h] = *reinterpret_cast<const v4f *>(from + 4 * h);
         }
     }
-    const int b = p.first ? kv_find(p, lane, [&](int, int first) { return first <= t; }) : (int)(t / p.Sq);
+    const int b = p.first ? kv_find(p, lane, [&](int, int first) { return first <= t; }) : (int)((unsigned)t / (unsigned)p.Sq);
     if (b >= p.B) return;
     const KvSeq s = kv_seq(p, b);
     const int i0 = (int)t - s.first, pos = s.len - s.n + i0;
@@ -127,16 +128,17 @@ template <int TYPE, int LANES>
 __global__ void __launch_bounds__(64 * WAVES) k_kv_read(RowsArgs a) {
     const KvPages &p = a.pages;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane % LANES;
-    const int64_t item = (a.first + blockIdx.x) * WAVES + wave, t = item / a.per_row;
+    const unsigned item = blockIdx.x * WAVES + wave, row = item / (unsigned)a.per_row;
+    const int64_t t = a.first + row;
     if (t >= p.T) return;
-    const int b = p.first ? kv_find(p, lane, [&](int, int first) { return first <= t; }) : (int)(t / p.Sq);
+    const int b = p.first ? kv_find(p, lane, [&](int, int first) { return first <= t; }) : (int)((unsigned)t / (unsigned)p.Sq);
     if (b >= p.B) return;
     const KvSeq s = kv_seq(p, b);
     const int i0 = (int)t - s.first, pos = s.len - s.n + i0;
     if (i0 < 0 || i0 >= s.n || pos < 0) return;
     const int page = kv_page(p, b, pos);
     if (page < 0) return;
-    const int task0 = (int)(item - t * a.per_row) * (AHEAD * 64 / LANES) + lane / LANES, tasks = 2 * p.heads;
+    const int task0 = (int)(item - row * (unsigned)a.per_row) * (AHEAD * 64 / LANES) + lane / LANES, tasks = 2 * p.heads;
 #pragma unroll
     for (int i = 0; i < AHEAD; i++) {
         const int task = task0 + i * (64 / LANES);
@@ -169,11 +171,12 @@ int rows_arguments(const char *who, RowsArgs &a, const axhip_kv_cache *cache, co
 
 template <typename Launch>
 int launch_rows(RowsArgs &a, const char *who, Launch launch) {
-    const int lanes = a.pages.dk <= 32 ? 4 : a.pages.dk <= 64 ? 8 : 16, at_once = AHEAD * 64 / lanes;
-    a.per_row = (2 * a.pages.heads + at_once - 1) / at_once;
-    const int64_t all = ((int64_t)a.pages.T * a.per_row + WAVES - 1) / WAVES;
-    for (a.first = 0; a.first < all; a.first += GRID_MOST) {
-        const dim3 grid((unsigned)(all - a.first < GRID_MOST ? all - a.first : GRID_MOST));
+    const int lanes = a.pages.dk <= 32 ? 4 : a.pages.dk <= 64 ? 8 : 16, heads = AHEAD * 64 / lanes;
+    a.per_row = (2 * a.pages.heads + heads - 1) / heads;
+    const int64_t at_once = GRID_MOST * WAVES / a.per_row;       // rows a launch; (a row has at most 2^17 waves)
+    for (a.first = 0; a.first < a.pages.T; a.first += at_once) {
+        const int64_t rows = a.pages.T - a.first < at_once ? a.pages.T - a.first : at_once;
+        const dim3 grid((unsigned)((rows * a.per_row + WAVES - 1) / WAVES));
         if (lanes == 4) launch(std::integral_constant<int, 4>(), grid);
         else if (lanes == 8) launch(std::integral_constant<int, 8>(), grid);
         else launch(std::integral_constant<int, 16>(), grid);

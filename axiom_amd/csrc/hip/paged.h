@@ -13,7 +13,7 @@ struct PagedArgs {
 };
 
 struct PagedFewGrid {
-    int64_t first;                               // the launch's first workgroup
+    int first;                                   // the launch's first sequence
     int row_tiles, splits;                       // of 16 rows each; ranges of keys
     int most;                                    // sequences with more rows (of all heads that share keys) are the tiles'
     float *parts;                                // what the ranges leave
@@ -21,15 +21,15 @@ struct PagedFewGrid {
 };
 
 struct PagedTileGrid {
-    int64_t first, slots;                        // slots: places for tiles, of which each sequence has as many as its rows could need
+    int64_t first, slots, per;                   // the launch's first slot; slots: places for tiles, of which each sequence has as many as its rows could need (`per`, where they are equal)
     int splits;                                  // ranges of keys
     int least;                                   // sequences with fewer rows are the few-rows form's
     float *parts;
     int *arrivals;
 };
 
-int paged_few(const PagedArgs &a, int type, int rows_most, int64_t keys);
-int paged_tiles(const PagedArgs &a, int type, int rows_least, int64_t keys);
+int paged_few(const PagedArgs &a, int type, int rows_most);
+int paged_tiles(const PagedArgs &a, int type, int rows_least);
 
 // What the cache holds, per type: bits of a number, and what the matrix core gets.  A row's numbers go in as f16 exactly, n or (MX4) n 2^12 under the largest scale of its groups; its
 // factor brings them back.  Numbers reach 2^TOP; where they are summed over (P V) their factors carry 2^BIAS beyond, and are infinite for values of 2^78 and more (VALUES_UP, f16x2.h).
@@ -84,6 +84,14 @@ __device__ __forceinline__ PagedTiles paged_tiles_of(const PagedArgs &a, int beg
     t.ahead = a.window > 0 ? min((int)(((int64_t)a.sinks + step) >> shift), t.from) : 0;
     t.all = t.ahead + last - t.from;
     return t;
+}
+
+// The most steps of 2^shift keys that rows of one sequence see together (above: from begin = p + 1 - window to the end of a row at most Sq - 1 further)
+inline int64_t paged_steps_most(const PagedArgs &a, int shift) {
+    const int64_t step = int64_t(1) << shift, all = (a.pages.room + step - 1) / step;
+    if (a.window == 0) return all;
+    const int64_t most = (a.window + (int64_t)a.pages.Sq - 1 + 2 * (step - 1)) / step + ((int64_t)a.sinks + step - 1) / step;
+    return most < all ? most : all;
 }
 
 // ---- one row by one wave with fp32 instructions: what the matrix kernels fall back to where sums are not finite.  64 keys at a time, a score a lane; then a value column a lane (two

@@ -51,14 +51,11 @@ extern "C" int axhip_attn_paged(const float *Q, int64_t ldq, const axhip_kv_cach
     a.window = r.window < PAST ? r.window : PAST;
     a.sinks = r.window == 0 ? 0 : r.sinks < PAST ? r.sinks : PAST;
     if (a.pages.room > Sk) a.pages.room = (int)Sk;
-    // the most keys that rows of one sequence see together
-    int64_t keys = a.pages.room;
-    if (a.window > 0 && keys > (int64_t)a.window + a.sinks + Sq) keys = (int64_t)a.window + a.sinks + Sq;
     // A sequence with few rows is read by the form that shares out its keys, others by tiles.  How many rows each sequence has is on the device, so both may have to be launched, each
     // for its own; not where all have the same number of rows, or none can have more than a few.
     const int64_t rows = (int64_t)t.G * Sq;
-    if (rows <= FEW_ROWS) return paged_few(a, cache->type, FEW_ROWS, keys);
-    if (!first || B == 1) return paged_tiles(a, cache->type, 0, keys);
-    if (int rc = paged_few(a, cache->type, FEW_ROWS, keys)) return rc;
-    return paged_tiles(a, cache->type, FEW_ROWS + 1, keys);
+    if (rows <= FEW_ROWS) return paged_few(a, cache->type, FEW_ROWS);
+    if (!first || B == 1) return paged_tiles(a, cache->type, 0);
+    if (int rc = paged_few(a, cache->type, FEW_ROWS)) return rc;
+    return paged_tiles(a, cache->type, FEW_ROWS + 1);
 }

@@ -14,9 +14,9 @@
 namespace {
 using namespace axhip;
 
-constexpr int WAVES = 4, SPLITS_MOST = 64, ROWS = 16;
+constexpr int SPLITS_MOST = 64, ROWS = 16;
 
-template <int DK>
+template <int DK, int WAVES>
 struct FewGeom {
     using B = Block<DK, 32>;
     static constexpr int PIECES = DK / 16;                       // a lane's output in pieces of four
@@ -25,7 +25,7 @@ struct FewGeom {
     static constexpr int BLOCKS = WAVES * BLOCK, JOINED = ML_AT + WAVES * 128, RANGES = SPLITS_MOST * ROWS * 8;
     static constexpr int MOST = BLOCKS > JOINED ? BLOCKS : JOINED, FLAGS_AT = MOST > RANGES ? MOST : RANGES;   // a word a wave: the rows whose sums are not finite; then who is last
     static constexpr int SMEM = FLAGS_AT + 4 * WAVES + 16;
-    static_assert(BLOCK % 256 == 0 && SMEM <= 64 * 1024, "LDS");
+    static_assert(BLOCK % 256 == 0 && SMEM <= 80 * 1024, "LDS");
     static constexpr int PART = PIECES * 256 + 2 * ROWS;         // floats that a range leaves in memory
 };
 
@@ -35,7 +35,7 @@ struct Quarter {
     static constexpr int WIDE = WORDS % 4 == 0 ? 4 : WORDS % 2 == 0 ? 2 : 1;
     unsigned w[WORDS];
     template <bool PAD>
-    __device__ __forceinline__ void load(const unsigned char *row, int part, int row_bytes) {
+    __device__ __forceinline__ void load(const unsigned char *quarter, int part, int row_bytes) {
 #pragma unroll
         for (int i = 0; i < WORDS; i += WIDE) {
             typedef unsigned wide __attribute__((ext_vector_type(WIDE)));
@@ -44,9 +44,9 @@ struct Quarter {
 #pragma unroll
                 for (int e = 0; e < WIDE; e++) w[i + e] = 0;
             } else if constexpr (WIDE == 1) {
-                w[i] = *reinterpret_cast<const unsigned *>(row + at);
+                w[i] = *reinterpret_cast<const unsigned *>(quarter + 4 * i);
             } else {
-                const wide v = *reinterpret_cast<const wide *>(row + at);
+                const wide v = *reinterpret_cast<const wide *>(quarter + 4 * i);
 #pragma unroll
                 for (int e = 0; e < WIDE; e++) w[i + e] = v[e];
             }
@@ -76,9 +76,9 @@ __device__ __forceinline__ v4i eight_halves(const Quarter<WORDS> &x, int s, int 
     if constexpr (TYPE == AXHIP_KV_MX4) return kv_nibbles(x.w[s], mx4_up(scales, top, (part * (DK / 4) + 8 * s) / 32));
 }
 
-template <int DK, int TYPE, bool PAD>
+template <int DK, int TYPE, bool PAD, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedFewGrid grid) {
-    using G = FewGeom<DK>;
+    using G = FewGeom<DK, WAVES>;
     using B = typename G::B;
     using T = KvType<TYPE>;
     constexpr int KS = DK / 32, PIECES = G::PIECES, MINE = (PIECES + WAVES - 1) / WAVES, WORDS = DK * T::BITS / 128;
@@ -87,10 +87,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
     const AttnArgs &at = a.attn;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 15, part = lane >> 4;
     // ranges of one set of rows follow each other, so that they go to different XCDs
-    const int64_t lin = grid.first + blockIdx.x, unit = lin / grid.splits;
-    const int split = (int)(lin - unit * grid.splits);
-    const int64_t bh = unit / grid.row_tiles;
-    const int rt = (int)(unit - bh * grid.row_tiles), b = (int)(bh / kv.heads), hk = (int)(bh - (int64_t)b * kv.heads);
+    const unsigned local = blockIdx.x / (unsigned)grid.splits, split = blockIdx.x - local * (unsigned)grid.splits, bh = local / (unsigned)grid.row_tiles, of_b = bh / (unsigned)kv.heads;
+    const int rt = (int)(local - bh * grid.row_tiles), b = grid.first + (int)of_b, hk = (int)(bh - of_b * kv.heads);
+    const int64_t unit = (int64_t)grid.first * kv.heads * grid.row_tiles + local;
     const KvSeq seq = kv_seq(kv, b);
     const int64_t rows = (int64_t)at.G * seq.n;
     if ((int64_t)rt * ROWS >= rows || rows > grid.most) return;
@@ -103,40 +102,51 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
     // what the rows see together: they go up with their positions
     const PagedRow low = paged_row(a, seq, rt * ROWS / at.G), high = paged_row(a, seq, (int)(min((int64_t)rt * ROWS + ROWS, rows) - 1) / at.G);
     const PagedTiles tiles = paged_tiles_of(a, low.begin, high.end, 5);
-    const int t_begin = (int)((int64_t)tiles.all * split / grid.splits), t_end = (int)((int64_t)tiles.all * (split + 1) / grid.splits);
+    const int t_begin = (int)((unsigned)tiles.all * split / (unsigned)grid.splits), t_end = (int)((unsigned)tiles.all * (split + 1) / (unsigned)grid.splits);
     const float slope2 = at.slopes ? at.slopes[head] * at.bias2 : 0.0f;
 
     unsigned char *const mine = lds + wave * G::BLOCK;
     float *const factors = reinterpret_cast<float *>(mine + G::FACTORS_AT);
     const unsigned base = lds_address(mine);
 
-    // keys frow and 16 + frow of a tile
+    // keys frow and 16 + frow of a tile, and the entries of the table for those of the next
     Quarter<WORDS> kq[2], vq[2];
     unsigned ks[2], vs[2];
     int entry[2];
     bool here[2];
+    const int32_t *const entries = kv.table + (int64_t)b * kv.table_ld;
+    // where this lane's quarter of row zero of a page zero is, and the scale of that row
+    const unsigned char *const k0 = kv.k + kv_row_at(kv, 0, hk, 0) + part * WORDS * 4;
+    const unsigned char *const s0 = kv.k_scale + kv_scale_at(kv, 0, hk, 0);
+    const int64_t to_v = kv.v - kv.k, to_v_scale = kv.v_scale - kv.k_scale;
     auto pos_of = [&](int n, int t) { return tiles.tile(n) * 32 + 16 * t + frow; };
     auto look = [&](int n) {
 #pragma unroll
-        for (int t = 0; t < 2; t++) entry[t] = kv_entry(kv, b, min(pos_of(n, t), high.end - 1));
+        for (int t = 0; t < 2; t++) entry[t] = entries[(unsigned)min(pos_of(n, t), high.end - 1) >> kv.shift];
     };
     auto fetch = [&](int n) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const int pos = pos_of(n, t);
             here[t] = pos < high.end && kv_is_page(kv, entry[t]);
-            kq[t].clear();
-            vq[t].clear();
             ks[t] = vs[t] = 0;
             if (here[t]) {
-                const uint64_t at_row = kv_row_at(kv, entry[t], hk, pos), at_scale = kv_scale_at(kv, entry[t], hk, pos);
-                kq[t].template load<PAD>(kv.k + at_row, part, kv.row_bytes);
-                vq[t].template load<PAD>(kv.v + at_row, part, kv.row_bytes);
-                ks[t] = *reinterpret_cast<const unsigned *>(kv.k_scale + at_scale);
-                vs[t] = *reinterpret_cast<const unsigned *>(kv.v_scale + at_scale);
+                const unsigned in_page = (unsigned)pos & ((1u << kv.shift) - 1);
+                const unsigned char *const row = k0 + ((uint64_t)(unsigned)entry[t] * kv.page_bytes + __umul24(in_page, (unsigned)kv.row_bytes));
+                const unsigned char *const scale = s0 + ((uint64_t)(unsigned)entry[t] * kv.page_scales + 4 * in_page);
+                ks[t] = *reinterpret_cast<const unsigned *>(scale);
+                vs[t] = *reinterpret_cast<const unsigned *>(scale + to_v_scale);
+                kq[t].template load<PAD>(row, part, kv.row_bytes);
+                vq[t].template load<PAD>(row + to_v, part, kv.row_bytes);
             }
         }
     };
+    // (where there is no page the numbers of an earlier tile stay, which are finite, under a factor of zero)
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        kq[t].clear();
+        vq[t].clear();
+    }
     int n = t_begin + wave;
     if (n < t_end) {
         look(n);
@@ -164,6 +174,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
     for (int d = 0; d < PIECES; d++) acc[d] = v4f{0.f, 0.f, 0.f, 0.f};
     float ref = ATTN_LOWEST, l_run = 0.0f;           // acc is 2^VALUE_BIAS times the sum
     const float one = hidden_one();
+    const bool plain = at.cap == 0.0f && !at.slopes;
+    const float down = plain ? q_down : 1.0f;        // what is left to the score in the exponential's multiply-add
     const unsigned column_at = B::column_place16(lane) + base;
 
     for (; n < t_end; n += WAVES) {
@@ -205,9 +217,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
         for (int t = 0; t < 2; t++) {
             const v4f kf = *reinterpret_cast<const v4f *>(factors + 16 * t + 4 * part);
             vf[t] = *reinterpret_cast<const v4f *>(factors + 32 + 16 * t + 4 * part);
-            s[t] = s[t] * kf * q_down;
+            s[t] *= kf;
+            if (!plain) s[t] *= q_down;
         }
-        if (at.cap > 0.0f) {
+        if (__builtin_expect(at.cap > 0.0f, 0)) {
             float big = 0.0f;
 #pragma unroll
             for (int v = 0; v < 8; v++) big = fmaxf(big, __builtin_fabsf(s[v >> 2][v & 3]));
@@ -218,14 +231,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
 #pragma unroll
                 for (int v = 0; v < 8; v++) s[v >> 2][v & 3] = capped_near(at, s[v >> 2][v & 3]).score;
         }
-        if (at.slopes) {
+        if (__builtin_expect(at.slopes != nullptr, 0)) {
             const float from = (float)(row.p - kt0 - 4 * part);
 #pragma unroll
             for (int v = 0; v < 8; v++) s[v >> 2][v & 3] = __builtin_fmaf(-slope2, from - (float)(16 * (v >> 2) + (v & 3)), s[v >> 2][v & 3]);
         }
         // (all rows see a tile before the first one's end and, where it is none of the first tokens only, behind the last one's beginning; rows that see nothing are not written)
         const bool partly = gone != 0 || kt0 + 32 > low.end || (kt0 < high.begin && kt0 + 32 > a.sinks);
-        if (partly) {
+        if (__builtin_expect(partly, 0)) {
             const int end = row.end - kt0 - 4 * part, begin = row.begin - kt0 - 4 * part, first = a.sinks - kt0 - 4 * part;
             const unsigned none = gone >> (4 * part);
 #pragma unroll
@@ -239,18 +252,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
             most = l_blk = 0.0f;
 #pragma unroll
             for (int v = 0; v < 8; v++) {
-                const float p = __builtin_amdgcn_exp2f(s[v >> 2][v & 3] - ref);
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v >> 2][v & 3], down, -ref));
                 l_blk += p;
                 x[v] = p * vf[v >> 2][v & 3];
                 most = fmaxf(most, x[v]);
             }
         };
         weigh();
-        if (__builtin_amdgcn_ballot_w64(most > ROOM)) {          // (always for the first finite scores)
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > ROOM) != 0, 0)) {          // (always for the first finite scores)
             most = most_of_parts(most);
             float top = -INFINITY;
 #pragma unroll
-            for (int v = 0; v < 8; v++) top = fmaxf(top, s[v >> 2][v & 3] + __builtin_amdgcn_logf(vf[v >> 2][v & 3]));
+            for (int v = 0; v < 8; v++) top = fmaxf(top, __builtin_fmaf(s[v >> 2][v & 3], down, __builtin_amdgcn_logf(vf[v >> 2][v & 3])));
             top = most_of_parts(top) - (float)LARGEST;
             const float next = most > ROOM ? fmaxf(ref, top) : ref, alpha = __builtin_amdgcn_exp2f(ref - next);
             l_run = scaled(l_run, ref - next);
@@ -262,11 +275,17 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
         l_run += l_blk;
         v4i pf[2];
         cut_scaled(x, one, pf);
+        // (columns are read two pieces ahead)
+        v4i f[3];
+        f[0] = B::columns16(column_at, 0, 0);
+        if (PIECES > 1) f[1] = B::columns16(column_at, 1, 0);
+        __builtin_amdgcn_sched_barrier(0x6);
 #pragma unroll
         for (int d = 0; d < PIECES; d++) {
-            const v8h f = __builtin_bit_cast(v8h, B::columns16(column_at, d, 0));
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, __builtin_bit_cast(v8h, pf[1]), acc[d], 0, 0, 0);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, __builtin_bit_cast(v8h, pf[0]), acc[d], 0, 0, 0);
+            if (d + 2 < PIECES) f[(d + 2) % 3] = B::columns16(column_at, d + 2, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, f[d % 3]), __builtin_bit_cast(v8h, pf[1]), acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, f[d % 3]), __builtin_bit_cast(v8h, pf[0]), acc[d], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0x6);
         }
     }
 
@@ -322,28 +341,17 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
         auto read = [&](int64_t from) {
             return __builtin_bit_cast(v2f, __hip_atomic_load(reinterpret_cast<const int64_t *>(theirs + from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
         };
-        // Every read is a trip to memory, so they go out together: maxima and sums by 16 groups of 16 lanes, then AHEAD ranges' outputs at a time.
+        // Every read is a trip to memory, so they go out together: maxima and sums by groups of 16 lanes, and AHEAD ranges' outputs at a time.
+        constexpr int AHEAD = 8, GROUPS = 4 * WAVES, EACH = SPLITS_MOST / GROUPS;
         v2f *const both = reinterpret_cast<v2f *>(lds + G::JOIN_AT) + frow;
-        v2f here[4];
+        v2f here[EACH];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int from = (int)(threadIdx.x >> 4) + 16 * k;
+        for (int k = 0; k < EACH; k++) {
+            const int from = (int)(threadIdx.x >> 4) + GROUPS * k;
             if (from < grid.splits) here[k] = read((int64_t)from * G::PART + PIECES * 256 + 2 * frow);
         }
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int from = (int)(threadIdx.x >> 4) + 16 * k;
-            if (from < grid.splits) both[ROWS * from] = here[k];
-        }
-        __syncthreads();
-        m_all = ATTN_LOWEST;
-        for (int from = 0; from < grid.splits; from++) m_all = fmaxf(m_all, both[ROWS * from][0]);
-        l_all = 0.0f;
-#pragma unroll
-        for (int d = 0; d < MINE; d++) out[d] = v4f{0.f, 0.f, 0.f, 0.f};
-        constexpr int AHEAD = 8;
-        for (int s0 = 0; s0 < grid.splits; s0 += AHEAD) {
-            v4f x[AHEAD][MINE];
+        v4f x[AHEAD][MINE];
+        auto outputs = [&](int s0) {
 #pragma unroll
             for (int k = 0; k < AHEAD; k++) {
                 if (s0 + k >= grid.splits) break;
@@ -355,6 +363,21 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
                     x[k][d] = v4f{p[0], p[1], q[0], q[1]};
                 }
             }
+        };
+        outputs(0);
+#pragma unroll
+        for (int k = 0; k < EACH; k++) {
+            const int from = (int)(threadIdx.x >> 4) + GROUPS * k;
+            if (from < grid.splits) both[ROWS * from] = here[k];
+        }
+        __syncthreads();
+        m_all = ATTN_LOWEST;
+        for (int from = 0; from < grid.splits; from++) m_all = fmaxf(m_all, both[ROWS * from][0]);
+        l_all = 0.0f;
+#pragma unroll
+        for (int d = 0; d < MINE; d++) out[d] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < grid.splits; s0 += AHEAD) {
+            if (s0 > 0) outputs(s0);
 #pragma unroll
             for (int k = 0; k < AHEAD; k++) {
                 if (s0 + k >= grid.splits) break;
@@ -400,52 +423,63 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
     }
 }
 
-template <int DK, int TYPE, bool PAD>
-int launch_few(const PagedArgs &a, PagedFewGrid grid, int64_t units) {
-    using G = FewGeom<DK>;
+template <int DK, int TYPE, bool PAD, int WAVES>
+int launch_few(const PagedArgs &a, PagedFewGrid grid) {
+    using G = FewGeom<DK, WAVES>;
+    static bool attr_set = false;
+    if (!attr_set) {
+        AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_paged_few<DK, TYPE, PAD, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
+        attr_set = true;
+    }
+    const int64_t of_b = (int64_t)a.pages.heads * grid.row_tiles, units = a.pages.B * of_b;
     if (grid.splits > 1) {
         grid.parts = static_cast<float *>(workspace((size_t)units * grid.splits * G::PART * sizeof(float)));
         grid.arrivals = strip_counters((size_t)units);
         if (!grid.parts || !grid.arrivals) return AXHIP_ERR_ALLOC;
     }
     note_kernel(grid.splits > 1 ? "paged_few_ranges" : "paged_few");
-    const int64_t all = units * grid.splits;
-    for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
-        const int64_t left = all - grid.first;
-        hipLaunchKernelGGL((k_paged_few<DK, TYPE, PAD>), dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
+    const int64_t at_once = GRID_MOST / (of_b * grid.splits);    // sequences a launch; (a sequence has at most 2^21 units, and ranges only where there are few)
+    for (grid.first = 0; grid.first < a.pages.B; grid.first += (int)at_once) {
+        const int64_t left = a.pages.B - grid.first, here = left < at_once ? left : at_once;
+        hipLaunchKernelGGL((k_paged_few<DK, TYPE, PAD, WAVES>), dim3((unsigned)(here * of_b * grid.splits)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
         if (int rc = check_launch("attn_paged")) return rc;
     }
     return AXHIP_OK;
 }
 
-template <int DK, int TYPE>
-int launch_few(const PagedArgs &a, const PagedFewGrid &grid, int64_t units) {
-    return a.pages.dk < DK ? launch_few<DK, TYPE, true>(a, grid, units) : launch_few<DK, TYPE, false>(a, grid, units);
+template <int DK, int TYPE, int WAVES>
+int launch_few(const PagedArgs &a, const PagedFewGrid &grid) {
+    return a.pages.dk < DK ? launch_few<DK, TYPE, true, WAVES>(a, grid) : launch_few<DK, TYPE, false, WAVES>(a, grid);
 }
-template <int DK>
-int launch_few(const PagedArgs &a, int type, const PagedFewGrid &grid, int64_t units) {
-    return type == AXHIP_KV_F16 ? launch_few<DK, AXHIP_KV_F16>(a, grid, units) : type == AXHIP_KV_I8 ? launch_few<DK, AXHIP_KV_I8>(a, grid, units) : launch_few<DK, AXHIP_KV_MX4>(a, grid, units);
+template <int DK, int WAVES>
+int launch_few(const PagedArgs &a, int type, const PagedFewGrid &grid) {
+    return type == AXHIP_KV_F16 ? launch_few<DK, AXHIP_KV_F16, WAVES>(a, grid) : type == AXHIP_KV_I8 ? launch_few<DK, AXHIP_KV_I8, WAVES>(a, grid) : launch_few<DK, AXHIP_KV_MX4, WAVES>(a, grid);
 }
 
 }  // namespace
 
 namespace axhip {
 
-int paged_few(const PagedArgs &a, int type, int rows_most, int64_t keys) {
+int paged_few(const PagedArgs &a, int type, int rows_most) {
     PagedFewGrid grid = {};
     grid.most = rows_most;
     const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, most = rows < rows_most ? rows : rows_most;
     grid.row_tiles = (int)((most + ROWS - 1) / ROWS);
-    const int64_t units = (int64_t)a.pages.B * a.pages.heads * grid.row_tiles, tiles = (keys + 31) / 32, cus = cu_count();
-    int64_t splits = (2 * cus + units - 1) / units;
-    if (splits > (tiles + WAVES - 1) / WAVES) splits = (tiles + WAVES - 1) / WAVES;
+    const int64_t units = (int64_t)a.pages.B * a.pages.heads * grid.row_tiles, tiles = paged_steps_most(a, 5), cus = cu_count();
+    const int waves = tiles > 4 ? 8 : 4;
+    int64_t splits = cus / units;
+    if (splits > (tiles + 2 * waves - 1) / (2 * waves)) splits = (tiles + 2 * waves - 1) / (2 * waves);
     if (splits > SPLITS_MOST) splits = SPLITS_MOST;
     if (splits < 1) splits = 1;
     grid.splits = (int)splits;
-    if (a.pages.dk <= 32) return launch_few<32>(a, type, grid, units);
-    if (a.pages.dk <= 64) return launch_few<64>(a, type, grid, units);
-    if (a.pages.dk <= 96) return launch_few<96>(a, type, grid, units);
-    return launch_few<128>(a, type, grid, units);
+    auto run = [&](auto width) {
+        constexpr int DK = decltype(width)::value;
+        return waves == 8 ? launch_few<DK, 8>(a, type, grid) : launch_few<DK, 4>(a, type, grid);
+    };
+    if (a.pages.dk <= 32) return run(std::integral_constant<int, 32>());
+    if (a.pages.dk <= 64) return run(std::integral_constant<int, 64>());
+    if (a.pages.dk <= 96) return run(std::integral_constant<int, 96>());
+    return run(std::integral_constant<int, 128>());
 }
 
 }  // namespace axhip

@@ -7,6 +7,8 @@
 // What rows see goes up with their positions: blocks before the window of a workgroup's first row, but for the first tokens that stay visible, and behind its last row's position are not
 // fetched, 32-key tiles that no row of a wave sees not computed, and only tiles that some row sees in part pay for the mask.
 // Where tiles would leave CUs idle, ranges of their keys go to workgroups of their own, and a second launch adds what they leave, in order.
+#include <algorithm>
+
 #include "attn_launch.h"
 #include "attn_tiles.h"
 #include "paged.h"
@@ -29,29 +31,35 @@ struct TileGeom {
     static constexpr int PART = SETS * (PIECES * 256 + 64);      // floats that a range leaves in memory: of each 32 rows the pieces, then maxima and sums
 };
 
-// Where a workgroup's rows are
+// Where a workgroup's rows are: `rows` of them (0: none of this form's), the first of which is the row of token i0 of sequence b and of head g0 of those that share keys
 struct Place {
-    int b;
-    int64_t tile, rows;                          // rows: of the sequence, for all heads that share keys; 0: none of this form's
+    int b, rows, i0;
+    unsigned g0;
 };
 template <int BQ>
 __device__ __forceinline__ Place place_of(const PagedArgs &a, const PagedTileGrid &grid, int64_t slot, int lane, KvSeq &seq) {
     const KvPages &kv = a.pages;
     const int64_t G = a.attn.G;
-    Place p = {0, 0, 0};
+    Place p = {0, 0, 0, 0};
+    int64_t tile;
     if (kv.first) {
         // sequence b's slots are those from first[b] G / BQ + b on
         p.b = kv_find(kv, lane, [&](int k, int first) { return first * G / BQ + k <= slot; });
         if (p.b >= kv.B) return p;
-        p.tile = slot - (min(max(kv.first[p.b], 0), kv.T) * G / BQ + p.b);
+        tile = slot - (min(max(kv.first[p.b], 0), kv.T) * G / BQ + p.b);
+    } else if (grid.slots >> 32 == 0) {
+        p.b = (int)((unsigned)slot / (unsigned)grid.per);
+        tile = (unsigned)slot - (unsigned)p.b * (unsigned)grid.per;
     } else {
-        const int64_t per = (kv.Sq * G + BQ - 1) / BQ;
-        p.b = (int)(slot / per);
-        p.tile = slot - p.b * per;
+        p.b = (int)(slot / grid.per);
+        tile = slot - p.b * grid.per;
     }
     seq = kv_seq(kv, p.b);
-    const int64_t rows = G * seq.n;
-    if (rows >= grid.least && p.tile >= 0 && p.tile * BQ < rows) p.rows = rows;
+    const int64_t rows = G * seq.n, r0 = tile * BQ;
+    if (rows < grid.least || tile < 0 || r0 >= rows) return p;
+    p.rows = (int)min(rows - r0, (int64_t)BQ);
+    p.i0 = r0 >> 32 == 0 ? (int)((unsigned)r0 / (unsigned)a.attn.G) : (int)(r0 / G);
+    p.g0 = (unsigned)(r0 - p.i0 * G);
     return p;
 }
 
@@ -68,27 +76,29 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
 
     // a sequence's last tiles, the longest, first; heads of keys go to the XCDs in turn
-    const int64_t lin = grid.first + blockIdx.x, rest = lin / kv.heads, slot = grid.slots - 1 - rest / grid.splits;
-    const int hk = (int)(lin - rest * kv.heads), split = (int)(rest % grid.splits);
+    const unsigned rest = blockIdx.x / (unsigned)kv.heads, of_slot = rest / (unsigned)grid.splits, split = rest - of_slot * (unsigned)grid.splits;
+    const int64_t slot = grid.slots - 1 - (grid.first + of_slot);
+    const int hk = (int)(blockIdx.x - rest * (unsigned)kv.heads);
     KvSeq seq = {0, 0, 0};
     const Place place = place_of<BQ>(a, grid, slot, lane, seq);
     if (place.rows == 0) return;
     const int b = place.b;
-    const int64_t r0 = place.tile * BQ;
-    const int rows_here = (int)min(place.rows - r0, (int64_t)BQ), mine = wave % SETS * 32 + frow;
+    const int rows_here = place.rows, mine = wave % SETS * 32 + frow;
     const bool valid = mine < rows_here;
-    const int64_t r = r0 + (valid ? mine : rows_here - 1);
-    const int i = (int)(r / at.G), head = hk * at.G + (int)(r - (int64_t)i * at.G);
+    // (the tile's first row is one of token i0, its group's head number g0)
+    const unsigned G0 = (unsigned)at.G, r = place.g0 + (unsigned)(valid ? mine : rows_here - 1), over = r / G0;
+    const int i = place.i0 + (int)over, head = hk * at.G + (int)(r - over * G0);
+    auto token = [&](int of) { return place.i0 + (int)((place.g0 + (unsigned)of) / G0); };
     PagedRow row = paged_row(a, seq, i);
     if (!valid) row.end = 0;
     const bool live = row.end > 0;
     // what the workgroup's rows see together, and the wave's
-    const PagedRow wg_low = paged_row(a, seq, (int)(r0 / at.G)), wg_high = paged_row(a, seq, (int)((r0 + rows_here - 1) / at.G));
+    const PagedRow wg_low = paged_row(a, seq, place.i0), wg_high = paged_row(a, seq, token(rows_here - 1));
     const int w0 = min(wave % SETS * 32, rows_here - 1), w1 = min(wave % SETS * 32 + 31, rows_here - 1);
-    const PagedRow low = paged_row(a, seq, (int)((r0 + w0) / at.G)), high = paged_row(a, seq, (int)((r0 + w1) / at.G));
+    const PagedRow low = paged_row(a, seq, token(w0)), high = paged_row(a, seq, token(w1));
     const int last = wave % SETS * 32 < rows_here ? high.end : 0;
     const PagedTiles blocks = paged_tiles_of(a, wg_low.begin, wg_high.end, G::SHIFT);
-    const int n_begin = (int)((int64_t)blocks.all * split / grid.splits), n_end = (int)((int64_t)blocks.all * (split + 1) / grid.splits);
+    const int n_begin = (int)((unsigned)blocks.all * split / (unsigned)grid.splits), n_end = (int)((unsigned)blocks.all * (split + 1) / (unsigned)grid.splits);
     const float slope2 = at.slopes ? at.slopes[head] * at.bias2 : 0.0f;
 
     const unsigned base = lds_address(lds);
@@ -98,11 +108,15 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
     unsigned scales[PASSES];
     int entry[PLACES];
     unsigned gone = 0;                               // a bit a place: its key has no page
+    const int32_t *const entries = kv.table + (int64_t)b * kv.table_ld;
+    // where this lane's bytes of row zero of a page zero are, and the scale of that row
+    const unsigned char *const k0 = kv.k + kv_row_at(kv, 0, hk, 0) + 16 * ((int)threadIdx.x % LANES), *const s0 = kv.k_scale + kv_scale_at(kv, 0, hk, 0);
+    const int64_t to_v = kv.v - kv.k, to_v_scale = kv.v_scale - kv.k_scale;
     auto row_of = [&](int pass) { return (pass * 64 * WAVES + (int)threadIdx.x) / LANES; };      // from BKV on a value's; from 2 BKV on none
     auto pos_of = [&](int n, int place) { return blocks.tile(n) * BKV + row_of(place) % BKV; };
     auto look = [&](int n) {
 #pragma unroll
-        for (int p = 0; p < PLACES; p++) entry[p] = kv_entry(kv, b, min(pos_of(n, p), wg_high.end - 1));
+        for (int p = 0; p < PLACES; p++) entry[p] = entries[(unsigned)min(pos_of(n, p), wg_high.end - 1) >> kv.shift];
     };
     auto fetch = [&](int n) {
         const int c = (int)threadIdx.x % LANES;
@@ -116,19 +130,21 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
         for (int p = 0; p < PLACES; p++) {
             const int pos = pos_of(n, p);
             if (pos < wg_high.end && kv_is_page(kv, entry[p]) && (2 * BKV * LANES >= 64 * WAVES || row_of(p) < 2 * BKV)) {
-                const uint64_t at_row = kv_row_at(kv, entry[p], hk, pos) + 16 * c, at_scale = kv_scale_at(kv, entry[p], hk, pos);
+                const unsigned in_page = (unsigned)pos & ((1u << kv.shift) - 1);
+                const unsigned char *const k = k0 + ((uint64_t)(unsigned)entry[p] * kv.page_bytes + __umul24(in_page, (unsigned)kv.row_bytes));
+                const unsigned char *const k_scale = s0 + ((uint64_t)(unsigned)entry[p] * kv.page_scales + 4 * in_page);
                 const bool some = (!PAD && DK != 96) || 16 * c < kv.row_bytes;
                 if (PASSES > 1) {
                     if (some) {
-                        x[p] = *reinterpret_cast<const v4i *>(kv.k + at_row);
-                        x[(p + PLACES) % PASSES] = *reinterpret_cast<const v4i *>(kv.v + at_row);
+                        x[p] = *reinterpret_cast<const v4i *>(k);
+                        x[(p + PLACES) % PASSES] = *reinterpret_cast<const v4i *>(k + to_v);
                     }
-                    scales[p] = *reinterpret_cast<const unsigned *>(kv.k_scale + at_scale);
-                    scales[(p + PLACES) % PASSES] = *reinterpret_cast<const unsigned *>(kv.v_scale + at_scale);
+                    scales[p] = *reinterpret_cast<const unsigned *>(k_scale);
+                    scales[(p + PLACES) % PASSES] = *reinterpret_cast<const unsigned *>(k_scale + to_v_scale);
                 } else {
                     const bool of_v = row_of(p) >= BKV;
-                    if (some) x[p] = *reinterpret_cast<const v4i *>((of_v ? kv.v : kv.k) + at_row);
-                    scales[p] = *reinterpret_cast<const unsigned *>((of_v ? kv.v_scale : kv.k_scale) + at_scale);
+                    if (some) x[p] = *reinterpret_cast<const v4i *>(of_v ? k + to_v : k);
+                    scales[p] = *reinterpret_cast<const unsigned *>(of_v ? k_scale + to_v_scale : k_scale);
                 }
             } else {
                 gone |= 1u << p;
@@ -240,10 +256,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
             // what is left to the score: q_down, here where more is done to it, in the exponential's multiply-add otherwise
             const bool plain = at.cap == 0.0f && !at.slopes;
             const float down = plain ? q_down : 1.0f;
-            if (!plain)
+            if (__builtin_expect(!plain, 0))
 #pragma unroll
                 for (int v = 0; v < 16; v++) s[v] *= q_down;
-            if (at.cap > 0.0f) {
+            if (__builtin_expect(at.cap > 0.0f, 0)) {
                 float big = 0.0f;
 #pragma unroll
                 for (int v = 0; v < 16; v++) big = fmaxf(big, __builtin_fabsf(s[v]));
@@ -254,12 +270,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
 #pragma unroll
                     for (int v = 0; v < 16; v++) s[v] = capped_near(at, s[v]).score;
             }
-            if (at.slopes) {
+            if (__builtin_expect(at.slopes != nullptr, 0)) {
                 const float from = (float)(row.p - kt0 - 4 * fhalf);
 #pragma unroll
                 for (int v = 0; v < 16; v++) s[v] = __builtin_fmaf(-slope2, from - (float)(8 * (v >> 2) + (v & 3)), s[v]);
             }
-            if (partly) {
+            if (__builtin_expect(partly, 0)) {
                 const int end = row.end - kt0 - 4 * fhalf, begin = row.begin - kt0 - 4 * fhalf, first = a.sinks - kt0 - 4 * fhalf;
 #pragma unroll
                 for (int v = 0; v < 16; v++) {
@@ -285,7 +301,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
                 }
             };
             weigh();
-            if (__builtin_amdgcn_ballot_w64(most > ROOM)) {      // (always for the first finite scores)
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > ROOM) != 0, 0)) {      // (always for the first finite scores)
                 most = fmaxf(most, __shfl_xor(most, 32, 64));
                 float top = -INFINITY;
 #pragma unroll
@@ -414,16 +430,16 @@ __global__ void __launch_bounds__(2 * DK) k_paged_join(PagedArgs a, PagedTileGri
     const KvPages &kv = a.pages;
     const AttnArgs &at = a.attn;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
-    const int64_t lin = grid.first + blockIdx.x, unit = lin / SETS, slot = unit / kv.heads;
-    const int set = (int)(lin - unit * SETS), hk = (int)(unit - slot * kv.heads);
+    const unsigned of_set = blockIdx.x / SETS, set = blockIdx.x % SETS, of_slot = of_set / (unsigned)kv.heads;
+    const int hk = (int)(of_set - of_slot * (unsigned)kv.heads);
+    const int64_t slot = grid.first + of_slot, unit = slot * kv.heads + hk;
     KvSeq seq = {0, 0, 0};
     const Place place = place_of<BQ>(a, grid, slot, lane, seq);
-    const int64_t r0 = place.tile * BQ + 32 * set;
-    if (place.rows == 0 || r0 >= place.rows) return;
-    const int rows_here = (int)min(place.rows - r0, (int64_t)32);
+    const int rows_here = place.rows - 32 * (int)set;
+    if (rows_here <= 0) return;
     const bool valid = frow < rows_here;
-    const int64_t r = r0 + (valid ? frow : rows_here - 1);
-    const int i = (int)(r / at.G), head = hk * at.G + (int)(r - (int64_t)i * at.G);
+    const unsigned r = place.g0 + 32 * set + (unsigned)(valid ? frow : rows_here - 1), over = r / (unsigned)at.G;
+    const int i = place.i0 + (int)over, head = hk * at.G + (int)(r - over * (unsigned)at.G);
     const bool live = valid && paged_row(a, seq, i).end > 0;
     const float *parts = grid.parts + unit * grid.splits * G::PART + set * (G::PART / SETS);
     float m = ATTN_LOWEST, l = 0.0f;
@@ -477,32 +493,34 @@ int launch_tiles(const PagedArgs &a, PagedTileGrid grid) {
         AXHIP_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(k_paged_tiles<DK, SETS, TYPE, PAD>), hipFuncAttributeMaxDynamicSharedMemorySize, G::SMEM), "hipFuncSetAttribute");
         attr_set = true;
     }
-    const int64_t units = grid.slots * a.pages.heads, all = units * grid.splits;
     if (grid.splits > 1) {
-        grid.parts = static_cast<float *>(workspace((size_t)all * G::PART * sizeof(float)));
+        grid.parts = static_cast<float *>(workspace((size_t)grid.slots * a.pages.heads * grid.splits * G::PART * sizeof(float)));
         if (!grid.parts) return AXHIP_ERR_ALLOC;
     }
     note_kernel(grid.splits > 1 ? (SETS == 8 ? "paged_tiles_256_ranges" : "paged_tiles_128_ranges") : SETS == 8 ? "paged_tiles_256" : "paged_tiles_128");
-    for (grid.first = 0; grid.first < all; grid.first += GRID_MOST) {
-        const int64_t left = all - grid.first;
-        hipLaunchKernelGGL((k_paged_tiles<DK, SETS, TYPE, PAD>), dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
+    // as many slots a launch as it holds
+    const int64_t at_once = std::max<int64_t>(1, GRID_MOST / ((int64_t)a.pages.heads * grid.splits)), join_at_once = std::max<int64_t>(1, GRID_MOST / ((int64_t)a.pages.heads * SETS));
+    for (grid.first = 0; grid.first < grid.slots; grid.first += at_once) {
+        const int64_t here = std::min(grid.slots - grid.first, at_once);
+        hipLaunchKernelGGL((k_paged_tiles<DK, SETS, TYPE, PAD>), dim3((unsigned)(here * a.pages.heads * grid.splits)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
         if (int rc = check_launch("attn_paged")) return rc;
     }
-    if (grid.splits > 1)                             // (few tiles: a launch holds them)
-        for (grid.first = 0; grid.first < units * SETS; grid.first += GRID_MOST) {
-            const int64_t left = units * SETS - grid.first;
-            hipLaunchKernelGGL((k_paged_join<DK, SETS, TYPE>), dim3((unsigned)(left < GRID_MOST ? left : GRID_MOST)), dim3(2 * DK), 0, kStream, a, grid);
+    if (grid.splits > 1)
+        for (grid.first = 0; grid.first < grid.slots; grid.first += join_at_once) {
+            const int64_t here = std::min(grid.slots - grid.first, join_at_once);
+            hipLaunchKernelGGL((k_paged_join<DK, SETS, TYPE>), dim3((unsigned)(here * a.pages.heads * SETS)), dim3(2 * DK), 0, kStream, a, grid);
             if (int rc = check_launch("attn_paged")) return rc;
         }
     return AXHIP_OK;
 }
 
 template <int DK, int SETS>
-int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid, int64_t keys) {
+int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid) {
     using G = TileGeom<DK, SETS>;
     const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, all_rows = (int64_t)a.attn.G * a.pages.T, cus = cu_count();
-    grid.slots = a.pages.first ? all_rows / G::BQ + a.pages.B : a.pages.B * ((rows + G::BQ - 1) / G::BQ);
-    const int64_t likely = (a.pages.first ? all_rows / G::BQ + 1 : grid.slots) * a.pages.heads, blocks = (keys + G::BKV - 1) / G::BKV;
+    grid.per = (rows + G::BQ - 1) / G::BQ;
+    grid.slots = a.pages.first ? all_rows / G::BQ + a.pages.B : a.pages.B * grid.per;
+    const int64_t likely = (a.pages.first ? all_rows / G::BQ + 1 : grid.slots) * a.pages.heads, blocks = paged_steps_most(a, G::SHIFT);
     int64_t splits = cus / likely;
     if (splits > blocks / 4) splits = blocks / 4;
     if (splits > SPLITS_MOST) splits = SPLITS_MOST;
@@ -520,14 +538,14 @@ int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid, int64_t keys)
 
 namespace axhip {
 
-int paged_tiles(const PagedArgs &a, int type, int rows_least, int64_t keys) {
+int paged_tiles(const PagedArgs &a, int type, int rows_least) {
     PagedTileGrid grid = {};
     grid.least = rows_least;
     const int64_t wide_tiles = ((int64_t)a.attn.G * a.pages.T + 255) / 256 * a.pages.heads;
     const bool wide = wide_tiles >= cu_count();
     auto run = [&](auto width) {
         constexpr int DK = decltype(width)::value;
-        return wide ? launch_tiles<DK, 8>(a, type, grid, keys) : launch_tiles<DK, 4>(a, type, grid, keys);
+        return wide ? launch_tiles<DK, 8>(a, type, grid) : launch_tiles<DK, 4>(a, type, grid);
     };
     return a.pages.dk <= 32 ? run(std::integral_constant<int, 32>()) : a.pages.dk <= 64 ? run(std::integral_constant<int, 64>()) : a.pages.dk <= 96 ? run(std::integral_constant<int, 96>())
                                                                                                                                                 : run(std::integral_constant<int, 128>());
