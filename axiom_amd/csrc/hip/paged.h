@@ -22,7 +22,7 @@ struct PagedFewGrid {
 
 struct PagedTileGrid {
     int64_t first, slots, per;                   // the launch's first slot; slots: places for tiles, of which each sequence has as many as its rows could need (`per`, where they are equal)
-    int splits;                                  // ranges of keys
+    int splits, range;                           // the most ranges of keys that a tile has, one for every `range` blocks
     int least;                                   // sequences with fewer rows are the few-rows form's
     float *parts;
     int *arrivals;
@@ -97,7 +97,7 @@ inline int64_t paged_steps_most(const PagedArgs &a, int shift) {
 // ---- one row by one wave with fp32 instructions: what the matrix kernels fall back to where sums are not finite.  64 keys at a time, a score a lane; then a value column a lane (two
 // where dk > 64), and only keys that are seen are touched. ----
 template <int TYPE>
-__device__ __forceinline__ void paged_again(const PagedArgs &a, int b, const KvSeq &s, int head, int i, int lane) {
+__device__ __forceinline__ void paged_again(const PagedArgs &a, int b, const KvSeq &s, int head, int i, int lane, int c0 = 0, int c1 = 128) {
     const KvPages &kv = a.pages;
     const PagedRow r = paged_row(a, s, i);
     const int hk = head / a.attn.G, dk = kv.dk;
@@ -167,10 +167,10 @@ __device__ __forceinline__ void paged_again(const PagedArgs &a, int b, const KvS
     }
     float *o = a.attn.O + at * a.attn.ldo + (int64_t)head * dk;
     const float inv = any ? 1.0f / l : 0.0f;
-    if (lane < dk) o[lane] = any ? o0 * inv : 0.0f;
-    if (lane + 64 < dk) o[lane + 64] = any ? o1 * inv : 0.0f;
+    if (lane < dk && lane >= c0 && lane < c1) o[lane] = any ? o0 * inv : 0.0f;
+    if (lane + 64 < dk && lane + 64 >= c0 && lane + 64 < c1) o[lane + 64] = any ? o1 * inv : 0.0f;
     // (a row that saw nothing but scores of -infinity: 0 / 0 above, and NaN here)
-    if (a.attn.L && lane == 0) a.attn.L[at * a.attn.H + head] = !any ? -INFINITY : l == 0.0f ? NAN : (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (a.attn.L && lane == 0 && c0 == 0) a.attn.L[at * a.attn.H + head] = !any ? -INFINITY : l == 0.0f ? NAN : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 }  // namespace axhip

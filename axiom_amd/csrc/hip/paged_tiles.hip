@@ -63,6 +63,11 @@ __device__ __forceinline__ Place place_of(const PagedArgs &a, const PagedTileGri
     return p;
 }
 
+// How many ranges a tile's blocks are shared out in: as many as their count asks for
+__device__ __forceinline__ unsigned ranges_of(const PagedTileGrid &grid, const PagedTiles &blocks) {
+    return (unsigned)min(max((blocks.all + grid.range - 1) / grid.range, 1), grid.splits);
+}
+
 template <int DK, int SETS, int TYPE, bool PAD>
 __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, PagedTileGrid grid) {
     using G = TileGeom<DK, SETS>;
@@ -98,7 +103,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
     const PagedRow low = paged_row(a, seq, token(w0)), high = paged_row(a, seq, token(w1));
     const int last = wave % SETS * 32 < rows_here ? high.end : 0;
     const PagedTiles blocks = paged_tiles_of(a, wg_low.begin, wg_high.end, G::SHIFT);
-    const int n_begin = (int)((unsigned)blocks.all * split / (unsigned)grid.splits), n_end = (int)((unsigned)blocks.all * (split + 1) / (unsigned)grid.splits);
+    const unsigned ranges = ranges_of(grid, blocks);
+    if (split >= ranges) return;
+    const int n_begin = (int)((unsigned)blocks.all * split / ranges), n_end = (int)((unsigned)blocks.all * (split + 1) / ranges);
     const float slope2 = at.slopes ? at.slopes[head] * at.bias2 : 0.0f;
 
     const unsigned base = lds_address(lds);
@@ -375,7 +382,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
                 for (int e = 0; e < 4; e++) acc[d][4 * g + e] = __builtin_fmaf(acc[d][4 * g + e], ours, sum[e] * theirs);
             }
     }
-    if (grid.splits > 1) {
+    if (ranges > 1) {
         float *part = grid.parts + ((slot * kv.heads + hk) * grid.splits + split) * G::PART + wave * (G::PART / SETS);
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -421,17 +428,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
     }
 }
 
-// What ranges of keys left, added in order: a workgroup for 32 rows, a wave for 32 columns
+// What ranges of keys left, added in order: a workgroup for 32 rows and 32 columns, a quarter of the ranges a wave
 template <int DK, int SETS, int TYPE>
-__global__ void __launch_bounds__(2 * DK) k_paged_join(PagedArgs a, PagedTileGrid grid) {
+__global__ void __launch_bounds__(256) k_paged_join(PagedArgs a, PagedTileGrid grid) {
     using G = TileGeom<DK, SETS>;
     constexpr int BQ = G::BQ, DT = DK / 32;
-    __shared__ unsigned flags[DT];
+    __shared__ v4f sums[3][4][64];
+    __shared__ float of_rows[4][2][32];
     const KvPages &kv = a.pages;
     const AttnArgs &at = a.attn;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
-    const unsigned of_set = blockIdx.x / SETS, set = blockIdx.x % SETS, of_slot = of_set / (unsigned)kv.heads;
-    const int hk = (int)(of_set - of_slot * (unsigned)kv.heads);
+    const unsigned of_set = blockIdx.x / DT, d = blockIdx.x % DT, of_unit = of_set / SETS, set = of_set % SETS, of_slot = of_unit / (unsigned)kv.heads;
+    const int hk = (int)(of_unit - of_slot * (unsigned)kv.heads);
     const int64_t slot = grid.first + of_slot, unit = slot * kv.heads + hk;
     KvSeq seq = {0, 0, 0};
     const Place place = place_of<BQ>(a, grid, slot, lane, seq);
@@ -440,48 +448,72 @@ __global__ void __launch_bounds__(2 * DK) k_paged_join(PagedArgs a, PagedTileGri
     const bool valid = frow < rows_here;
     const unsigned r = place.g0 + 32 * set + (unsigned)(valid ? frow : rows_here - 1), over = r / (unsigned)at.G;
     const int i = place.i0 + (int)over, head = hk * at.G + (int)(r - over * (unsigned)at.G);
+    const PagedRow low = paged_row(a, seq, place.i0), high = paged_row(a, seq, place.i0 + (int)((place.g0 + (unsigned)place.rows - 1) / (unsigned)at.G));
+    const int ranges = (int)ranges_of(grid, paged_tiles_of(a, low.begin, high.end, G::SHIFT));
+    if (ranges == 1) return;                         // (it wrote its rows itself)
     const bool live = valid && paged_row(a, seq, i).end > 0;
     const float *parts = grid.parts + unit * grid.splits * G::PART + set * (G::PART / SETS);
+    // this wave's ranges, against their largest reference
+    const int from = ranges * wave / 4, to = ranges * (wave + 1) / 4;
     float m = ATTN_LOWEST, l = 0.0f;
-    for (int s = 0; s < grid.splits; s++) m = fmaxf(m, parts[(int64_t)s * G::PART + G::PIECES * 256 + frow]);
     v4f sum[4];
 #pragma unroll
     for (int g = 0; g < 4; g++) sum[g] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = 0; s < grid.splits; s++) {
+    for (int s = from; s < to; s++) {
         const float *part = parts + (int64_t)s * G::PART;
-        const float ref = part[G::PIECES * 256 + frow], weight = __builtin_amdgcn_exp2f(ref - m);
-        l += scaled(part[G::PIECES * 256 + 32 + frow], ref - m);
+        const float ref = part[G::PIECES * 256 + frow], more = part[G::PIECES * 256 + 32 + frow], both = fmaxf(m, ref);
+        const float ours = __builtin_amdgcn_exp2f(m - both), theirs = __builtin_amdgcn_exp2f(ref - both);
+        l = scaled(l, m - both) + scaled(more, ref - both);
+        m = both;
 #pragma unroll
-        for (int g = 0; g < 4; g++) sum[g] += *reinterpret_cast<const v4f *>(part + ((4 * wave + g) * 64 + lane) * 4) * weight;
+        for (int g = 0; g < 4; g++) sum[g] = sum[g] * ours + *reinterpret_cast<const v4f *>(part + ((4 * d + g) * 64 + lane) * 4) * theirs;
+    }
+    if (wave > 0)
+#pragma unroll
+        for (int g = 0; g < 4; g++) sums[wave - 1][g][lane] = sum[g];
+    if (fhalf == 0) {
+        of_rows[wave][0][frow] = m;
+        of_rows[wave][1][frow] = l;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    float top = m;
+#pragma unroll
+    for (int w = 1; w < 4; w++) top = fmaxf(top, of_rows[w][0][frow]);
+    l = scaled(l, m - top);
+    const float first = __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+    for (int g = 0; g < 4; g++) sum[g] *= first;
+#pragma unroll
+    for (int w = 1; w < 4; w++) {
+        const float ref = of_rows[w][0][frow], weight = __builtin_amdgcn_exp2f(ref - top);
+        l += scaled(of_rows[w][1][frow], ref - top);
+#pragma unroll
+        for (int g = 0; g < 4; g++) sum[g] += sums[w - 1][g][lane] * weight;
     }
     float seen = l * 0.0f;
 #pragma unroll
     for (int g = 0; g < 4; g++)
 #pragma unroll
         for (int e = 0; e < 4; e++) seen = __builtin_fmaf(sum[g][e], 0.0f, seen);
-    const uint64_t unfit = __builtin_amdgcn_ballot_w64(live && (!(seen == 0.0f) || l == 0.0f));
-    if (lane == 0) flags[wave] = (unsigned)(unfit | unfit >> 32);
-    __syncthreads();
-    unsigned again = 0;
-#pragma unroll
-    for (int w = 0; w < DT; w++) again |= flags[w];
-    again = __builtin_amdgcn_readfirstlane(again);
+    uint64_t again = __builtin_amdgcn_ballot_w64(live && (!(seen == 0.0f) || l == 0.0f));
+    again |= again >> 32;
     if (valid && !((again >> frow) & 1)) {
-        const int64_t to = (int64_t)seq.first + i;
-        float *o = at.O + to * at.ldo + (int64_t)head * kv.dk;
+        const int64_t row = (int64_t)seq.first + i;
+        float *o = at.O + row * at.ldo + (int64_t)head * kv.dk;
         const float inv = 1.0f / l;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-            const int col = 32 * wave + 8 * g + 4 * fhalf;
+            const int col = 32 * (int)d + 8 * g + 4 * fhalf;
             if (col < kv.dk) *reinterpret_cast<v4f *>(o + col) = live ? sum[g] * inv : v4f{0.f, 0.f, 0.f, 0.f};
         }
-        if (at.L && wave == 0 && fhalf == 0) at.L[to * at.H + head] = live ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+        if (at.L && d == 0 && fhalf == 0) at.L[row * at.H + head] = live ? (top + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
     }
-    int nth = 0;
-    for (unsigned rest = again; rest; rest &= rest - 1, nth++) {
+    // (each workgroup its own columns of a row, and the first one its sum)
+    for (unsigned rest = (unsigned)again; rest; rest &= rest - 1) {
         const int n = __builtin_ctz(rest);
-        if (nth % DT == wave) paged_again<TYPE>(a, place.b, seq, __builtin_amdgcn_readlane(head, n), __builtin_amdgcn_readlane(i, n), lane);
+        paged_again<TYPE>(a, place.b, seq, __builtin_amdgcn_readlane(head, n), __builtin_amdgcn_readlane(i, n), lane, 32 * (int)d, 32 * (int)d + 32);
     }
 }
 
@@ -499,7 +531,7 @@ int launch_tiles(const PagedArgs &a, PagedTileGrid grid) {
     }
     note_kernel(grid.splits > 1 ? (SETS == 8 ? "paged_tiles_256_ranges" : "paged_tiles_128_ranges") : SETS == 8 ? "paged_tiles_256" : "paged_tiles_128");
     // as many slots a launch as it holds
-    const int64_t at_once = std::max<int64_t>(1, GRID_MOST / ((int64_t)a.pages.heads * grid.splits)), join_at_once = std::max<int64_t>(1, GRID_MOST / ((int64_t)a.pages.heads * SETS));
+    const int64_t at_once = std::max<int64_t>(1, GRID_MOST / ((int64_t)a.pages.heads * grid.splits)), join_at_once = std::max<int64_t>(1, GRID_MOST / ((int64_t)a.pages.heads * SETS * (DK / 32)));
     for (grid.first = 0; grid.first < grid.slots; grid.first += at_once) {
         const int64_t here = std::min(grid.slots - grid.first, at_once);
         hipLaunchKernelGGL((k_paged_tiles<DK, SETS, TYPE, PAD>), dim3((unsigned)(here * a.pages.heads * grid.splits)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
@@ -508,7 +540,7 @@ int launch_tiles(const PagedArgs &a, PagedTileGrid grid) {
     if (grid.splits > 1)
         for (grid.first = 0; grid.first < grid.slots; grid.first += join_at_once) {
             const int64_t here = std::min(grid.slots - grid.first, join_at_once);
-            hipLaunchKernelGGL((k_paged_join<DK, SETS, TYPE>), dim3((unsigned)(here * a.pages.heads * SETS)), dim3(2 * DK), 0, kStream, a, grid);
+            hipLaunchKernelGGL((k_paged_join<DK, SETS, TYPE>), dim3((unsigned)(here * a.pages.heads * SETS * (DK / 32))), dim3(256), 0, kStream, a, grid);
             if (int rc = check_launch("attn_paged")) return rc;
         }
     return AXHIP_OK;
@@ -521,11 +553,12 @@ int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid) {
     grid.per = (rows + G::BQ - 1) / G::BQ;
     grid.slots = a.pages.first ? all_rows / G::BQ + a.pages.B : a.pages.B * grid.per;
     const int64_t likely = (a.pages.first ? all_rows / G::BQ + 1 : grid.slots) * a.pages.heads, blocks = paged_steps_most(a, G::SHIFT);
-    int64_t splits = cus / likely;
+    int64_t splits = (cus + likely / 2) / likely;
     if (splits > blocks / 4) splits = blocks / 4;
     if (splits > SPLITS_MOST) splits = SPLITS_MOST;
     if (splits < 1) splits = 1;
     grid.splits = (int)splits;
+    grid.range = (int)std::max<int64_t>((blocks + splits - 1) / splits, 1);
     auto run = [&](auto of) {
         constexpr int TYPE = decltype(of)::value;
         return a.pages.dk < DK ? launch_tiles<DK, SETS, TYPE, true>(a, grid) : launch_tiles<DK, SETS, TYPE, false>(a, grid);
@@ -541,8 +574,7 @@ namespace axhip {
 int paged_tiles(const PagedArgs &a, int type, int rows_least) {
     PagedTileGrid grid = {};
     grid.least = rows_least;
-    const int64_t wide_tiles = ((int64_t)a.attn.G * a.pages.T + 255) / 256 * a.pages.heads;
-    const bool wide = wide_tiles >= cu_count();
+    const bool wide = (int64_t)a.attn.G * a.pages.Sq > 128;
     auto run = [&](auto width) {
         constexpr int DK = decltype(width)::value;
         return wide ? launch_tiles<DK, 8>(a, type, grid) : launch_tiles<DK, 4>(a, type, grid);

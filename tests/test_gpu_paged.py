@@ -292,8 +292,9 @@ def test_chunks(hip, kind, rules, dk, heads, G, page_rows):
 
 @TYPES
 @pytest.mark.parametrize("dk", [64, 128, 72])
-@pytest.mark.parametrize("new,lens,kernel", [([1], [2000], "paged_few_ranges"), ([1] * 600, [40] * 600, "paged_few"), ([64], [2000], "paged_tiles_128_ranges"),
-                                             ([700] * 3, [800, 700, 5], "paged_tiles_128"), ([257] * 12, [300] * 12, "paged_tiles_256")], ids=lambda v: str(v)[:12])
+@pytest.mark.parametrize("new,lens,kernel", [([1], [2000], "paged_few_ranges"), ([1] * 600, [40] * 600, "paged_few"), ([30], [2000], "paged_tiles_128_ranges"),
+                                             ([20] * 300, [40] * 299 + [3], "paged_tiles_128"), ([100] * 2, [2000, 700], "paged_tiles_256_ranges"),
+                                             ([700] * 3, [1800, 700, 5], "paged_tiles_256_ranges"), ([257] * 12, [300] * 12, "paged_tiles_256")], ids=lambda v: str(v)[:12])
 def test_forms(hip, kind, dk, new, lens, kernel):
     """Each form, by the kernel that it says it is."""
     say("forms", kind, dk, kernel)
