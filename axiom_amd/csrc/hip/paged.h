@@ -94,6 +94,12 @@ inline int64_t paged_steps_most(const PagedArgs &a, int shift) {
     return most < all ? most : all;
 }
 
+// In how many ranges the keys of `units` groups of rows are shared out: as many as fill the CUs with a workgroup each, a wave with two tiles or more (few rows), a workgroup with four blocks or
+// more (tiles).
+constexpr int PAGED_SPLITS = 64;
+int64_t paged_few_splits(int64_t units, int64_t tiles);
+int64_t paged_tile_splits(int64_t units, int64_t blocks);
+
 // ---- one row by one wave with fp32 instructions: what the matrix kernels fall back to where sums are not finite.  64 keys at a time, a score a lane; then a value column a lane (two
 // where dk > 64), and only keys that are seen are touched. ----
 template <int TYPE>

@@ -7,8 +7,25 @@
 namespace {
 using namespace axhip;
 
-// Sequences with more rows than this (new tokens, times the query heads that share keys) go over tiles
-constexpr int FEW_ROWS = 32;
+// Which form takes rows of equal counts, by what each takes, in us: rounds of workgroups over the CUs, each its start and its steps of keys, and for tiles in ranges the launch that joins them.
+// (16-row units of 8 waves that take 32 keys each; tiles of 256 rows, or 128, in blocks.)  Within a tenth or so of what was measured (us, tiles -> few rows: 1 x 128 tokens over 128 keys, 32 heads, 8
+// of keys, of 128 19.6 -> 7.8, 1 x 512 over 512, 8 heads 31 -> 15.5, 4 x 64 over 500, 32 heads, 8 of keys 33 -> 25; the other side 64 x 32 over 100, 32 heads, 8 of keys 38 -> 58, 16 x 64 over 64, 16 heads, 4
+// of keys, of 64 14.3 -> 20.7).  Up to 64 rows of a sequence few rows won throughout (8 x 8 tokens over 4096, 64 heads, 8 of keys 49 -> 44, 1 x 8 24 -> 17).
+constexpr int FEW_ROWS = 64, LIKE_ROWS = 32;
+bool few_is_faster(const PagedArgs &a) {
+    const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, cus = cu_count();
+    if (rows <= FEW_ROWS) return true;
+    const int width = (a.pages.dk + 31) / 32 - 1;
+    constexpr double FEW_STEP[] = {0.9, 1.3, 2.2, 2.5}, BLOCK[] = {3.0, 4.4, 4.0, 4.7};
+    const int64_t units = a.pages.B * (int64_t)a.pages.heads * ((rows + 15) / 16), keys = paged_steps_most(a, 5);
+    if (units > 64 * cus) return false;
+    const int64_t splits = paged_few_splits(units, keys), rounds = (units * splits + cus - 1) / cus, steps = ((keys + splits - 1) / splits + 7) / 8;
+    const double few = (double)rounds * (5.5 + (double)steps * FEW_STEP[width]);
+    const int64_t tile_rows = rows > 128 ? 256 : 128, tiles = a.pages.B * (int64_t)a.pages.heads * ((rows + tile_rows - 1) / tile_rows), blocks = paged_steps_most(a, a.pages.dk <= 64 ? 7 : 6);
+    const int64_t ranges = paged_tile_splits(tiles, blocks), tile_rounds = (tiles * ranges + cus - 1) / cus;
+    const double by_tiles = (double)tile_rounds * (10.0 + (double)((blocks + ranges - 1) / ranges) * BLOCK[width] * (tile_rows == 256 ? 1.0 : 0.7)) + (ranges > 1 ? 9.0 : 0.0);
+    return few < by_tiles;
+}
 
 }  // namespace
 
@@ -51,11 +68,10 @@ extern "C" int axhip_attn_paged(const float *Q, int64_t ldq, const axhip_kv_cach
     a.window = r.window < PAST ? r.window : PAST;
     a.sinks = r.window == 0 ? 0 : r.sinks < PAST ? r.sinks : PAST;
     if (a.pages.room > Sk) a.pages.room = (int)Sk;
-    // A sequence with few rows is read by the form that shares out its keys, others by tiles.  How many rows each sequence has is on the device, so both may have to be launched, each
-    // for its own; not where all have the same number of rows, or none can have more than a few.
-    const int64_t rows = (int64_t)t.G * Sq;
-    if (rows <= FEW_ROWS) return paged_few(a, cache->type, FEW_ROWS);
-    if (!first || B == 1) return paged_tiles(a, cache->type, 0);
-    if (int rc = paged_few(a, cache->type, FEW_ROWS)) return rc;
-    return paged_tiles(a, cache->type, FEW_ROWS + 1);
+    // How many rows each sequence has is on the device: where some may have many and others few, both forms are launched, each for its own.  (There a sequence is few rows' with 32 of them, or one
+    // token of many heads.)
+    if (!first || B == 1 || (int64_t)t.G * Sq <= FEW_ROWS) return few_is_faster(a) ? paged_few(a, cache->type, 0x7fffffff) : paged_tiles(a, cache->type, 0);
+    const int like = t.G > LIKE_ROWS ? (t.G + 15) / 16 * 16 : LIKE_ROWS;
+    if (int rc = paged_few(a, cache->type, like)) return rc;
+    return paged_tiles(a, cache->type, like + 1);
 }

@@ -14,7 +14,7 @@
 namespace {
 using namespace axhip;
 
-constexpr int SPLITS_MOST = 64, ROWS = 16;
+constexpr int SPLITS_MOST = PAGED_SPLITS, ROWS = 16;
 
 template <int DK, int WAVES>
 struct FewGeom {
@@ -460,18 +460,22 @@ int launch_few(const PagedArgs &a, int type, const PagedFewGrid &grid) {
 
 namespace axhip {
 
+int64_t paged_few_splits(int64_t units, int64_t tiles) {
+    int64_t splits = cu_count() / units;
+    if (splits > (tiles + 15) / 16) splits = (tiles + 15) / 16;
+    if (splits > SPLITS_MOST) splits = SPLITS_MOST;
+    return splits < 1 ? 1 : splits;
+}
+
 int paged_few(const PagedArgs &a, int type, int rows_most) {
     PagedFewGrid grid = {};
     grid.most = rows_most;
-    const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, most = rows < rows_most ? rows : rows_most;
+    const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, most = rows < rows_most ? rows : rows_most, tiles = paged_steps_most(a, 5);
     grid.row_tiles = (int)((most + ROWS - 1) / ROWS);
-    const int64_t units = (int64_t)a.pages.B * a.pages.heads * grid.row_tiles, tiles = paged_steps_most(a, 5), cus = cu_count();
+    // (where only some of the sequences are this form's, most of those have a single new token)
+    const int64_t of_b = rows <= rows_most ? grid.row_tiles : (a.attn.G + ROWS - 1) / ROWS;
+    grid.splits = (int)paged_few_splits(a.pages.B * a.pages.heads * of_b, tiles);
     const int waves = tiles > 4 ? 8 : 4;
-    int64_t splits = cus / units;
-    if (splits > (tiles + 2 * waves - 1) / (2 * waves)) splits = (tiles + 2 * waves - 1) / (2 * waves);
-    if (splits > SPLITS_MOST) splits = SPLITS_MOST;
-    if (splits < 1) splits = 1;
-    grid.splits = (int)splits;
     auto run = [&](auto width) {
         constexpr int DK = decltype(width)::value;
         return waves == 8 ? launch_few<DK, 8>(a, type, grid) : launch_few<DK, 4>(a, type, grid);

@@ -16,7 +16,7 @@
 namespace {
 using namespace axhip;
 
-constexpr int WAVES = 8, SPLITS_MOST = 64;
+constexpr int WAVES = 8, SPLITS_MOST = PAGED_SPLITS;
 
 template <int DK, int SETS>
 struct TileGeom {
@@ -250,11 +250,29 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = 0.0f;
             __builtin_amdgcn_s_setprio(1);
+            if constexpr (DK <= 64) {
+                v4i f[KS];
+#pragma unroll
+                for (int k = 0; k < KS; k++) f[k] = B::rows(row_place, k, 0);
+                __builtin_amdgcn_sched_barrier(0x6);
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    s = mfma_halves(f[k], qf[k][1], s);
+                    s = mfma_halves(f[k], qf[k][0], s);
+                }
+            } else
             products<KS>([&](int k, v4i (&f)[2]) { f[0] = B::rows(row_place, k, 0); },
                          [&](int k, const v4i (&f)[2]) {
                              s = mfma_halves(f[0], qf[k][1], s);
                              s = mfma_halves(f[0], qf[k][0], s);
                          });
+            v4i vfrag[2 * DT];
+            if constexpr (DK <= 64) {
+                __builtin_amdgcn_sched_barrier(0x6);
+#pragma unroll
+                for (int m = 0; m < 2 * DT; m++) vfrag[m] = B::columns(column_place, 16 * (m / DT), m % DT, 0);
+                __builtin_amdgcn_sched_barrier(0x6);
+            }
             __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int g = 0; g < 4; g++)
@@ -329,6 +347,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
             cut_scaled(w, 0, one, pf[0]);
             cut_scaled(w, 1, one, pf[1]);
             __builtin_amdgcn_s_setprio(1);
+            if constexpr (DK <= 64) {
+#pragma unroll
+                for (int m = 0; m < 2 * DT; m++) {
+                    acc[m % DT] = mfma_halves(vfrag[m], pf[m / DT][1], acc[m % DT]);
+                    acc[m % DT] = mfma_halves(vfrag[m], pf[m / DT][0], acc[m % DT]);
+                }
+            } else
             products<2 * DT>([&](int m, v4i (&f)[2]) { f[0] = B::columns(column_place, 16 * (m / DT), m % DT, 0); },
                              [&](int m, const v4i (&f)[2]) {
                                  acc[m % DT] = mfma_halves(f[0], pf[m / DT][1], acc[m % DT]);
@@ -549,16 +574,12 @@ int launch_tiles(const PagedArgs &a, PagedTileGrid grid) {
 template <int DK, int SETS>
 int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid) {
     using G = TileGeom<DK, SETS>;
-    const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, all_rows = (int64_t)a.attn.G * a.pages.T, cus = cu_count();
+    const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, all_rows = (int64_t)a.attn.G * a.pages.T;
     grid.per = (rows + G::BQ - 1) / G::BQ;
     grid.slots = a.pages.first ? all_rows / G::BQ + a.pages.B : a.pages.B * grid.per;
     const int64_t likely = (a.pages.first ? all_rows / G::BQ + 1 : grid.slots) * a.pages.heads, blocks = paged_steps_most(a, G::SHIFT);
-    int64_t splits = (cus + likely / 2) / likely;
-    if (splits > blocks / 4) splits = blocks / 4;
-    if (splits > SPLITS_MOST) splits = SPLITS_MOST;
-    if (splits < 1) splits = 1;
-    grid.splits = (int)splits;
-    grid.range = (int)std::max<int64_t>((blocks + splits - 1) / splits, 1);
+    grid.splits = (int)paged_tile_splits(likely, blocks);
+    grid.range = (int)std::max<int64_t>((blocks + grid.splits - 1) / grid.splits, 1);
     auto run = [&](auto of) {
         constexpr int TYPE = decltype(of)::value;
         return a.pages.dk < DK ? launch_tiles<DK, SETS, TYPE, true>(a, grid) : launch_tiles<DK, SETS, TYPE, false>(a, grid);
@@ -570,6 +591,13 @@ int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid) {
 }  // namespace
 
 namespace axhip {
+
+int64_t paged_tile_splits(int64_t units, int64_t blocks) {
+    int64_t splits = (cu_count() + units / 2) / units;
+    if (splits > blocks / 4) splits = blocks / 4;
+    if (splits > SPLITS_MOST) splits = SPLITS_MOST;
+    return splits < 1 ? 1 : splits;
+}
 
 int paged_tiles(const PagedArgs &a, int type, int rows_least) {
     PagedTileGrid grid = {};

@@ -292,13 +292,13 @@ def test_chunks(hip, kind, rules, dk, heads, G, page_rows):
 
 @TYPES
 @pytest.mark.parametrize("dk", [64, 128, 72])
-@pytest.mark.parametrize("new,lens,kernel", [([1], [2000], "paged_few_ranges"), ([1] * 600, [40] * 600, "paged_few"), ([30], [2000], "paged_tiles_128_ranges"),
-                                             ([20] * 300, [40] * 299 + [3], "paged_tiles_128"), ([100] * 2, [2000, 700], "paged_tiles_256_ranges"),
-                                             ([700] * 3, [1800, 700, 5], "paged_tiles_256_ranges"), ([257] * 12, [300] * 12, "paged_tiles_256")], ids=lambda v: str(v)[:12])
+@pytest.mark.parametrize("new,lens,kernel", [([1], [2000], "paged_few_ranges"), ([1] * 600, [40] * 600, "paged_few"), ([70], [300], "paged_few"), ([30] * 30, [3000] * 30, "paged_tiles_128_ranges"),
+                                             ([30] * 100, [40] * 99 + [3], "paged_tiles_128"), ([700] * 3, [1800, 700, 5], "paged_tiles_256_ranges"), ([257] * 12, [300] * 12, "paged_tiles_256")],
+                         ids=lambda v: str(v)[:12])
 def test_forms(hip, kind, dk, new, lens, kernel):
     """Each form, by the kernel that it says it is."""
     say("forms", kind, dk, kernel)
-    heads, G = (23, 1) if kernel == "paged_tiles_256" else (2, 4) if len(new) < 100 else (1, 2)
+    heads, G = (23, 1) if kernel == "paged_tiles_256" else (2, 4) if len(new) <= 100 else (1, 2)
     check(hip, kind, heads, G, dk, 64, new, lens, dict(window=1500, sinks=70) if dk == 72 else {}, uniform=True, kernel=kernel)
 
 

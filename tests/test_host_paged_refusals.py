@@ -58,16 +58,17 @@ assert all(f(t, dk) == 0 for t, dk in ((-1, 64), (3, 64), (0, 0), (0, 132), (1, 
 
 
 def test_which_launches(stub):  # noqa: F811
-    """Few rows of every sequence: one launch; many of every one: tiles alone; unlike ones: both."""
+    """Few rows of every sequence, or not many in all: one launch; many of every one: tiles alone; unlike ones: both."""
     run(stub, PAGED + """
 def names(**more):
     before = stub.stub_launches()
     assert attend(**more) == 0
     return [("few" if b"paged_few" in x.kernel else "tiles" if b"paged_tiles" in x.kernel else "join" if b"paged_join" in x.kernel else "?") for x in launched()[before:]]
 assert names(Sq=1, T=3, first=None) == ["few"] and names(Sq=4, T=9) == ["few"] and names(Sq=16, T=9) == ["few"]
-assert names(Sq=100, T=300, first=None, Sk=100)[0] == "tiles" and "few" not in names(Sq=100, T=100, B=1)
-assert names(Sq=100, T=120)[:2] == ["few", "tiles"]
-assert names(Sq=100, T=100, B=1, Sk=100000, table_ld=10000)[-1] == "join"
+assert names(Sq=100, T=300, first=None, Sk=100) == ["few"] and names(Sq=100, T=100, B=1) == ["few"]
+assert names(Sq=4000, T=12000, first=None) == ["tiles"] and names(Sq=8000, T=8000, B=1) == ["tiles"]
+assert names(Sq=100, T=120) == ["few", "tiles"]
+assert names(Sq=2000, T=2000, B=1, Sk=100000, table_ld=10000) == ["tiles", "join"]
 """)
 
 
