@@ -13,7 +13,7 @@ struct PagedArgs {
 };
 
 struct PagedFewGrid {
-    int first;                                   // the launch's first sequence
+    int first, here;                             // the launch's first sequence, and how many
     int row_tiles, splits;                       // of 16 rows each; ranges of keys
     int most;                                    // sequences with more rows (of all heads that share keys) are the tiles'
     float *parts;                                // what the ranges leave
@@ -86,17 +86,30 @@ __device__ __forceinline__ PagedTiles paged_tiles_of(const PagedArgs &a, int beg
     return t;
 }
 
-// The most steps of 2^shift keys that rows of one sequence see together (above: from begin = p + 1 - window to the end of a row at most Sq - 1 further)
-inline int64_t paged_steps_most(const PagedArgs &a, int shift) {
-    const int64_t step = int64_t(1) << shift, all = (a.pages.room + step - 1) / step;
+// The most steps of 2^shift keys that `rows` rows of one sequence, one token after the other, see together (above: from begin = p + 1 - window to the end of a later row)
+inline int64_t paged_steps_most(const PagedArgs &a, int shift, int64_t rows) {
+    const int64_t step = int64_t(1) << shift, all = (a.pages.room + step - 1) / step, tokens = rows / a.attn.G + 2 < a.pages.Sq ? rows / a.attn.G + 2 : a.pages.Sq;
     if (a.window == 0) return all;
-    const int64_t most = (a.window + (int64_t)a.pages.Sq - 1 + 2 * (step - 1)) / step + ((int64_t)a.sinks + step - 1) / step;
+    const int64_t most = (a.window + tokens - 1 + 2 * (step - 1)) / step + ((int64_t)a.sinks + step - 1) / step;
     return most < all ? most : all;
 }
 
-// In how many ranges the keys of `units` groups of rows are shared out: as many as fill the CUs with a workgroup each, a wave with two tiles or more (few rows), a workgroup with four blocks or
-// more (tiles).
+// In how many ranges the keys of `units` groups of rows are shared out, a workgroup each: of 1 to `most` (a wave with two tiles of keys or more for few rows, a workgroup with four blocks for tiles) those
+// that take the fewest rounds over the CUs times their steps, `start` more for each round and `join` for the ranges' sums.
 constexpr int PAGED_SPLITS = 64;
+inline int64_t best_splits(int64_t units, int64_t steps, int64_t most, int64_t start, int64_t join) {
+    const int64_t cus = cu_count();
+    int64_t best = 1, least = INT64_MAX;
+    if (units >= 2 * cus) return 1;                  // (groups of unlike length fill up the rounds)
+    for (int64_t s = 1; s == 1 || (s <= most && s <= PAGED_SPLITS && units * s <= 8 * cus); s++) {
+        const int64_t cost = (units * s + cus - 1) / cus * ((steps + s - 1) / s + start) + (s > 1 ? join : 0);
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
+}
 int64_t paged_few_splits(int64_t units, int64_t tiles);
 int64_t paged_tile_splits(int64_t units, int64_t blocks);
 

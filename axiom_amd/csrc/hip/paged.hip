@@ -17,11 +17,11 @@ bool few_is_faster(const PagedArgs &a) {
     if (rows <= FEW_ROWS) return true;
     const int width = (a.pages.dk + 31) / 32 - 1;
     constexpr double FEW_STEP[] = {0.9, 1.3, 2.2, 2.5}, BLOCK[] = {3.0, 4.4, 4.0, 4.7};
-    const int64_t units = a.pages.B * (int64_t)a.pages.heads * ((rows + 15) / 16), keys = paged_steps_most(a, 5);
+    const int64_t units = a.pages.B * (int64_t)a.pages.heads * ((rows + 15) / 16), keys = paged_steps_most(a, 5, 16);
     if (units > 64 * cus) return false;
     const int64_t splits = paged_few_splits(units, keys), rounds = (units * splits + cus - 1) / cus, steps = ((keys + splits - 1) / splits + 7) / 8;
     const double few = (double)rounds * (5.5 + (double)steps * FEW_STEP[width]);
-    const int64_t tile_rows = rows > 128 ? 256 : 128, tiles = a.pages.B * (int64_t)a.pages.heads * ((rows + tile_rows - 1) / tile_rows), blocks = paged_steps_most(a, a.pages.dk <= 64 ? 7 : 6);
+    const int64_t tile_rows = rows > 128 ? 256 : 128, tiles = a.pages.B * (int64_t)a.pages.heads * ((rows + tile_rows - 1) / tile_rows), blocks = paged_steps_most(a, a.pages.dk <= 64 ? 7 : 6, tile_rows);
     const int64_t ranges = paged_tile_splits(tiles, blocks), tile_rounds = (tiles * ranges + cus - 1) / cus;
     const double by_tiles = (double)tile_rounds * (10.0 + (double)((blocks + ranges - 1) / ranges) * BLOCK[width] * (tile_rows == 256 ? 1.0 : 0.7)) + (ranges > 1 ? 9.0 : 0.0);
     return few < by_tiles;

@@ -86,9 +86,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_few(PagedArgs a, PagedF
     const KvPages &kv = a.pages;
     const AttnArgs &at = a.attn;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 15, part = lane >> 4;
-    // ranges of one set of rows follow each other, so that they go to different XCDs
-    const unsigned local = blockIdx.x / (unsigned)grid.splits, split = blockIdx.x - local * (unsigned)grid.splits, bh = local / (unsigned)grid.row_tiles, of_b = bh / (unsigned)kv.heads;
-    const int rt = (int)(local - bh * grid.row_tiles), b = grid.first + (int)of_b, hk = (int)(bh - of_b * kv.heads);
+    // Ranges of one set of rows follow each other, so that they go to different XCDs; the sequences' second sets of rows, which few may have, come behind all first ones, so that those do.
+    const unsigned local = blockIdx.x / (unsigned)grid.splits, split = blockIdx.x - local * (unsigned)grid.splits, each = (unsigned)grid.here * (unsigned)kv.heads, of_b = local % each;
+    const int rt = (int)(local / each), b = grid.first + (int)(of_b / (unsigned)kv.heads), hk = (int)(of_b % (unsigned)kv.heads);
     const int64_t unit = (int64_t)grid.first * kv.heads * grid.row_tiles + local;
     const KvSeq seq = kv_seq(kv, b);
     const int64_t rows = (int64_t)at.G * seq.n;
@@ -441,6 +441,7 @@ int launch_few(const PagedArgs &a, PagedFewGrid grid) {
     const int64_t at_once = GRID_MOST / (of_b * grid.splits);    // sequences a launch; (a sequence has at most 2^21 units, and ranges only where there are few)
     for (grid.first = 0; grid.first < a.pages.B; grid.first += (int)at_once) {
         const int64_t left = a.pages.B - grid.first, here = left < at_once ? left : at_once;
+        grid.here = (int)here;
         hipLaunchKernelGGL((k_paged_few<DK, TYPE, PAD, WAVES>), dim3((unsigned)(here * of_b * grid.splits)), dim3(64 * WAVES), G::SMEM, kStream, a, grid);
         if (int rc = check_launch("attn_paged")) return rc;
     }
@@ -460,17 +461,12 @@ int launch_few(const PagedArgs &a, int type, const PagedFewGrid &grid) {
 
 namespace axhip {
 
-int64_t paged_few_splits(int64_t units, int64_t tiles) {
-    int64_t splits = cu_count() / units;
-    if (splits > (tiles + 15) / 16) splits = (tiles + 15) / 16;
-    if (splits > SPLITS_MOST) splits = SPLITS_MOST;
-    return splits < 1 ? 1 : splits;
-}
+int64_t paged_few_splits(int64_t units, int64_t tiles) { return best_splits(units, (tiles + 7) / 8, (tiles + 15) / 16, 2, 1); }
 
 int paged_few(const PagedArgs &a, int type, int rows_most) {
     PagedFewGrid grid = {};
     grid.most = rows_most;
-    const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, most = rows < rows_most ? rows : rows_most, tiles = paged_steps_most(a, 5);
+    const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, most = rows < rows_most ? rows : rows_most, tiles = paged_steps_most(a, 5, ROWS);
     grid.row_tiles = (int)((most + ROWS - 1) / ROWS);
     // (where only some of the sequences are this form's, most of those have a single new token)
     const int64_t of_b = rows <= rows_most ? grid.row_tiles : (a.attn.G + ROWS - 1) / ROWS;

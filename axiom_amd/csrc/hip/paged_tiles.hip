@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
     const AttnArgs &at = a.attn;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, frow = lane & 31, fhalf = lane >> 5;
 
-    // a sequence's last tiles, the longest, first; heads of keys go to the XCDs in turn
+    // a sequence's last tiles, the longest, first; heads of keys, and then ranges, go to the XCDs in turn, each of which has an L2 (the ranges behind all first ones: 175 us for 159)
     const unsigned rest = blockIdx.x / (unsigned)kv.heads, of_slot = rest / (unsigned)grid.splits, split = rest - of_slot * (unsigned)grid.splits;
     const int64_t slot = grid.slots - 1 - (grid.first + of_slot);
     const int hk = (int)(blockIdx.x - rest * (unsigned)kv.heads);
@@ -577,7 +577,7 @@ int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid) {
     const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, all_rows = (int64_t)a.attn.G * a.pages.T;
     grid.per = (rows + G::BQ - 1) / G::BQ;
     grid.slots = a.pages.first ? all_rows / G::BQ + a.pages.B : a.pages.B * grid.per;
-    const int64_t likely = (a.pages.first ? all_rows / G::BQ + 1 : grid.slots) * a.pages.heads, blocks = paged_steps_most(a, G::SHIFT);
+    const int64_t likely = (a.pages.first ? all_rows / G::BQ + 1 : grid.slots) * a.pages.heads, blocks = paged_steps_most(a, G::SHIFT, G::BQ);
     grid.splits = (int)paged_tile_splits(likely, blocks);
     grid.range = (int)std::max<int64_t>((blocks + grid.splits - 1) / grid.splits, 1);
     auto run = [&](auto of) {
@@ -592,12 +592,7 @@ int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid) {
 
 namespace axhip {
 
-int64_t paged_tile_splits(int64_t units, int64_t blocks) {
-    int64_t splits = (cu_count() + units / 2) / units;
-    if (splits > blocks / 4) splits = blocks / 4;
-    if (splits > SPLITS_MOST) splits = SPLITS_MOST;
-    return splits < 1 ? 1 : splits;
-}
+int64_t paged_tile_splits(int64_t units, int64_t blocks) { return best_splits(units, blocks, blocks / 4, 2, 3); }
 
 int paged_tiles(const PagedArgs &a, int type, int rows_least) {
     PagedTileGrid grid = {};
