@@ -37,17 +37,18 @@ __device__ __forceinline__ KvSeq kv_seq(const KvPages &a, int b) {
 }
 
 // How many of first[1 .. B] the predicate holds for, which holds for the first of them and no longer from some place on: the sequence that a row, or a tile, belongs to.  By all
-// lanes of a wave together, 64 sequences at a time.
+// lanes of a wave together, 64 places at a time: one trip to memory for up to 64 sequences, two for 4096.
 template <typename Before>
 __device__ __forceinline__ int kv_find(const KvPages &a, int lane, Before before) {
-    int b = 0;
-    for (int k0 = 1; k0 <= a.B; k0 += 64) {
-        const int k = k0 + lane;
-        const int here = __builtin_popcountll(__builtin_amdgcn_ballot_w64(k <= a.B && before(k, min(max(a.first[k], 0), a.T))));
-        b += here;
-        if (here < 64) break;
+    int low = 0, high = a.B;                         // it holds for `low`, and for none past `high`
+    while (low < high) {
+        const int step = (high - low + 63) / 64, k = min(low + (lane + 1) * step, high);
+        const int here = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before(k, min(max(a.first[k], 0), a.T))));
+        const int from = low;
+        low = min(from + here * step, high);
+        if (here < 64) high = max(min(from + (here + 1) * step, high) - 1, low);
     }
-    return b;
+    return low;
 }
 
 // The table's entry for a position below a sequence's length, and whether it is a page: apart, so that entries can be under way while nothing waits for them

@@ -172,6 +172,19 @@ def test_rows_of_equal_counts(hip, kind):
     assert np.array_equal(got[0][4], want)
 
 
+@TYPES
+@pytest.mark.parametrize("B", [64, 65, 4096, 5000])
+def test_many_sequences(hip, kind, B):
+    """Rows of unlike counts, none and one mostly, of so many sequences that the search for a row's takes one, two and three steps: written, read and attended to by both forms."""
+    say("kv many", kind, B)
+    rng = np.random.default_rng(B)
+    heads, G, dk, page_rows = 1, 2, 32, 4
+    new = rng.integers(0, 3, B)
+    new[[0, B // 3, B - 1]] = [0, 70, 5]
+    lens = new + rng.integers(0, 4, B)
+    check(hip, kind, heads, G, dk, page_rows, new.tolist(), lens.tolist(), seed=B, behind=1)
+
+
 def test_offsets_that_pass_32_bits(hip):
     """Pages past 4 GiB of a pool: written, read and attended to there."""
     say("kv far")
@@ -272,7 +285,7 @@ RULES = {"plain": {}, "window": dict(window=19), "sinks": dict(window=40, sinks=
 
 @TYPES
 @pytest.mark.parametrize("rules", RULES)
-@pytest.mark.parametrize("dk,heads,G", [(64, 2, 4), (128, 1, 8), (80, 2, 1), (32, 1, 2), (20, 2, 3)])
+@pytest.mark.parametrize("dk,heads,G", [(64, 2, 4), (128, 1, 8), (80, 2, 1), (32, 1, 2), (20, 2, 3), (4, 3, 5), (104, 1, 16)])
 def test_tokens(hip, kind, rules, dk, heads, G):
     """One token, a few, none, more than there are positions: the form for few rows."""
     say("tokens", kind, rules, dk, heads, G)
@@ -282,7 +295,7 @@ def test_tokens(hip, kind, rules, dk, heads, G):
 
 @TYPES
 @pytest.mark.parametrize("rules", RULES)
-@pytest.mark.parametrize("dk,heads,G,page_rows", [(64, 2, 4, 32), (128, 2, 2, 16), (96, 1, 3, 64), (40, 1, 40, 8), (112, 2, 1, 128), (32, 1, 8, 1)])
+@pytest.mark.parametrize("dk,heads,G,page_rows", [(64, 2, 4, 32), (128, 2, 2, 16), (96, 1, 3, 64), (40, 1, 40, 8), (112, 2, 1, 128), (32, 1, 8, 1), (4, 2, 3, 16)])
 def test_chunks(hip, kind, rules, dk, heads, G, page_rows):
     """Chunks of unlike lengths, single tokens and nothing beside them: both forms in one call."""
     say("chunks", kind, rules, dk, heads, G, page_rows)

@@ -45,3 +45,10 @@ def test_attention_under_score_rules_keeps_its_registers(kernels):
         wide = "k_attn_fwdILi128" in name
         assert int(re.search(r"\.private_segment_fixed_size: (\d+)\n", note).group(1)) <= (32 if wide else 0), name
         assert int(re.search(r"\.vgpr_spill_count: (\d+)\n", note).group(1)) <= (7 if wide else 0), name
+
+
+def test_attention_over_pages_keeps_its_registers(kernels):
+    mine = {name: note for name, note in kernels.items() if re.search("k_paged_(few|tiles|join)I|k_kv_(write|read)I", name)}
+    assert len(mine) == 48 + 48 + 24 + 18 + 6, len(mine)
+    for name, note in mine.items():
+        assert re.search(r"\.private_segment_fixed_size: 0\n", note) and re.search(r"\.vgpr_spill_count: 0\n", note), name
