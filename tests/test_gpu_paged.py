@@ -433,6 +433,28 @@ def test_sizes_far_apart(hip, kind, new):
     hold(k, [x * np.float32(2.0 ** 80) for x in draw().__next__()], q, 0.125, {})
 
 
+@pytest.mark.parametrize("seed", range(48))
+def test_drawn(hip, seed):
+    """Any types, heads, pages, rules, counts and holes together."""
+    rng = np.random.default_rng(1000 + seed)
+    kind, heads, G, dk, page_rows = int(rng.integers(3)), int(rng.integers(1, 5)), int(rng.integers(1, 20)), 4 * int(rng.integers(1, 33)), 1 << int(rng.integers(0, 9))
+    B, most = int(rng.integers(1, 9)), int(rng.choice([1, 2, 9, 40, 150, 400]))
+    new = rng.integers(0, most + 1, B)
+    new[0] = most
+    lens = np.maximum(new + rng.integers(-2, 300, B) * rng.integers(0, 2, B), 0)
+    if rng.random() < 0.3:
+        new[:] = most
+    rules = {}
+    if rng.random() < 0.5:
+        rules.update(window=int(rng.choice([1, 3, 31, 32, 33, 64, 100, 257])), sinks=int(rng.choice([0, 1, 4, 32, 33, 130])))
+    if rng.random() < 0.3:
+        rules.update(cap=float(rng.choice([0.5, 5.0, 50.0])))
+    holes = [(b, int(rng.integers(0, max(1, -(-int(lens[b]) // page_rows))))) for b in range(B) if lens[b] and rng.random() < 0.3]
+    say("drawn", seed, kind, heads, G, dk, page_rows, new.tolist(), lens.tolist(), rules, holes)
+    check(hip, kind, heads, G, dk, page_rows, new.tolist(), lens.tolist(), rules, bool(rng.random() < 0.3), holes, seed, pitch=4 * int(rng.integers(0, 3)), behind=int(rng.integers(0, 3)),
+          uniform=False)
+
+
 # ---- together --------------------------------------------------------------------------------------------------------
 
 @TYPES
