@@ -472,7 +472,8 @@ typedef struct {
  * multiple of them: query head h reads head h / (H / heads)).  Rows of Q and O hold H * dk floats; L [T, H] is the log-sum-exp of each row of scores, or NULL.  Sk is the most
  * positions that any sequence has (lens is taken as Sk above it).  A row that sees no key, padding among them, gets O = 0 and L = -infinity; rows of no sequence are left as they
  * were.  What a query does not see has no part in its results, whatever it holds.  Pitches multiples of 4 floats up to 2^22, Q and O 16-byte aligned, outputs apart from all
- * else.  cap and scale as for axhip_attn_fwd; precision too, with what the cache holds taken exactly (of F16 and I8; an MX4 number below 2^-36 of its row's largest loses bits).
+ * else.  cap and scale as for axhip_attn_fwd; precision too, with what the cache holds taken exactly (an MX4 number below 2^-36 of its row's largest, or of a row below
+ * 2^-100, loses bits).
  * The rules are read before the call returns. */
 int axhip_attn_paged(const float *Q, int64_t ldq, const axhip_kv_cache *cache, float *O, int64_t ldo, float *L, const int32_t *first, const int32_t *lens, int64_t B,
                      int64_t T, int64_t H, int64_t Sq, int64_t Sk, float scale, const axhip_kv_rules *rules);

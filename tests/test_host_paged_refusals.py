@@ -67,7 +67,8 @@ def names(**more):
 assert names(Sq=1, T=3, first=None) == ["few"] and names(Sq=4, T=9) == ["few"] and names(Sq=16, T=9) == ["few"]
 assert names(Sq=100, T=300, first=None, Sk=100) == ["few"] and names(Sq=100, T=100, B=1) == ["few"]
 assert names(Sq=4000, T=12000, first=None) == ["tiles"] and names(Sq=8000, T=8000, B=1) == ["tiles"]
-assert names(Sq=100, T=120) == ["few", "tiles"]
+assert names(Sq=100, T=120) == ["few", "tiles"] and names(Sq=100, T=150) == ["few"]
+assert names(Sq=4000, T=12000) == ["tiles"] and names(Sq=4000, T=11999) == ["few", "tiles"]
 assert names(Sq=2000, T=2000, B=1, Sk=100000, table_ld=10000) == ["tiles", "join"]
 """)
 
