@@ -381,6 +381,27 @@ def test_infinities_and_nans(hip, kind, new):
 
 
 @TYPES
+@pytest.mark.parametrize("new", [1, 40, 130])
+@pytest.mark.parametrize("garbage", [0xff, 0x7c])
+def test_rows_that_were_never_written(hip, kind, new, garbage):
+    """Positions behind a window that hold bytes of all kinds (NaNs and infinities as f16 and as scales), on pages that are there: as if they were not."""
+    say("never written", kind, new, garbage)
+    rng = np.random.default_rng(13)
+    heads, G, dk, length, window = 2, 4, 64, 300, 30
+    written = new + window
+    table, pages = table_of(rng, [length], 16)
+    cache = Cache(hip, kind, heads, dk, 16, table, pages, fill=garbage)
+    k, v = (rng.normal(size=(written, heads, dk)).astype(np.float32) for _ in range(2))
+    write(hip, cache, k, v, None, [length], written)
+    q = rng.normal(size=(new, heads * G, dk)).astype(np.float32)
+    o, lse = attend(hip, cache, q, [new], [length], dict(window=window))
+    kk, vv = (np.concatenate([np.zeros((length - written, heads, dk)), quantised(kind, x)[2]]) for x in (k, v))
+    w = paged_attention(q, kk, vv, np.ones(length, bool), dk ** -0.5, window=window)
+    within(o, w, "o")
+    within(lse, w, "lse")
+
+
+@TYPES
 @pytest.mark.parametrize("new", [[1, 2], [60, 70]])
 def test_sizes_far_apart(hip, kind, new):
     """Huge values and keys that a window hides, rows of zeros, tiny rows, huge keys under tiny queries."""
