@@ -582,7 +582,9 @@ int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid) {
     grid.per = (rows + G::BQ - 1) / G::BQ;
     grid.slots = a.pages.first ? all_rows / G::BQ + a.pages.B : a.pages.B * grid.per;
     const int64_t likely = (a.pages.first ? all_rows / G::BQ + 1 : grid.slots) * a.pages.heads, blocks = paged_steps_most(a, G::SHIFT, G::BQ);
-    grid.splits = (int)paged_tile_splits(likely, blocks);
+    // (each slot has a place for what its ranges leave, also those of sequences that turn out to have few rows: 256 MiB at most)
+    const int64_t of_range = grid.slots * a.pages.heads * G::PART * (int64_t)sizeof(float);
+    grid.splits = (int)std::max<int64_t>(1, std::min(paged_tile_splits(likely, blocks), (int64_t(256) << 20) / of_range));
     grid.range = (int)std::max<int64_t>((blocks + grid.splits - 1) / grid.splits, 1);
     auto run = [&](auto of) {
         constexpr int TYPE = decltype(of)::value;

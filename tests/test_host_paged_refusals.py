@@ -90,3 +90,16 @@ for rules in (None, KvRules(window=1000, sinks=4, cap=10.0)):
 for x in launched():
     assert 0 < x.grid[0] < 1 << 31 and x.grid[0] * x.block[0] < 1 << 32 and x.block[0] <= 1024 and x.shared <= 160 * 1024, (x.kernel, list(x.grid), list(x.block))
 """ % ((B, T, H, heads, Sq, Sk, dk, kind, uniform),))
+
+
+@pytest.mark.parametrize("B,T,H,heads,Sq,Sk,dk", [(2000, 6000, 8, 8, 2000, 4000, 128), (300, 3000, 32, 8, 1000, 100000, 128), (24, 2217, 16, 4, 600, 3000, 80), (1, 64, 32, 8, 64, 1 << 20, 128),
+                                                  (128, 128, 8, 1, 1, 1 << 20, 128), (8388607, 1 << 20, 8, 1, 1000, 100000, 64)])
+def test_what_ranges_keep(stub, B, T, H, heads, Sq, Sk, dk):  # noqa: F811
+    """The shared workspace holds what ranges of keys leave, and stays at 256 MiB or what it started with, however many sequences a call has."""
+    run(stub, PAGED + """
+B, T, H, heads, Sq, Sk, dk = %r
+hip.check(attend(ldq=H * dk, ldo=H * dk, H=H, Sk=Sk, heads=heads, dk=dk, pages=1 << 12, table_ld=1 << 20, B=B, T=T, Sq=Sq))
+have = C.c_size_t()
+hip.check(L.axhip_workspace_reserve(0, C.byref(have)))
+assert have.value <= 256 * MIB, have.value
+""" % ((B, T, H, heads, Sq, Sk, dk),))
