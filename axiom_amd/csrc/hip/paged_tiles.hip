@@ -16,6 +16,7 @@
 #include "attn_launch.h"
 #include "attn_tiles.h"
 #include "paged.h"
+#include "paged_share.h"
 
 namespace {
 using namespace axhip;
@@ -78,7 +79,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
     using B = typename G::B;
     using T = KvType<TYPE>;
     constexpr int KS = DK / 16, DT = DK / 32, BKV = G::BKV, TILES = BKV / 32, BQ = G::BQ;
-    constexpr int COLS = 128 / T::BITS, LANES = (DK == 96 ? 128 : DK) / COLS, PASSES = 2 * BKV * LANES > 64 * WAVES ? 2 * BKV * LANES / (64 * WAVES) : 1;
+    using S = BlockShare<DK, T::BITS, BKV, 64 * WAVES>;
+    constexpr int COLS = S::COLS, LANES = S::LANES, PASSES = S::PASSES, PLACES = S::PLACES;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const KvPages &kv = a.pages;
     const AttnArgs &at = a.attn;
@@ -113,8 +115,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
     const float slope2 = at.slopes ? at.slopes[head] * at.bias2 : 0.0f;
 
     const unsigned base = lds_address(lds);
-    // A pass brings 16 bytes a thread: LANES threads a row, rows of keys and then of values.
-    constexpr int PLACES = PASSES > 1 ? PASSES / 2 : 1;          // with two passes or more, the second half brings the values of the first half's keys
+    // A pass brings 16 bytes a thread (paged_share.h).
     v4i x[PASSES];
     unsigned scales[PASSES];
     int entry[PLACES];
@@ -123,7 +124,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
     // where this lane's bytes of row zero of a page zero are, and the scale of that row
     const unsigned char *const k0 = kv.k + kv_row_at(kv, 0, hk, 0) + 16 * ((int)threadIdx.x % LANES), *const s0 = kv.k_scale + kv_scale_at(kv, 0, hk, 0);
     const int64_t to_v = kv.v - kv.k, to_v_scale = kv.v_scale - kv.k_scale;
-    auto row_of = [&](int pass) { return (pass * 64 * WAVES + (int)threadIdx.x) / LANES; };      // from BKV on a value's; from 2 BKV on none
+    auto row_of = [&](int pass) { return S::row((int)threadIdx.x, pass); };
+    auto has_row = [&](int pass) { return S::has_row((int)threadIdx.x, pass); };
     auto pos_of = [&](int n, int place) { return blocks.tile(n) * BKV + row_of(place) % BKV; };
     auto look = [&](int n) {
 #pragma unroll
@@ -140,7 +142,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
 #pragma unroll
         for (int p = 0; p < PLACES; p++) {
             const int pos = pos_of(n, p);
-            if (pos < wg_high.end && kv_is_page(kv, entry[p]) && (2 * BKV * LANES >= 64 * WAVES || row_of(p) < 2 * BKV)) {
+            const bool page = pos < wg_high.end && kv_is_page(kv, entry[p]);
+            if (S::misses((int)threadIdx.x, p, page)) gone |= 1u << p;
+            if (page && has_row(p)) {
                 const unsigned in_page = (unsigned)pos & ((1u << kv.shift) - 1);
                 const unsigned char *const k = k0 + ((uint64_t)(unsigned)entry[p] * kv.page_bytes + __umul24(in_page, (unsigned)kv.row_bytes));
                 const unsigned char *const k_scale = s0 + ((uint64_t)(unsigned)entry[p] * kv.page_scales + 4 * in_page);
@@ -157,8 +161,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
                     if (some) x[p] = *reinterpret_cast<const v4i *>(of_v ? k + to_v : k);
                     scales[p] = *reinterpret_cast<const unsigned *>(of_v ? k_scale + to_v_scale : k_scale);
                 }
-            } else {
-                gone |= 1u << p;
             }
         }
     };
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_paged_tiles(PagedArgs a, Page
 #pragma unroll
         for (int p = 0; p < PASSES; p++) {
             const int at_row = row_of(p), c = (int)threadIdx.x % LANES, in_block = at_row % BKV;
-            if (2 * BKV * LANES >= 64 * WAVES || at_row < 2 * BKV) {
+            if (has_row(p)) {
                 const bool of_v = PASSES > 1 ? p >= PLACES : at_row >= BKV;
                 const unsigned to = base + cur + (of_v ? G::V_AT : 0);
                 if (DK != 96 || c * COLS < DK) {
