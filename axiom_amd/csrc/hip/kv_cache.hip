@@ -262,7 +262,7 @@ int kv_arguments(const char *who, KvPages &a, const axhip_kv_cache *cache, const
     a.page_scales = (uint32_t)(c.heads * c.page_rows * 4);
     a.B = (int)B;
     a.T = (int)T;
-    a.Sq = (int)Sq;
+    a.Sq = (int)(first && T < Sq ? T : Sq);          // (a bound: no sequence has more rows than there are)
     a.room = (int)(c.table_ld < LONG >> a.shift ? c.table_ld << a.shift : LONG);
     return AXHIP_OK;
 }

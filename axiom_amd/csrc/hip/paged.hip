@@ -70,8 +70,9 @@ extern "C" int axhip_attn_paged(const float *Q, int64_t ldq, const axhip_kv_cach
     if (a.pages.room > Sk) a.pages.room = (int)Sk;
     // How many rows each sequence has is on the device: where some may have many and others few, both forms are launched, each for its own.  (There a sequence is few rows' with 32 of them, or one
     // token of many heads.)  Either form is right for any counts; as many rows as there can be are taken to be equal ones, and half as many to be near enough for few rows to take all.
-    const bool equal = !first || T == B * Sq;
-    if ((equal || B == 1 || 2 * T >= B * Sq || (int64_t)t.G * Sq <= FEW_ROWS) && few_is_faster(a)) return paged_few(a, cache->type, 0x7fffffff);
+    const int64_t most = a.pages.Sq;
+    const bool equal = !first || T == B * most;
+    if ((equal || B == 1 || 2 * T >= B * most || t.G * most <= FEW_ROWS) && few_is_faster(a)) return paged_few(a, cache->type, 0x7fffffff);
     if (equal || B == 1) return paged_tiles(a, cache->type, 0);
     const int like = t.G > LIKE_ROWS ? (t.G + 15) / 16 * 16 : LIKE_ROWS;
     if (int rc = paged_few(a, cache->type, like)) return rc;

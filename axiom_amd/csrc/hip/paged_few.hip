@@ -10,6 +10,8 @@
 //
 // One token over 500 int8 keys, 16 heads, 4 of keys, of 64: 7.8 us (9.2 with four waves and ranges); of 32 sequences over up to 4096, 32 heads, 8 of keys, of 128 49 us, 4.3 TB/s of cache (53 with four waves); equal ones of 8192 5.4
 // TB/s; two tokens of 8 over up to 32768 of 4 bits, 64 heads, 8 of keys 62 us.  Entries checked where they are read, which waits for all that is under way: 73 instead of 53, and 87 instead of 63.
+#include <algorithm>
+
 #include "attn_launch.h"
 #include "attn_tiles.h"
 #include "paged.h"
@@ -471,9 +473,14 @@ int paged_few(const PagedArgs &a, int type, int rows_most) {
     grid.most = rows_most;
     const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, most = rows < rows_most ? rows : rows_most, tiles = paged_steps_most(a, 5, ROWS);
     grid.row_tiles = (int)((most + ROWS - 1) / ROWS);
-    // (where only some of the sequences are this form's, most of those have a single new token)
-    const int64_t of_b = rows <= rows_most ? grid.row_tiles : (a.attn.G + ROWS - 1) / ROWS;
-    grid.splits = (int)paged_few_splits(a.pages.B * a.pages.heads * of_b, tiles);
+    // In how many ranges goes by the sets of rows that there are; where only some of the sequences are this form's, most of those have a single new token.  Where a sequence may have all rows of the
+    // call, they are taken to be one token each and the others in full sets: eight single tokens over 4096 int8 keys, 64 heads, 8 of keys, of 128, with Sq = 8 or more 21 us as with Sq = 1, and 38 by the most
+    // that each may have.  (Not so for counts between: workgroups that find nothing delay others, and ranges make more of those.  16 tokens of one of 16 sequences and one of each other, 4 bits: 25 instead of 19.)
+    const int64_t B = a.pages.B, T = a.pages.T, of_token = (a.attn.G + ROWS - 1) / ROWS, some = std::min(B, T);
+    int64_t sets = B * (rows <= rows_most ? grid.row_tiles : of_token);
+    if (a.pages.first && rows <= rows_most && T == a.pages.Sq)
+        sets = std::min(sets, std::max(some * of_token + (a.attn.G * (T - some) + ROWS - 1) / ROWS, sets / 4));      // (a quarter at least: of what finds nothing, and what it could leave, there is no more than four times)
+    grid.splits = (int)paged_few_splits(a.pages.heads * sets, tiles);
     const int waves = tiles > 4 ? 8 : 4;
     auto run = [&](auto width) {
         constexpr int DK = decltype(width)::value;

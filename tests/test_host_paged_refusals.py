@@ -103,3 +103,38 @@ have = C.c_size_t()
 hip.check(L.axhip_workspace_reserve(0, C.byref(have)))
 assert have.value <= 256 * MIB, have.value
 """ % ((B, T, H, heads, Sq, Sk, dk),))
+
+
+def test_a_bound_on_rows_is_no_count_of_them(stub):  # noqa: F811
+    """Sq is the most rows that a sequence may have, and none has more than there are: callers with a bound of their own launch for the rows that come."""
+    run(stub, PAGED + """
+def shapes(**more):
+    before = stub.stub_launches()
+    assert attend(**more) == 0
+    return [(x.kernel, list(x.grid), list(x.block)) for x in launched()[before:]]
+for B, T in ((1, 1), (1, 3), (8, 8), (3, 10), (1, 40), (1, 300)):
+    for heads, H, dk in ((2, 4, 64), (8, 64, 128), (1, 1, 32)):
+        for rules in (None, KvRules(window=30, sinks=4)):
+            more = dict(B=B, T=T, heads=heads, H=H, dk=dk, ldq=H * dk, ldo=H * dk, rules=rules)
+            want = shapes(Sq=T, **more)
+            for Sq in (T + 1, 4096, 1 << 24):
+                assert shapes(Sq=Sq, **more) == want, (B, T, heads, Sq)
+assert all(b"paged_few" in x[0] for T in (1, 8) for x in shapes(B=T, T=T, Sq=4096, heads=8, H=64, dk=128, ldq=8192, ldo=8192)[:1])
+assert len(shapes(B=1, T=1, Sq=4096, heads=8, H=64, dk=128, ldq=8192, ldo=8192)) == 1
+# eight single tokens with room for eight each: as many ranges of keys, a workgroup for each of the four sets of rows that each could have
+one, more = (shapes(B=8, T=8, Sq=Sq, heads=8, H=64, dk=128, ldq=8192, ldo=8192, Sk=4096, table_ld=256)[0] for Sq in (1, 4096))
+assert one[1][0] > 8 * 8 and more[1][0] == 4 * one[1][0] and one[2] == more[2], (one, more)
+""")
+
+
+@pytest.mark.parametrize("B,T,H,heads,dk", [(1000, 64, 1, 1, 128), (8, 8, 64, 8, 128), (100000, 16, 4, 1, 128), (3, 60, 8, 8, 64), (2, 500, 8, 8, 128), (300, 3, 64, 4, 64)])
+@pytest.mark.parametrize("Sq", [0, 1 << 24])
+def test_what_ranges_of_few_rows_keep(stub, B, T, H, heads, dk, Sq):  # noqa: F811
+    """... and where any sequence may have all of the rows, ranges are counted by the rows that there are, within what the workspace and the counters start with."""
+    run(stub, PAGED + """
+B, T, H, heads, dk, Sq = %r
+hip.check(attend(ldq=H * dk, ldo=H * dk, H=H, Sk=100000, heads=heads, dk=dk, pages=1 << 12, table_ld=1 << 20, B=B, T=T, Sq=Sq or T))
+have = C.c_size_t()
+hip.check(L.axhip_workspace_reserve(0, C.byref(have)))
+assert have.value == 160 * MIB and all(x.grid[0] < 1 << 22 for x in launched()), have.value
+""" % ((B, T, H, heads, dk, Sq),))
