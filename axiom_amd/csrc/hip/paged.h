@@ -25,7 +25,6 @@ struct PagedTileGrid {
     int splits, range;                           // the most ranges of keys that a tile has, one for every `range` blocks
     int least;                                   // sequences with fewer rows are the few-rows form's
     float *parts;
-    int *arrivals;
 };
 
 int paged_few(const PagedArgs &a, int type, int rows_most);

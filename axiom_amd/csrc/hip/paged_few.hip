@@ -443,7 +443,7 @@ int launch_few(const PagedArgs &a, PagedFewGrid grid) {
         if (!grid.parts || !grid.arrivals) return AXHIP_ERR_ALLOC;
     }
     note_kernel(grid.splits > 1 ? "paged_few_ranges" : "paged_few");
-    const int64_t at_once = GRID_MOST / (of_b * grid.splits);    // sequences a launch; (a sequence has at most 2^21 units, and ranges only where there are few)
+    const int64_t at_once = std::max<int64_t>(1, GRID_MOST / (of_b * grid.splits));      // sequences a launch; (one has at most 2^22 units, of 2^20 heads with 64 rows, and ranges only where there are few)
     for (grid.first = 0; grid.first < a.pages.B; grid.first += (int)at_once) {
         const int64_t left = a.pages.B - grid.first, here = left < at_once ? left : at_once;
         grid.here = (int)here;

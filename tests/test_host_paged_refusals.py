@@ -138,3 +138,11 @@ have = C.c_size_t()
 hip.check(L.axhip_workspace_reserve(0, C.byref(have)))
 assert have.value == 160 * MIB and all(x.grid[0] < 1 << 22 for x in launched()), have.value
 """ % ((B, T, H, heads, dk, Sq),))
+
+
+def test_as_many_workgroups_a_sequence_as_a_launch_holds(stub):  # noqa: F811
+    """2^20 heads of four sets of rows each: a launch a sequence."""
+    run(stub, PAGED + """
+hip.check(attend(ldq=1 << 22, ldo=1 << 22, H=1 << 20, heads=1 << 20, dk=4, pages=1 << 12, table_ld=1 << 20, Sk=100, B=3, T=192, Sq=64, first=None))
+assert [x.grid[0] for x in launched()] == [1 << 22] * 3 and all(b"paged_few" in x.kernel for x in launched())
+""")
