@@ -122,71 +122,84 @@ __device__ __forceinline__ void paged_again(const PagedArgs &a, int b, const KvS
     const int64_t at = (int64_t)s.first + i;
     const float *q = a.attn.Q + at * a.attn.ldq + (int64_t)head * dk;
     const float slope2 = a.attn.slopes ? a.attn.slopes[head] * a.attn.bias2 : 0.0f;
-    float m = ATTN_LOWEST, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    bool any = false;
-    for (int k0 = 0; k0 < r.end; k0 += 64) {
-        if (k0 + 64 <= r.begin && k0 >= a.sinks) {   // nothing before the window's first 64
-            k0 = (r.begin & ~63) - 64;
-            continue;
-        }
-        const int key = k0 + lane;
-        bool sees = key < r.end && (key >= r.begin || key < a.sinks);
-        int page = 0;
-        if (sees) {
-            page = kv_page(kv, b, key);
-            sees = page >= 0;
-        }
-        float x = -INFINITY;
-        if (sees) {
-            const unsigned scale = *reinterpret_cast<const unsigned *>(kv.k_scale + kv_scale_at(kv, page, hk, key));
-            const unsigned char *row = kv.k + kv_row_at(kv, page, hk, key);
-            float sum = 0.0f;
-            for (int c = 0; 8 * c < dk; c++) {
-                float k[8];
-                kv_eight<TYPE>(row, scale, c, k);
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (8 * c + e < dk) sum = __builtin_fmaf(q[8 * c + e] * a.attn.q_up, k[e], sum);
+    // Sums of values near the largest float may pass it where their mean does not: such columns are formed once more, with 2^-25 of each weight, since there are up to 2^24 keys.
+    float m, l, o0, o1, once0, once1, down = 1.0f;
+    bool any;
+#pragma unroll 1
+    for (;;) {
+        m = ATTN_LOWEST;
+        l = o0 = o1 = 0.0f;
+        any = false;
+        for (int k0 = 0; k0 < r.end; k0 += 64) {
+            if (k0 + 64 <= r.begin && k0 >= a.sinks) {   // nothing before the window's first 64
+                k0 = (r.begin & ~63) - 64;
+                continue;
             }
-            if (a.attn.cap > 0.0f) sum = capped(a.attn, sum).score;
-            x = a.attn.slopes ? __builtin_fmaf(-slope2, (float)(r.p - key), sum) : sum;
-        }
-        uint64_t seen = __builtin_amdgcn_ballot_w64(sees);
-        if (!seen) continue;
-        any = true;
-        const float m_new = fmaxf(m, wave_max(x)), alpha = __builtin_amdgcn_exp2f(m - m_new);
-        const float p = sees ? __builtin_amdgcn_exp2f(x - m_new) : 0.0f;
-        m = m_new;
-        l = l * alpha + wave_sum(p);
-        o0 *= alpha;
-        o1 *= alpha;
-        for (; seen; seen &= seen - 1) {
-            const int j = __builtin_ctzll(seen);
-            const float pj = from_lane(p, j);
-            const int of_j = __builtin_amdgcn_readlane(page, j);
-            const unsigned scale = *reinterpret_cast<const unsigned *>(kv.v_scale + kv_scale_at(kv, of_j, hk, k0 + j));
-            const unsigned char *row = kv.v + kv_row_at(kv, of_j, hk, k0 + j);
-            float v[8];
-            if (lane < dk) {
-                kv_eight<TYPE>(row, scale, lane >> 3, v);
-                float mine = v[0];
-#pragma unroll
-                for (int e = 1; e < 8; e++) mine = (lane & 7) == e ? v[e] : mine;
-                o0 = __builtin_fmaf(pj, mine, o0);
+            const int key = k0 + lane;
+            bool sees = key < r.end && (key >= r.begin || key < a.sinks);
+            int page = 0;
+            if (sees) {
+                page = kv_page(kv, b, key);
+                sees = page >= 0;
             }
-            if (lane + 64 < dk) {
-                kv_eight<TYPE>(row, scale, 8 + (lane >> 3), v);
-                float mine = v[0];
+            float x = -INFINITY;
+            if (sees) {
+                const unsigned scale = *reinterpret_cast<const unsigned *>(kv.k_scale + kv_scale_at(kv, page, hk, key));
+                const unsigned char *row = kv.k + kv_row_at(kv, page, hk, key);
+                float sum = 0.0f;
+                for (int c = 0; 8 * c < dk; c++) {
+                    float k[8];
+                    kv_eight<TYPE>(row, scale, c, k);
 #pragma unroll
-                for (int e = 1; e < 8; e++) mine = (lane & 7) == e ? v[e] : mine;
-                o1 = __builtin_fmaf(pj, mine, o1);
+                    for (int e = 0; e < 8; e++)
+                        if (8 * c + e < dk) sum = __builtin_fmaf(q[8 * c + e] * a.attn.q_up, k[e], sum);
+                }
+                if (a.attn.cap > 0.0f) sum = capped(a.attn, sum).score;
+                x = a.attn.slopes ? __builtin_fmaf(-slope2, (float)(r.p - key), sum) : sum;
+            }
+            uint64_t seen = __builtin_amdgcn_ballot_w64(sees);
+            if (!seen) continue;
+            any = true;
+            const float m_new = fmaxf(m, wave_max(x)), alpha = __builtin_amdgcn_exp2f(m - m_new);
+            const float p = sees ? __builtin_amdgcn_exp2f(x - m_new) : 0.0f;
+            m = m_new;
+            l = l * alpha + wave_sum(p);
+            o0 *= alpha;
+            o1 *= alpha;
+            for (; seen; seen &= seen - 1) {
+                const int j = __builtin_ctzll(seen);
+                const float pj = from_lane(p, j) * down;
+                const int of_j = __builtin_amdgcn_readlane(page, j);
+                const unsigned scale = *reinterpret_cast<const unsigned *>(kv.v_scale + kv_scale_at(kv, of_j, hk, k0 + j));
+                const unsigned char *row = kv.v + kv_row_at(kv, of_j, hk, k0 + j);
+                float v[8];
+                if (lane < dk) {
+                    kv_eight<TYPE>(row, scale, lane >> 3, v);
+                    float mine = v[0];
+#pragma unroll
+                    for (int e = 1; e < 8; e++) mine = (lane & 7) == e ? v[e] : mine;
+                    o0 = __builtin_fmaf(pj, mine, o0);
+                }
+                if (lane + 64 < dk) {
+                    kv_eight<TYPE>(row, scale, 8 + (lane >> 3), v);
+                    float mine = v[0];
+#pragma unroll
+                    for (int e = 1; e < 8; e++) mine = (lane & 7) == e ? v[e] : mine;
+                    o1 = __builtin_fmaf(pj, mine, o1);
+                }
             }
         }
+        if (down < 1.0f) break;
+        once0 = o0;
+        once1 = o1;
+        if (!(l > 0.0f) || !__builtin_amdgcn_ballot_w64(!(__builtin_fabsf(o0) < INFINITY && __builtin_fabsf(o1) < INFINITY))) break;
+        down = 0x1p-25f;
     }
-    float *o = a.attn.O + at * a.attn.ldo + (int64_t)head * dk;
     const float inv = any ? 1.0f / l : 0.0f;
-    if (lane < dk && lane >= c0 && lane < c1) o[lane] = any ? o0 * inv : 0.0f;
-    if (lane + 64 < dk && lane + 64 >= c0 && lane + 64 < c1) o[lane + 64] = any ? o1 * inv : 0.0f;
+    auto mean = [&](float once, float again) { return __builtin_fabsf(once) < INFINITY ? once * inv : again * inv * 0x1p25f; };
+    float *o = a.attn.O + at * a.attn.ldo + (int64_t)head * dk;
+    if (lane < dk && lane >= c0 && lane < c1) o[lane] = any ? mean(once0, o0) : 0.0f;
+    if (lane + 64 < dk && lane + 64 >= c0 && lane + 64 < c1) o[lane + 64] = any ? mean(once1, o1) : 0.0f;
     // (a row that saw nothing but scores of -infinity: 0 / 0 above, and NaN here)
     if (a.attn.L && lane == 0 && c0 == 0) a.attn.L[at * a.attn.H + head] = !any ? -INFINITY : l == 0.0f ? NAN : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
