@@ -583,7 +583,9 @@ int launch_tiles(const PagedArgs &a, int type, PagedTileGrid grid) {
     const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, all_rows = (int64_t)a.attn.G * a.pages.T;
     grid.per = (rows + G::BQ - 1) / G::BQ;
     grid.slots = a.pages.first ? all_rows / G::BQ + a.pages.B : a.pages.B * grid.per;
-    const int64_t likely = (a.pages.first ? all_rows / G::BQ + 1 : grid.slots) * a.pages.heads, blocks = paged_steps_most(a, G::SHIFT, G::BQ);
+    // (tiles of equal counts as they are, however those are given: 64 tokens over 8192 int8 keys, 32 heads, 8 of keys, of 128, counted as the two tiles that rows anywhere could touch took 50 us, so 42)
+    const bool equal = !a.pages.first || a.pages.B == 1 || a.pages.T == (int64_t)a.pages.B * a.pages.Sq;
+    const int64_t likely = (equal ? a.pages.B * grid.per : all_rows / G::BQ + 1) * a.pages.heads, blocks = paged_steps_most(a, G::SHIFT, G::BQ);
     // (each slot has a place for what its ranges leave, also those of sequences that turn out to have few rows: 256 MiB at most)
     const int64_t of_range = grid.slots * a.pages.heads * G::PART * (int64_t)sizeof(float);
     grid.splits = (int)std::max<int64_t>(1, std::min(paged_tile_splits(likely, blocks), (int64_t(256) << 20) / of_range));

@@ -146,3 +146,23 @@ def test_as_many_workgroups_a_sequence_as_a_launch_holds(stub):  # noqa: F811
 hip.check(attend(ldq=1 << 22, ldo=1 << 22, H=1 << 20, heads=1 << 20, dk=4, pages=1 << 12, table_ld=1 << 20, Sk=100, B=3, T=192, Sq=64, first=None))
 assert [x.grid[0] for x in launched()] == [1 << 22] * 3 and all(b"paged_few" in x.kernel for x in launched())
 """)
+
+
+@pytest.mark.parametrize("B,n,H,heads,dk,Sk", [(1, 64, 32, 8, 128, 8192), (2, 150, 16, 4, 64, 30000), (1, 300, 8, 8, 80, 20000), (3, 257, 4, 1, 128, 50000)])
+def test_ranges_of_equal_counts_however_they_are_given(stub, B, n, H, heads, dk, Sk):  # noqa: F811
+    """Sequences of n rows each, with `first` and without: tiles have as many ranges of keys."""
+    run(stub, PAGED + """
+B, n, H, heads, dk, Sk = %r
+G = H // heads
+BQ = 256 if G * n > 128 else 128
+def splits(first, slots, Sq=n):
+    before = stub.stub_launches()
+    hip.check(attend(ldq=H * dk, ldo=H * dk, H=H, Sk=Sk, heads=heads, dk=dk, pages=1 << 12, table_ld=1 << 12, B=B, T=B * n, Sq=Sq, first=first))
+    tiles, join = launched()[before:]
+    assert b"paged_tiles" in tiles.kernel and b"paged_join" in join.kernel and tiles.grid[0] %% (slots * heads) == 0
+    return tiles.grid[0] // (slots * heads)
+want = splits(None, B * -(-G * n // BQ))
+assert want > 1 and splits(P[7], G * B * n // BQ + B) == want, want
+if B == 1:
+    assert splits(P[7], G * n // BQ + 1, Sq=4096) == want
+""" % ((B, n, H, heads, dk, Sk),))
