@@ -3,7 +3,8 @@
 // One pass each.  Writing: a wave takes a row of both arrays, LANES lanes a head of it, eight columns a lane (two 16-byte accesses); the largest magnitude is an integer maximum of the bits over
 // the lanes of a head (of a group of 32 columns, four lanes), which infinities and NaNs pass.  Many rows are HBM-bound, AHEAD heads of a lane group under way at once; few rows are five trips to
 // memory one after the other (arguments, the row's sequence, its length, the page, the row), with a head a lane group.
-// 13156 rows of 8 heads of 128 into 4 bits 32 us, 4.9 TB/s, and back 25, 5.1 TB/s; 16 rows into int8 3.5 to 3.9 (5.6 with four heads a lane group).
+// 14768 rows of 8 heads of 128 into 4 bits 33 us, 4.1 TB/s, and back 25, 5.4 TB/s; into f16 48, 3.8 TB/s, and back 29, 6.2 TB/s, of 80 32, 3.6 TB/s (six of sixteen lanes hold nothing), and back 22; 16 rows into int8 3.3 to
+// 3.7 (5.6 with four heads a lane group).
 #include "kv_pages.h"
 
 namespace {

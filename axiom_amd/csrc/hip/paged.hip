@@ -11,6 +11,9 @@ using namespace axhip;
 // (16-row units of 8 waves that take 32 keys each; tiles of 256 rows, or 128, in blocks.)  Within a tenth or so of what was measured (us, tiles -> few rows: 1 x 128 tokens over 128 keys, 32 heads, 8
 // of keys, of 128 19.6 -> 7.8, 1 x 512 over 512, 8 heads 31 -> 15.5, 4 x 64 over 500, 32 heads, 8 of keys 33 -> 25; the other side 64 x 32 over 100, 32 heads, 8 of keys 38 -> 58, 16 x 64 over 64, 16 heads, 4
 // of keys, of 64 14.3 -> 20.7).  Up to 64 rows of a sequence few rows won throughout (8 x 8 tokens over 4096, 64 heads, 8 of keys 49 -> 44, 1 x 8 24 -> 17).
+// Beside sequences of many rows those of more than 32 are the tiles': few rows run before the tiles and not beside them, so what they take is added, while tiles that few rows fill in part run in rounds that others fill.
+// (us, of 32 -> of 64: 600 tokens and 16 sequences of 8 over up to 4096, 32 heads, 4 of keys, of 128, 64 rows each, int8 159 -> 174, f16 163 -> 203, 4 bits 162 -> 167; of 5, 64 heads, 8 of keys, f16 305 -> 341; 2000 and 8 of
+// 64 over 500, 8 heads of 64, f16 46 -> 66; the other side four of 512 and 32 of 8, 8 heads, one of keys, int8 149 -> 139, and 1000 and 30 of 9, 16 heads, 4 of keys, of 80, f16 132 -> 122.)
 constexpr int FEW_ROWS = 64, LIKE_ROWS = 32;
 bool few_is_faster(const PagedArgs &a) {
     const int64_t rows = (int64_t)a.attn.G * a.pages.Sq, cus = cu_count();

@@ -8,9 +8,10 @@
 // fetched, 32-key tiles that no row of a wave sees not computed, and only tiles that some row sees in part pay for the mask.
 // Where tiles would leave CUs idle, ranges of their keys go to workgroups of their own, as many as a tile's blocks ask for, and a second launch adds what they leave, in order.
 //
-// Bound by vector instructions (some 150 for a tile of 32 x 32 and, of the block's conversion, 25 to 75) and products (32 for heads of 128, 16 for 64), which the two waves of a SIMD overlap little.  Two chunks of 2048 tokens over
-// 4096 int8 keys, 32 heads, 8 of keys, of 128 take 311 us, 498 TFLOP/s of fp32 products (two f16 products each: a large library product in f16 does 1175); four prompts of up to 4096 in windows of 1024, 16 heads of 64, 4 bits 197,
-// of which conversion is 11 %, barriers 6 and the scores' products 22; 64 tokens over 8192 int8 keys, 32 heads, 8 of keys 33 and 9 for the sums of 32 ranges (38 and 15 with 128 rows and 16 ranges).
+// Bound by vector instructions (some 150 for a tile of 32 x 32 and, of the block's conversion, 25 to 75) and products (32 for heads of 128, 16 for 64), one kind after the other in a wave, of which the two
+// waves of a SIMD overlap little.  Two chunks of 2048 and 1564 tokens over up to 4096 int8 keys, 32 heads, 8 of keys, of 128 take 307 to 319 us, 504 to 486 TFLOP/s of fp32 products (two f16 products each: a large library product
+// in f16 does 1175); f16 317 to 331; four prompts of 2636 to 4096 in windows of 1024, 16 heads of 64, 4 bits 191, of which conversion is 11 %, barriers 6 and the scores' products 22; 64 tokens over 8192 int8 keys, 32 heads, 8 of keys 29 to 31 and 9
+// for the sums of 32 ranges (with 128 rows 33 and 7: level; the ranges leave 34 MB, twice the cache that is read).
 #include <algorithm>
 
 #include "attn_launch.h"

@@ -450,7 +450,8 @@ int64_t axhip_kv_row_bytes(int type, int64_t dk);
 
 /* The new rows of a call, in all three of the following: those of sequence b are rows first[b] .. first[b + 1] - 1 (at most Sq of them; first NULL: b * Sq .. b * Sq + Sq - 1,
  * and T = B * Sq) of arrays of T rows, and they are the last of its lens[b] positions: n rows, row i at position p = lens[b] - n + i.  Rows with p < 0 are padding, and
- * lens[b] is taken as 0 below 0 and as the table's room above it.  first [B + 1] must not fall; lens [B]; Sq, T and positions up to 2^24. */
+ * lens[b] is taken as 0 below 0 and as the table's room above it.  first [B + 1] must not fall; lens [B]; Sq, T and positions up to 2^24.  Sq, and Sk below, may be more than
+ * any sequence has, at the price of launches made for it. */
 
 /* Quantises rows of K and V (heads * dk floats, row pitches ldk and ldv) into their places.  Padding is not written. */
 int axhip_kv_write(const axhip_kv_cache *cache, const float *K, int64_t ldk, const float *V, int64_t ldv, const int32_t *first, const int32_t *lens, int64_t B,
